@@ -201,6 +201,98 @@ int vh_attention(vh_context *ctx, int sequences, int length, int heads, const vo
 int vh_attention_noalloc(vh_context *ctx, int sequences, int length, int heads, const void *qkv, void *out,
                          int apply_rotary, int flags);
 
+/* ---- layer norm ---------------------------------------------------------- */
+/* Type of activations and of their gradients; weights, statistics and the
+   weights' gradients are fp32. */
+#define VH_TYPE_FP32 0
+#define VH_TYPE_BF16 1
+/* Layer norm rows, beside vh_rmsnorm: y = (x - mean) * rstd * gamma + beta with
+   rstd = 1 / sqrt(mean of (x - mean)^2 + eps); fp32 inside, y rounded once.
+   Device x[rows][ldx], y[rows][ldy] of `type`, gamma[dim], beta[dim] (may be
+   null: 0); stats[rows][2] (may be null) receives (mean, rstd) for the backward
+   pass.  dim 1 to 16384, any pitch from dim up, rows from 0; y may be x.  Rows
+   of a pitch and dim that are multiples of 4, in tensors (and gamma, beta)
+   aligned to four elements, are read four elements at a time.  Issues one
+   kernel: no allocation, no synchronisation, fit for stream capture. */
+int vh_layernorm(vh_context *ctx, int type, int64_t rows, int dim, const void *x, int64_t ldx, const float *gamma,
+                 const float *beta, float eps, void *y, int64_t ldy, float *stats);
+/* Its backward pass from dy, x and the forward's stats:
+     h = (x - mean) rstd, g = dy gamma, dx = rstd (g - mean(g) - h mean(g h)),
+     dgamma = sum over rows of dy h, dbeta = sum over rows of dy
+   dgamma and dbeta (device [dim], written, not added to; each may be null) are
+   summed in a fixed order: equal calls give equal bits.  They need `workspace`,
+   vh_layernorm_workspace_bytes(rows, dim) bytes of device memory, 16-byte
+   aligned, the caller's: it is free again when the call's work is done, and two
+   captured graphs that may run at once need one each.  dx may be dy or x.  With
+   0 rows dgamma and dbeta are 0.  Issues kernels only. */
+int vh_layernorm_backward(vh_context *ctx, int type, int64_t rows, int dim, const void *dy, int64_t lddy, const void *x,
+                          int64_t ldx, const float *gamma, const float *stats, void *dx, int64_t lddx, float *dgamma,
+                          float *dbeta, void *workspace);
+/* 0: refused (vh_last_error). */
+size_t vh_layernorm_workspace_bytes(int64_t rows, int dim);
+
+/* ---- attention over another sequence's states ----------------------------- */
+/* Layout of vh_cross_attention, beside vh_attention (one packed projection, one
+   length, rotary): q [sequences][query_length][heads][64] attends to k and v
+   [sequences][key_length][kv_heads][64], heads a multiple of kv_heads (query
+   head h reads key head h / (heads / kv_heads)).  Heads are 64 wide. */
+typedef struct {
+    int type; /* VH_TYPE_* of q, k, v, out and of their gradients */
+    int sequences, heads, kv_heads, query_length, key_length;
+    int causal;  /* 1: query i of sequence s sees keys j <= query_start[s] + i */
+    float scale; /* of the scores q.k, e.g. 0.125 */
+    /* elements between sequences, rows and heads; a head's 64 are consecutive.
+       Each a multiple of 16 bytes, none negative, rows at most 2^26 bytes apart.
+       dq, dk and dv are laid out as q, k and v, dout as out; where a gradient or
+       out is written, no two (sequence, row, head) may share a place. */
+    int64_t q_strides[3], k_strides[3], v_strides[3], out_strides[3];
+    /* device [sequences], each may be null.  Rows from a sequence's query length
+       on are padding: their out and dq are 0.  Keys from its key length on are
+       never read; their dk and dv are 0.  Lengths beyond 0 and the tensors'
+       lengths act as those. */
+    const int32_t *query_lengths, *key_lengths;
+    /* position of query row 0 among the keys (null: 0), for causal and the bias:
+       a step of decoding gives the number of keys before its new tokens */
+    const int32_t *query_start;
+    /* learned relative position bias, null for none: device fp32
+       [buckets][heads], added to the scaled scores at bucket(j - (query_start +
+       i)), vh_relative_bucket's */
+    const float *bias_table;
+    int buckets, max_distance, bidirectional;
+} vh_cross;
+/* out = softmax(scale q k^T + bias) v over the keys a row sees.  A row that sees
+   none (no keys, causal before the first one, or a bias of -inf at all of them)
+   is 0.  The products run on the matrix cores (bf16 operands as they are, P
+   rounded to bf16; fp32 in fp32), scores, softmax and sums in fp32.
+   saved (may be null): vh_cross_saved_bytes bytes for the backward pass (the
+   rows' softmax statistics and, for bf16, what rounding took from out).
+   workspace: vh_cross_workspace_bytes(c, 0) bytes.  Tensors, saved and workspace
+   16-byte aligned device memory.  Issues kernels only, without allocation or
+   synchronisation, so it may be captured; workspace is free again when the
+   call's work is done, and graphs that may run at once need one each. */
+int vh_cross_attention(vh_context *ctx, const vh_cross *c, const void *q, const void *k, const void *v, void *out,
+                       void *saved, void *workspace);
+/* Its backward pass, from the forward's q, k, v, out and saved (unchanged) and
+   dout: dq, dk, dv (written, not added to; dk and dv may both be null) and, when
+   not null, dbias [buckets][heads], the table's gradient.  Shared key heads
+   receive the sum over their query heads; a bias table shared by several calls
+   and inputs that several sequences share are summed by the caller.  Every sum
+   has a fixed order: equal calls give equal bits.  workspace:
+   vh_cross_workspace_bytes(c, 1) bytes. */
+int vh_cross_attention_backward(vh_context *ctx, const vh_cross *c, const void *q, const void *k, const void *v,
+                                const void *out, const void *saved, const void *dout, void *dq, void *dk, void *dv,
+                                float *dbias, void *workspace);
+/* 0: refused (vh_last_error). */
+size_t vh_cross_saved_bytes(const vh_cross *c);
+size_t vh_cross_workspace_bytes(const vh_cross *c, int backward);
+/* Bucket of a relative position rel = key's - query's.  n = |rel| (one-sided:
+   max(-rel, 0)), side = buckets / 2 (one-sided: buckets), near = side / 2:
+   n for n < near, else min(side - 1, near + floor(log(n / near) /
+   log(max_distance / near) * (side - near))), borders that whole numbers meet
+   counted as reached; bidirectional adds side for rel > 0.  2 to 128 buckets
+   (bidirectional: even, from 4), near < max_distance <= 4096.  -1: refused. */
+int vh_relative_bucket(int rel, int buckets, int max_distance, int bidirectional);
+
 /* ---- model -------------------------------------------------------------- */
 /* Upload a VSCNAT01 pack (native/vocalarc_separation.c:528-589) laid out for
    `dims` from host memory.  Returns NULL on a malformed pack. */

@@ -1,0 +1,388 @@
+// Launchers of the layer norm and of the attention over another sequence's
+// states (layernorm.hpp, cross_attention.hpp).
+#include "runtime.hpp"
+
+#include <math.h>
+
+#include <algorithm>
+#include <initializer_list>
+#include <utility>
+
+#include "cross_attention.hpp"
+#include "layernorm.hpp"
+
+namespace vh {
+
+// --------------------------------------------------------------- layer norm
+constexpr int LN_MAX_DIM = 16384;
+// Workgroups of the backward pass: each keeps its rows' weight gradients, so
+// more of them are more sums to add up afterwards.
+static int layernorm_parts(int64_t rows, int dim) {
+    return (int)std::min<int64_t>(dim <= 1024 ? (rows + 3) / 4 : rows, 512);
+}
+
+static bool layernorm_ok(const char *what, int type, int64_t rows, int dim, std::initializer_list<int64_t> pitches) {
+    if ((type != VH_TYPE_FP32 && type != VH_TYPE_BF16) || rows < 0 || rows > INT32_MAX || dim < 1 || dim > LN_MAX_DIM) {
+        set_error("%s: unsupported type %d, rows %lld or dim %d (1 to %d)", what, type, (long long)rows, dim,
+                  LN_MAX_DIM);
+        return false;
+    }
+    for (int64_t ld : pitches)
+        if (ld < dim) {
+            set_error("%s: a row pitch of %lld is below dim %d", what, (long long)ld, dim);
+            return false;
+        }
+    return true;
+}
+
+size_t layernorm_workspace_bytes(int64_t rows, int dim) {
+    if (!layernorm_ok("vh_layernorm_workspace_bytes", VH_TYPE_FP32, rows, dim, {})) return 0;
+    return std::max<size_t>(16, (size_t)layernorm_parts(rows, dim) * 2 * dim * sizeof(float));
+}
+
+// Vectors of four where every row and array starts on one.
+static bool by_fours(int type, int dim, std::initializer_list<int64_t> pitches,
+                     std::initializer_list<const void *> tensors, std::initializer_list<const void *> floats) {
+    const uintptr_t bytes = type == VH_TYPE_BF16 ? 8 : 16;
+    int64_t odd = dim % 4;
+    uintptr_t at = 0;
+    for (int64_t ld : pitches) odd |= ld % 4;
+    for (const void *p : tensors) at |= (uintptr_t)p & (bytes - 1);
+    for (const void *p : floats) at |= (uintptr_t)p & 15;
+    return !odd && !at;
+}
+
+template <typename T, int LANES, int N, int NV>
+static void layernorm_launch(hipStream_t s, const NormArgs &a, bool backward, unsigned parts) {
+    constexpr int threads = LANES > 256 ? LANES : 256;
+    if (backward)
+        hipLaunchKernelGGL((layernorm_backward_kernel<T, LANES, N, NV>), dim3(parts), dim3(threads), 0, s, a);
+    else
+        hipLaunchKernelGGL((layernorm_kernel<T, LANES, N, NV>), dim3((unsigned)(LANES == 64 ? (a.rows + 3) / 4 : a.rows)),
+                           dim3(threads), 0, s, a);
+}
+
+template <typename T>
+static void layernorm_dispatch(hipStream_t s, const NormArgs &a, bool fours, bool backward, unsigned parts) {
+    const int d = a.dim;
+    if (fours) {
+        if (d <= 256) layernorm_launch<T, 64, 4, 1>(s, a, backward, parts);
+        else if (d <= 512) layernorm_launch<T, 64, 4, 2>(s, a, backward, parts);
+        else if (d <= 1024) layernorm_launch<T, 64, 4, 4>(s, a, backward, parts);
+        else if (d <= 2048) layernorm_launch<T, 256, 4, 2>(s, a, backward, parts);
+        else if (d <= 4096) layernorm_launch<T, 256, 4, 4>(s, a, backward, parts);
+        else layernorm_launch<T, 1024, 4, 4>(s, a, backward, parts);
+    } else {
+        if (d <= 256) layernorm_launch<T, 64, 1, 4>(s, a, backward, parts);
+        else if (d <= 512) layernorm_launch<T, 64, 1, 8>(s, a, backward, parts);
+        else if (d <= 1024) layernorm_launch<T, 64, 1, 16>(s, a, backward, parts);
+        else if (d <= 4096) layernorm_launch<T, 256, 1, 16>(s, a, backward, parts);
+        else layernorm_launch<T, 1024, 1, 16>(s, a, backward, parts);
+    }
+}
+
+bool layernorm(hipStream_t s, const LayerNorm &n, KernelTimer *t) {
+    if (!layernorm_ok("vh_layernorm", n.type, n.rows, n.dim, {n.ldx, n.ldy})) return false;
+    if (!(n.eps >= 0.0f) || isinf(n.eps) || !n.gamma || (n.rows && (!n.x || !n.y))) {
+        set_error("vh_layernorm: null x, gamma or y, or an eps that is no number from 0 up");
+        return false;
+    }
+    if (!n.rows) return true;
+    NormArgs a{};
+    a.x = n.x; a.y = n.y; a.ldx = n.ldx; a.ldy = n.ldy;
+    a.gamma = n.gamma; a.beta = n.beta;
+    a.stats = reinterpret_cast<float2 *>(n.stats);
+    a.rows = n.rows; a.dim = n.dim; a.eps = n.eps;
+    const bool fours = by_fours(n.type, n.dim, {n.ldx, n.ldy}, {n.x, n.y}, {n.gamma, n.beta});
+    Scope sc(t, s, "layernorm");
+    if (n.type == VH_TYPE_BF16) layernorm_dispatch<bf16>(s, a, fours, false, 0);
+    else layernorm_dispatch<float>(s, a, fours, false, 0);
+    return sync_debug(s, "layernorm_kernel");
+}
+
+bool layernorm_backward(hipStream_t s, const LayerNorm &n, KernelTimer *t) {
+    if (!layernorm_ok("vh_layernorm_backward", n.type, n.rows, n.dim, {n.ldx, n.ldy, n.lddx})) return false;
+    if (!n.gamma || (n.rows && (!n.x || !n.dy || !n.dx || !n.stats))) {
+        set_error("vh_layernorm_backward: null dy, x, gamma, stats or dx");
+        return false;
+    }
+    const bool weights = n.dgamma || n.dbeta;
+    if (weights && (!n.workspace || ((uintptr_t)n.workspace & 15))) {
+        set_error("vh_layernorm_backward: the weights' gradients need a 16-byte aligned workspace "
+                  "(vh_layernorm_workspace_bytes)");
+        return false;
+    }
+    const int parts = layernorm_parts(n.rows, n.dim);
+    Scope sc(t, s, "layernorm_backward");
+    if (n.rows) {
+        NormArgs a{};
+        a.x = n.x; a.dy = n.dy; a.dx = n.dx; a.ldx = n.ldx; a.lddy = n.ldy; a.lddx = n.lddx;
+        a.gamma = n.gamma;
+        a.stats = reinterpret_cast<float2 *>(n.stats);
+        a.part = weights ? static_cast<float *>(n.workspace) : nullptr;
+        a.rows = n.rows; a.dim = n.dim;
+        const bool fours = by_fours(n.type, n.dim, {n.ldx, n.ldy, n.lddx}, {n.x, n.dy, n.dx}, {n.gamma});
+        if (n.type == VH_TYPE_BF16) layernorm_dispatch<bf16>(s, a, fours, true, (unsigned)parts);
+        else layernorm_dispatch<float>(s, a, fours, true, (unsigned)parts);
+        if (!sync_debug(s, "layernorm_backward_kernel")) return false;
+    }
+    if (!weights) return true;
+    hipLaunchKernelGGL(layernorm_columns_kernel, dim3((unsigned)(2 * n.dim + 63) / 64), dim3(256), 0, s,
+                       static_cast<const float *>(n.workspace), parts, n.dim, n.dgamma, n.dbeta);
+    return sync_debug(s, "layernorm_columns_kernel");
+}
+
+// ---------------------------------------------------------- cross attention
+// Distances from which the far buckets of a side begin.  Bucket near + i is
+// reached at the first whole n with n^far >= max_distance^i near^(far - i), far
+// = side - near: in logarithms, with a difference within their rounding taken
+// as equal (whole numbers that meet the border exactly).
+static int bucket_edges(int side, int near, int max_distance, int *edge) {
+    const int far = side - near;
+    const long double step = logl((long double)max_distance / near) / far;
+    int n = near;
+    for (int i = 0; i < far; i++) {
+        while (logl((long double)n / near) < step * i - 1e-13L) n++;
+        edge[i] = n;
+    }
+    return far;
+}
+
+static bool bias_ok(const char *what, int buckets, int max_distance, int bidirectional) {
+    const int side = bidirectional ? buckets / 2 : buckets;
+    if (buckets < 2 || buckets > CA_MAX_BUCKETS || (bidirectional && buckets % 2) || side < 2 || max_distance > 4096 ||
+        max_distance <= side / 2) {
+        set_error("%s: %d buckets (2 to %d, bidirectional: even and from 4) up to a distance of %d (more than the %d "
+                  "buckets of single distances, at most 4096)",
+                  what, buckets, CA_MAX_BUCKETS, max_distance, side / 2);
+        return false;
+    }
+    return true;
+}
+
+static void bias_args(CrossArgs &a, int buckets, int max_distance, int bidirectional) {
+    a.buckets = buckets;
+    a.max_distance = max_distance;
+    a.bidirectional = bidirectional ? 1 : 0;
+    a.side = bidirectional ? buckets / 2 : buckets;
+    a.near = a.side / 2;
+    a.edges = bucket_edges(a.side, a.near, max_distance, a.edge);
+}
+
+int relative_bucket(int rel, int buckets, int max_distance, int bidirectional) {
+    if (!bias_ok("vh_relative_bucket", buckets, max_distance, bidirectional)) return -1;
+    CrossArgs a{};
+    bias_args(a, buckets, max_distance, bidirectional);
+    return cross_bucket(a, std::max(rel, -INT32_MAX));
+}
+
+// Whether different (sequence, row, head) have different places: each stride, in
+// ascending order, at least what the smaller ones span.
+static bool apart(const int64_t *strides, int64_t seqs, int64_t rows, int64_t heads) {
+    std::pair<int64_t, int64_t> d[3] = {{strides[0], seqs}, {strides[1], rows}, {strides[2], heads}};
+    std::sort(d, d + 3);
+    int64_t span = CA_D;
+    for (const auto &[stride, n] : d) {
+        if (n <= 1) continue;
+        if (stride < span) return false;
+        span = stride * (n - 1) + span;
+    }
+    return true;
+}
+
+constexpr int64_t CA_MAX_ROW = 1 << 26;      // bytes of a row stride: 32 rows' offsets fit 32 bits
+constexpr int CA_MAX_LENGTH = 1 << 29;
+
+static bool cross_ok(const char *what, const vh_cross *c, bool backward) {
+    if (!c) {
+        set_error("%s: null layout", what);
+        return false;
+    }
+    if ((c->type != VH_TYPE_FP32 && c->type != VH_TYPE_BF16) || c->sequences < 0 || c->heads < 1 || c->kv_heads < 1 ||
+        c->heads % c->kv_heads || c->query_length < 0 || c->key_length < 0 || c->query_length > CA_MAX_LENGTH ||
+        c->key_length > CA_MAX_LENGTH) {
+        set_error("%s: unsupported type %d, %d sequences, %d heads over %d, lengths %d and %d", what, c->type,
+                  c->sequences, c->heads, c->kv_heads, c->query_length, c->key_length);
+        return false;
+    }
+    if (!isfinite(c->scale)) {
+        set_error("%s: the scale is no finite number", what);
+        return false;
+    }
+    if (c->bias_table && !bias_ok(what, c->buckets, c->max_distance, c->bidirectional)) return false;
+    const int64_t size = c->type == VH_TYPE_BF16 ? 2 : 4;
+    struct {
+        const char *name;
+        const int64_t *strides;
+        int64_t rows, heads;
+        bool written;
+    } tensors[] = {{"q", c->q_strides, c->query_length, c->heads, backward},
+                   {"k", c->k_strides, c->key_length, c->kv_heads, backward},
+                   {"v", c->v_strides, c->key_length, c->kv_heads, backward},
+                   {"out", c->out_strides, c->query_length, c->heads, true}};
+    for (const auto &t : tensors) {
+        for (int i = 0; i < 3; i++)
+            if (t.strides[i] < 0 || t.strides[i] * size % 16 || t.strides[i] > ((int64_t)1 << 46)) {
+                set_error("%s: %s's strides %lld, %lld, %lld: none negative, whole multiples of 16 bytes", what, t.name,
+                          (long long)t.strides[0], (long long)t.strides[1], (long long)t.strides[2]);
+                return false;
+            }
+        if (t.strides[1] * size > CA_MAX_ROW) {
+            set_error("%s: %s's row stride of %lld is over %lld bytes", what, t.name, (long long)t.strides[1],
+                      (long long)CA_MAX_ROW);
+            return false;
+        }
+        if (t.written && !apart(t.strides, c->sequences, t.rows, t.heads)) {
+            set_error("%s: %s's strides %lld, %lld, %lld let rows overlap, and %s is written", what, t.name,
+                      (long long)t.strides[0], (long long)t.strides[1], (long long)t.strides[2],
+                      t.name[0] == 'o' ? "out" : "its gradient");
+            return false;
+        }
+    }
+    const int64_t tasks = (int64_t)c->sequences * c->heads * ((std::max(c->query_length, c->key_length) + 127) / 128 + 1);
+    if (tasks > INT32_MAX) {
+        set_error("%s: %lld workgroups", what, (long long)tasks);
+        return false;
+    }
+    return true;
+}
+
+static int64_t cross_rows(const vh_cross *c) { return (int64_t)c->sequences * c->heads * c->query_length; }
+static size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+
+size_t cross_saved_bytes(const vh_cross *c) {
+    if (!cross_ok("vh_cross_saved_bytes", c, false)) return 0;
+    return std::max<size_t>(16, (size_t)cross_rows(c) * (8 + (c->type == VH_TYPE_BF16 ? 2 * CA_D : 0)));
+}
+
+size_t cross_workspace_bytes(const vh_cross *c, bool backward) {
+    if (!cross_ok("vh_cross_workspace_bytes", c, backward)) return 0;
+    if (!backward) return 16;
+    size_t n = round16((size_t)cross_rows(c) * sizeof(float));
+    if (c->bias_table)
+        n += (size_t)c->sequences * c->heads * ((c->query_length + 127) / 128) * c->buckets * sizeof(float);
+    return std::max<size_t>(16, n);
+}
+
+static CrossTensor cross_tensor(const void *p, const int64_t *strides, int64_t size) {
+    return {const_cast<char *>(static_cast<const char *>(p)), strides[0] * size, strides[1] * size, strides[2] * size};
+}
+
+static CrossArgs cross_args(const vh_cross *c, const CrossBuffers &b) {
+    CrossArgs a{};
+    const int64_t size = c->type == VH_TYPE_BF16 ? 2 : 4;
+    a.q = cross_tensor(b.q, c->q_strides, size);
+    a.k = cross_tensor(b.k, c->k_strides, size);
+    a.v = cross_tensor(b.v, c->v_strides, size);
+    a.out = cross_tensor(b.out, c->out_strides, size);
+    a.dout = cross_tensor(b.dout, c->out_strides, size);
+    a.dq = cross_tensor(b.dq, c->q_strides, size);
+    a.dk = cross_tensor(b.dk, c->k_strides, size);
+    a.dv = cross_tensor(b.dv, c->v_strides, size);
+    a.S = c->sequences; a.H = c->heads; a.KV = c->kv_heads;
+    a.Lq = c->query_length; a.Lk = c->key_length;
+    a.causal = c->causal ? 1 : 0;
+    a.scale = c->scale;
+    a.query_lengths = c->query_lengths; a.key_lengths = c->key_lengths; a.query_start = c->query_start;
+    a.table = c->bias_table;
+    if (a.table) bias_args(a, c->buckets, c->max_distance, c->bidirectional);
+    a.stats = static_cast<float2 *>(b.saved);
+    if (b.saved && c->type == VH_TYPE_BF16) a.rest = reinterpret_cast<bf16 *>(a.stats + cross_rows(c));
+    return a;
+}
+
+static bool aligned(const char *what, std::initializer_list<const void *> pointers) {
+    for (const void *p : pointers)
+        if ((uintptr_t)p & 15) {
+            set_error("%s: a tensor, saved or workspace is not 16-byte aligned", what);
+            return false;
+        }
+    return true;
+}
+
+static size_t window_bytes(const CrossArgs &a) { return a.table ? (size_t)(2 * (a.max_distance + CA_PAD) + 1) * 4 : 0; }
+
+template <typename T, bool BIAS>
+static void forward_launch(hipStream_t s, const CrossArgs &a) {
+    const unsigned grid = (unsigned)((int64_t)a.S * a.H * ((a.Lq + 127) / 128));
+    const size_t lds = 2 * Tile<T>::BYTES + window_bytes(a);
+    if (a.stats) hipLaunchKernelGGL((cross_forward_kernel<T, BIAS, true>), dim3(grid), dim3(256), lds, s, a);
+    else hipLaunchKernelGGL((cross_forward_kernel<T, BIAS, false>), dim3(grid), dim3(256), lds, s, a);
+}
+
+template <typename T>
+static void dq_launch(hipStream_t s, const CrossArgs &a) {
+    const unsigned grid = (unsigned)((int64_t)a.S * a.H * ((a.Lq + 127) / 128));
+    const size_t lds = 2 * Tile<T>::BYTES;
+    const size_t bias = a.table ? sizeof(DbiasLds) + 128 * (size_t)a.buckets * 4 + window_bytes(a) : 0;
+    if (a.table) hipLaunchKernelGGL((cross_dq_kernel<T, true>), dim3(grid), dim3(256), lds + bias, s, a);
+    else hipLaunchKernelGGL((cross_dq_kernel<T, false>), dim3(grid), dim3(256), lds, s, a);
+}
+
+template <typename T>
+static void dkv_launch(hipStream_t s, const CrossArgs &a) {
+    const unsigned grid = (unsigned)((int64_t)a.S * a.KV * ((a.Lk + 127) / 128));
+    const size_t lds = 2 * Tile<T>::BYTES + sizeof(RowStats) + window_bytes(a);
+    if (a.table) hipLaunchKernelGGL((cross_dkv_kernel<T, true>), dim3(grid), dim3(256), lds, s, a);
+    else hipLaunchKernelGGL((cross_dkv_kernel<T, false>), dim3(grid), dim3(256), lds, s, a);
+}
+
+bool cross_attention(hipStream_t s, const vh_cross *c, const CrossBuffers &b, KernelTimer *t) {
+    const char *what = "vh_cross_attention";
+    if (!cross_ok(what, c, false)) return false;
+    if (cross_rows(c) == 0) return true;
+    if (!b.q || !b.out || (c->key_length && (!b.k || !b.v))) {
+        set_error("%s: null q, k, v or out", what);
+        return false;
+    }
+    if (!aligned(what, {b.q, b.k, b.v, b.out, b.saved, b.workspace})) return false;
+    const CrossArgs a = cross_args(c, b);
+    Scope sc(t, s, "cross_attention");
+    if (c->type == VH_TYPE_BF16) a.table ? forward_launch<bf16, true>(s, a) : forward_launch<bf16, false>(s, a);
+    else a.table ? forward_launch<float, true>(s, a) : forward_launch<float, false>(s, a);
+    return sync_debug(s, "cross_forward_kernel");
+}
+
+bool cross_attention_backward(hipStream_t s, const vh_cross *c, const CrossBuffers &b, KernelTimer *t) {
+    const char *what = "vh_cross_attention_backward";
+    if (!cross_ok(what, c, true)) return false;
+    if ((b.dk != nullptr) != (b.dv != nullptr)) {
+        set_error("%s: dk and dv are given together, or neither", what);
+        return false;
+    }
+    if (b.dbias && !c->bias_table) {
+        set_error("%s: dbias without a bias table", what);
+        return false;
+    }
+    const bool rows = cross_rows(c) > 0, keys = (int64_t)c->sequences * c->key_length > 0;
+    if ((rows && (!b.q || !b.out || !b.saved || !b.dout || !b.dq)) || (rows && keys && (!b.k || !b.v)) || !b.workspace) {
+        set_error("%s: null q, k, v, out, saved, dout, dq or workspace", what);
+        return false;
+    }
+    if (!aligned(what, {b.q, b.k, b.v, b.out, b.saved, b.workspace, b.dout, b.dq, b.dk, b.dv})) return false;
+    CrossArgs a = cross_args(c, b);
+    a.delta = static_cast<float *>(b.workspace);
+    a.dbias = b.dbias;
+    if (b.dbias)
+        a.dbias_part = reinterpret_cast<float *>(static_cast<char *>(b.workspace) +
+                                                 round16((size_t)cross_rows(c) * sizeof(float)));
+    if (rows) {
+        Scope sc(t, s, "cross_attention_dq");
+        if (c->type == VH_TYPE_BF16) dq_launch<bf16>(s, a);
+        else dq_launch<float>(s, a);
+        if (!sync_debug(s, "cross_dq_kernel")) return false;
+    }
+    if (b.dbias) {
+        hipLaunchKernelGGL(cross_dbias_kernel, dim3((unsigned)a.H), dim3(128), 0, s, a);
+        if (!sync_debug(s, "cross_dbias_kernel")) return false;
+    }
+    if (b.dk && keys) {
+        Scope sc(t, s, "cross_attention_dkv");
+        if (c->type == VH_TYPE_BF16) dkv_launch<bf16>(s, a);
+        else dkv_launch<float>(s, a);
+        if (!sync_debug(s, "cross_dkv_kernel")) return false;
+    }
+    return true;
+}
+
+}  // namespace vh

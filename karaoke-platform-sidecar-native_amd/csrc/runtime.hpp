@@ -282,6 +282,42 @@ bool attention(hipStream_t s, const void *qkv, int ld, void *out, int ld_out, co
                bool split = false, const float *bound = nullptr, bool out_h2 = false, bool kv_scaled = false,
                bool device_choice = false, bool kv_pieces = false);
 
+// Layer norm of rows (layernorm.hpp); type: VH_TYPE_* of x, y and their
+// gradients.  Backward: y's pitch is dy's.
+struct LayerNorm {
+    int type;
+    int64_t rows;
+    int dim;
+    const void *x; int64_t ldx;
+    const float *gamma, *beta;
+    float eps;
+    void *y; int64_t ldy;
+    float *stats;
+    const void *dy = nullptr;
+    void *dx = nullptr; int64_t lddx = 0;
+    float *dgamma = nullptr, *dbeta = nullptr;
+    void *workspace = nullptr;
+};
+bool layernorm(hipStream_t s, const LayerNorm &n, KernelTimer *t = nullptr);
+bool layernorm_backward(hipStream_t s, const LayerNorm &n, KernelTimer *t = nullptr);
+size_t layernorm_workspace_bytes(int64_t rows, int dim);
+
+// Attention over another sequence's states and its backward pass
+// (cross_attention.hpp).
+struct CrossBuffers {
+    const void *q, *k, *v;
+    void *out, *saved, *workspace;
+    const void *dout = nullptr;
+    void *dq = nullptr, *dk = nullptr, *dv = nullptr;
+    float *dbias = nullptr;
+};
+bool cross_attention(hipStream_t s, const vh_cross *c, const CrossBuffers &b, KernelTimer *t = nullptr);
+bool cross_attention_backward(hipStream_t s, const vh_cross *c, const CrossBuffers &b, KernelTimer *t = nullptr);
+size_t cross_saved_bytes(const vh_cross *c);
+size_t cross_workspace_bytes(const vh_cross *c, bool backward);
+// Bucket of a relative position; -1 where the buckets are none.
+int relative_bucket(int rel, int buckets, int max_distance, int bidirectional);
+
 // ------------------------------------------------------------------- dims
 struct Dims {
     int dim, depth, bands, heads, dim_head, ff_dim, ffn_glu, gated, mask_hidden, n_fft, hop, channels;

@@ -426,6 +426,73 @@ extern "C" int vh_attention_noalloc(vh_context *ctx, int sequences, int length, 
                : 0;
 }
 
+// ------------------------------------- layer norm, attention over other states
+// The context's device, whichever is current when the call is made.
+struct OnDevice {
+    int before = -1;
+    bool ok;
+    explicit OnDevice(const vh_context *ctx) {
+        ok = check(hipGetDevice(&before), "hipGetDevice");
+        if (ok && before != ctx->device) ok = check(hipSetDevice(ctx->device), "hipSetDevice");
+        else before = -1;
+    }
+    ~OnDevice() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+    OnDevice(const OnDevice &) = delete;
+};
+
+static bool have_context(const vh_context *ctx, const char *what) {
+    if (!ctx) set_error("%s: null context", what);
+    return ctx != nullptr;
+}
+
+extern "C" int vh_layernorm(vh_context *ctx, int type, int64_t rows, int dim, const void *x, int64_t ldx,
+                            const float *gamma, const float *beta, float eps, void *y, int64_t ldy, float *stats) {
+    if (!have_context(ctx, "vh_layernorm")) return 0;
+    const OnDevice on(ctx);
+    return on.ok && layernorm(ctx->stream, {type, rows, dim, x, ldx, gamma, beta, eps, y, ldy, stats}, &ctx->timer);
+}
+
+extern "C" int vh_layernorm_backward(vh_context *ctx, int type, int64_t rows, int dim, const void *dy, int64_t lddy,
+                                     const void *x, int64_t ldx, const float *gamma, const float *stats, void *dx,
+                                     int64_t lddx, float *dgamma, float *dbeta, void *workspace) {
+    if (!have_context(ctx, "vh_layernorm_backward")) return 0;
+    const OnDevice on(ctx);
+    LayerNorm n{type, rows, dim, x, ldx, gamma, nullptr, 0.0f, nullptr, lddy, const_cast<float *>(stats)};
+    n.dy = dy; n.dx = dx; n.lddx = lddx;
+    n.dgamma = dgamma; n.dbeta = dbeta; n.workspace = workspace;
+    return on.ok && layernorm_backward(ctx->stream, n, &ctx->timer);
+}
+
+extern "C" size_t vh_layernorm_workspace_bytes(int64_t rows, int dim) { return layernorm_workspace_bytes(rows, dim); }
+
+extern "C" int vh_cross_attention(vh_context *ctx, const vh_cross *c, const void *q, const void *k, const void *v,
+                                  void *out, void *saved, void *workspace) {
+    if (!have_context(ctx, "vh_cross_attention")) return 0;
+    const OnDevice on(ctx);
+    return on.ok && cross_attention(ctx->stream, c, {q, k, v, out, saved, workspace}, &ctx->timer);
+}
+
+extern "C" int vh_cross_attention_backward(vh_context *ctx, const vh_cross *c, const void *q, const void *k,
+                                           const void *v, const void *out, const void *saved, const void *dout,
+                                           void *dq, void *dk, void *dv, float *dbias, void *workspace) {
+    if (!have_context(ctx, "vh_cross_attention_backward")) return 0;
+    const OnDevice on(ctx);
+    return on.ok && cross_attention_backward(ctx->stream, c,
+                                             {q, k, v, const_cast<void *>(out), const_cast<void *>(saved), workspace,
+                                              dout, dq, dk, dv, dbias},
+                                             &ctx->timer);
+}
+
+extern "C" size_t vh_cross_saved_bytes(const vh_cross *c) { return cross_saved_bytes(c); }
+extern "C" size_t vh_cross_workspace_bytes(const vh_cross *c, int backward) {
+    return cross_workspace_bytes(c, backward != 0);
+}
+extern "C" int vh_relative_bucket(int rel, int buckets, int max_distance, int bidirectional) {
+    return relative_bucket(rel, buckets, max_distance, bidirectional);
+}
+
 // -------------------------------------------------------------------- model
 namespace {
 

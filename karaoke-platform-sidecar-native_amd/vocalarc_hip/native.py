@@ -24,12 +24,23 @@ PRECISION_FP32, PRECISION_BF16, PRECISION_FP32_MFMA = 0, 1, 2
 BF16_A, BF16_C, BF16_STAGED = 1, 2, 4  # vh_gemm_bf16 operand flags; STAGED forces the register-staged kernel
 ATT_OUT_BF16, ATT_BF16, ATT_SPLIT, ATT_H2, ATT_OUT_H2 = 1, 2, 4, 8, 16  # vh_attention flags
 NOALLOC_MAX_LENGTH = 4096  # VH_NOALLOC_MAX_LENGTH
+TYPE_FP32, TYPE_BF16 = 0, 1  # VH_TYPE_*
 SPEC_REFERENCE, SPEC_FRAME_MAJOR = 0, 1  # spectrum layouts: [F][C][T][2] / [C][T][F][2]
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _I64 = ctypes.c_int64
 _lib = None
+
+
+class CCross(ctypes.Structure):
+    """vh_cross"""
+    _fields_ = ([(n, _I) for n in ("type", "sequences", "heads", "kv_heads", "query_length", "key_length", "causal")] +
+                [("scale", ctypes.c_float)] +
+                [(n, _I64 * 3) for n in ("q_strides", "k_strides", "v_strides", "out_strides")] +
+                [(n, _P) for n in ("query_lengths", "key_lengths", "query_start", "bias_table")] +
+                [(n, _I) for n in ("buckets", "max_distance", "bidirectional")])
+
 
 # Signatures (result, arguments) of every entry point declared in
 # include/vocalarc_hip.h (vh_*) and include/native_gpu.h (native_gpu_*).
@@ -55,6 +66,14 @@ SIGNATURES = {
     "vh_to_bf16": (_I, [_P, _I64, _I, _P, _P, _I]),
     "vh_attention": (_I, [_P, _I, _I, _I, _P, _P, _I, _I]),
     "vh_attention_noalloc": (_I, [_P, _I, _I, _I, _P, _P, _I, _I]),
+    "vh_layernorm": (_I, [_P, _I, _I64, _I, _P, _I64, _P, _P, ctypes.c_float, _P, _I64, _P]),
+    "vh_layernorm_backward": (_I, [_P, _I, _I64, _I, _P, _I64, _P, _I64, _P, _P, _P, _I64, _P, _P, _P]),
+    "vh_layernorm_workspace_bytes": (ctypes.c_size_t, [_I64, _I]),
+    "vh_cross_attention": (_I, [_P, ctypes.POINTER(CCross), _P, _P, _P, _P, _P, _P]),
+    "vh_cross_attention_backward": (_I, [_P, ctypes.POINTER(CCross)] + [_P] * 11),
+    "vh_cross_saved_bytes": (ctypes.c_size_t, [ctypes.POINTER(CCross)]),
+    "vh_cross_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(CCross), _I]),
+    "vh_relative_bucket": (_I, [_I, _I, _I, _I]),
     "vh_model_load": (_P, [_P, ctypes.POINTER(CDims), _P, ctypes.c_size_t]),
     "vh_model_free": (None, [_P]), "vh_model_set_precision": (_I, [_P, _I]),
     "vh_transformer": (_I, [_P, _P, _I, _I, _P, _I, _I]),
@@ -276,6 +295,27 @@ class Context:
         return lib().vh_attention_noalloc(self.h, sequences, length, heads, ptr(qkv), ptr(out), int(rotary),
                                           _att_flags(out_bf16, bf16, split, h2))
 
+    def layernorm(self, x, gamma, beta, y, rows: int, dim: int, eps: float = 1e-5, stats=None, ldx: int | None = None,
+                  ldy: int | None = None, bf16: bool = False):
+        """Layer norm rows; bf16: x and y are bf16; stats [rows][2] receives (mean, rstd) for the backward pass."""
+        _ok(lib().vh_layernorm(self.h, int(bf16), rows, dim, ptr(x), ldx or dim, ptr(gamma), _opt(beta), eps, ptr(y),
+                               ldy or dim, _opt(stats)), "vh_layernorm")
+
+    @staticmethod
+    def layernorm_workspace_bytes(rows: int, dim: int) -> int:
+        """Bytes of layernorm_backward's workspace."""
+        n = int(lib().vh_layernorm_workspace_bytes(rows, dim))
+        _ok(n, "vh_layernorm_workspace_bytes")
+        return n
+
+    def layernorm_backward(self, dy, x, gamma, stats, dx, rows: int, dim: int, dgamma=None, dbeta=None, workspace=None,
+                           lddy: int | None = None, ldx: int | None = None, lddx: int | None = None,
+                           bf16: bool = False):
+        """dx, and dgamma and dbeta where given (then with the workspace, layernorm_workspace_bytes(rows, dim))."""
+        _ok(lib().vh_layernorm_backward(self.h, int(bf16), rows, dim, ptr(dy), lddy or dim, ptr(x), ldx or dim,
+                                        ptr(gamma), ptr(stats), ptr(dx), lddx or dim, _opt(dgamma), _opt(dbeta),
+                                        _opt(workspace)), "vh_layernorm_backward")
+
     # -- timing --
     def timing(self, classes: str | None = "*"):
         """Time the named kernel classes (comma list, "*" = all, None = off)."""
@@ -290,6 +330,61 @@ class Context:
         if not lib().vh_timing_get(self.h, name.encode(), ctypes.byref(ms), ctypes.byref(n)):
             return 0.0, 0
         return ms.value, n.value
+
+
+class CrossAttention:
+    """The layout of an attention over another sequence's states (vh_cross), for tensors q [S][Lq][H][64], k and v
+    [S][Lk][KV heads][64] and out as q, of any strides that vh_cross takes.  Later calls may pass other tensors of the
+    same layout.  query_lengths, key_lengths, query_start: int32 device tensors [S]; bias_table: fp32 [buckets][H].
+    Shapes, types and devices are checked here; strides and sizes by the library."""
+
+    def __init__(self, ctx: Context, q, k, v, out, *, causal: bool = False, scale: float = 0.125, query_lengths=None,
+                 key_lengths=None, query_start=None, bias_table=None, max_distance: int = 128,
+                 bidirectional: bool = True):
+        import torch
+        S, Lq, H, D = q.shape
+        if q.dtype not in (torch.float32, torch.bfloat16) or D != 64 or k.dim() != 4 or k.shape[0] != S or \
+                k.shape[3] != 64 or tuple(v.shape) != tuple(k.shape) or tuple(out.shape) != tuple(q.shape) or \
+                len({t.dtype for t in (q, k, v, out)}) != 1:
+            raise NativeError("CrossAttention: q and out [S][Lq][H][64], k and v [S][Lk][KV][64], all fp32 or all bf16")
+        if any(t.stride(3) != 1 for t in (q, k, v, out)):
+            raise NativeError("CrossAttention: a head's 64 elements are consecutive")
+        for t in (query_lengths, key_lengths, query_start):
+            if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (S,) or not t.is_contiguous()):
+                raise NativeError("CrossAttention: lengths and starts are contiguous int32 [S]")
+        if bias_table is not None and (bias_table.dtype != torch.float32 or bias_table.dim() != 2 or
+                                       bias_table.shape[1] != H or not bias_table.is_contiguous()):
+            raise NativeError("CrossAttention: the bias table is contiguous fp32 [buckets][H]")
+        self.ctx = ctx
+        self._kept = (query_lengths, key_lengths, query_start, bias_table)
+        self.c = CCross(int(q.dtype == torch.bfloat16), S, H, k.shape[2], Lq, k.shape[1], int(causal), scale)
+        for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
+            setattr(self.c, name + "_strides", (_I64 * 3)(*t.stride()[:3]))
+        for name, t in zip(("query_lengths", "key_lengths", "query_start", "bias_table"), self._kept):
+            setattr(self.c, name, _opt(t))
+        if bias_table is not None:
+            self.c.buckets, self.c.max_distance = bias_table.shape[0], max_distance
+            self.c.bidirectional = int(bidirectional)
+        self._ref = ctypes.byref(self.c)
+
+    def saved_bytes(self) -> int:
+        n = int(lib().vh_cross_saved_bytes(self._ref))
+        _ok(n, "vh_cross_saved_bytes")
+        return n
+
+    def workspace_bytes(self, backward: bool = False) -> int:
+        n = int(lib().vh_cross_workspace_bytes(self._ref, int(backward)))
+        _ok(n, "vh_cross_workspace_bytes")
+        return n
+
+    def forward(self, q, k, v, out, saved=None, workspace=None):
+        _ok(lib().vh_cross_attention(self.ctx.h, self._ref, ptr(q), ptr(k), ptr(v), ptr(out), _opt(saved),
+                                     _opt(workspace)), "vh_cross_attention")
+
+    def backward(self, q, k, v, out, saved, dout, dq, dk=None, dv=None, dbias=None, workspace=None):
+        _ok(lib().vh_cross_attention_backward(self.ctx.h, self._ref, ptr(q), ptr(k), ptr(v), ptr(out), ptr(saved),
+                                              ptr(dout), ptr(dq), _opt(dk), _opt(dv), _opt(dbias), _opt(workspace)),
+            "vh_cross_attention_backward")
 
 
 class Model:

@@ -1,0 +1,135 @@
+"""Layer norm and cross attention without a GPU: refusals, sizes and the bias's buckets."""
+
+import ctypes
+
+import pytest
+import torch
+
+import norm_cross_ref as R
+from vocalarc_hip import native
+
+pytestmark = pytest.mark.skipif(not native.LIB_PATH.exists(), reason="library not built")
+
+
+def layout(**change):
+    c = native.CCross(0, 2, 8, 4, 5, 7, 0, 0.125)
+    c.q_strides[:] = c.out_strides[:] = (5 * 512, 512, 64)
+    c.k_strides[:] = c.v_strides[:] = (7 * 256, 256, 64)
+    for name, value in change.items():
+        if isinstance(value, tuple):
+            getattr(c, name)[:] = value
+        else:
+            setattr(c, name, value)
+    return c
+
+
+def refused(c, backward, text):
+    n = native.lib().vh_cross_workspace_bytes(ctypes.byref(c), backward)
+    assert n == 0 and text in native.last_error(), (n, native.last_error())
+    return True
+
+
+@pytest.mark.parametrize("change,text", [
+    ({"type": 2}, "type"), ({"sequences": -1}, "sequences"), ({"heads": 0}, "heads"), ({"kv_heads": 0}, "heads"),
+    ({"kv_heads": 3}, "heads"), ({"query_length": -1}, "lengths"), ({"key_length": -1}, "lengths"),
+    ({"key_length": (1 << 29) + 1}, "lengths"), ({"scale": float("nan")}, "scale"), ({"scale": float("inf")}, "scale"),
+    ({"q_strides": (2560, 510, 64)}, "q's strides"), ({"k_strides": (1792, 256, 2)}, "k's strides"),
+    ({"v_strides": (-1792, 256, 64)}, "v's strides"), ({"v_strides": (1792, 1 << 25, 64)}, "row stride"),
+    ({"out_strides": (0, 512, 64)}, "overlap"), ({"out_strides": (2560, 512, 32)}, "overlap"),
+    ({"out_strides": (2048, 512, 64)}, "overlap"),
+    ({"bias_table": 16, "buckets": 1, "max_distance": 128}, "buckets"),
+    ({"bias_table": 16, "buckets": 130, "max_distance": 128}, "buckets"),
+    ({"bias_table": 16, "buckets": 31, "max_distance": 128, "bidirectional": 1}, "buckets"),
+    ({"bias_table": 16, "buckets": 2, "max_distance": 128, "bidirectional": 1}, "buckets"),
+    ({"bias_table": 16, "buckets": 32, "max_distance": 16}, "buckets"),
+    ({"bias_table": 16, "buckets": 32, "max_distance": 4097}, "buckets"),
+    ({"sequences": 1 << 20, "heads": 1 << 12, "kv_heads": 1, "query_length": 1, "key_length": 1,
+      "q_strides": (1 << 18, 64, 64), "out_strides": (1 << 18, 64, 64)}, "workgroups"),
+])
+def test_layout_refused(change, text):
+    assert refused(layout(**change), 0, text)
+
+
+def test_broadcast_inputs_have_no_gradient():
+    """Keys that all sequences share, or heads on one place: fine to read, refused where a gradient goes there."""
+    for name, strides in (("k_strides", (0, 256, 64)), ("v_strides", (1792, 0, 64)), ("q_strides", (2560, 512, 0))):
+        c = layout(**{name: strides})
+        assert native.lib().vh_cross_workspace_bytes(ctypes.byref(c), 0) > 0
+        assert refused(c, 1, "overlap")
+
+
+def test_layouts_taken():
+    for change in ({}, {"sequences": 0}, {"query_length": 0}, {"key_length": 0}, {"type": 1},
+                   {"q_strides": (2560, 64, 320), "out_strides": (2560, 64, 320)},  # [S][H][L][64]
+                   {"q_strides": (64, 1024, 128), "out_strides": (64, 1024, 128)},  # rows outermost
+                   {"bias_table": 16, "buckets": 2, "max_distance": 2},
+                   {"bias_table": 16, "buckets": 4, "max_distance": 2, "bidirectional": 1},
+                   {"bias_table": 16, "buckets": 128, "max_distance": 4096}):
+        c = layout(**change)
+        for backward in (0, 1):
+            assert native.lib().vh_cross_workspace_bytes(ctypes.byref(c), backward) > 0, (change, native.last_error())
+        assert native.lib().vh_cross_saved_bytes(ctypes.byref(c)) > 0
+
+
+def test_null_context_and_layout():
+    L = native.lib()
+    c = layout()
+    assert not L.vh_cross_attention(None, ctypes.byref(c), None, None, None, None, None, None)
+    assert "null context" in native.last_error()
+    assert not L.vh_cross_attention_backward(None, ctypes.byref(c), *[None] * 11)
+    assert not L.vh_layernorm(None, 0, 1, 4, None, 4, None, None, 1e-5, None, 4, None)
+    assert not L.vh_layernorm_backward(None, 0, 1, 4, None, 4, None, 4, None, None, None, 4, None, None, None)
+    assert not L.vh_cross_workspace_bytes(None, 0) and "null layout" in native.last_error()
+
+
+@pytest.mark.parametrize("rows,dim", [(-1, 4), (1 << 31, 4), (1, 0), (1, 16385)])
+def test_layernorm_refused(rows, dim):
+    with pytest.raises(native.NativeError, match="unsupported"):
+        native.Context.layernorm_workspace_bytes(rows, dim)
+
+
+def test_layernorm_workspace():
+    # the backward pass's workgroups, a row of dgamma and one of dbeta each
+    assert native.Context.layernorm_workspace_bytes(0, 1) >= 16
+    for rows, dim in ((1, 1), (7, 384), (49662, 384), (3, 16384), (100000, 2048)):
+        n = native.Context.layernorm_workspace_bytes(rows, dim)
+        assert 8 * dim <= n <= 8 * dim * 512 and n % (8 * dim) == 0
+
+
+@pytest.mark.parametrize("bidirectional", [0, 1])
+@pytest.mark.parametrize("buckets,max_distance", [(32, 128), (16, 96), (64, 800), (4, 2), (4, 7), (128, 4096), (6, 27),
+                                                  (32, 256), (20, 1000), (128, 65), (8, 64)])
+def test_buckets(buckets, max_distance, bidirectional):
+    """Every distance, the borders' own among them (16 of 8 to 128 in 8 steps meets them in whole numbers)."""
+    if max_distance <= (buckets // 2 if bidirectional else buckets) // 2:  # no distance left for the far buckets
+        assert native.lib().vh_relative_bucket(1, buckets, max_distance, bidirectional) == -1
+        return
+    far = max_distance + 40
+    rel = torch.arange(-far, far + 1)
+    want = R.bucket(rel, buckets, max_distance, bool(bidirectional))
+    got = [native.lib().vh_relative_bucket(int(r), buckets, max_distance, bidirectional) for r in rel]
+    assert got == want.tolist()
+    for r in (-2 ** 31, 2 ** 31 - 1):
+        assert native.lib().vh_relative_bucket(r, buckets, max_distance, bidirectional) == \
+            int(want[0] if r < 0 else want[-1])
+
+
+def test_bucket_refused():
+    for args in ((0, 1, 128, 0), (0, 33, 128, 1), (0, 32, 8, 1), (0, 32, 5000, 1)):
+        assert native.lib().vh_relative_bucket(*args) == -1 and "buckets" in native.last_error()
+
+
+def test_binding_checks_shapes():
+    q, k = torch.zeros(2, 5, 8, 64), torch.zeros(2, 7, 4, 64)
+    table = torch.zeros(32, 8)
+    good = dict(q=q, k=k, v=k, out=q)
+    for bad in ({"q": q[..., :32]}, {"v": k[:, :3]}, {"k": k.bfloat16()}, {"out": q[:, :4]}, {"k": k[:1], "v": k[:1]},
+                {"q": q.double(), "k": k.double(), "v": k.double(), "out": q.double()},
+                {"q": torch.zeros(2, 5, 8, 128)[..., ::2]},
+                {"key_lengths": torch.zeros(2)}, {"key_lengths": torch.zeros(3, dtype=torch.int32)},
+                {"bias_table": table[:, :4]}, {"bias_table": table.double()}):
+        with pytest.raises(native.NativeError):
+            native.CrossAttention(None, **{**good, **bad})
+    c = native.CrossAttention(None, **good, bias_table=table).c
+    assert (c.sequences, c.heads, c.kv_heads, c.query_length, c.key_length, c.buckets) == (2, 8, 4, 5, 7, 32)
+    assert list(c.k_strides) == [7 * 256, 256, 64]
