@@ -210,10 +210,9 @@ int vh_attention_noalloc(vh_context *ctx, int sequences, int length, int heads, 
    rstd = 1 / sqrt(mean of (x - mean)^2 + eps); fp32 inside, y rounded once.
    Device x[rows][ldx], y[rows][ldy] of `type`, gamma[dim], beta[dim] (may be
    null: 0); stats[rows][2] (may be null) receives (mean, rstd) for the backward
-   pass.  dim 1 to 16384, any pitch from dim up, rows from 0; y may be x.  Rows
-   of a pitch and dim that are multiples of 4, in tensors (and gamma, beta)
-   aligned to four elements, are read four elements at a time.  Issues one
-   kernel: no allocation, no synchronisation, fit for stream capture. */
+   pass.  dim 1 to 16384, any pitch from dim up, any alignment, rows from 0; y may
+   be x.  Issues one kernel: no allocation, no synchronisation, fit for stream
+   capture. */
 int vh_layernorm(vh_context *ctx, int type, int64_t rows, int dim, const void *x, int64_t ldx, const float *gamma,
                  const float *beta, float eps, void *y, int64_t ldy, float *stats);
 /* Its backward pass from dy, x and the forward's stats:
@@ -235,7 +234,7 @@ size_t vh_layernorm_workspace_bytes(int64_t rows, int dim);
 /* Layout of vh_cross_attention, beside vh_attention (one packed projection, one
    length, rotary): q [sequences][query_length][heads][64] attends to k and v
    [sequences][key_length][kv_heads][64], heads a multiple of kv_heads (query
-   head h reads key head h / (heads / kv_heads)).  Heads are 64 wide. */
+   head h reads key head h / (heads / kv_heads)) and at most 65536.  Heads are 64 wide. */
 typedef struct {
     int type; /* VH_TYPE_* of q, k, v, out and of their gradients */
     int sequences, heads, kv_heads, query_length, key_length;

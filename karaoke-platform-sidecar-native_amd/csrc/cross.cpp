@@ -2,6 +2,7 @@
 // states (layernorm.hpp, cross_attention.hpp).
 #include "runtime.hpp"
 
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -18,7 +19,7 @@ constexpr int LN_MAX_DIM = 16384;
 // Workgroups of the backward pass: each keeps its rows' weight gradients, so
 // more of them are more sums to add up afterwards.
 static int layernorm_parts(int64_t rows, int dim) {
-    return (int)std::min<int64_t>(dim <= 1024 ? (rows + 3) / 4 : rows, 512);
+    return (int)std::min<int64_t>(dim <= 1024 ? (rows + 7) / 8 : rows, 512);
 }
 
 static bool layernorm_ok(const char *what, int type, int64_t rows, int dim, std::initializer_list<int64_t> pitches) {
@@ -40,45 +41,27 @@ size_t layernorm_workspace_bytes(int64_t rows, int dim) {
     return std::max<size_t>(16, (size_t)layernorm_parts(rows, dim) * 2 * dim * sizeof(float));
 }
 
-// Vectors of four where every row and array starts on one.
-static bool by_fours(int type, int dim, std::initializer_list<int64_t> pitches,
-                     std::initializer_list<const void *> tensors, std::initializer_list<const void *> floats) {
-    const uintptr_t bytes = type == VH_TYPE_BF16 ? 8 : 16;
-    int64_t odd = dim % 4;
-    uintptr_t at = 0;
-    for (int64_t ld : pitches) odd |= ld % 4;
-    for (const void *p : tensors) at |= (uintptr_t)p & (bytes - 1);
-    for (const void *p : floats) at |= (uintptr_t)p & 15;
-    return !odd && !at;
-}
-
 template <typename T, int LANES, int N, int NV>
-static void layernorm_launch(hipStream_t s, const NormArgs &a, bool backward, unsigned parts) {
-    constexpr int threads = LANES > 256 ? LANES : 256;
+static void layernorm_launch(hipStream_t s, const NormArgs &a, bool backward, int parts) {
+    using S = NormShape<LANES>;
     if (backward)
-        hipLaunchKernelGGL((layernorm_backward_kernel<T, LANES, N, NV>), dim3(parts), dim3(threads), 0, s, a);
+        hipLaunchKernelGGL((layernorm_backward_kernel<T, LANES, N, NV>), dim3((unsigned)parts), dim3(S::THREADS), 0, s, a);
     else
-        hipLaunchKernelGGL((layernorm_kernel<T, LANES, N, NV>), dim3((unsigned)(LANES == 64 ? (a.rows + 3) / 4 : a.rows)),
-                           dim3(threads), 0, s, a);
+        hipLaunchKernelGGL((layernorm_kernel<T, LANES, N, NV>), dim3((unsigned)((a.rows + S::ROWS - 1) / S::ROWS)),
+                           dim3(S::THREADS), 0, s, a);
 }
 
+// 16 bytes a lane and load (8 where a row is short), a wave a row up to 1024.
 template <typename T>
-static void layernorm_dispatch(hipStream_t s, const NormArgs &a, bool fours, bool backward, unsigned parts) {
+static void layernorm_dispatch(hipStream_t s, const NormArgs &a, bool backward, int parts) {
+    constexpr int N = 16 / sizeof(T);
     const int d = a.dim;
-    if (fours) {
-        if (d <= 256) layernorm_launch<T, 64, 4, 1>(s, a, backward, parts);
-        else if (d <= 512) layernorm_launch<T, 64, 4, 2>(s, a, backward, parts);
-        else if (d <= 1024) layernorm_launch<T, 64, 4, 4>(s, a, backward, parts);
-        else if (d <= 2048) layernorm_launch<T, 256, 4, 2>(s, a, backward, parts);
-        else if (d <= 4096) layernorm_launch<T, 256, 4, 4>(s, a, backward, parts);
-        else layernorm_launch<T, 1024, 4, 4>(s, a, backward, parts);
-    } else {
-        if (d <= 256) layernorm_launch<T, 64, 1, 4>(s, a, backward, parts);
-        else if (d <= 512) layernorm_launch<T, 64, 1, 8>(s, a, backward, parts);
-        else if (d <= 1024) layernorm_launch<T, 64, 1, 16>(s, a, backward, parts);
-        else if (d <= 4096) layernorm_launch<T, 256, 1, 16>(s, a, backward, parts);
-        else layernorm_launch<T, 1024, 1, 16>(s, a, backward, parts);
-    }
+    if (d <= 256) layernorm_launch<T, 64, 4, 1>(s, a, backward, parts);
+    else if (d <= 512) layernorm_launch<T, 64, N, 8 / N>(s, a, backward, parts);
+    else if (d <= 1024) layernorm_launch<T, 64, N, 16 / N>(s, a, backward, parts);
+    else if (d <= 2048) layernorm_launch<T, 256, N, 8 / N>(s, a, backward, parts);
+    else if (d <= 4096) layernorm_launch<T, 256, N, 16 / N>(s, a, backward, parts);
+    else layernorm_launch<T, 1024, N, 16 / N>(s, a, backward, parts);
 }
 
 bool layernorm(hipStream_t s, const LayerNorm &n, KernelTimer *t) {
@@ -93,10 +76,9 @@ bool layernorm(hipStream_t s, const LayerNorm &n, KernelTimer *t) {
     a.gamma = n.gamma; a.beta = n.beta;
     a.stats = reinterpret_cast<float2 *>(n.stats);
     a.rows = n.rows; a.dim = n.dim; a.eps = n.eps;
-    const bool fours = by_fours(n.type, n.dim, {n.ldx, n.ldy}, {n.x, n.y}, {n.gamma, n.beta});
     Scope sc(t, s, "layernorm");
-    if (n.type == VH_TYPE_BF16) layernorm_dispatch<bf16>(s, a, fours, false, 0);
-    else layernorm_dispatch<float>(s, a, fours, false, 0);
+    if (n.type == VH_TYPE_BF16) layernorm_dispatch<bf16>(s, a, false, 0);
+    else layernorm_dispatch<float>(s, a, false, 0);
     return sync_debug(s, "layernorm_kernel");
 }
 
@@ -121,13 +103,12 @@ bool layernorm_backward(hipStream_t s, const LayerNorm &n, KernelTimer *t) {
         a.stats = reinterpret_cast<float2 *>(n.stats);
         a.part = weights ? static_cast<float *>(n.workspace) : nullptr;
         a.rows = n.rows; a.dim = n.dim;
-        const bool fours = by_fours(n.type, n.dim, {n.ldx, n.ldy, n.lddx}, {n.x, n.dy, n.dx}, {n.gamma});
-        if (n.type == VH_TYPE_BF16) layernorm_dispatch<bf16>(s, a, fours, true, (unsigned)parts);
-        else layernorm_dispatch<float>(s, a, fours, true, (unsigned)parts);
+        if (n.type == VH_TYPE_BF16) layernorm_dispatch<bf16>(s, a, true, parts);
+        else layernorm_dispatch<float>(s, a, true, parts);
         if (!sync_debug(s, "layernorm_backward_kernel")) return false;
     }
     if (!weights) return true;
-    hipLaunchKernelGGL(layernorm_columns_kernel, dim3((unsigned)(2 * n.dim + 63) / 64), dim3(256), 0, s,
+    hipLaunchKernelGGL(layernorm_columns_kernel, dim3((unsigned)(2 * n.dim + 63) / 64), dim3(1024), 0, s,
                        static_cast<const float *>(n.workspace), parts, n.dim, n.dgamma, n.dbeta);
     return sync_debug(s, "layernorm_columns_kernel");
 }
@@ -199,7 +180,7 @@ static bool cross_ok(const char *what, const vh_cross *c, bool backward) {
         return false;
     }
     if ((c->type != VH_TYPE_FP32 && c->type != VH_TYPE_BF16) || c->sequences < 0 || c->heads < 1 || c->kv_heads < 1 ||
-        c->heads % c->kv_heads || c->query_length < 0 || c->key_length < 0 || c->query_length > CA_MAX_LENGTH ||
+        c->heads > 65536 || c->heads % c->kv_heads || c->query_length < 0 || c->key_length < 0 || c->query_length > CA_MAX_LENGTH ||
         c->key_length > CA_MAX_LENGTH) {
         set_error("%s: unsupported type %d, %d sequences, %d heads over %d, lengths %d and %d", what, c->type,
                   c->sequences, c->heads, c->kv_heads, c->query_length, c->key_length);
@@ -252,16 +233,118 @@ static size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 
 size_t cross_saved_bytes(const vh_cross *c) {
     if (!cross_ok("vh_cross_saved_bytes", c, false)) return 0;
-    return std::max<size_t>(16, (size_t)cross_rows(c) * (8 + (c->type == VH_TYPE_BF16 ? 2 * CA_D : 0)));
+    const size_t rows = (size_t)cross_rows(c);
+    const size_t rest = c->type == VH_TYPE_BF16 ? (c->bias_table ? sizeof(float) : sizeof(bf16)) * CA_D : 0;
+    return std::max<size_t>(16, round16(rows * sizeof(float2)) + rows * rest);
+}
+
+constexpr size_t CA_LDS = 160 * 1024;  // of a workgroup
+static size_t window_bytes(const vh_cross *c) {
+    return c->bias_table ? (size_t)(2 * (c->max_distance + CA_PAD) + 1) * sizeof(float) : 0;
+}
+static size_t tiles_lds(const vh_cross *c, bool split) {
+    if (c->type == VH_TYPE_BF16) return split ? SplitLds<bf16>::BYTES : 4 * Tile<bf16>::BYTES;
+    return split ? SplitLds<float>::BYTES : 4 * Tile<float>::BYTES;
+}
+static size_t dq_lds(const vh_cross *c, bool split) {
+    if (!c->bias_table) return tiles_lds(c, split);
+    size_t tiles = tiles_lds(c, false);
+    if (split) tiles = c->type == VH_TYPE_BF16 ? DqLds<bf16, true>::BYTES : DqLds<float, true>::BYTES;
+    return tiles + window_bytes(c) + sizeof(DbiasLds) + 128 * sizeof(float) * c->buckets + window_bytes(c) / sizeof(float);
+}
+static size_t pack_lds(const vh_cross *c) {
+    return tiles_lds(c, true) +
+           (c->bias_table ? sizeof(float) * c->buckets * (c->heads / c->kv_heads) + window_bytes(c) / sizeof(float) : 0);
+}
+
+// How a call is cut into workgroups.  split: the kernels whose four waves share 32
+// rows, in `parts` pieces; else those of 128 rows.
+struct CrossCut {
+    bool split = false, pack = false;
+    int parts = 1;
+    int64_t groups = 0;  // workgroups
+};
+// From about two 128-row workgroups per CU on, their sharing of tiles wins over
+// even work.  Below, pieces of at least 8 tiles (two a wave) until there are about
+// two workgroups per CU.
+constexpr int64_t CA_ENOUGH = 512;
+static CrossCut cross_cut(int64_t columns, int rows, int pack, int across, bool fits) {
+    CrossCut cut;
+    cut.groups = columns * ((rows + 127) / 128);
+    if ((cut.groups >= CA_ENOUGH && rows >= 64) || !fits) return cut;
+    cut.split = true;
+    cut.pack = pack > 1 && rows < 32;
+    if (cut.pack) columns /= pack;
+    const int64_t base = columns * (((int64_t)rows * (cut.pack ? pack : 1) + 31) / 32);
+    const int tiles = (across + 31) / 32;
+    if (base > 0) cut.parts = (int)std::max<int64_t>(1, std::min<int64_t>({CA_ENOUGH / base, tiles / 8, 64}));
+    cut.groups = base * cut.parts;
+    return cut;
+}
+static CrossCut forward_cut(const vh_cross *c, bool keep) {
+    const int shared = c->heads / c->kv_heads;
+    const bool pack = !keep && (!c->bias_table || pack_lds(c) <= CA_LDS);
+    return cross_cut((int64_t)c->sequences * c->heads, c->query_length, pack ? shared : 1, c->key_length, true);
+}
+static CrossCut dq_cut(const vh_cross *c) {
+    return cross_cut((int64_t)c->sequences * c->heads, c->query_length, 1, c->key_length, dq_lds(c, true) <= CA_LDS);
+}
+static CrossCut dkv_cut(const vh_cross *c) {
+    CrossCut cut = cross_cut((int64_t)c->sequences * c->kv_heads, c->key_length, 1, c->query_length, true);
+    if (!cut.split) return cut;
+    // the heads that share the keys are pieces of their own
+    const int64_t base = (int64_t)c->sequences * c->heads * ((c->key_length + 31) / 32);
+    const int tiles = (c->query_length + 31) / 32;
+    cut.parts = base > 0 ? (int)std::max<int64_t>(1, std::min<int64_t>({CA_ENOUGH / base, tiles / 8, 64})) : 1;
+    cut.groups = base * cut.parts;
+    return cut;
+}
+
+// The workspace's sections, in bytes from its start.
+struct CrossWork {
+    CrossCut rows, keys;  // backward: of dq, of dk and dv
+    size_t stats = 0, part_o = 0, part_ml = 0, part_dk = 0, part_dv = 0, dbias = 0, bytes = 0;
+    int dbias_parts = 0;
+    size_t take(size_t n) {
+        const size_t at = bytes;
+        bytes += round16(n);
+        return at;
+    }
+};
+static CrossWork forward_work(const vh_cross *c, bool keep) {
+    CrossWork w;
+    w.rows = forward_cut(c, keep);
+    if (w.rows.split && w.rows.parts > 1) {
+        const size_t rows = (size_t)cross_rows(c) * w.rows.parts;
+        w.part_o = w.take(rows * CA_D * sizeof(float));
+        w.part_ml = w.take(rows * sizeof(float2));
+    }
+    return w;
+}
+static int kv_pieces(const vh_cross *c, const CrossCut &cut) { return cut.split ? c->heads / c->kv_heads * cut.parts : 1; }
+static CrossWork backward_work(const vh_cross *c) {
+    CrossWork w;
+    w.rows = dq_cut(c);
+    w.keys = dkv_cut(c);
+    w.stats = w.take((size_t)c->sequences * c->heads * ((c->query_length + 31) / 32) * sizeof(RowStats));
+    if (w.rows.split && w.rows.parts > 1) w.part_o = w.take((size_t)cross_rows(c) * w.rows.parts * CA_D * sizeof(float));
+    const int pieces = kv_pieces(c, w.keys);
+    if (pieces > 1) {
+        const size_t n = (size_t)pieces * c->sequences * c->kv_heads * c->key_length * CA_D * sizeof(float);
+        w.part_dk = w.take(n);
+        w.part_dv = w.take(n);
+    }
+    if (c->bias_table) {
+        w.dbias_parts = (int)(w.rows.groups / c->heads);
+        w.dbias = w.take((size_t)w.rows.groups * c->buckets * sizeof(float));
+    }
+    return w;
 }
 
 size_t cross_workspace_bytes(const vh_cross *c, bool backward) {
     if (!cross_ok("vh_cross_workspace_bytes", c, backward)) return 0;
-    if (!backward) return 16;
-    size_t n = round16((size_t)cross_rows(c) * sizeof(float));
-    if (c->bias_table)
-        n += (size_t)c->sequences * c->heads * ((c->query_length + 127) / 128) * c->buckets * sizeof(float);
-    return std::max<size_t>(16, n);
+    if (backward) return std::max<size_t>(16, backward_work(c).bytes);
+    return std::max<size_t>({16, forward_work(c, false).bytes, forward_work(c, true).bytes});
 }
 
 static CrossTensor cross_tensor(const void *p, const int64_t *strides, int64_t size) {
@@ -283,11 +366,12 @@ static CrossArgs cross_args(const vh_cross *c, const CrossBuffers &b) {
     a.Lq = c->query_length; a.Lk = c->key_length;
     a.causal = c->causal ? 1 : 0;
     a.scale = c->scale;
+    a.scale2 = std::max(fabsf(c->scale) * 1.4426950408889634f, FLT_MIN);  // 0 times a hidden score is no number
     a.query_lengths = c->query_lengths; a.key_lengths = c->key_lengths; a.query_start = c->query_start;
     a.table = c->bias_table;
     if (a.table) bias_args(a, c->buckets, c->max_distance, c->bidirectional);
     a.stats = static_cast<float2 *>(b.saved);
-    if (b.saved && c->type == VH_TYPE_BF16) a.rest = reinterpret_cast<bf16 *>(a.stats + cross_rows(c));
+    if (b.saved && c->type == VH_TYPE_BF16) a.rest = static_cast<char *>(b.saved) + round16((size_t)cross_rows(c) * sizeof(float2));
     return a;
 }
 
@@ -300,31 +384,31 @@ static bool aligned(const char *what, std::initializer_list<const void *> pointe
     return true;
 }
 
-static size_t window_bytes(const CrossArgs &a) { return a.table ? (size_t)(2 * (a.max_distance + CA_PAD) + 1) * 4 : 0; }
+template <typename F>
+static void launch(F kernel, int64_t groups, size_t lds, hipStream_t s, const CrossArgs &a) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), lds, s, a);
+}
 
 template <typename T, bool BIAS>
-static void forward_launch(hipStream_t s, const CrossArgs &a) {
-    const unsigned grid = (unsigned)((int64_t)a.S * a.H * ((a.Lq + 127) / 128));
-    const size_t lds = 2 * Tile<T>::BYTES + window_bytes(a);
-    if (a.stats) hipLaunchKernelGGL((cross_forward_kernel<T, BIAS, true>), dim3(grid), dim3(256), lds, s, a);
-    else hipLaunchKernelGGL((cross_forward_kernel<T, BIAS, false>), dim3(grid), dim3(256), lds, s, a);
-}
-
-template <typename T>
-static void dq_launch(hipStream_t s, const CrossArgs &a) {
-    const unsigned grid = (unsigned)((int64_t)a.S * a.H * ((a.Lq + 127) / 128));
-    const size_t lds = 2 * Tile<T>::BYTES;
-    const size_t bias = a.table ? sizeof(DbiasLds) + 128 * (size_t)a.buckets * 4 + window_bytes(a) : 0;
-    if (a.table) hipLaunchKernelGGL((cross_dq_kernel<T, true>), dim3(grid), dim3(256), lds + bias, s, a);
-    else hipLaunchKernelGGL((cross_dq_kernel<T, false>), dim3(grid), dim3(256), lds, s, a);
-}
-
-template <typename T>
-static void dkv_launch(hipStream_t s, const CrossArgs &a) {
-    const unsigned grid = (unsigned)((int64_t)a.S * a.KV * ((a.Lk + 127) / 128));
-    const size_t lds = 2 * Tile<T>::BYTES + sizeof(RowStats) + window_bytes(a);
-    if (a.table) hipLaunchKernelGGL((cross_dkv_kernel<T, true>), dim3(grid), dim3(256), lds, s, a);
-    else hipLaunchKernelGGL((cross_dkv_kernel<T, false>), dim3(grid), dim3(256), lds, s, a);
+static void forward_launch(hipStream_t s, const vh_cross *c, const CrossArgs &a, const CrossCut &cut) {
+    const bool keep = a.stats != nullptr;
+    const size_t lds = tiles_lds(c, cut.split) + window_bytes(c);
+    if (!cut.split) {
+        if (keep) launch(cross_forward_kernel<T, BIAS, true>, cut.groups, lds, s, a);
+        else launch(cross_forward_kernel<T, BIAS, false>, cut.groups, lds, s, a);
+        return;
+    }
+    if (cut.pack) {
+        launch(cross_forward_split_kernel<T, BIAS, false, true>, cut.groups, pack_lds(c), s, a);
+    } else if (keep) {
+        launch(cross_forward_split_kernel<T, BIAS, true, false>, cut.groups, lds, s, a);
+    } else {
+        launch(cross_forward_split_kernel<T, BIAS, false, false>, cut.groups, lds, s, a);
+    }
+    if (cut.parts == 1) return;
+    const int64_t groups = (cross_rows(c) + 15) / 16;
+    if (keep) launch(cross_join_kernel<T, BIAS, true>, groups, 0, s, a);
+    else launch(cross_join_kernel<T, BIAS, false>, groups, 0, s, a);
 }
 
 bool cross_attention(hipStream_t s, const vh_cross *c, const CrossBuffers &b, KernelTimer *t) {
@@ -336,11 +420,34 @@ bool cross_attention(hipStream_t s, const vh_cross *c, const CrossBuffers &b, Ke
         return false;
     }
     if (!aligned(what, {b.q, b.k, b.v, b.out, b.saved, b.workspace})) return false;
-    const CrossArgs a = cross_args(c, b);
+    CrossArgs a = cross_args(c, b);
+    const CrossWork w = forward_work(c, a.stats != nullptr);
+    if (w.bytes && !b.workspace) {
+        set_error("%s: null workspace (vh_cross_workspace_bytes)", what);
+        return false;
+    }
+    a.parts = w.rows.parts;
+    a.part_o = reinterpret_cast<float *>(static_cast<char *>(b.workspace) + w.part_o);
+    a.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(b.workspace) + w.part_ml);
     Scope sc(t, s, "cross_attention");
-    if (c->type == VH_TYPE_BF16) a.table ? forward_launch<bf16, true>(s, a) : forward_launch<bf16, false>(s, a);
-    else a.table ? forward_launch<float, true>(s, a) : forward_launch<float, false>(s, a);
+    if (c->type == VH_TYPE_BF16)
+        a.table ? forward_launch<bf16, true>(s, c, a, w.rows) : forward_launch<bf16, false>(s, c, a, w.rows);
+    else a.table ? forward_launch<float, true>(s, c, a, w.rows) : forward_launch<float, false>(s, c, a, w.rows);
     return sync_debug(s, "cross_forward_kernel");
+}
+
+template <typename T, bool BIAS>
+static void dq_launch(hipStream_t s, const vh_cross *c, const CrossArgs &a, const CrossCut &cut) {
+    if (cut.split) launch(cross_dq_split_kernel<T, BIAS>, cut.groups, dq_lds(c, true), s, a);
+    else launch(cross_dq_kernel<T, BIAS>, cut.groups, dq_lds(c, false), s, a);
+}
+
+template <typename T, bool BIAS>
+static void dkv_launch(hipStream_t s, const vh_cross *c, const CrossArgs &a, const CrossCut &cut) {
+    const size_t lds = tiles_lds(c, cut.split) + (cut.split ? 4 * SplitLds<T>::BUFS * sizeof(RowStats) + window_bytes(c)
+                                                        : 2 * sizeof(RowStats) + 2 * window_bytes(c));
+    if (cut.split) launch(cross_dkv_split_kernel<T, BIAS>, cut.groups, lds, s, a);
+    else launch(cross_dkv_kernel<T, BIAS>, cut.groups, lds, s, a);
 }
 
 bool cross_attention_backward(hipStream_t s, const vh_cross *c, const CrossBuffers &b, KernelTimer *t) {
@@ -361,28 +468,40 @@ bool cross_attention_backward(hipStream_t s, const vh_cross *c, const CrossBuffe
     }
     if (!aligned(what, {b.q, b.k, b.v, b.out, b.saved, b.workspace, b.dout, b.dq, b.dk, b.dv})) return false;
     CrossArgs a = cross_args(c, b);
-    a.delta = static_cast<float *>(b.workspace);
+    const CrossWork w = backward_work(c);
+    auto at = [&](size_t n) { return reinterpret_cast<float *>(static_cast<char *>(b.workspace) + n); };
+    a.rows = at(w.stats);
+    a.parts = w.rows.parts;
+    a.kv_parts = w.keys.parts;
+    a.part_o = at(w.part_o);
+    a.part_dk = at(w.part_dk);
+    a.part_dv = at(w.part_dv);
     a.dbias = b.dbias;
-    if (b.dbias)
-        a.dbias_part = reinterpret_cast<float *>(static_cast<char *>(b.workspace) +
-                                                 round16((size_t)cross_rows(c) * sizeof(float)));
+    a.dbias_part = b.dbias ? at(w.dbias) : nullptr;
+    a.dbias_parts = w.dbias_parts;
+    const bool is_bf16 = c->type == VH_TYPE_BF16;
     if (rows) {
         Scope sc(t, s, "cross_attention_dq");
-        if (c->type == VH_TYPE_BF16) dq_launch<bf16>(s, a);
-        else dq_launch<float>(s, a);
+        if (is_bf16) a.table ? dq_launch<bf16, true>(s, c, a, w.rows) : dq_launch<bf16, false>(s, c, a, w.rows);
+        else a.table ? dq_launch<float, true>(s, c, a, w.rows) : dq_launch<float, false>(s, c, a, w.rows);
         if (!sync_debug(s, "cross_dq_kernel")) return false;
     }
-    if (b.dbias) {
-        hipLaunchKernelGGL(cross_dbias_kernel, dim3((unsigned)a.H), dim3(128), 0, s, a);
-        if (!sync_debug(s, "cross_dbias_kernel")) return false;
-    }
-    if (b.dk && keys) {
+    const bool dkv = b.dk && keys;
+    if (dkv) {
         Scope sc(t, s, "cross_attention_dkv");
-        if (c->type == VH_TYPE_BF16) dkv_launch<bf16>(s, a);
-        else dkv_launch<float>(s, a);
+        if (is_bf16) a.table ? dkv_launch<bf16, true>(s, c, a, w.keys) : dkv_launch<bf16, false>(s, c, a, w.keys);
+        else a.table ? dkv_launch<float, true>(s, c, a, w.keys) : dkv_launch<float, false>(s, c, a, w.keys);
         if (!sync_debug(s, "cross_dkv_kernel")) return false;
     }
-    return true;
+    FinishArgs f{};
+    if (rows && w.rows.split && w.rows.parts > 1) f.dq = (cross_rows(c) + 15) / 16;
+    if (dkv && kv_pieces(c, w.keys) > 1) f.dkv = ((int64_t)c->sequences * c->kv_heads * c->key_length + 15) / 16;
+    const int64_t groups = f.dq + 2 * f.dkv + (b.dbias ? c->heads : 0);
+    if (!groups) return true;
+    Scope sc(t, s, "cross_attention_sums");
+    if (is_bf16) hipLaunchKernelGGL(cross_finish_kernel<bf16>, dim3((unsigned)groups), dim3(256), 0, s, a, f);
+    else hipLaunchKernelGGL(cross_finish_kernel<float>, dim3((unsigned)groups), dim3(256), 0, s, a, f);
+    return sync_debug(s, "cross_finish_kernel");
 }
 
 }  // namespace vh

@@ -14,10 +14,18 @@
 // exponentials and dS are fp32.  bf16 operands are the tensors as they are;
 // P and dS are rounded to bf16 (by up to 2^-8 of themselves, as the outputs are)
 // where they enter a product, and nowhere else: scale, bias, statistics and the
-// table's gradient see the fp32 values.  A forward that keeps its state for the
-// backward pass multiplies v by P in two bf16 pieces (to 2^-16): delta is the
-// sum of P dP, and the table's gradient, whose terms cancel in every row, would
-// show an error of 2^-8 in it as one of 2e-3 of its own norm.
+// table's gradient see the fp32 values.  delta stands for the sum of P dP, and out
+// rounded to bf16, or made of rounded P, would put an error of 2^-8 into it.  So a
+// forward that keeps its state for the backward pass multiplies v by P in two bf16
+// pieces and keeps what rounding takes from out; with a bias in three pieces, and
+// the rest in fp32, since dS sums to 0 over a row and the table's gradient is what
+// is left of such sums (14 x 8 x 4089 rows over 60 keys, nearly all in one bucket:
+// off by 2.8e-5 of its norm with two pieces and a bf16 rest).
+//
+// Scores are kept times log2(e): without a bias as s = q.k, the factor scale log2(e)
+// being multiplied in the exponential's argument, exp2(s c - m c), one operation a
+// score (a negative scale turns q's, or k's, sign instead); with a bias as s c + b
+// log2(e), where a finite b stays finite.
 //
 // Operand order (both types).  v_mfma_f32_32x32x16_bf16 takes 8 values of the
 // summed index per lane: lane (li = l % 32, lh = l / 32) holds row or column li
@@ -49,13 +57,26 @@ struct CrossArgs {
     int S, H, KV, Lq, Lk;
     int causal;
     float scale;
+    float scale2;    // |scale| log2(e), at least the smallest normal number
     const int *query_lengths, *key_lengths, *query_start;  // [S] or null
     const float *table;                                    // [buckets][H] or null
     int buckets, max_distance, bidirectional;
-    float2 *stats;   // [S][H][Lq]: the maximum's place m and -log2 of sum exp(x - m); (0, -inf) without a key
-    bf16 *rest;      // bf16: [S][H][Lq][64], out's rounding error, so that delta is exact; null: not kept
-    float *delta;    // [S][H][Lq]
-    float *dbias_part;  // [S][H][ceil(Lq / 128)][buckets]
+    // [S][H][Lq], in powers of two: (M, -) with P = exp2(x log2(e) - M); with a bias
+    // (m, n) with P = exp2((x log2(e) - m) + n), since one as low as the type goes
+    // leaves no bits for n beside it
+    float2 *stats;
+    void *rest;      // bf16: [S][H][Lq][64], what rounding took from out, in bf16 (with a bias in fp32)
+    float *rows;     // backward: [S][H][ceil(Lq / 32)] tiles of RowStats
+    // Sums over a part of the keys (forward, dq) or queries (dk, dv), when a row
+    // tile's work is split: parts pieces, [part][S][H][Lq][64] and their (m, l);
+    // [part][S][KV][Lk][64] for dk, dv, part = head among those that share the
+    // keys * kv_parts + piece
+    int parts, kv_parts;
+    float *part_o;
+    float2 *part_ml;
+    float *part_dk, *part_dv;
+    float *dbias_part;  // [H][dbias_parts][buckets]
+    int dbias_parts;    // per head: sequences x row tiles x pieces
     float *dbias;       // [buckets][H]
     // far buckets of one side: bucket near + i begins at distance edge[i]
     int side, near, edges;
@@ -98,15 +119,22 @@ VH_DEVICE void frag_mfma(floatx16 &acc, const Frag<float> &a, const Frag<float> 
 VH_DEVICE Frag<bf16> frag_load(const bf16 *p) { return {*reinterpret_cast<const bf16x8 *>(p)}; }
 VH_DEVICE Frag<float> frag_load(const float *p) { return {{ld4(p), ld4(p + 4)}}; }
 
+VH_DEVICE void frag_negate(Frag<bf16> &f) { f.v = -f.v; }
+VH_DEVICE void frag_negate(Frag<float> &f) {
+    f.v[0] = -f.v[0];
+    f.v[1] = -f.v[1];
+}
+
 // Registers 8 st .. 8 st + 7 of a result as a B operand.
 VH_DEVICE void frag_from(Frag<bf16> &f, const floatx16 &x, int st) {
 #pragma unroll
     for (int e = 0; e < 8; e++) f.v[e] = (bf16)x[8 * st + e];
 }
-// What rounding took from them.
-VH_DEVICE void frag_rest(Frag<bf16> &rest, const Frag<bf16> &f, const floatx16 &x, int st) {
+// What rounding took from them: x becomes it, f its next piece.
+VH_DEVICE void frag_rest(Frag<bf16> &f, floatx16 &x, int st) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) rest.v[e] = (bf16)(x[8 * st + e] - (float)f.v[e]);
+    for (int e = 0; e < 8; e++) x[8 * st + e] -= (float)f.v[e];
+    frag_from(f, x, st);
 }
 VH_DEVICE void frag_from(Frag<float> &f, const floatx16 &x, int st) {
 #pragma unroll
@@ -178,14 +206,14 @@ VH_DEVICE Frag<float> tile_col(const unsigned char *tile, int st, int t, int lan
 }
 
 // Copies rows row0 .. row0 + 31 of a tensor's sequence and head (base: its row 0)
-// into a tile, 1 KB a load, the loads dealt out to the four waves.  Rows past
-// `last` are copies of row `last`: what lies behind the valid rows is never read.
-template <typename T>
+// into a tile, 1 KB a load, the loads dealt out to WAVES waves.  Rows past `last`
+// are copies of row `last`: what lies behind the valid rows is never read.
+template <typename T, int WAVES>
 VH_DEVICE void tile_issue(const char *base, int64_t row_bytes, int row0, int last, uint32_t tile_lds, int wave,
                           int lane) {
     using L = Tile<T>;
     const char *sbase = base + (int64_t)row0 * row_bytes;
-    constexpr int LOADS = CA_TILE / L::DMA_ROWS / 4;
+    constexpr int LOADS = CA_TILE / L::DMA_ROWS / WAVES;
 #pragma unroll
     for (int i = 0; i < LOADS; i++) {
         const int r0 = (LOADS * wave + i) * L::DMA_ROWS;
@@ -194,6 +222,7 @@ VH_DEVICE void tile_issue(const char *base, int64_t row_bytes, int row0, int las
         lds_dma16s(off, sbase, tile_lds + (uint32_t)(r0 * L::ROW));
     }
 }
+VH_DEVICE void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 VH_DEVICE int row_of(int r, int lh) { return 8 * (r >> 2) + 4 * lh + (r & 3); }
 VH_DEVICE void zero16(floatx16 &x) {
@@ -222,44 +251,134 @@ VH_DEVICE int cross_start(const CrossArgs &a, int s) {
 // max_distance the bucket is the last), so that a 32 x 32 tile that is not
 // wholly beyond it looks its pairs up without a clamp.
 VH_DEVICE int cross_window(const CrossArgs &a) { return 2 * (a.max_distance + CA_PAD) + 1; }
+VH_DEVICE float bias_log2(float b) {
+    const float y = b * CA_LOG2E;
+    return __builtin_isinf(y) && !__builtin_isinf(b) ? __builtin_copysignf(3.402823466e38f, b) : y;
+}
 VH_DEVICE void fill_bias_window(const CrossArgs &a, int h, float *window, int tid) {
     for (int i = tid; i < cross_window(a); i += 256)
-        window[i] = a.table[(int64_t)cross_bucket(a, i - a.max_distance - CA_PAD) * a.H + h];
+        window[i] = bias_log2(a.table[(int64_t)cross_bucket(a, i - a.max_distance - CA_PAD) * a.H + h]);
+}
+VH_DEVICE void fill_bucket_window(const CrossArgs &a, unsigned char *window, int tid) {
+    for (int i = tid; i < cross_window(a); i += 256)
+        window[i] = (unsigned char)cross_bucket(a, i - a.max_distance - CA_PAD);
 }
 
-// Scores of a tile: x = scale s + bias, -inf where the pair is hidden.  rel0: the
-// relative position of register row 0 (lh 0) against the lane's column; step: +1
-// where rows are keys, -1 where they are queries.
-template <bool BIAS>
-VH_DEVICE void scores(const CrossArgs &a, floatx16 &x, const float *window, int tile_lo, int tile_hi, int rel0, int step,
-                      int lh) {
-    if constexpr (BIAS) {
-        const int md = a.max_distance;
-        if (tile_hi <= -md || tile_lo >= md) {
-            const float b = window[tile_hi <= -md ? CA_PAD : 2 * md + CA_PAD];
+// Scores of a tile with the bias.  rel0: the relative position of register row 0
+// (lh 0) against the lane's column; step: +1 where rows are keys, -1 where they
+// are queries.
+VH_DEVICE void add_bias(const CrossArgs &a, floatx16 &x, const float *window, int tile_lo, int tile_hi, int rel0,
+                        int step, int lh) {
+    const int md = a.max_distance;
+    if (tile_hi <= -md || tile_lo >= md) {
+        const float b = window[tile_hi <= -md ? CA_PAD : 2 * md + CA_PAD];
 #pragma unroll
-            for (int r = 0; r < 16; r++) x[r] = __builtin_fmaf(x[r], a.scale, b);
-        } else {
-            const float *w = window + rel0 + step * 4 * lh + md + CA_PAD;
-#pragma unroll
-            for (int r = 0; r < 16; r++) x[r] = __builtin_fmaf(x[r], a.scale, w[step * row_of(r, 0)]);
-        }
+        for (int r = 0; r < 16; r++) x[r] = __builtin_fmaf(x[r], a.scale2, b);
     } else {
+        const float *w = window + rel0 + step * 4 * lh + md + CA_PAD;
 #pragma unroll
-        for (int r = 0; r < 16; r++) x[r] *= a.scale;
+        for (int r = 0; r < 16; r++) x[r] = __builtin_fmaf(x[r], a.scale2, w[step * row_of(r, 0)]);
     }
 }
 
 // ------------------------------------------------------------------ forward
-// Workgroup: 4 waves x 32 queries of one head, tiles of 32 keys.  Per wave and
-// tile S^T = K Q^T, so that a lane holds 16 scores of one query, the online
-// softmax, and out^T += V^T P^T from the same registers.
-// KEEP: statistics, rest, and P in two pieces.
+// A wave's 32 query rows as columns: running maximum (of s, or of s c + b with a
+// bias), the same in the exponent (0 while the row has seen no key: -inf - -inf is
+// no number), sum and out^T.
+struct RowState {
+    floatx16 o[2];
+    float m, mc, l;
+    VH_DEVICE void clear() {
+        zero16(o[0]);
+        zero16(o[1]);
+        m = -INFINITY;
+        mc = 0.0f;
+        l = 0.0f;
+    }
+    VH_DEVICE float top() const { return m == -INFINITY ? m : mc; }  // the maximum in powers of two
+};
+
+// One tile of keys: x holds its scores on entry; seen: rows of the tile that the
+// lane's query sees, -inf past them where mask says that a lane has fewer than 32.
+// The maximum is raised only when a tile exceeds it by more than 2^8, which fp32
+// sums absorb: the rescaling runs on a few tiles of a row.
 template <typename T, bool BIAS, bool KEEP>
-__global__ __launch_bounds__(256, 2) void cross_forward_kernel(CrossArgs a) {
-    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-    unsigned char *Ks = smem, *Vs = smem + Tile<T>::BYTES;
-    float *window = reinterpret_cast<float *>(smem + 2 * Tile<T>::BYTES);
+VH_DEVICE void softmax_tile(RowState &st, floatx16 &x, const unsigned char *Vs, float c, bool mask, int seen, int lane) {
+    const int lh = lane >> 5;
+    if (mask) {
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+            if (row_of(r, lh) >= seen) x[r] = -INFINITY;
+    }
+    float mt = x[0];
+#pragma unroll
+    for (int r = 1; r < 16; r++) mt = fmaxf(mt, x[r]);
+    mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+    const bool grow = BIAS ? mt - 8.0f > st.m : (mt - st.m) * c > 8.0f;
+    if (__any(grow)) {
+        const float mn = fmaxf(st.m, mt);
+        const float mc = mn == -INFINITY ? 0.0f : BIAS ? mn : mn * c;
+        const float f = st.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(BIAS ? st.m - mn : (st.m - mn) * c);
+        st.m = mn;
+        st.mc = mc;
+        st.l *= f;
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            st.o[0][r] *= f;
+            st.o[1][r] *= f;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+        x[r] = __builtin_amdgcn_exp2f(BIAS ? x[r] - st.mc : __builtin_fmaf(x[r], c, -st.mc));
+        st.l += x[r];
+    }
+#pragma unroll
+    for (int g = 0; g < 2; g++) {
+        Frag<T> pb, vf[2];
+        frag_from(pb, x, g);
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            vf[t] = tile_col(Vs, g, t, lane, T());
+            frag_mfma(st.o[t], vf[t], pb);
+        }
+        if constexpr (KEEP && sizeof(T) == 2) {
+#pragma unroll
+            for (int i = 0; i < (BIAS ? 2 : 1); i++) {
+                frag_rest(pb, x, g);
+#pragma unroll
+                for (int t = 0; t < 2; t++) frag_mfma(st.o[t], vf[t], pb);
+            }
+        }
+    }
+}
+
+// Four dims of a finished row: out, and what rounding took from it.
+template <typename T, bool BIAS, bool KEEP>
+VH_DEVICE void store_out(const CrossArgs &a, T *op, int64_t row, int d, floatx4 y) {
+    st4(op + d, y);
+    if constexpr (KEEP && sizeof(T) == 2) {
+        const bf16x4 yr = to_bf16x4(y);
+#pragma unroll
+        for (int r = 0; r < 4; r++) y[r] -= (float)yr[r];
+        if constexpr (BIAS) st4(static_cast<float *>(a.rest) + row * CA_D + d, y);
+        else st4(static_cast<bf16 *>(a.rest) + row * CA_D + d, y);
+    }
+}
+VH_DEVICE float2 row_stats(bool bias, bool seen, float m, float l) {
+    if (!seen) return make_float2(bias ? 0.0f : INFINITY, -INFINITY);
+    const float n = log2f(l);
+    return make_float2(bias ? m : m + n, -n);
+}
+
+// Workgroup: 4 waves x 32 queries of one head, tiles of 32 keys that they share,
+// the next one's copies in flight while one is worked on.  Per wave and tile S^T =
+// K Q^T, so that a lane holds 16 scores of one query, the online softmax, and out^T
+// += V^T P^T from the same registers.  KEEP: statistics, rest, and P in two pieces.
+template <typename T, bool BIAS, bool KEEP>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) void cross_forward_kernel(CrossArgs a) {
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];  // [2] K and V tiles
+    float *window = reinterpret_cast<float *>(smem + 4 * Tile<T>::BYTES);
 
     const int qtiles = (a.Lq + 127) / 128;
     const int task = xcd_swizzle((int)blockIdx.x, (int)gridDim.x);
@@ -275,117 +394,483 @@ __global__ __launch_bounds__(256, 2) void cross_forward_kernel(CrossArgs a) {
     if (a.causal) keys = min(keys, start + min(128 * qt + 128, qlen));
     if (128 * qt >= qlen) keys = 0;
 
-    if constexpr (BIAS) {
-        fill_bias_window(a, h, window, tid);
-        __syncthreads();
-    }
+    const char *kp = a.k.p + s * a.k.seq + kh * a.k.head, *vp = a.v.p + s * a.v.seq + kh * a.v.head;
+    const uint32_t lds = (uint32_t)(uintptr_t)smem;
+    auto issue = [&](int k0) {
+        const uint32_t at = lds + (uint32_t)(k0 / CA_TILE & 1) * 2 * Tile<T>::BYTES;
+        tile_issue<T, 4>(kp, a.k.row, k0, klen - 1, at, wave, lane);
+        tile_issue<T, 4>(vp, a.v.row, k0, klen - 1, at + Tile<T>::BYTES, wave, lane);
+    };
+    if (keys > 0) issue(0);
+    if constexpr (BIAS) fill_bias_window(a, h, window, tid);  // read after the loop's first barrier
     Frag<T> qf[4];
     if (active) {
         const char *qp = a.q.p + s * a.q.seq + (int64_t)min(q, qlen - 1) * a.q.row + h * a.q.head;
 #pragma unroll
-        for (int g = 0; g < 4; g++) qf[g] = frag_load(reinterpret_cast<const T *>(qp) + 16 * g + 8 * lh);
+        for (int g = 0; g < 4; g++) {
+            qf[g] = frag_load(reinterpret_cast<const T *>(qp) + 16 * g + 8 * lh);
+            if (a.scale < 0.0f) frag_negate(qf[g]);
+        }
     }
-    floatx16 o[2];
-    zero16(o[0]);
-    zero16(o[1]);
-    float m = -INFINITY, l = 0.0f;
-    const char *kp = a.k.p + s * a.k.seq + kh * a.k.head, *vp = a.v.p + s * a.v.seq + kh * a.v.head;
-    const uint32_t k_lds = (uint32_t)(uintptr_t)Ks, v_lds = (uint32_t)(uintptr_t)Vs;
+    RowState st;
+    st.clear();
     for (int k0 = 0; k0 < keys; k0 += CA_TILE) {
-        tile_issue<T>(kp, a.k.row, k0, klen - 1, k_lds, wave, lane);
-        tile_issue<T>(vp, a.v.row, k0, klen - 1, v_lds, wave, lane);
         wait_vmcnt<0>();
-        __syncthreads();
+        __syncthreads();  // this tile is there, and the last one has been read
+        if (k0 + CA_TILE < keys) issue(k0 + CA_TILE);
         if (active && (!a.causal || k0 <= start + q0 + 31)) {
+            const unsigned char *Ks = smem + (k0 / CA_TILE & 1) * 2 * Tile<T>::BYTES;
             floatx16 x;
             zero16(x);
 #pragma unroll
             for (int g = 0; g < 4; g++) frag_mfma(x, tile_row(Ks, li, g, lh, T()), qf[g]);
             const int lo = k0 - (start + q0 + 31), hi = k0 + 31 - (start + q0);
-            scores<BIAS>(a, x, window, lo, hi, k0 - (start + q), 1, lh);
-            const int seen = (a.causal ? min(klen, start + q + 1) : klen) - k0;  // rows of the tile that the lane's query sees
-            if (k0 + 32 > klen || (a.causal && hi > 0)) {
-#pragma unroll
-                for (int r = 0; r < 16; r++)
-                    if (row_of(r, lh) >= seen) x[r] = -INFINITY;
-            }
-            float mt = x[0];
-#pragma unroll
-            for (int r = 1; r < 16; r++) mt = fmaxf(mt, x[r]);
-            mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-            const float mn = fmaxf(m, mt);
-            const float base = mn == -INFINITY ? 0.0f : mn;  // -inf - -inf is no number
-            const float c = __builtin_amdgcn_exp2f((m - base) * CA_LOG2E);
-            m = mn;
-            l *= c;
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                x[r] = __builtin_amdgcn_exp2f((x[r] - base) * CA_LOG2E);
-                l += x[r];
-                o[0][r] *= c;
-                o[1][r] *= c;
-            }
-#pragma unroll
-            for (int st = 0; st < 2; st++) {
-                Frag<T> pb;
-                frag_from(pb, x, st);
-#pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const Frag<T> vf = tile_col(Vs, st, t, lane, T());
-                    frag_mfma(o[t], vf, pb);
-                    if constexpr (KEEP && sizeof(T) == 2) {
-                        Frag<T> pr;
-                        frag_rest(pr, pb, x, st);
-                        frag_mfma(o[t], vf, pr);
-                    }
-                }
-            }
+            if constexpr (BIAS) add_bias(a, x, window, lo, hi, k0 - (start + q), 1, lh);
+            softmax_tile<T, BIAS, KEEP>(st, x, Ks + Tile<T>::BYTES, a.scale2, k0 + 32 > klen || (a.causal && hi > 0),
+                                        (a.causal ? min(klen, start + q + 1) : klen) - k0, lane);
         }
-        __syncthreads();
     }
     if (q >= a.Lq) return;
-    l += __shfl_xor(l, 32, 64);
+    const float l = st.l + __shfl_xor(st.l, 32, 64);
     const bool seen = q < qlen && (l > 0.0f || l != l);  // a row of NaN stays one
     const float inv = seen ? 1.0f / l : 0.0f;
     const int64_t row = ((int64_t)s * a.H + h) * a.Lq + q;
-    if (KEEP && lh == 0) a.stats[row] = make_float2(seen ? m : 0.0f, seen ? -log2f(l) : -INFINITY);
+    if (KEEP && lh == 0) a.stats[row] = row_stats(BIAS, seen, st.mc, l);
     T *op = reinterpret_cast<T *>(a.out.p + s * a.out.seq + (int64_t)q * a.out.row + h * a.out.head);
 #pragma unroll
     for (int t = 0; t < 2; t++)
 #pragma unroll
         for (int rq = 0; rq < 4; rq++) {
-            const int d = 32 * t + 8 * rq + 4 * lh;
             floatx4 y;
 #pragma unroll
-            for (int r = 0; r < 4; r++) y[r] = seen ? o[t][4 * rq + r] * inv : 0.0f;
-            st4(op + d, y);
-            if constexpr (KEEP && sizeof(T) == 2) {
-                const bf16x4 yr = to_bf16x4(y);
-#pragma unroll
-                for (int r = 0; r < 4; r++) y[r] -= (float)yr[r];
-                st4(a.rest + row * CA_D + d, y);
-            }
+            for (int r = 0; r < 4; r++) y[r] = seen ? st.o[t][4 * rq + r] * inv : 0.0f;
+            store_out<T, BIAS, KEEP>(a, op, row, 32 * t + 8 * rq + 4 * lh, y);
         }
 }
 
+// The same where that makes too few workgroups: 4 waves take the same 32 rows
+// and every fourth tile of keys, each in tiles of its own, so that no wave waits
+// for another before the end; a.parts workgroups share a row tile's keys.  PACK:
+// a tile's rows are the queries' heads that share the key head, head by head
+// within a query, so that single tokens of shared heads fill it.
+template <typename T, int B = sizeof(T) == 2 ? 2 : 1>  // fp32's matrix instructions outlast a tile's copy
+struct SplitLds {
+    static constexpr int BUFS = B;
+    static constexpr int WAVE = BUFS * 2 * Tile<T>::BYTES;
+    static constexpr int PITCH = CA_D + 4;
+    static constexpr int RESULTS = 4 * 32 * PITCH * 4 + 4 * 32 * 8;  // the waves' [32][CA_D] and (m, l), over the tiles
+    static constexpr int BYTES = 4 * WAVE > RESULTS ? 4 * WAVE : RESULTS;
+};
+
+// A wave's own tiles [first, last) of keys (or queries), every fourth one from
+// its own number on: issue(tile, buffer) starts the copies, LOADS of them, use(tile,
+// buffer) works on them.
+template <int BUFS, int LOADS, typename Issue, typename Use>
+VH_DEVICE void wave_tiles(int first, int last, Issue issue, Use use) {
+    if constexpr (BUFS == 2) {
+        int buf = 0;
+        if (first < last) issue(first, 0);
+        for (int t = first; t < last; t += 4, buf ^= 1) {
+            if (t + 4 < last) {
+                wait_lds();  // the other buffer's reads have returned
+                issue(t + 4, buf ^ 1);
+                wait_vmcnt<LOADS>();
+            } else {
+                wait_vmcnt<0>();
+            }
+            use(t, buf);
+        }
+    } else {
+        for (int t = first; t < last; t += 4) {
+            wait_lds();
+            issue(t, 0);
+            wait_vmcnt<0>();
+            use(t, 0);
+        }
+    }
+}
+
+// The bias where a tile's columns belong to several heads: the bucket by relative
+// position, and the heads' tables.
+struct PackedBias {
+    const unsigned char *bucket;  // as the window of one head
+    const float *table;           // [heads][buckets], times log2(e)
+};
+VH_DEVICE void scores_packed(const CrossArgs &a, floatx16 &x, const PackedBias &pb, int tile_lo, int tile_hi, int rel0,
+                             int head, int lh) {
+    const int md = a.max_distance;
+    const float *table = pb.table + head * a.buckets;
+    if (tile_hi <= -md || tile_lo >= md) {
+        const float b = table[pb.bucket[tile_hi <= -md ? CA_PAD : 2 * md + CA_PAD]];
+#pragma unroll
+        for (int r = 0; r < 16; r++) x[r] = __builtin_fmaf(x[r], a.scale2, b);
+    } else {
+        const unsigned char *w = pb.bucket + rel0 + 4 * lh + md + CA_PAD;
+#pragma unroll
+        for (int r = 0; r < 16; r++) x[r] = __builtin_fmaf(x[r], a.scale2, table[w[row_of(r, 0)]]);
+    }
+}
+
+template <typename T, bool BIAS, bool KEEP, bool PACK>
+__global__ __launch_bounds__(256, 2) void cross_forward_split_kernel(CrossArgs a) {
+    using L = SplitLds<T>;
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+    float *window = reinterpret_cast<float *>(smem + L::BYTES);
+    const int G = a.H / a.KV, per = PACK ? G : 1, HH = a.H / per;
+    const int rtiles = (int)(((int64_t)a.Lq * per + 31) / 32);
+    const int task = xcd_swizzle((int)blockIdx.x, (int)gridDim.x);
+    const int rt = task % rtiles, part = task / rtiles % a.parts;
+    const int hh = task / rtiles / a.parts % HH, s = task / rtiles / a.parts / HH;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int li = lane & 31, lh = lane >> 5;
+    const int kh = PACK ? hh : hh / G;
+    const int start = cross_start(a, s);
+    const int qlen = cross_length(a.query_lengths, s, a.Lq), klen = cross_length(a.key_lengths, s, a.Lk);
+    const int q_lo = 32 * rt / per, q_hi = min((32 * rt + 31) / per, qlen - 1);
+    const int q = (32 * rt + li) / per, head = PACK ? kh * G + (32 * rt + li) % per : hh;
+    const bool active = q_lo < qlen;
+    int keys = active ? klen : 0;
+    if (a.causal) keys = min(keys, start + q_hi + 1);
+    const int tiles = (max(keys, 0) + 31) / 32;
+    const int first = (int)((int64_t)tiles * part / a.parts), last = (int)((int64_t)tiles * (part + 1) / a.parts);
+
+    PackedBias pb{reinterpret_cast<const unsigned char *>(window + per * a.buckets), window};
+    if constexpr (BIAS) {
+        if constexpr (PACK) {
+            for (int i = tid; i < per * a.buckets; i += 256)
+                window[i] = bias_log2(a.table[(int64_t)(i % a.buckets) * a.H + kh * G + i / a.buckets]);
+            fill_bucket_window(a, const_cast<unsigned char *>(pb.bucket), tid);
+        } else {
+            fill_bias_window(a, hh, window, tid);
+        }
+        __syncthreads();
+    }
+    Frag<T> qf[4];
+    if (active) {
+        const char *qp = a.q.p + s * a.q.seq + (int64_t)min(q, qlen - 1) * a.q.row + head * a.q.head;
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            qf[g] = frag_load(reinterpret_cast<const T *>(qp) + 16 * g + 8 * lh);
+            if (a.scale < 0.0f) frag_negate(qf[g]);
+        }
+    }
+    RowState st;
+    st.clear();
+    const char *kp = a.k.p + s * a.k.seq + kh * a.k.head, *vp = a.v.p + s * a.v.seq + kh * a.v.head;
+    unsigned char *tile = smem + wave * L::WAVE;
+    const uint32_t lds = (uint32_t)(uintptr_t)tile;
+    wave_tiles<L::BUFS, 2 * CA_TILE / Tile<T>::DMA_ROWS>(
+        first + wave, last,
+        [&](int t, int buf) {
+            tile_issue<T, 1>(kp, a.k.row, 32 * t, klen - 1, lds + 2 * buf * Tile<T>::BYTES, 0, lane);
+            tile_issue<T, 1>(vp, a.v.row, 32 * t, klen - 1, lds + (2 * buf + 1) * Tile<T>::BYTES, 0, lane);
+        },
+        [&](int t, int buf) {
+            const unsigned char *Ks = tile + 2 * buf * Tile<T>::BYTES, *Vs = Ks + Tile<T>::BYTES;
+            const int k0 = 32 * t;
+            floatx16 x;
+            zero16(x);
+#pragma unroll
+            for (int g = 0; g < 4; g++) frag_mfma(x, tile_row(Ks, li, g, lh, T()), qf[g]);
+            const int lo = k0 - (start + q_hi), hi = k0 + 31 - (start + q_lo);
+            if constexpr (BIAS && PACK) scores_packed(a, x, pb, lo, hi, k0 - (start + q), head - kh * G, lh);
+            else if constexpr (BIAS) add_bias(a, x, window, lo, hi, k0 - (start + q), 1, lh);
+            softmax_tile<T, BIAS, KEEP>(st, x, Vs, a.scale2, k0 + 32 > klen || (a.causal && hi > 0),
+                                        (a.causal ? min(klen, start + q + 1) : klen) - k0, lane);
+        });
+
+    // the four waves' results joined: row tid / 8, dims 8 (tid % 8) .. + 7
+    __syncthreads();
+    float *res = reinterpret_cast<float *>(smem);
+    float2 *ml = reinterpret_cast<float2 *>(res + 4 * 32 * L::PITCH);
+    const float l_wave = st.l + __shfl_xor(st.l, 32, 64);
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int rq = 0; rq < 4; rq++) {
+            floatx4 y;
+#pragma unroll
+            for (int r = 0; r < 4; r++) y[r] = st.o[t][4 * rq + r];
+            st4(res + (wave * 32 + li) * L::PITCH + 32 * t + 8 * rq + 4 * lh, y);
+        }
+    if (lh == 0) ml[wave * 32 + li] = make_float2(st.top(), l_wave);
+    __syncthreads();
+    const int rr = tid >> 3, d = 8 * (tid & 7);
+    const int oq = (32 * rt + rr) / per, oh = PACK ? kh * G + (32 * rt + rr) % per : hh;
+    if (oq >= a.Lq) return;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; w++) m = fmaxf(m, ml[w * 32 + rr].x);
+    const float base = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+    floatx4 y[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        const float2 v = ml[w * 32 + rr];
+        const float c = __builtin_amdgcn_exp2f(v.x - base);
+        l += v.y * c;
+#pragma unroll
+        for (int e = 0; e < 2; e++) y[e] += ld4(res + (w * 32 + rr) * L::PITCH + d + 4 * e) * c;
+    }
+    const int64_t row = ((int64_t)s * a.H + oh) * a.Lq + oq;
+    if (a.parts > 1) {
+        const int64_t at = (int64_t)part * a.S * a.H * a.Lq + row;
+        st4(a.part_o + at * CA_D + d, y[0]);
+        st4(a.part_o + at * CA_D + d + 4, y[1]);
+        if (d == 0) a.part_ml[at] = make_float2(m, l);
+        return;
+    }
+    const bool seen = oq < qlen && (l > 0.0f || l != l);
+    const float inv = seen ? 1.0f / l : 0.0f;
+    if (KEEP && d == 0) a.stats[row] = row_stats(BIAS, seen, m, l);
+    T *op = reinterpret_cast<T *>(a.out.p + s * a.out.seq + (int64_t)oq * a.out.row + oh * a.out.head);
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) y[e][r] = seen ? y[e][r] * inv : 0.0f;
+        store_out<T, BIAS, KEEP>(a, op, row, d + 4 * e, y[e]);
+    }
+}
+
+// The pieces of every row joined: 16 lanes a row, 4 dims each.
+template <typename T, bool BIAS, bool KEEP>
+__global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
+    const int64_t rows = (int64_t)a.S * a.H * a.Lq, row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (row >= rows) return;
+    const int d = 4 * ((int)threadIdx.x & 15);
+    const int q = (int)(row % a.Lq), h = (int)(row / a.Lq % a.H), s = (int)(row / a.Lq / a.H);
+    float m = -INFINITY;
+    for (int p = 0; p < a.parts; p++) m = fmaxf(m, a.part_ml[p * rows + row].x);
+    const float base = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+    floatx4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int p = 0; p < a.parts; p++) {
+        const float2 v = a.part_ml[p * rows + row];
+        const float c = __builtin_amdgcn_exp2f(v.x - base);
+        l += v.y * c;
+        y += ld4(a.part_o + (p * rows + row) * CA_D + d) * c;
+    }
+    const bool seen = q < cross_length(a.query_lengths, s, a.Lq) && (l > 0.0f || l != l);
+    const float inv = seen ? 1.0f / l : 0.0f;
+    if (KEEP && d == 0) a.stats[row] = row_stats(BIAS, seen, m, l);
+#pragma unroll
+    for (int r = 0; r < 4; r++) y[r] = seen ? y[r] * inv : 0.0f;
+    T *op = reinterpret_cast<T *>(a.out.p + s * a.out.seq + (int64_t)q * a.out.row + h * a.out.head);
+    store_out<T, BIAS, KEEP>(a, op, row, d, y);
+}
+
 // ----------------------------------------------------------------- backward
-// dq, delta and the table's gradient: workgroup and tiles as the forward's.
-// dbias: a tile's dS are summed along its 63 diagonals in the wave's own LDS by
-// ds_add_f32, whose lanes take different diagonals (the half-waves have an array
-// each), then each diagonal is added to its bucket's slot of that lane: the order
-// of every sum is fixed.  Tiles wholly beyond max_distance have one bucket and
-// are summed in registers.
+// A query tile's statistics and delta: the dq kernels leave them for the dk and dv
+// ones, which copy a tile's into LDS beside its q and dout.  Rows past the length
+// have no probability.
+struct RowStats {
+    float m[CA_TILE], n[CA_TILE], delta[CA_TILE];  // delta: its negative
+};
+static_assert(sizeof(RowStats) == 24 * 16, "24 lanes copy it");
+VH_DEVICE RowStats *row_tile(const CrossArgs &a, int s, int h, int t) {
+    return reinterpret_cast<RowStats *>(a.rows) + ((int64_t)s * a.H + h) * ((a.Lq + CA_TILE - 1) / CA_TILE) + t;
+}
+
+// Copies a tile's into LDS: 24 lanes of a wave, 16 bytes each.
+VH_DEVICE void row_tile_issue(const RowStats *from, uint32_t lds, int lane) {
+    const uint64_t p = (uint64_t)from;
+    const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32 |
+                          (uint32_t)__builtin_amdgcn_readfirstlane((int)p);
+    lds = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds);
+    if (lane < 24) lds_dma16s(16u * (uint32_t)lane, reinterpret_cast<const void *>(base), lds);
+}
+
+// What a wave's 32 query rows need as columns, besides their tiles.
+template <typename T>
+struct QueryRows {
+    Frag<T> q[4], dout[4];
+    floatx16 delta;  // -delta, dP's product's initial value
+    float m, n;
+};
+// Rows q (clamped into qlen) of head h; their statistics are also left where `leave`.
+template <typename T, bool BIAS>
+VH_DEVICE void load_rows(const CrossArgs &a, QueryRows<T> &w, int s, int h, int q, int qlen, bool leave, int lane) {
+    const int lh = lane >> 5;
+    const int64_t qr = min(q, qlen - 1), row = ((int64_t)s * a.H + h) * a.Lq + qr;
+    const T *qp = reinterpret_cast<const T *>(a.q.p + s * a.q.seq + qr * a.q.row + h * a.q.head);
+    const T *dp = reinterpret_cast<const T *>(a.dout.p + s * a.dout.seq + qr * a.dout.row + h * a.dout.head);
+    const T *op = reinterpret_cast<const T *>(a.out.p + s * a.out.seq + qr * a.out.row + h * a.out.head);
+    float delta = 0.0f;
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+        const int d = 16 * g + 8 * lh;
+        w.q[g] = frag_load(qp + d);
+        if (a.scale < 0.0f) frag_negate(w.q[g]);
+        w.dout[g] = frag_load(dp + d);
+        const Frag<T> of = frag_load(op + d);
+        if constexpr (sizeof(T) == 2) {
+            if constexpr (BIAS) {
+                const Frag<float> rf = frag_load(static_cast<const float *>(a.rest) + row * CA_D + d);
+#pragma unroll
+                for (int e = 0; e < 8; e++) delta += (float)w.dout[g].v[e] * ((float)of.v[e] + rf.v[e >> 2][e & 3]);
+            } else {
+                const Frag<bf16> rf = frag_load(static_cast<const bf16 *>(a.rest) + row * CA_D + d);
+#pragma unroll
+                for (int e = 0; e < 8; e++) delta += (float)w.dout[g].v[e] * ((float)of.v[e] + (float)rf.v[e]);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) delta += w.dout[g].v[e >> 2][e & 3] * of.v[e >> 2][e & 3];
+        }
+    }
+    delta = -(delta + __shfl_xor(delta, 32, 64));
+    float2 st = a.stats[row];
+    if (q >= qlen) {  // no probability
+        st = make_float2(INFINITY, -INFINITY);
+        delta = 0.0f;
+    }
+    w.m = st.x;
+    w.n = st.y;
+#pragma unroll
+    for (int r = 0; r < 16; r++) w.delta[r] = delta;
+    if (leave && lh == 0) {
+        RowStats *to = row_tile(a, s, h, q / CA_TILE);
+        to->m[lane] = st.x;
+        to->n[lane] = st.y;
+        to->delta[lane] = delta;
+    }
+}
+
+// The table's gradient.  A tile's dS are summed along its 63 diagonals: 16 keys at
+// a time, the pair of key i and query j is stored at [i - j + 31][i] of the wave's
+// own array, whose other places stay 0, and lane d adds up the 16 of diagonal d
+// (ds_add_f32 instead, straight into the sums, made the whole kernel 3 times as
+// long).  Each diagonal is then added to its bucket's slot of that lane: the order
+// of every sum is fixed.  Tiles wholly beyond max_distance have one bucket and are
+// summed in registers.
+constexpr int CA_DIAG = 20;  // pitch: 16-byte reads, and stores of 32 lanes in 32 banks
 struct DbiasLds {
-    float diag[4][2][64];
+    float diag[4][48 * CA_DIAG];
     float far[4][2];
 };
+struct Dbias {
+    DbiasLds *db;
+    float *slots;           // [4][buckets][32]
+    unsigned char *bucket;  // by relative position, as the bias window
+    float lo = 0.0f, hi = 0.0f;
+    // behind the tiles: where the gradient is wanted the sums, and the bias window
+    VH_DEVICE void lay(const CrossArgs &a, unsigned char *at, float *&window) {
+        db = reinterpret_cast<DbiasLds *>(at);
+        slots = reinterpret_cast<float *>(db + 1);
+        window = slots + 128 * a.buckets;
+        bucket = reinterpret_cast<unsigned char *>(window + cross_window(a));
+    }
+    VH_DEVICE void clear(const CrossArgs &a, int tid) {
+        for (int i = tid; i < 128 * a.buckets; i += 256) slots[i] = 0.0f;
+        for (int i = tid; i < 4 * 48 * CA_DIAG; i += 256) (&db->diag[0][0])[i] = 0.0f;
+        fill_bucket_window(a, bucket, tid);
+    }
+    // x: dS of a tile whose pairs have the relative positions tile_lo .. tile_hi
+    VH_DEVICE void add(const CrossArgs &a, const floatx16 &x, int tile_lo, int tile_hi, int wave, int lane) {
+        const int md = a.max_distance, li = lane & 31, lh = lane >> 5;
+        if (tile_hi <= -md || tile_lo >= md) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 16; r++) sum += x[r];
+            if (tile_hi <= -md) lo += sum;
+            else hi += sum;
+            return;
+        }
+        float *diag = &db->diag[wave][0];
+        float sum[2];
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            wave_order();
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int i = row_of(e, lh);  // of the 16
+                diag[(i - li + 31) * CA_DIAG + i] = x[8 * g + e];
+            }
+            wave_order();
+            const float *d = diag + min(lane, 46) * CA_DIAG;
+            const floatx4 v = (ld4(d) + ld4(d + 4)) + (ld4(d + 8) + ld4(d + 12));
+            sum[g] = lane < 47 ? (v[0] + v[1]) + (v[2] + v[3]) : 0.0f;
+        }
+        // diagonal d of the tile: d of the first 16 keys, d - 16 of the second
+        const float up = __shfl(sum[1], (lane - 16) & 63, 64);
+        const float v = sum[0] + (lane >= 16 ? up : 0.0f);
+        const float v1 = __shfl(v, (lane & 31) + 32, 64);
+        wave_order();
+        if (lane < 32) {  // the second may be the first one's bucket
+            float *sl = slots + wave * a.buckets * 32 + lane;
+            const unsigned char *bw = bucket + tile_lo + lane + md + CA_PAD;
+            sl[32 * bw[0]] += v;
+            sl[32 * bw[lane < 31 ? 32 : 31]] += v1;  // there are 63: the last lane's is 0
+        }
+        wave_order();
+    }
+    // the workgroup's sums into part `at` of head h
+    VH_DEVICE void finish(const CrossArgs &a, int h, int at, int tid) {
+        const int wave = tid >> 6;
+        lo = wave_sum(lo);
+        hi = wave_sum(hi);
+        __syncthreads();  // cleared, where no tile was worked on
+        if ((tid & 63) == 0) {
+            db->far[wave][0] = lo;
+            db->far[wave][1] = hi;
+        }
+        __syncthreads();
+        for (int b = tid; b < a.buckets; b += 256) {
+            float sum = 0.0f;
+            for (int w = 0; w < 4; w++) {
+                for (int i = 0; i < 32; i++) sum += slots[(w * a.buckets + b) * 32 + (i + b) % 32];
+                if (b == cross_bucket(a, -a.max_distance)) sum += db->far[w][0];
+                if (b == cross_bucket(a, a.max_distance)) sum += db->far[w][1];
+            }
+            a.dbias_part[((int64_t)h * a.dbias_parts + at) * a.buckets + b] = sum;
+        }
+    }
+};
+
+// One tile of keys: dq^T += K^T dS^T, and the table's gradient.
+template <typename T, bool BIAS>
+VH_DEVICE void dq_tile(const CrossArgs &a, const QueryRows<T> &w, floatx16 (&acc)[2], Dbias &db, const float *window,
+                       const unsigned char *Ks, const unsigned char *Vs, int k0, int pos, int pos_lo, int klen, int wave,
+                       int lane) {
+    const int li = lane & 31, lh = lane >> 5;
+    floatx16 x, dp = w.delta;
+    zero16(x);
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+        frag_mfma(x, tile_row(Ks, li, g, lh, T()), w.q[g]);
+        frag_mfma(dp, tile_row(Vs, li, g, lh, T()), w.dout[g]);
+    }
+    const int lo = k0 - (pos_lo + 31), hi = k0 + 31 - pos_lo;
+    const int seen = (a.causal ? min(klen, pos + 1) : klen) - k0;  // rows of the tile that the lane's query sees
+    const bool mask = k0 + 32 > klen || (a.causal && hi > 0);
+    if constexpr (BIAS) add_bias(a, x, window, lo, hi, k0 - pos, 1, lh);
+#pragma unroll
+    for (int r = 0; r < 16; r++)
+        x[r] = __builtin_amdgcn_exp2f(BIAS ? (x[r] - w.m) + w.n : __builtin_fmaf(x[r], a.scale2, -w.m)) * dp[r];
+    if (mask) {
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+            if (row_of(r, lh) >= seen) x[r] = 0.0f;
+    }
+    if constexpr (BIAS) {
+        if (a.dbias_part) db.add(a, x, lo, hi, wave, lane);
+    }
+#pragma unroll
+    for (int g = 0; g < 2; g++) {
+        Frag<T> sb;
+        frag_from(sb, x, g);
+#pragma unroll
+        for (int t = 0; t < 2; t++) frag_mfma(acc[t], tile_col(Ks, g, t, lane, T()), sb);
+    }
+}
+
+// dq, delta and the table's gradient: workgroup and tiles as the forward's.
 template <typename T, bool BIAS>
 __global__ __launch_bounds__(256, 2) void cross_dq_kernel(CrossArgs a) {
-    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-    unsigned char *Ks = smem, *Vs = smem + Tile<T>::BYTES;
-    DbiasLds *db = reinterpret_cast<DbiasLds *>(smem + 2 * Tile<T>::BYTES);
-    float *slots = reinterpret_cast<float *>(db + 1);  // [4][buckets][32]
-    float *window = slots + 128 * a.buckets;
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];  // [2] K and V tiles
+    float *window;
+    Dbias db;
+    db.lay(a, smem + 4 * Tile<T>::BYTES, window);
 
     const int qtiles = (a.Lq + 127) / 128;
     const int task = xcd_swizzle((int)blockIdx.x, (int)gridDim.x);
@@ -400,132 +885,35 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(CrossArgs a) {
     int keys = klen;
     if (a.causal) keys = min(keys, start + min(128 * qt + 128, qlen));
     if (128 * qt >= qlen) keys = 0;
-    const bool with_dbias = BIAS && a.dbias_part != nullptr;
 
-    if constexpr (BIAS) {
+    const char *kp = a.k.p + s * a.k.seq + kh * a.k.head, *vp = a.v.p + s * a.v.seq + kh * a.v.head;
+    const uint32_t lds = (uint32_t)(uintptr_t)smem;
+    auto issue = [&](int k0) {
+        const uint32_t at = lds + (uint32_t)(k0 / CA_TILE & 1) * 2 * Tile<T>::BYTES;
+        tile_issue<T, 4>(kp, a.k.row, k0, klen - 1, at, wave, lane);
+        tile_issue<T, 4>(vp, a.v.row, k0, klen - 1, at + Tile<T>::BYTES, wave, lane);
+    };
+    if (keys > 0) issue(0);
+    if constexpr (BIAS) {  // read after the loop's first barrier
         fill_bias_window(a, h, window, tid);
-        if (with_dbias) {
-            for (int i = tid; i < 128 * a.buckets; i += 256) slots[i] = 0.0f;
-            for (int i = tid; i < 4 * 2 * 64; i += 256) (&db->diag[0][0][0])[i] = 0.0f;
-        }
-        __syncthreads();
+        if (a.dbias_part) db.clear(a, tid);
     }
-    Frag<T> qf[4], df[4];
-    float delta = 0.0f, m = 0.0f, nl = -INFINITY;
-    const int64_t row = ((int64_t)s * a.H + h) * a.Lq + min(q, qlen - 1);
-    if (active) {
-        const int64_t qr = min(q, qlen - 1);
-        const T *qp = reinterpret_cast<const T *>(a.q.p + s * a.q.seq + qr * a.q.row + h * a.q.head);
-        const T *dp = reinterpret_cast<const T *>(a.dout.p + s * a.dout.seq + qr * a.dout.row + h * a.dout.head);
-        const T *op = reinterpret_cast<const T *>(a.out.p + s * a.out.seq + qr * a.out.row + h * a.out.head);
-#pragma unroll
-        for (int g = 0; g < 4; g++) {
-            const int d = 16 * g + 8 * lh;
-            qf[g] = frag_load(qp + d);
-            df[g] = frag_load(dp + d);
-            const Frag<T> of = frag_load(op + d);
-            if constexpr (sizeof(T) == 2) {
-                const Frag<T> rf = frag_load(a.rest + row * CA_D + d);
-#pragma unroll
-                for (int e = 0; e < 8; e++) delta += (float)df[g].v[e] * ((float)of.v[e] + (float)rf.v[e]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; e++) delta += df[g].v[e >> 2][e & 3] * of.v[e >> 2][e & 3];
-            }
-        }
-        delta += __shfl_xor(delta, 32, 64);
-        const float2 st = a.stats[row];
-        m = st.x;
-        nl = st.y;
-        if (lh == 0 && q < qlen) a.delta[row] = delta;
-    }
+    QueryRows<T> w;
+    if (active) load_rows<T, BIAS>(a, w, s, h, q, qlen, true, lane);
     floatx16 acc[2];
     zero16(acc[0]);
     zero16(acc[1]);
-    float far_lo = 0.0f, far_hi = 0.0f;
-    const char *kp = a.k.p + s * a.k.seq + kh * a.k.head, *vp = a.v.p + s * a.v.seq + kh * a.v.head;
-    const uint32_t k_lds = (uint32_t)(uintptr_t)Ks, v_lds = (uint32_t)(uintptr_t)Vs;
     for (int k0 = 0; k0 < keys; k0 += CA_TILE) {
-        tile_issue<T>(kp, a.k.row, k0, klen - 1, k_lds, wave, lane);
-        tile_issue<T>(vp, a.v.row, k0, klen - 1, v_lds, wave, lane);
         wait_vmcnt<0>();
         __syncthreads();
+        if (k0 + CA_TILE < keys) issue(k0 + CA_TILE);
         if (active && (!a.causal || k0 <= start + q0 + 31)) {
-            floatx16 x, dp;
-            zero16(x);
-            zero16(dp);
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-                frag_mfma(x, tile_row(Ks, li, g, lh, T()), qf[g]);
-                frag_mfma(dp, tile_row(Vs, li, g, lh, T()), df[g]);
-            }
-            const int lo = k0 - (start + q0 + 31), hi = k0 + 31 - (start + q0);
-            scores<BIAS>(a, x, window, lo, hi, k0 - (start + q), 1, lh);
-            int seen = (a.causal ? min(klen, start + q + 1) : klen) - k0;
-            if (q >= qlen) seen = 0;
-#pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r] - m, CA_LOG2E, nl));
-                x[r] = row_of(r, lh) < seen ? p * (dp[r] - delta) : 0.0f;
-            }
-            if constexpr (BIAS) {
-                if (with_dbias) {
-                    const int md = a.max_distance;
-                    if (hi <= -md || lo >= md) {
-                        float sum = 0.0f;
-#pragma unroll
-                        for (int r = 0; r < 16; r++) sum += x[r];
-                        if (hi <= -md) far_lo += sum;
-                        else far_hi += sum;
-                    } else {
-                        float *w = &db->diag[wave][lh][31 - li + 4 * lh];
-#pragma unroll
-                        for (int r = 0; r < 16; r++)
-                            __hip_atomic_fetch_add(w + row_of(r, 0), x[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
-                        wave_order();
-                        float *d = &db->diag[wave][0][lane];
-                        const float v = d[0] + d[64];
-                        d[0] = 0.0f;
-                        d[64] = 0.0f;
-                        const float v1 = __shfl(v, (lane & 31) + 32, 64);
-                        if (lane < 32) {  // the second may be the first one's bucket
-                            float *sl = slots + wave * a.buckets * 32 + lane;
-                            sl[32 * cross_bucket(a, lo + lane)] += v;
-                            sl[32 * cross_bucket(a, lo + lane + 32)] += v1;
-                        }
-                        wave_order();
-                    }
-                }
-            }
-#pragma unroll
-            for (int st = 0; st < 2; st++) {
-                Frag<T> sb;
-                frag_from(sb, x, st);
-#pragma unroll
-                for (int t = 0; t < 2; t++) frag_mfma(acc[t], tile_col(Ks, st, t, lane, T()), sb);
-            }
+            const unsigned char *Ks = smem + (k0 / CA_TILE & 1) * 2 * Tile<T>::BYTES;
+            dq_tile<T, BIAS>(a, w, acc, db, window, Ks, Ks + Tile<T>::BYTES, k0, start + q, start + q0, klen, wave, lane);
         }
-        __syncthreads();
     }
     if constexpr (BIAS) {
-        if (with_dbias) {
-            far_lo = wave_sum(far_lo);
-            far_hi = wave_sum(far_hi);
-            if (lane == 0) {
-                db->far[wave][0] = far_lo;
-                db->far[wave][1] = far_hi;
-            }
-            __syncthreads();
-            for (int b = tid; b < a.buckets; b += 256) {
-                float sum = 0.0f;
-                for (int w = 0; w < 4; w++) {
-                    for (int i = 0; i < 32; i++) sum += slots[(w * a.buckets + b) * 32 + (i + b) % 32];
-                    if (b == cross_bucket(a, -a.max_distance)) sum += db->far[w][0];
-                    if (b == cross_bucket(a, a.max_distance)) sum += db->far[w][1];
-                }
-                a.dbias_part[(((int64_t)s * a.H + h) * qtiles + qt) * a.buckets + b] = sum;
-            }
-        }
+        if (a.dbias_part) db.finish(a, h, s * qtiles + qt, tid);
     }
     if (q >= a.Lq) return;
     T *out = reinterpret_cast<T *>(a.dq.p + s * a.dq.seq + (int64_t)q * a.dq.row + h * a.dq.head);
@@ -540,18 +928,175 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(CrossArgs a) {
         }
 }
 
-// dk and dv: workgroup of 4 waves x 32 keys of one key head, tiles of 32 queries
-// of every query head that shares it.  S = Q K^T with the keys as columns, so
-// that P and dS are B operands of dv^T += dout^T P and dk^T += Q^T dS as they are.
-struct RowStats {
-    float m[CA_TILE], nl[CA_TILE], delta[CA_TILE];
+// A wave's column of 32 x 64 sums added over the workgroup's four waves: thread
+// tid gets dims 8 (tid % 8) .. + 7 of row tid / 8.
+template <typename T>
+VH_DEVICE void waves_sum(float *res, const floatx16 (&acc)[2], int tid, floatx4 (&y)[2]) {
+    using L = SplitLds<T>;
+    const int lane = tid & 63, li = lane & 31, lh = lane >> 5, wave = tid >> 6;
+    __syncthreads();  // what lay there has been read
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int rq = 0; rq < 4; rq++) {
+            floatx4 v;
+#pragma unroll
+            for (int r = 0; r < 4; r++) v[r] = acc[t][4 * rq + r];
+            st4(res + (wave * 32 + li) * L::PITCH + 32 * t + 8 * rq + 4 * lh, v);
+        }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        const float *p = res + (tid >> 3) * L::PITCH + 8 * (tid & 7) + 4 * e;
+        y[e] = (ld4(p) + ld4(p + 32 * L::PITCH)) + (ld4(p + 64 * L::PITCH) + ld4(p + 96 * L::PITCH));
+    }
+}
+
+// The same in too few workgroups: as cross_forward_split_kernel.  With a bias one
+// buffer a wave, so that three workgroups with their sums' slots share a CU's LDS.
+template <typename T, bool BIAS>
+using DqLds = SplitLds<T, BIAS ? 1 : SplitLds<T>::BUFS>;
+template <typename T, bool BIAS>
+__global__ __launch_bounds__(256, 2) void cross_dq_split_kernel(CrossArgs a) {
+    using L = DqLds<T, BIAS>;
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+    float *window;
+    Dbias db;
+    db.lay(a, smem + L::BYTES, window);
+
+    const int rtiles = (a.Lq + 31) / 32;
+    const int task = xcd_swizzle((int)blockIdx.x, (int)gridDim.x);
+    const int rt = task % rtiles, part = task / rtiles % a.parts;
+    const int h = task / rtiles / a.parts % a.H, s = task / rtiles / a.parts / a.H;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int kh = h / (a.H / a.KV);
+    const int start = cross_start(a, s);
+    const int qlen = cross_length(a.query_lengths, s, a.Lq), klen = cross_length(a.key_lengths, s, a.Lk);
+    const int q0 = 32 * rt, q = q0 + (lane & 31);
+    int keys = q0 < qlen ? klen : 0;
+    if (a.causal) keys = min(keys, start + min(q0 + 32, qlen));
+    const int tiles = (max(keys, 0) + 31) / 32;
+    const int first = (int)((int64_t)tiles * part / a.parts), last = (int)((int64_t)tiles * (part + 1) / a.parts);
+
+    if constexpr (BIAS) {
+        fill_bias_window(a, h, window, tid);
+        if (a.dbias_part) db.clear(a, tid);
+        __syncthreads();
+    }
+    QueryRows<T> w;
+    if (q0 < qlen) load_rows<T, BIAS>(a, w, s, h, q, qlen, part == 0 && wave == 0, lane);
+    floatx16 acc[2];
+    zero16(acc[0]);
+    zero16(acc[1]);
+    const char *kp = a.k.p + s * a.k.seq + kh * a.k.head, *vp = a.v.p + s * a.v.seq + kh * a.v.head;
+    unsigned char *tile = smem + wave * L::WAVE;
+    const uint32_t lds = (uint32_t)(uintptr_t)tile;
+    wave_tiles<L::BUFS, 2 * CA_TILE / Tile<T>::DMA_ROWS>(
+        first + wave, last,
+        [&](int t, int buf) {
+            tile_issue<T, 1>(kp, a.k.row, 32 * t, klen - 1, lds + 2 * buf * Tile<T>::BYTES, 0, lane);
+            tile_issue<T, 1>(vp, a.v.row, 32 * t, klen - 1, lds + (2 * buf + 1) * Tile<T>::BYTES, 0, lane);
+        },
+        [&](int t, int buf) {
+            const unsigned char *Ks = tile + 2 * buf * Tile<T>::BYTES;
+            dq_tile<T, BIAS>(a, w, acc, db, window, Ks, Ks + Tile<T>::BYTES, 32 * t, start + q, start + q0, klen, wave,
+                             lane);
+        });
+    if constexpr (BIAS) {
+        if (a.dbias_part) db.finish(a, h, (s * rtiles + rt) * a.parts + part, tid);
+    }
+    floatx4 y[2];
+    waves_sum<T>(reinterpret_cast<float *>(smem), acc, tid, y);
+    const int oq = q0 + (tid >> 3), d = 8 * (tid & 7);
+    if (oq >= a.Lq) return;
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) y[e][r] = oq < qlen ? y[e][r] * a.scale : 0.0f;
+    if (a.parts > 1) {
+        float *p = a.part_o + (((int64_t)part * a.S * a.H + (int64_t)s * a.H + h) * a.Lq + oq) * CA_D + d;
+        st4(p, y[0]);
+        st4(p + 4, y[1]);
+        return;
+    }
+    T *out = reinterpret_cast<T *>(a.dq.p + s * a.dq.seq + (int64_t)oq * a.dq.row + h * a.dq.head) + d;
+    st4(out, y[0]);
+    st4(out + 4, y[1]);
+}
+
+// A wave's 32 keys as columns, and their gradients' sums.
+template <typename T>
+struct KeyRows {
+    Frag<T> k[4], v[4];
+    floatx16 dk[2], dv[2];
 };
+template <typename T>
+VH_DEVICE void load_keys(const CrossArgs &a, KeyRows<T> &w, int s, int kh, int key, int klen, int lh) {
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        zero16(w.dk[t]);
+        zero16(w.dv[t]);
+    }
+    if (klen <= 0) return;
+    const int64_t kr = min(key, klen - 1);
+    const T *kp = reinterpret_cast<const T *>(a.k.p + s * a.k.seq + kr * a.k.row + kh * a.k.head);
+    const T *vp = reinterpret_cast<const T *>(a.v.p + s * a.v.seq + kr * a.v.row + kh * a.v.head);
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+        w.k[g] = frag_load(kp + 16 * g + 8 * lh);
+        if (a.scale < 0.0f) frag_negate(w.k[g]);
+        w.v[g] = frag_load(vp + 16 * g + 8 * lh);
+    }
+}
+// One tile of queries: S = Q K^T with the keys as columns, so that P and dS are B
+// operands of dv^T += dout^T P and dk^T += Q^T dS as they are.
+template <typename T, bool BIAS>
+VH_DEVICE void dkv_tile(const CrossArgs &a, KeyRows<T> &w, const float *window, const unsigned char *Qs,
+                        const unsigned char *Ds, const RowStats *rs, int q0, int start, int key, int k0, int lane) {
+    const int li = lane & 31, lh = lane >> 5;
+    floatx16 x, dp;
+    zero16(x);
+#pragma unroll
+    for (int r = 0; r < 16; r++) dp[r] = rs->delta[row_of(r, lh)];
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+        frag_mfma(x, tile_row(Qs, li, g, lh, T()), w.k[g]);
+        frag_mfma(dp, tile_row(Ds, li, g, lh, T()), w.v[g]);
+    }
+    const int lo = k0 - (start + q0 + 31), hi = k0 + 31 - (start + q0);
+    if constexpr (BIAS) add_bias(a, x, window, lo, hi, key - (start + q0), -1, lh);
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+        const int i = row_of(r, lh);
+        x[r] = __builtin_amdgcn_exp2f(BIAS ? (x[r] - rs->m[i]) + rs->n[i] : __builtin_fmaf(x[r], a.scale2, -rs->m[i]));
+        dp[r] *= x[r];
+    }
+    if (a.causal && hi > 0) {
+        const int hidden = key - start - q0;  // rows below it come before the lane's key
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+            if (row_of(r, lh) < hidden) x[r] = dp[r] = 0.0f;
+    }
+#pragma unroll
+    for (int g = 0; g < 2; g++) {
+        Frag<T> pb, sb;
+        frag_from(pb, x, g);
+        frag_from(sb, dp, g);
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            frag_mfma(w.dv[t], tile_col(Ds, g, t, lane, T()), pb);
+            frag_mfma(w.dk[t], tile_col(Qs, g, t, lane, T()), sb);
+        }
+    }
+}
+
+// dk and dv: workgroup of 4 waves x 32 keys of one key head, tiles of 32 queries
+// of every query head that shares it.
 template <typename T, bool BIAS>
 __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(CrossArgs a) {
-    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-    unsigned char *Qs = smem, *Ds = smem + Tile<T>::BYTES;
-    RowStats *rs = reinterpret_cast<RowStats *>(smem + 2 * Tile<T>::BYTES);
-    float *window = reinterpret_cast<float *>(rs + 1);
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];  // [2] Q and dout tiles
+    RowStats *rs = reinterpret_cast<RowStats *>(smem + 4 * Tile<T>::BYTES);  // [2]
+    float *window = reinterpret_cast<float *>(rs + 2);                       // [2]: of two heads in turn
 
     const int ktiles = (a.Lk + 127) / 128;
     const int task = xcd_swizzle((int)blockIdx.x, (int)gridDim.x);
@@ -567,78 +1112,31 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(CrossArgs a) {
     if (a.causal) first = max(0, min(128 * kt - start, qlen)) / CA_TILE * CA_TILE;
     if (128 * kt >= klen) first = qlen;
 
-    Frag<T> kf[4], vf[4];
-    if (active) {
-        const int64_t kr = min(key, klen - 1);
-        const T *kp = reinterpret_cast<const T *>(a.k.p + s * a.k.seq + kr * a.k.row + kh * a.k.head);
-        const T *vp = reinterpret_cast<const T *>(a.v.p + s * a.v.seq + kr * a.v.row + kh * a.v.head);
-#pragma unroll
-        for (int g = 0; g < 4; g++) {
-            kf[g] = frag_load(kp + 16 * g + 8 * lh);
-            vf[g] = frag_load(vp + 16 * g + 8 * lh);
-        }
-    }
-    floatx16 dk[2], dv[2];
-#pragma unroll
-    for (int t = 0; t < 2; t++) {
-        zero16(dk[t]);
-        zero16(dv[t]);
-    }
-    const uint32_t q_lds = (uint32_t)(uintptr_t)Qs, d_lds = (uint32_t)(uintptr_t)Ds;
+    const uint32_t lds = (uint32_t)(uintptr_t)smem, rs_lds = (uint32_t)(uintptr_t)rs;
     const int G = a.H / a.KV;
-    for (int h = kh * G; h < kh * G + G; h++) {
-        const char *qp = a.q.p + s * a.q.seq + h * a.q.head, *dp_ = a.dout.p + s * a.dout.seq + h * a.dout.head;
-        const int64_t row = ((int64_t)s * a.H + h) * a.Lq;
-        if constexpr (BIAS) {
-            __syncthreads();  // the last head's window has been read
-            fill_bias_window(a, h, window, tid);
-        }
-        for (int q0 = first; q0 < qlen; q0 += CA_TILE) {
-            tile_issue<T>(qp, a.q.row, q0, qlen - 1, q_lds, wave, lane);
-            tile_issue<T>(dp_, a.dout.row, q0, qlen - 1, d_lds, wave, lane);
-            if (tid < CA_TILE) {
-                const int q = min(q0 + tid, qlen - 1);
-                const float2 st = a.stats[row + q];
-                rs->m[tid] = st.x;
-                rs->nl[tid] = q0 + tid < qlen ? st.y : -INFINITY;
-                rs->delta[tid] = a.delta[row + q];
-            }
+    auto issue = [&](int h, int q0, int buf) {
+        const char *qp = a.q.p + s * a.q.seq + h * a.q.head, *dp = a.dout.p + s * a.dout.seq + h * a.dout.head;
+        const uint32_t at = lds + (uint32_t)buf * 2 * Tile<T>::BYTES;
+        tile_issue<T, 4>(qp, a.q.row, q0, qlen - 1, at, wave, lane);
+        tile_issue<T, 4>(dp, a.dout.row, q0, qlen - 1, at + Tile<T>::BYTES, wave, lane);
+        if (wave == 0) row_tile_issue(row_tile(a, s, h, q0 / CA_TILE), rs_lds + (uint32_t)buf * sizeof(RowStats), lane);
+    };
+    if (first < qlen) issue(kh * G, first, 0);
+    KeyRows<T> w;
+    load_keys(a, w, s, kh, key, klen, lh);
+    int buf = 0;
+    for (int g = 0; g < G; g++) {
+        // the window before last is free: its head's tiles ended a barrier ago
+        float *bias = window + (g & 1) * (BIAS ? cross_window(a) : 0);
+        if constexpr (BIAS) fill_bias_window(a, kh * G + g, bias, tid);
+        for (int q0 = first; q0 < qlen; q0 += CA_TILE, buf ^= 1) {
             wait_vmcnt<0>();
             __syncthreads();
-            if (active && (!a.causal || k0 <= start + q0 + 31)) {
-                floatx16 x, dp;
-                zero16(x);
-                zero16(dp);
-#pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    frag_mfma(x, tile_row(Qs, li, g, lh, T()), kf[g]);
-                    frag_mfma(dp, tile_row(Ds, li, g, lh, T()), vf[g]);
-                }
-                const int lo = k0 - (start + q0 + 31), hi = k0 + 31 - (start + q0);
-                scores<BIAS>(a, x, window, lo, hi, key - (start + q0), -1, lh);
-                // rows below `hidden` come before the lane's key
-                const int hidden = a.causal ? key - start - q0 : -1;
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int i = row_of(r, lh);
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[r] - rs->m[i], CA_LOG2E, rs->nl[i]));
-                    const bool vis = i >= hidden && q0 + i < qlen;
-                    x[r] = vis ? p : 0.0f;
-                    dp[r] = vis ? p * (dp[r] - rs->delta[i]) : 0.0f;
-                }
-#pragma unroll
-                for (int st = 0; st < 2; st++) {
-                    Frag<T> pb, sb;
-                    frag_from(pb, x, st);
-                    frag_from(sb, dp, st);
-#pragma unroll
-                    for (int t = 0; t < 2; t++) {
-                        frag_mfma(dv[t], tile_col(Ds, st, t, lane, T()), pb);
-                        frag_mfma(dk[t], tile_col(Qs, st, t, lane, T()), sb);
-                    }
-                }
-            }
-            __syncthreads();
+            if (q0 + CA_TILE < qlen) issue(kh * G + g, q0 + CA_TILE, buf ^ 1);
+            else if (g + 1 < G) issue(kh * G + g + 1, first, buf ^ 1);
+            const unsigned char *Qs = smem + buf * 2 * Tile<T>::BYTES;
+            if (active && (!a.causal || k0 <= start + q0 + 31))
+                dkv_tile<T, BIAS>(a, w, bias, Qs, Qs + Tile<T>::BYTES, rs + buf, q0, start, key, k0, lane);
         }
     }
     if (key >= a.Lk) return;
@@ -651,22 +1149,129 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(CrossArgs a) {
             floatx4 y, z;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                y[r] = key < klen ? dk[t][4 * rq + r] * a.scale : 0.0f;
-                z[r] = key < klen ? dv[t][4 * rq + r] : 0.0f;
+                y[r] = key < klen ? w.dk[t][4 * rq + r] * a.scale : 0.0f;
+                z[r] = key < klen ? w.dv[t][4 * rq + r] : 0.0f;
             }
             st4(pk + 32 * t + 8 * rq + 4 * lh, y);
             st4(pv + 32 * t + 8 * rq + 4 * lh, z);
         }
 }
 
-// dtable[b][h]: the workgroups' sums in the order of sequences and query tiles.
-static __global__ __launch_bounds__(128) void cross_dbias_kernel(CrossArgs a) {
-    const int h = (int)blockIdx.x, b = (int)threadIdx.x;
-    if (b >= a.buckets) return;
-    const int qtiles = (a.Lq + 127) / 128;
+// The same in too few workgroups: 4 waves take the same 32 keys and every fourth
+// tile of one head's queries; the heads that share the keys, and a.kv_parts pieces
+// of their queries, are workgroups of their own.
+template <typename T, bool BIAS>
+__global__ __launch_bounds__(256, 2) void cross_dkv_split_kernel(CrossArgs a) {
+    using L = SplitLds<T>;
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+    RowStats *stats = reinterpret_cast<RowStats *>(smem + L::BYTES);  // [4][BUFS]
+    float *window = reinterpret_cast<float *>(stats + 4 * L::BUFS);
+
+    const int ktiles = (a.Lk + 31) / 32, G = a.H / a.KV;
+    const int task = xcd_swizzle((int)blockIdx.x, (int)gridDim.x);
+    const int kt = task % ktiles, part = task / ktiles % a.kv_parts;
+    const int h = task / ktiles / a.kv_parts % a.H, s = task / ktiles / a.kv_parts / a.H;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lh = lane >> 5, kh = h / G;
+    const int start = cross_start(a, s);
+    const int qlen = cross_length(a.query_lengths, s, a.Lq), klen = cross_length(a.key_lengths, s, a.Lk);
+    const int k0 = 32 * kt, key = k0 + (lane & 31);
+    int begin = 0, tiles = k0 < klen ? (qlen + 31) / 32 : 0;
+    if (a.causal) begin = min(tiles, max(0, min(k0 - start, qlen)) / 32);
+    const int first = begin + (int)((int64_t)(tiles - begin) * part / a.kv_parts);
+    const int last = begin + (int)((int64_t)(tiles - begin) * (part + 1) / a.kv_parts);
+
+    if constexpr (BIAS) {
+        fill_bias_window(a, h, window, tid);
+        __syncthreads();
+    }
+    KeyRows<T> w;
+    load_keys(a, w, s, kh, key, klen, lh);
+    const char *qp = a.q.p + s * a.q.seq + h * a.q.head, *dp = a.dout.p + s * a.dout.seq + h * a.dout.head;
+    unsigned char *tile = smem + wave * L::WAVE;
+    const uint32_t lds = (uint32_t)(uintptr_t)tile;
+    RowStats *rs = stats + wave * L::BUFS;
+    wave_tiles<L::BUFS, 2 * CA_TILE / Tile<T>::DMA_ROWS + 1>(
+        first + wave, last,
+        [&](int t, int buf) {
+            tile_issue<T, 1>(qp, a.q.row, 32 * t, qlen - 1, lds + 2 * buf * Tile<T>::BYTES, 0, lane);
+            tile_issue<T, 1>(dp, a.dout.row, 32 * t, qlen - 1, lds + (2 * buf + 1) * Tile<T>::BYTES, 0, lane);
+            row_tile_issue(row_tile(a, s, h, t), (uint32_t)(uintptr_t)(rs + buf), lane);
+        },
+        [&](int t, int buf) {
+            const unsigned char *Qs = tile + 2 * buf * Tile<T>::BYTES;
+            dkv_tile<T, BIAS>(a, w, window, Qs, Qs + Tile<T>::BYTES, rs + buf, 32 * t, start, key, k0, lane);
+        });
+    floatx4 y[2], z[2];
+    waves_sum<T>(reinterpret_cast<float *>(smem), w.dk, tid, y);
+    waves_sum<T>(reinterpret_cast<float *>(smem), w.dv, tid, z);
+    const int ok = k0 + (tid >> 3), d = 8 * (tid & 7);
+    if (ok >= a.Lk) return;
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            y[e][r] = ok < klen ? y[e][r] * a.scale : 0.0f;
+            z[e][r] = ok < klen ? z[e][r] : 0.0f;
+        }
+    if (G * a.kv_parts > 1) {
+        const int64_t at = ((((int64_t)(h % G) * a.kv_parts + part) * a.S + s) * a.KV + kh) * a.Lk + ok;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            st4(a.part_dk + at * CA_D + d + 4 * e, y[e]);
+            st4(a.part_dv + at * CA_D + d + 4 * e, z[e]);
+        }
+        return;
+    }
+    T *pk = reinterpret_cast<T *>(a.dk.p + s * a.dk.seq + (int64_t)ok * a.dk.row + kh * a.dk.head) + d;
+    T *pv = reinterpret_cast<T *>(a.dv.p + s * a.dv.seq + (int64_t)ok * a.dv.row + kh * a.dv.head) + d;
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        st4(pk + 4 * e, y[e]);
+        st4(pv + 4 * e, z[e]);
+    }
+}
+
+// The pieces added up, in their order: workgroups of 16 rows of dq, then of dk and
+// of dv, then one for each head's bias.
+struct FinishArgs {
+    int64_t dq, dkv;  // workgroups of dq; of dk (and as many of dv)
+};
+template <typename T>
+VH_DEVICE void sum_parts(const float *part, int parts, int64_t rows, int64_t row, int len, int heads,
+                         const CrossTensor &to) {
+    if (row >= rows) return;
+    const int d = 4 * ((int)threadIdx.x & 15);
+    floatx4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int p = 0; p < parts; p++) y += ld4(part + (p * rows + row) * CA_D + d);
+    const int64_t i = row % len, h = row / len % heads, s = row / len / heads;
+    st4(reinterpret_cast<T *>(to.p + s * to.seq + i * to.row + h * to.head) + d, y);
+}
+template <typename T>
+__global__ __launch_bounds__(256) void cross_finish_kernel(CrossArgs a, FinishArgs f) {
+    __shared__ float sums[256];
+    int64_t block = blockIdx.x;
+    const int tid = (int)threadIdx.x, sub = tid >> 4;
+    if (block < f.dq) {
+        sum_parts<T>(a.part_o, a.parts, (int64_t)a.S * a.H * a.Lq, block * 16 + sub, a.Lq, a.H, a.dq);
+        return;
+    }
+    block -= f.dq;
+    if (block < 2 * f.dkv) {
+        const bool v = block >= f.dkv;
+        sum_parts<T>(v ? a.part_dv : a.part_dk, a.H / a.KV * a.kv_parts, (int64_t)a.S * a.KV * a.Lk,
+                     (block - (v ? f.dkv : 0)) * 16 + sub, a.Lk, a.KV, v ? a.dv : a.dk);
+        return;
+    }
+    const int h = (int)(block - 2 * f.dkv), lanes = 256 / a.buckets;  // threads that share a bucket
+    const int b = tid % a.buckets, l = tid / a.buckets;
     float sum = 0.0f;
-    for (int s = 0; s < a.S; s++)
-        for (int t = 0; t < qtiles; t++) sum += a.dbias_part[(((int64_t)s * a.H + h) * qtiles + t) * a.buckets + b];
+    if (l < lanes)
+        for (int i = l; i < a.dbias_parts; i += lanes) sum += a.dbias_part[((int64_t)h * a.dbias_parts + i) * a.buckets + b];
+    sums[tid] = sum;
+    __syncthreads();
+    if (tid >= a.buckets) return;
+    for (int i = 1; i < lanes; i++) sum += sums[i * a.buckets + b];
     a.dbias[(int64_t)b * a.H + h] = sum;
 }
 

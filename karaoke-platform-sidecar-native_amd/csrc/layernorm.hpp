@@ -26,38 +26,43 @@ struct NormArgs {
     float eps;
 };
 
+// N consecutive elements (16 bytes, or 8) of any element's alignment: the hardware
+// takes such an access as one, also across lines.  n: how many of them belong to
+// the row; the others are 0 and not touched.
 template <int N>
 struct Vec {
     float v[N];
 };
-template <int N>
-VH_DEVICE Vec<N> ldv(const float *p) {
-    Vec<N> r;
-    if constexpr (N == 4) {
-        const floatx4 a = ld4(p);
+template <typename T, int N>
+struct Packed {
+    typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+template <int N, typename T>
+VH_DEVICE Vec<N> ldv(const T *p, int n) {
+    Vec<N> r = {};
+    if (n >= N) {
+        const typename Packed<T, N>::type a = *reinterpret_cast<const typename Packed<T, N>::type *>(p);
 #pragma unroll
-        for (int e = 0; e < 4; e++) r.v[e] = a[e];
+        for (int e = 0; e < N; e++) r.v[e] = (float)a[e];
     } else {
-        r.v[0] = p[0];
-    }
-    return r;
-}
-template <int N>
-VH_DEVICE Vec<N> ldv(const bf16 *p) {
-    Vec<N> r;
-    if constexpr (N == 4) {
-        const bf16x4 a = *reinterpret_cast<const bf16x4 *>(p);
 #pragma unroll
-        for (int e = 0; e < 4; e++) r.v[e] = (float)a[e];
-    } else {
-        r.v[0] = (float)p[0];
+        for (int e = 0; e < N; e++)
+            if (e < n) r.v[e] = (float)p[e];
     }
     return r;
 }
 template <int N, typename T>
-VH_DEVICE void stv(T *p, const Vec<N> &a) {
-    if constexpr (N == 4) st4(p, floatx4{a.v[0], a.v[1], a.v[2], a.v[3]});
-    else p[0] = (T)a.v[0];
+VH_DEVICE void stv(T *p, const Vec<N> &v, int n) {
+    if (n >= N) {
+        typename Packed<T, N>::type a;
+#pragma unroll
+        for (int e = 0; e < N; e++) a[e] = (T)v.v[e];
+        *reinterpret_cast<typename Packed<T, N>::type *>(p) = a;
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e++)
+            if (e < n) p[e] = (T)v.v[e];
+    }
 }
 
 // Sums over a row's LANES lanes: a wave, or a workgroup of LANES / 64 waves by
@@ -83,11 +88,16 @@ VH_DEVICE void row_sums(float (&v)[K], float *red, int &turn) {
     }
 }
 
-// LANES lanes per row (64: a wave, four rows a workgroup of 256; else the
-// workgroup), NV vectors of N elements each.
+// LANES lanes per row (64: a wave, ROWS rows a workgroup; else the workgroup), NV
+// vectors of N elements each.
+template <int LANES>
+struct NormShape {
+    static constexpr int ROWS = LANES == 64 ? 8 : 1;
+    static constexpr int THREADS = LANES * ROWS;
+};
 template <typename T, int LANES, int N, int NV>
-static __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layernorm_kernel(NormArgs a) {
-    constexpr int ROWS = LANES == 64 ? 4 : 1;
+static __global__ __launch_bounds__(NormShape<LANES>::THREADS) void layernorm_kernel(NormArgs a) {
+    constexpr int ROWS = NormShape<LANES>::ROWS;
     __shared__ float red[4 * (LANES / 64)];
     int turn = 0;
     const int64_t row = (int64_t)blockIdx.x * ROWS + (LANES == 64 ? (int)threadIdx.x >> 6 : 0);
@@ -100,12 +110,9 @@ static __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layernorm_ke
 #pragma unroll
     for (int i = 0; i < NV; i++) {
         const int c = (lane + LANES * i) * N;
-        if (c < a.dim) v[i] = ldv<N>(x + c);
+        v[i] = ldv<N>(x + c, a.dim - c);
 #pragma unroll
-        for (int e = 0; e < N; e++) {
-            if (c >= a.dim) v[i].v[e] = 0.0f;
-            sum[0] += v[i].v[e];
-        }
+        for (int e = 0; e < N; e++) sum[0] += v[i].v[e];
     }
     row_sums<LANES>(sum, red, turn);
     const float mu = sum[0] / (float)a.dim;
@@ -116,7 +123,7 @@ static __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layernorm_ke
 #pragma unroll
         for (int e = 0; e < N; e++) {
             v[i].v[e] -= mu;
-            if (c < a.dim) sq[0] = __builtin_fmaf(v[i].v[e], v[i].v[e], sq[0]);
+            if (c + e < a.dim) sq[0] = __builtin_fmaf(v[i].v[e], v[i].v[e], sq[0]);
         }
     }
     row_sums<LANES>(sq, red, turn);
@@ -125,24 +132,22 @@ static __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layernorm_ke
 #pragma unroll
     for (int i = 0; i < NV; i++) {
         const int c = (lane + LANES * i) * N;
-        if (c < a.dim) {
-            const Vec<N> g = ldv<N>(a.gamma + c);
-            Vec<N> b = {};
-            if (a.beta) b = ldv<N>(a.beta + c);
+        const Vec<N> g = ldv<N>(a.gamma + c, a.dim - c);
+        Vec<N> b = {};
+        if (a.beta) b = ldv<N>(a.beta + c, a.dim - c);
 #pragma unroll
-            for (int e = 0; e < N; e++) v[i].v[e] = __builtin_fmaf(v[i].v[e] * rstd, g.v[e], b.v[e]);
-            stv<N>(y + c, v[i]);
-        }
+        for (int e = 0; e < N; e++) v[i].v[e] = __builtin_fmaf(v[i].v[e] * rstd, g.v[e], b.v[e]);
+        stv<N>(y + c, v[i], a.dim - c);
     }
 }
 
-// A workgroup takes every gridDim-th row (or four), and keeps its rows' sums of
-// dgamma and dbeta in registers: lane's columns are the same in every row.
+// A workgroup takes every gridDim-th row (or eight), and keeps its rows' sums of
+// dgamma and dbeta in registers: a lane's columns are the same in every row.
 template <typename T, int LANES, int N, int NV>
-static __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layernorm_backward_kernel(NormArgs a) {
-    constexpr int ROWS = LANES == 64 ? 4 : 1;
+static __global__ __launch_bounds__(NormShape<LANES>::THREADS) void layernorm_backward_kernel(NormArgs a) {
+    constexpr int ROWS = NormShape<LANES>::ROWS, COLS = LANES * N * NV;
     __shared__ float red[4 * (LANES / 64)];
-    __shared__ float cols[ROWS == 4 ? 2 * 64 * N * NV : 1];
+    __shared__ float cols[ROWS > 1 ? 2 * COLS : 1];
     int turn = 0;
     const int lane = (int)threadIdx.x % LANES, sub = LANES == 64 ? (int)threadIdx.x >> 6 : 0;
     Vec<N> dg[NV] = {}, db[NV] = {};
@@ -155,19 +160,22 @@ static __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layernorm_ba
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int c = (lane + LANES * i) * N;
-            if (c < a.dim) {
-                h[i] = ldv<N>(x + c);
-                g[i] = ldv<N>(dy + c);
-                const Vec<N> w = ldv<N>(a.gamma + c);
+            h[i] = ldv<N>(x + c, a.dim - c);
+            g[i] = ldv<N>(dy + c, a.dim - c);
+        }
 #pragma unroll
-                for (int e = 0; e < N; e++) {
-                    h[i].v[e] = (h[i].v[e] - st.x) * st.y;
-                    dg[i].v[e] = __builtin_fmaf(g[i].v[e], h[i].v[e], dg[i].v[e]);
-                    db[i].v[e] += g[i].v[e];
-                    g[i].v[e] *= w.v[e];
-                    sum[0] += g[i].v[e];
-                    sum[1] = __builtin_fmaf(g[i].v[e], h[i].v[e], sum[1]);
-                }
+        for (int i = 0; i < NV; i++) {
+            const int c = (lane + LANES * i) * N;
+            const Vec<N> w = ldv<N>(a.gamma + c, a.dim - c);
+#pragma unroll
+            for (int e = 0; e < N; e++) {  // past the row's end g is 0
+                h[i].v[e] = (h[i].v[e] - st.x) * st.y;
+                if (c + e >= a.dim) h[i].v[e] = 0.0f;
+                dg[i].v[e] = __builtin_fmaf(g[i].v[e], h[i].v[e], dg[i].v[e]);
+                db[i].v[e] += g[i].v[e];
+                g[i].v[e] *= w.v[e];
+                sum[0] += g[i].v[e];
+                sum[1] = __builtin_fmaf(g[i].v[e], h[i].v[e], sum[1]);
             }
         }
         row_sums<LANES>(sum, red, turn);
@@ -175,58 +183,56 @@ static __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void layernorm_ba
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int c = (lane + LANES * i) * N;
-            if (c < a.dim) {
 #pragma unroll
-                for (int e = 0; e < N; e++) g[i].v[e] = st.y * (g[i].v[e] - c1 - h[i].v[e] * c2);
-                stv<N>(dx + c, g[i]);
-            }
+            for (int e = 0; e < N; e++) g[i].v[e] = st.y * (g[i].v[e] - c1 - h[i].v[e] * c2);
+            stv<N>(dx + c, g[i], a.dim - c);
         }
     }
     if (!a.part) return;
     float *part = a.part + (int64_t)blockIdx.x * 2 * a.dim;
-    if constexpr (ROWS == 4) {  // the four waves' sums, one after the other
-        for (int w = 0; w < 4; w++) {
+    if constexpr (ROWS > 1) {  // the waves' sums, one after the other
+        for (int w = 0; w < ROWS; w++) {
             if (sub == w)
 #pragma unroll
                 for (int i = 0; i < NV; i++)
 #pragma unroll
                     for (int e = 0; e < N; e++) {
-                        const int c = (lane + 64 * i) * N + e;
+                        const int c = (i * N + e) * 64 + lane;  // a column's place: its own lane's
                         if (w) {
                             dg[i].v[e] += cols[c];
-                            db[i].v[e] += cols[64 * N * NV + c];
+                            db[i].v[e] += cols[COLS + c];
                         }
                         cols[c] = dg[i].v[e];
-                        cols[64 * N * NV + c] = db[i].v[e];
+                        cols[COLS + c] = db[i].v[e];
                     }
             __syncthreads();
         }
-        if (sub != 3) return;
+        if (sub != ROWS - 1) return;
     }
 #pragma unroll
     for (int i = 0; i < NV; i++) {
         const int c = (lane + LANES * i) * N;
-        if (c < a.dim) {
-            stv<N>(part + c, dg[i]);
-            stv<N>(part + a.dim + c, db[i]);
-        }
+        stv<N>(part + c, dg[i], a.dim - c);
+        stv<N>(part + a.dim + c, db[i], a.dim - c);
     }
 }
 
-// Column sums of the workgroups' parts [parts][2 dim]: 64 columns x 4 rows a
+// Column sums of the workgroups' parts [parts][2 dim]: 64 columns x 16 rows a
 // workgroup.  out: dgamma, then dbeta (either may be null).
-static __global__ __launch_bounds__(256) void layernorm_columns_kernel(const float *part, int parts, int dim,
-                                                                        float *dgamma, float *dbeta) {
-    __shared__ float sums[4][64];
-    const int c = (int)blockIdx.x * 64 + ((int)threadIdx.x & 63), w = (int)threadIdx.x >> 6;
+static __global__ __launch_bounds__(1024) void layernorm_columns_kernel(const float *part, int parts, int dim,
+                                                                         float *dgamma, float *dbeta) {
+    __shared__ float sums[16][64];
+    const int i = (int)threadIdx.x & 63, c = (int)blockIdx.x * 64 + i, w = (int)threadIdx.x >> 6;
     float sum = 0.0f;
-    if (c < 2 * dim)
-        for (int p = w; p < parts; p += 4) sum += part[(int64_t)p * 2 * dim + c];
-    sums[w][threadIdx.x & 63] = sum;
+    if (c < 2 * dim) {
+#pragma unroll 8
+        for (int p = w; p < parts; p += 16) sum += part[(int64_t)p * 2 * dim + c];
+    }
+    sums[w][i] = sum;
     __syncthreads();
     if (w || c >= 2 * dim) return;
-    const int i = (int)threadIdx.x;
-    sum = (sums[0][i] + sums[1][i]) + (sums[2][i] + sums[3][i]);
+#pragma unroll
+    for (int k = 1; k < 16; k++) sum += sums[k][i];
     float *out = c < dim ? dgamma : dbeta;
     if (out) out[c < dim ? c : c - dim] = sum;
 }

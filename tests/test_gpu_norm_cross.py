@@ -368,6 +368,14 @@ def test_peaked_and_flat(ctx, size, dtype):
     check(ctx, q, k, v, dout, str(size))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1.0])
+def test_scale(ctx, scale, dtype):
+    q, k, v, dout = make(2, 4, 2, 45, 75, dtype)
+    check(ctx, q, k, v, dout, str(scale), scale=scale, causal=True, query_start=[20, 0])
+    check(ctx, q, k, v, dout, str(scale), scale=scale, bias_table=randn(9, 32, 4))
+
+
 def test_values_past_range(ctx):
     """NaN and infinity in a query stay in its row, in a key or value go where it is seen."""
     q, k, v, _ = make(1, 2, 2, 70, 60, F32)
