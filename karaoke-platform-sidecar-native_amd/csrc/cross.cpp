@@ -248,9 +248,7 @@ static size_t tiles_lds(const vh_cross *c, bool split) {
 }
 static size_t dq_lds(const vh_cross *c, bool split) {
     if (!c->bias_table) return tiles_lds(c, split);
-    size_t tiles = tiles_lds(c, false);
-    if (split) tiles = c->type == VH_TYPE_BF16 ? DqLds<bf16, true>::BYTES : DqLds<float, true>::BYTES;
-    return tiles + window_bytes(c) + sizeof(DbiasLds) + 128 * sizeof(float) * c->buckets + window_bytes(c) / sizeof(float);
+    return tiles_lds(c, split) + window_bytes(c) + sizeof(DbiasLds) + 128 * sizeof(float) * c->buckets + window_bytes(c) / sizeof(float);
 }
 static size_t pack_lds(const vh_cross *c) {
     return tiles_lds(c, true) +
@@ -264,10 +262,11 @@ struct CrossCut {
     int parts = 1;
     int64_t groups = 0;  // workgroups
 };
-// From about two 128-row workgroups per CU on, their sharing of tiles wins over
-// even work.  Below, pieces of at least 8 tiles (two a wave) until there are about
-// two workgroups per CU.
-constexpr int64_t CA_ENOUGH = 512;
+// From 1.5 128-row workgroups per CU on, their sharing of tiles wins over even work
+// (8 x 801 rows over 1723 keys, 448 of them: 42 us against 48; 4 x 1000 rows over
+// 1200 in fp32, 256: 101 against 94).  Below, pieces of at least 8 tiles (two a
+// wave) until there are about two workgroups per CU.
+constexpr int64_t CA_ENOUGH = 384, CA_PIECES = 512;
 static CrossCut cross_cut(int64_t columns, int rows, int pack, int across, bool fits) {
     CrossCut cut;
     cut.groups = columns * ((rows + 127) / 128);
@@ -277,7 +276,7 @@ static CrossCut cross_cut(int64_t columns, int rows, int pack, int across, bool 
     if (cut.pack) columns /= pack;
     const int64_t base = columns * (((int64_t)rows * (cut.pack ? pack : 1) + 31) / 32);
     const int tiles = (across + 31) / 32;
-    if (base > 0) cut.parts = (int)std::max<int64_t>(1, std::min<int64_t>({CA_ENOUGH / base, tiles / 8, 64}));
+    if (base > 0) cut.parts = (int)std::max<int64_t>(1, std::min<int64_t>({CA_PIECES / base, tiles / 8, 64}));
     cut.groups = base * cut.parts;
     return cut;
 }
@@ -295,7 +294,7 @@ static CrossCut dkv_cut(const vh_cross *c) {
     // the heads that share the keys are pieces of their own
     const int64_t base = (int64_t)c->sequences * c->heads * ((c->key_length + 31) / 32);
     const int tiles = (c->query_length + 31) / 32;
-    cut.parts = base > 0 ? (int)std::max<int64_t>(1, std::min<int64_t>({CA_ENOUGH / base, tiles / 8, 64})) : 1;
+    cut.parts = base > 0 ? (int)std::max<int64_t>(1, std::min<int64_t>({CA_PIECES / base, tiles / 8, 64})) : 1;
     cut.groups = base * cut.parts;
     return cut;
 }
@@ -444,7 +443,7 @@ static void dq_launch(hipStream_t s, const vh_cross *c, const CrossArgs &a, cons
 
 template <typename T, bool BIAS>
 static void dkv_launch(hipStream_t s, const vh_cross *c, const CrossArgs &a, const CrossCut &cut) {
-    const size_t lds = tiles_lds(c, cut.split) + (cut.split ? 4 * SplitLds<T>::BUFS * sizeof(RowStats) + window_bytes(c)
+    const size_t lds = tiles_lds(c, cut.split) + (cut.split ? 4 * sizeof(RowStats) + window_bytes(c)
                                                         : 2 * sizeof(RowStats) + 2 * window_bytes(c));
     if (cut.split) launch(cross_dkv_split_kernel<T, BIAS>, cut.groups, lds, s, a);
     else launch(cross_dkv_kernel<T, BIAS>, cut.groups, lds, s, a);

@@ -302,9 +302,8 @@ struct RowState {
 // lane's query sees, -inf past them where mask says that a lane has fewer than 32.
 // The maximum is raised only when a tile exceeds it by more than 2^8, which fp32
 // sums absorb: the rescaling runs on a few tiles of a row.
-template <typename T, bool BIAS, bool KEEP>
-VH_DEVICE void softmax_tile(RowState &st, floatx16 &x, const unsigned char *Vs, float c, bool mask, int seen, int lane) {
-    const int lh = lane >> 5;
+template <bool BIAS>
+VH_DEVICE void softmax_tile(RowState &st, floatx16 &x, float c, bool mask, int seen, int lh) {
     if (mask) {
 #pragma unroll
         for (int r = 0; r < 16; r++)
@@ -333,6 +332,10 @@ VH_DEVICE void softmax_tile(RowState &st, floatx16 &x, const unsigned char *Vs, 
         x[r] = __builtin_amdgcn_exp2f(BIAS ? x[r] - st.mc : __builtin_fmaf(x[r], c, -st.mc));
         st.l += x[r];
     }
+}
+// out^T += V^T P^T.
+template <typename T, bool BIAS, bool KEEP>
+VH_DEVICE void values_tile(RowState &st, floatx16 &x, const unsigned char *Vs, int lane) {
 #pragma unroll
     for (int g = 0; g < 2; g++) {
         Frag<T> pb, vf[2];
@@ -414,21 +417,29 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) void cross_forward_ker
     }
     RowState st;
     st.clear();
-    for (int k0 = 0; k0 < keys; k0 += CA_TILE) {
+    // the tiles of which the wave sees something, then the others' only for the rest
+    // of the workgroup (a branch in the loop would copy every accumulator each time)
+    const int mine = !active ? 0 : a.causal ? min(keys, start + q0 + 32) : keys;
+    int k0 = 0;
+    for (; k0 < mine; k0 += CA_TILE) {
         wait_vmcnt<0>();
         __syncthreads();  // this tile is there, and the last one has been read
         if (k0 + CA_TILE < keys) issue(k0 + CA_TILE);
-        if (active && (!a.causal || k0 <= start + q0 + 31)) {
-            const unsigned char *Ks = smem + (k0 / CA_TILE & 1) * 2 * Tile<T>::BYTES;
-            floatx16 x;
-            zero16(x);
+        const unsigned char *Ks = smem + (k0 / CA_TILE & 1) * 2 * Tile<T>::BYTES;
+        floatx16 x;
+        zero16(x);
 #pragma unroll
-            for (int g = 0; g < 4; g++) frag_mfma(x, tile_row(Ks, li, g, lh, T()), qf[g]);
-            const int lo = k0 - (start + q0 + 31), hi = k0 + 31 - (start + q0);
-            if constexpr (BIAS) add_bias(a, x, window, lo, hi, k0 - (start + q), 1, lh);
-            softmax_tile<T, BIAS, KEEP>(st, x, Ks + Tile<T>::BYTES, a.scale2, k0 + 32 > klen || (a.causal && hi > 0),
-                                        (a.causal ? min(klen, start + q + 1) : klen) - k0, lane);
-        }
+        for (int g = 0; g < 4; g++) frag_mfma(x, tile_row(Ks, li, g, lh, T()), qf[g]);
+        const int lo = k0 - (start + q0 + 31), hi = k0 + 31 - (start + q0);
+        if constexpr (BIAS) add_bias(a, x, window, lo, hi, k0 - (start + q), 1, lh);
+        softmax_tile<BIAS>(st, x, a.scale2, k0 + 32 > klen || (a.causal && hi > 0),
+                           (a.causal ? min(klen, start + q + 1) : klen) - k0, lh);
+        values_tile<T, BIAS, KEEP>(st, x, Ks + Tile<T>::BYTES, lane);
+    }
+    for (; k0 < keys; k0 += CA_TILE) {
+        wait_vmcnt<0>();
+        __syncthreads();
+        if (k0 + CA_TILE < keys) issue(k0 + CA_TILE);
     }
     if (q >= a.Lq) return;
     const float l = st.l + __shfl_xor(st.l, 32, 64);
@@ -452,42 +463,23 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) void cross_forward_ker
 // and every fourth tile of keys, each in tiles of its own, so that no wave waits
 // for another before the end; a.parts workgroups share a row tile's keys.  PACK:
 // a tile's rows are the queries' heads that share the key head, head by head
-// within a query, so that single tokens of shared heads fill it.
-template <typename T, int B = sizeof(T) == 2 ? 2 : 1>  // fp32's matrix instructions outlast a tile's copy
+// within a query, so that single tokens of shared heads fill it.  A wave has one
+// place for either tile and starts the next one's copies as soon as it has read the
+// last: half the LDS of two places (8 x 801 rows over 1723 keys 54 -> 48 us).
+template <typename T>
 struct SplitLds {
-    static constexpr int BUFS = B;
-    static constexpr int WAVE = BUFS * 2 * Tile<T>::BYTES;
+    static constexpr int WAVE = 2 * Tile<T>::BYTES;
     static constexpr int PITCH = CA_D + 4;
     static constexpr int RESULTS = 4 * 32 * PITCH * 4 + 4 * 32 * 8;  // the waves' [32][CA_D] and (m, l), over the tiles
     static constexpr int BYTES = 4 * WAVE > RESULTS ? 4 * WAVE : RESULTS;
+    static constexpr int LOADS = CA_TILE / Tile<T>::DMA_ROWS;  // copies of a tile
 };
-
-// A wave's own tiles [first, last) of keys (or queries), every fourth one from
-// its own number on: issue(tile, buffer) starts the copies, LOADS of them, use(tile,
-// buffer) works on them.
-template <int BUFS, int LOADS, typename Issue, typename Use>
-VH_DEVICE void wave_tiles(int first, int last, Issue issue, Use use) {
-    if constexpr (BUFS == 2) {
-        int buf = 0;
-        if (first < last) issue(first, 0);
-        for (int t = first; t < last; t += 4, buf ^= 1) {
-            if (t + 4 < last) {
-                wait_lds();  // the other buffer's reads have returned
-                issue(t + 4, buf ^ 1);
-                wait_vmcnt<LOADS>();
-            } else {
-                wait_vmcnt<0>();
-            }
-            use(t, buf);
-        }
-    } else {
-        for (int t = first; t < last; t += 4) {
-            wait_lds();
-            issue(t, 0);
-            wait_vmcnt<0>();
-            use(t, 0);
-        }
-    }
+// Waits until at most the newest N copies are still under way; none where there is
+// no next tile.
+template <int N>
+VH_DEVICE void wait_tile(bool next) {
+    if (next) wait_vmcnt<N>();
+    else wait_vmcnt<0>();
 }
 
 // The bias where a tile's columns belong to several heads: the bucket by relative
@@ -559,25 +551,34 @@ __global__ __launch_bounds__(256, 2) void cross_forward_split_kernel(CrossArgs a
     const char *kp = a.k.p + s * a.k.seq + kh * a.k.head, *vp = a.v.p + s * a.v.seq + kh * a.v.head;
     unsigned char *tile = smem + wave * L::WAVE;
     const uint32_t lds = (uint32_t)(uintptr_t)tile;
-    wave_tiles<L::BUFS, 2 * CA_TILE / Tile<T>::DMA_ROWS>(
-        first + wave, last,
-        [&](int t, int buf) {
-            tile_issue<T, 1>(kp, a.k.row, 32 * t, klen - 1, lds + 2 * buf * Tile<T>::BYTES, 0, lane);
-            tile_issue<T, 1>(vp, a.v.row, 32 * t, klen - 1, lds + (2 * buf + 1) * Tile<T>::BYTES, 0, lane);
-        },
-        [&](int t, int buf) {
-            const unsigned char *Ks = tile + 2 * buf * Tile<T>::BYTES, *Vs = Ks + Tile<T>::BYTES;
-            const int k0 = 32 * t;
-            floatx16 x;
-            zero16(x);
+    const unsigned char *Ks = tile, *Vs = tile + Tile<T>::BYTES;
+    auto issue_k = [&](int t) { tile_issue<T, 1>(kp, a.k.row, 32 * t, klen - 1, lds, 0, lane); };
+    auto issue_v = [&](int t) { tile_issue<T, 1>(vp, a.v.row, 32 * t, klen - 1, lds + Tile<T>::BYTES, 0, lane); };
+    int t = first + wave;
+    if (t < last) {
+        issue_k(t);
+        issue_v(t);
+    }
+    for (; t < last; t += 4) {
+        const bool next = t + 4 < last;
+        const int k0 = 32 * t;
+        floatx16 x;
+        zero16(x);
+        wait_vmcnt<L::LOADS>();  // K is there, V may be under way
 #pragma unroll
-            for (int g = 0; g < 4; g++) frag_mfma(x, tile_row(Ks, li, g, lh, T()), qf[g]);
-            const int lo = k0 - (start + q_hi), hi = k0 + 31 - (start + q_lo);
-            if constexpr (BIAS && PACK) scores_packed(a, x, pb, lo, hi, k0 - (start + q), head - kh * G, lh);
-            else if constexpr (BIAS) add_bias(a, x, window, lo, hi, k0 - (start + q), 1, lh);
-            softmax_tile<T, BIAS, KEEP>(st, x, Vs, a.scale2, k0 + 32 > klen || (a.causal && hi > 0),
-                                        (a.causal ? min(klen, start + q + 1) : klen) - k0, lane);
-        });
+        for (int g = 0; g < 4; g++) frag_mfma(x, tile_row(Ks, li, g, lh, T()), qf[g]);
+        wait_lds();
+        if (next) issue_k(t + 4);
+        const int lo = k0 - (start + q_hi), hi = k0 + 31 - (start + q_lo);
+        if constexpr (BIAS && PACK) scores_packed(a, x, pb, lo, hi, k0 - (start + q), head - kh * G, lh);
+        else if constexpr (BIAS) add_bias(a, x, window, lo, hi, k0 - (start + q), 1, lh);
+        softmax_tile<BIAS>(st, x, a.scale2, k0 + 32 > klen || (a.causal && hi > 0),
+                           (a.causal ? min(klen, start + q + 1) : klen) - k0, lh);
+        wait_tile<L::LOADS>(next);
+        values_tile<T, BIAS, KEEP>(st, x, Vs, lane);
+        wait_lds();
+        if (next) issue_v(t + 4);
+    }
 
     // the four waves' results joined: row tid / 8, dims 8 (tid % 8) .. + 7
     __syncthreads();
@@ -827,19 +828,21 @@ struct Dbias {
     }
 };
 
-// One tile of keys: dq^T += K^T dS^T, and the table's gradient.
-template <typename T, bool BIAS>
+// One tile of keys: dq^T += K^T dS^T, and the table's gradient.  have_k() is called
+// before K is read, had_v() when V has been.
+template <typename T, bool BIAS, typename HaveK, typename HadV>
 VH_DEVICE void dq_tile(const CrossArgs &a, const QueryRows<T> &w, floatx16 (&acc)[2], Dbias &db, const float *window,
                        const unsigned char *Ks, const unsigned char *Vs, int k0, int pos, int pos_lo, int klen, int wave,
-                       int lane) {
+                       int lane, HaveK have_k, HadV had_v) {
     const int li = lane & 31, lh = lane >> 5;
     floatx16 x, dp = w.delta;
     zero16(x);
 #pragma unroll
-    for (int g = 0; g < 4; g++) {
-        frag_mfma(x, tile_row(Ks, li, g, lh, T()), w.q[g]);
-        frag_mfma(dp, tile_row(Vs, li, g, lh, T()), w.dout[g]);
-    }
+    for (int g = 0; g < 4; g++) frag_mfma(dp, tile_row(Vs, li, g, lh, T()), w.dout[g]);
+    had_v();
+    have_k();
+#pragma unroll
+    for (int g = 0; g < 4; g++) frag_mfma(x, tile_row(Ks, li, g, lh, T()), w.q[g]);
     const int lo = k0 - (pos_lo + 31), hi = k0 + 31 - pos_lo;
     const int seen = (a.causal ? min(klen, pos + 1) : klen) - k0;  // rows of the tile that the lane's query sees
     const bool mask = k0 + 32 > klen || (a.causal && hi > 0);
@@ -903,14 +906,20 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(CrossArgs a) {
     floatx16 acc[2];
     zero16(acc[0]);
     zero16(acc[1]);
-    for (int k0 = 0; k0 < keys; k0 += CA_TILE) {
+    const int mine = !active ? 0 : a.causal ? min(keys, start + q0 + 32) : keys;  // as in the forward
+    int k0 = 0;
+    for (; k0 < mine; k0 += CA_TILE) {
         wait_vmcnt<0>();
         __syncthreads();
         if (k0 + CA_TILE < keys) issue(k0 + CA_TILE);
-        if (active && (!a.causal || k0 <= start + q0 + 31)) {
-            const unsigned char *Ks = smem + (k0 / CA_TILE & 1) * 2 * Tile<T>::BYTES;
-            dq_tile<T, BIAS>(a, w, acc, db, window, Ks, Ks + Tile<T>::BYTES, k0, start + q, start + q0, klen, wave, lane);
-        }
+        const unsigned char *Ks = smem + (k0 / CA_TILE & 1) * 2 * Tile<T>::BYTES;
+        dq_tile<T, BIAS>(
+            a, w, acc, db, window, Ks, Ks + Tile<T>::BYTES, k0, start + q, start + q0, klen, wave, lane, [] {}, [] {});
+    }
+    for (; k0 < keys; k0 += CA_TILE) {
+        wait_vmcnt<0>();
+        __syncthreads();
+        if (k0 + CA_TILE < keys) issue(k0 + CA_TILE);
     }
     if constexpr (BIAS) {
         if (a.dbias_part) db.finish(a, h, s * qtiles + qt, tid);
@@ -952,13 +961,10 @@ VH_DEVICE void waves_sum(float *res, const floatx16 (&acc)[2], int tid, floatx4 
     }
 }
 
-// The same in too few workgroups: as cross_forward_split_kernel.  With a bias one
-// buffer a wave, so that three workgroups with their sums' slots share a CU's LDS.
-template <typename T, bool BIAS>
-using DqLds = SplitLds<T, BIAS ? 1 : SplitLds<T>::BUFS>;
+// The same in too few workgroups: as cross_forward_split_kernel.
 template <typename T, bool BIAS>
 __global__ __launch_bounds__(256, 2) void cross_dq_split_kernel(CrossArgs a) {
-    using L = DqLds<T, BIAS>;
+    using L = SplitLds<T>;
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     float *window;
     Dbias db;
@@ -991,17 +997,26 @@ __global__ __launch_bounds__(256, 2) void cross_dq_split_kernel(CrossArgs a) {
     const char *kp = a.k.p + s * a.k.seq + kh * a.k.head, *vp = a.v.p + s * a.v.seq + kh * a.v.head;
     unsigned char *tile = smem + wave * L::WAVE;
     const uint32_t lds = (uint32_t)(uintptr_t)tile;
-    wave_tiles<L::BUFS, 2 * CA_TILE / Tile<T>::DMA_ROWS>(
-        first + wave, last,
-        [&](int t, int buf) {
-            tile_issue<T, 1>(kp, a.k.row, 32 * t, klen - 1, lds + 2 * buf * Tile<T>::BYTES, 0, lane);
-            tile_issue<T, 1>(vp, a.v.row, 32 * t, klen - 1, lds + (2 * buf + 1) * Tile<T>::BYTES, 0, lane);
-        },
-        [&](int t, int buf) {
-            const unsigned char *Ks = tile + 2 * buf * Tile<T>::BYTES;
-            dq_tile<T, BIAS>(a, w, acc, db, window, Ks, Ks + Tile<T>::BYTES, 32 * t, start + q, start + q0, klen, wave,
-                             lane);
-        });
+    auto issue_k = [&](int t) { tile_issue<T, 1>(kp, a.k.row, 32 * t, klen - 1, lds, 0, lane); };
+    auto issue_v = [&](int t) { tile_issue<T, 1>(vp, a.v.row, 32 * t, klen - 1, lds + Tile<T>::BYTES, 0, lane); };
+    int t = first + wave;
+    if (t < last) {
+        issue_v(t);
+        issue_k(t);
+    }
+    for (; t < last; t += 4) {
+        const bool next = t + 4 < last;
+        wait_vmcnt<L::LOADS>();  // V is there, K may be under way
+        dq_tile<T, BIAS>(
+            a, w, acc, db, window, tile, tile + Tile<T>::BYTES, 32 * t, start + q, start + q0, klen, wave, lane,
+            [&] { wait_tile<L::LOADS>(next); },
+            [&] {
+                wait_lds();
+                if (next) issue_v(t + 4);
+            });
+        wait_lds();
+        if (next) issue_k(t + 4);
+    }
     if constexpr (BIAS) {
         if (a.dbias_part) db.finish(a, h, (s * rtiles + rt) * a.parts + part, tid);
     }
@@ -1049,20 +1064,22 @@ VH_DEVICE void load_keys(const CrossArgs &a, KeyRows<T> &w, int s, int kh, int k
     }
 }
 // One tile of queries: S = Q K^T with the keys as columns, so that P and dS are B
-// operands of dv^T += dout^T P and dk^T += Q^T dS as they are.
-template <typename T, bool BIAS>
+// operands of dv^T += dout^T P and dk^T += Q^T dS as they are.  have_q() is called
+// before Q is read, had_dout() when dout and the statistics have been.
+template <typename T, bool BIAS, typename HaveQ, typename HadDout>
 VH_DEVICE void dkv_tile(const CrossArgs &a, KeyRows<T> &w, const float *window, const unsigned char *Qs,
-                        const unsigned char *Ds, const RowStats *rs, int q0, int start, int key, int k0, int lane) {
+                        const unsigned char *Ds, const RowStats *rs, int q0, int start, int key, int k0, int lane,
+                        HaveQ have_q, HadDout had_dout) {
     const int li = lane & 31, lh = lane >> 5;
     floatx16 x, dp;
     zero16(x);
 #pragma unroll
     for (int r = 0; r < 16; r++) dp[r] = rs->delta[row_of(r, lh)];
 #pragma unroll
-    for (int g = 0; g < 4; g++) {
-        frag_mfma(x, tile_row(Qs, li, g, lh, T()), w.k[g]);
-        frag_mfma(dp, tile_row(Ds, li, g, lh, T()), w.v[g]);
-    }
+    for (int g = 0; g < 4; g++) frag_mfma(dp, tile_row(Ds, li, g, lh, T()), w.v[g]);
+    have_q();
+#pragma unroll
+    for (int g = 0; g < 4; g++) frag_mfma(x, tile_row(Qs, li, g, lh, T()), w.k[g]);
     const int lo = k0 - (start + q0 + 31), hi = k0 + 31 - (start + q0);
     if constexpr (BIAS) add_bias(a, x, window, lo, hi, key - (start + q0), -1, lh);
 #pragma unroll
@@ -1079,14 +1096,18 @@ VH_DEVICE void dkv_tile(const CrossArgs &a, KeyRows<T> &w, const float *window, 
     }
 #pragma unroll
     for (int g = 0; g < 2; g++) {
-        Frag<T> pb, sb;
+        Frag<T> pb;
         frag_from(pb, x, g);
+#pragma unroll
+        for (int t = 0; t < 2; t++) frag_mfma(w.dv[t], tile_col(Ds, g, t, lane, T()), pb);
+    }
+    had_dout();
+#pragma unroll
+    for (int g = 0; g < 2; g++) {
+        Frag<T> sb;
         frag_from(sb, dp, g);
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            frag_mfma(w.dv[t], tile_col(Ds, g, t, lane, T()), pb);
-            frag_mfma(w.dk[t], tile_col(Qs, g, t, lane, T()), sb);
-        }
+        for (int t = 0; t < 2; t++) frag_mfma(w.dk[t], tile_col(Qs, g, t, lane, T()), sb);
     }
 }
 
@@ -1111,6 +1132,9 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(CrossArgs a) {
     int first = 0;
     if (a.causal) first = max(0, min(128 * kt - start, qlen)) / CA_TILE * CA_TILE;
     if (128 * kt >= klen) first = qlen;
+    // and one of the wave's own: the tiles before it are the other waves' (as in the forward)
+    int mine = active ? first : qlen;
+    if (active && a.causal) mine = max(first, max(0, min(k0 - start, qlen)) / CA_TILE * CA_TILE);
 
     const uint32_t lds = (uint32_t)(uintptr_t)smem, rs_lds = (uint32_t)(uintptr_t)rs;
     const int G = a.H / a.KV;
@@ -1129,14 +1153,19 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(CrossArgs a) {
         // the window before last is free: its head's tiles ended a barrier ago
         float *bias = window + (g & 1) * (BIAS ? cross_window(a) : 0);
         if constexpr (BIAS) fill_bias_window(a, kh * G + g, bias, tid);
-        for (int q0 = first; q0 < qlen; q0 += CA_TILE, buf ^= 1) {
+        auto begin = [&](int q0) {
             wait_vmcnt<0>();
             __syncthreads();
             if (q0 + CA_TILE < qlen) issue(kh * G + g, q0 + CA_TILE, buf ^ 1);
             else if (g + 1 < G) issue(kh * G + g + 1, first, buf ^ 1);
+        };
+        int q0 = first;
+        for (; q0 < mine; q0 += CA_TILE, buf ^= 1) begin(q0);
+        for (; q0 < qlen; q0 += CA_TILE, buf ^= 1) {
+            begin(q0);
             const unsigned char *Qs = smem + buf * 2 * Tile<T>::BYTES;
-            if (active && (!a.causal || k0 <= start + q0 + 31))
-                dkv_tile<T, BIAS>(a, w, bias, Qs, Qs + Tile<T>::BYTES, rs + buf, q0, start, key, k0, lane);
+            dkv_tile<T, BIAS>(
+                a, w, bias, Qs, Qs + Tile<T>::BYTES, rs + buf, q0, start, key, k0, lane, [] {}, [] {});
         }
     }
     if (key >= a.Lk) return;
@@ -1164,8 +1193,8 @@ template <typename T, bool BIAS>
 __global__ __launch_bounds__(256, 2) void cross_dkv_split_kernel(CrossArgs a) {
     using L = SplitLds<T>;
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
-    RowStats *stats = reinterpret_cast<RowStats *>(smem + L::BYTES);  // [4][BUFS]
-    float *window = reinterpret_cast<float *>(stats + 4 * L::BUFS);
+    RowStats *stats = reinterpret_cast<RowStats *>(smem + L::BYTES);  // [4]
+    float *window = reinterpret_cast<float *>(stats + 4);
 
     const int ktiles = (a.Lk + 31) / 32, G = a.H / a.KV;
     const int task = xcd_swizzle((int)blockIdx.x, (int)gridDim.x);
@@ -1190,18 +1219,29 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_split_kernel(CrossArgs a) {
     const char *qp = a.q.p + s * a.q.seq + h * a.q.head, *dp = a.dout.p + s * a.dout.seq + h * a.dout.head;
     unsigned char *tile = smem + wave * L::WAVE;
     const uint32_t lds = (uint32_t)(uintptr_t)tile;
-    RowStats *rs = stats + wave * L::BUFS;
-    wave_tiles<L::BUFS, 2 * CA_TILE / Tile<T>::DMA_ROWS + 1>(
-        first + wave, last,
-        [&](int t, int buf) {
-            tile_issue<T, 1>(qp, a.q.row, 32 * t, qlen - 1, lds + 2 * buf * Tile<T>::BYTES, 0, lane);
-            tile_issue<T, 1>(dp, a.dout.row, 32 * t, qlen - 1, lds + (2 * buf + 1) * Tile<T>::BYTES, 0, lane);
-            row_tile_issue(row_tile(a, s, h, t), (uint32_t)(uintptr_t)(rs + buf), lane);
-        },
-        [&](int t, int buf) {
-            const unsigned char *Qs = tile + 2 * buf * Tile<T>::BYTES;
-            dkv_tile<T, BIAS>(a, w, window, Qs, Qs + Tile<T>::BYTES, rs + buf, 32 * t, start, key, k0, lane);
-        });
+    RowStats *rs = stats + wave;
+    auto issue_q = [&](int t) { tile_issue<T, 1>(qp, a.q.row, 32 * t, qlen - 1, lds, 0, lane); };
+    auto issue_dout = [&](int t) {
+        tile_issue<T, 1>(dp, a.dout.row, 32 * t, qlen - 1, lds + Tile<T>::BYTES, 0, lane);
+        row_tile_issue(row_tile(a, s, h, t), (uint32_t)(uintptr_t)rs, lane);
+    };
+    int t = first + wave;
+    if (t < last) {
+        issue_dout(t);
+        issue_q(t);
+    }
+    for (; t < last; t += 4) {
+        const bool next = t + 4 < last;
+        wait_vmcnt<L::LOADS>();  // dout is there, Q may be under way
+        dkv_tile<T, BIAS>(
+            a, w, window, tile, tile + Tile<T>::BYTES, rs, 32 * t, start, key, k0, lane, [&] { wait_vmcnt<0>(); },
+            [&] {
+                wait_lds();
+                if (next) issue_dout(t + 4);
+            });
+        wait_lds();
+        if (next) issue_q(t + 4);
+    }
     floatx4 y[2], z[2];
     waves_sum<T>(reinterpret_cast<float *>(smem), w.dk, tid, y);
     waves_sum<T>(reinterpret_cast<float *>(smem), w.dv, tid, z);
