@@ -221,7 +221,7 @@ static bool cross_ok(const char *what, const vh_cross *c, bool backward) {
         }
     }
     const int64_t tasks = (int64_t)c->sequences * c->heads * ((std::max(c->query_length, c->key_length) + 127) / 128 + 1);
-    if (tasks > INT32_MAX) {
+    if (tasks > INT32_MAX / 8) {
         set_error("%s: %lld workgroups", what, (long long)tasks);
         return false;
     }
@@ -242,16 +242,16 @@ constexpr size_t CA_LDS = 160 * 1024;  // of a workgroup
 static size_t window_bytes(const vh_cross *c) {
     return c->bias_table ? (size_t)(2 * (c->max_distance + CA_PAD) + 1) * sizeof(float) : 0;
 }
-static size_t tiles_lds(const vh_cross *c, bool split) {
+static size_t tiles_lds(const vh_cross *c, bool split, bool forward = false) {
     if (c->type == VH_TYPE_BF16) return split ? SplitLds<bf16>::BYTES : 4 * Tile<bf16>::BYTES;
-    return split ? SplitLds<float>::BYTES : 4 * Tile<float>::BYTES;
+    return !split ? 4 * Tile<float>::BYTES : forward ? SplitLds<float, true>::BYTES : SplitLds<float>::BYTES;
 }
 static size_t dq_lds(const vh_cross *c, bool split) {
     if (!c->bias_table) return tiles_lds(c, split);
     return tiles_lds(c, split) + window_bytes(c) + sizeof(DbiasLds) + 128 * sizeof(float) * c->buckets + window_bytes(c) / sizeof(float);
 }
 static size_t pack_lds(const vh_cross *c) {
-    return tiles_lds(c, true) +
+    return tiles_lds(c, true, true) +
            (c->bias_table ? sizeof(float) * c->buckets * (c->heads / c->kv_heads) + window_bytes(c) / sizeof(float) : 0);
 }
 
@@ -260,24 +260,30 @@ static size_t pack_lds(const vh_cross *c) {
 struct CrossCut {
     bool split = false, pack = false;
     int parts = 1;
-    int64_t groups = 0;  // workgroups
+    int64_t pairs = 0, tiles = 0;  // (sequence, head) pairs, and workgroups of each
+    int64_t groups() const { return pairs * tiles; }
+    int64_t grid() const { return (pairs_by_xcd(pairs) ? (pairs + 7) / 8 * 8 : pairs) * tiles; }
 };
 // From 1.5 128-row workgroups per CU on, their sharing of tiles wins over even work
 // (8 x 801 rows over 1723 keys, 448 of them: 42 us against 48; 4 x 1000 rows over
 // 1200 in fp32, 256: 101 against 94).  Below, pieces of at least 8 tiles (two a
 // wave) until there are about two workgroups per CU.
 constexpr int64_t CA_ENOUGH = 384, CA_PIECES = 512;
-static CrossCut cross_cut(int64_t columns, int rows, int pack, int across, bool fits) {
+static int pieces(int64_t groups, int across) {
+    const int tiles = (across + 31) / 32;
+    return groups > 0 ? (int)std::max<int64_t>(1, std::min<int64_t>({CA_PIECES / groups, tiles / 8, 64})) : 1;
+}
+static CrossCut cross_cut(int64_t pairs, int rows, int pack, int across, bool fits) {
     CrossCut cut;
-    cut.groups = columns * ((rows + 127) / 128);
-    if ((cut.groups >= CA_ENOUGH && rows >= 64) || !fits) return cut;
+    cut.pairs = pairs;
+    cut.tiles = (rows + 127) / 128;
+    if ((cut.groups() >= CA_ENOUGH && rows >= 64) || !fits) return cut;
     cut.split = true;
     cut.pack = pack > 1 && rows < 32;
-    if (cut.pack) columns /= pack;
-    const int64_t base = columns * (((int64_t)rows * (cut.pack ? pack : 1) + 31) / 32);
-    const int tiles = (across + 31) / 32;
-    if (base > 0) cut.parts = (int)std::max<int64_t>(1, std::min<int64_t>({CA_PIECES / base, tiles / 8, 64}));
-    cut.groups = base * cut.parts;
+    if (cut.pack) cut.pairs /= pack;
+    cut.tiles = ((int64_t)rows * (cut.pack ? pack : 1) + 31) / 32;
+    cut.parts = pieces(cut.groups(), across);
+    cut.tiles *= cut.parts;
     return cut;
 }
 static CrossCut forward_cut(const vh_cross *c, bool keep) {
@@ -291,11 +297,11 @@ static CrossCut dq_cut(const vh_cross *c) {
 static CrossCut dkv_cut(const vh_cross *c) {
     CrossCut cut = cross_cut((int64_t)c->sequences * c->kv_heads, c->key_length, 1, c->query_length, true);
     if (!cut.split) return cut;
-    // the heads that share the keys are pieces of their own
-    const int64_t base = (int64_t)c->sequences * c->heads * ((c->key_length + 31) / 32);
-    const int tiles = (c->query_length + 31) / 32;
-    cut.parts = base > 0 ? (int)std::max<int64_t>(1, std::min<int64_t>({CA_PIECES / base, tiles / 8, 64})) : 1;
-    cut.groups = base * cut.parts;
+    // the heads that share the keys are pairs of their own, their sums pieces
+    cut.pairs = (int64_t)c->sequences * c->heads;
+    cut.tiles = (c->key_length + 31) / 32;
+    cut.parts = pieces(cut.groups(), c->query_length);
+    cut.tiles *= cut.parts;
     return cut;
 }
 
@@ -334,8 +340,8 @@ static CrossWork backward_work(const vh_cross *c) {
         w.part_dv = w.take(n);
     }
     if (c->bias_table) {
-        w.dbias_parts = (int)(w.rows.groups / c->heads);
-        w.dbias = w.take((size_t)w.rows.groups * c->buckets * sizeof(float));
+        w.dbias_parts = (int)(w.rows.groups() / c->heads);
+        w.dbias = w.take((size_t)w.rows.groups() * c->buckets * sizeof(float));
     }
     return w;
 }
@@ -391,18 +397,18 @@ static void launch(F kernel, int64_t groups, size_t lds, hipStream_t s, const Cr
 template <typename T, bool BIAS>
 static void forward_launch(hipStream_t s, const vh_cross *c, const CrossArgs &a, const CrossCut &cut) {
     const bool keep = a.stats != nullptr;
-    const size_t lds = tiles_lds(c, cut.split) + window_bytes(c);
+    const size_t lds = tiles_lds(c, cut.split, true) + window_bytes(c);
     if (!cut.split) {
-        if (keep) launch(cross_forward_kernel<T, BIAS, true>, cut.groups, lds, s, a);
-        else launch(cross_forward_kernel<T, BIAS, false>, cut.groups, lds, s, a);
+        if (keep) launch(cross_forward_kernel<T, BIAS, true>, cut.grid(), lds, s, a);
+        else launch(cross_forward_kernel<T, BIAS, false>, cut.grid(), lds, s, a);
         return;
     }
     if (cut.pack) {
-        launch(cross_forward_split_kernel<T, BIAS, false, true>, cut.groups, pack_lds(c), s, a);
+        launch(cross_forward_split_kernel<T, BIAS, false, true>, cut.grid(), pack_lds(c), s, a);
     } else if (keep) {
-        launch(cross_forward_split_kernel<T, BIAS, true, false>, cut.groups, lds, s, a);
+        launch(cross_forward_split_kernel<T, BIAS, true, false>, cut.grid(), lds, s, a);
     } else {
-        launch(cross_forward_split_kernel<T, BIAS, false, false>, cut.groups, lds, s, a);
+        launch(cross_forward_split_kernel<T, BIAS, false, false>, cut.grid(), lds, s, a);
     }
     if (cut.parts == 1) return;
     const int64_t groups = (cross_rows(c) + 15) / 16;
@@ -437,16 +443,16 @@ bool cross_attention(hipStream_t s, const vh_cross *c, const CrossBuffers &b, Ke
 
 template <typename T, bool BIAS>
 static void dq_launch(hipStream_t s, const vh_cross *c, const CrossArgs &a, const CrossCut &cut) {
-    if (cut.split) launch(cross_dq_split_kernel<T, BIAS>, cut.groups, dq_lds(c, true), s, a);
-    else launch(cross_dq_kernel<T, BIAS>, cut.groups, dq_lds(c, false), s, a);
+    if (cut.split) launch(cross_dq_split_kernel<T, BIAS>, cut.grid(), dq_lds(c, true), s, a);
+    else launch(cross_dq_kernel<T, BIAS>, cut.grid(), dq_lds(c, false), s, a);
 }
 
 template <typename T, bool BIAS>
 static void dkv_launch(hipStream_t s, const vh_cross *c, const CrossArgs &a, const CrossCut &cut) {
     const size_t lds = tiles_lds(c, cut.split) + (cut.split ? 4 * sizeof(RowStats) + window_bytes(c)
                                                         : 2 * sizeof(RowStats) + 2 * window_bytes(c));
-    if (cut.split) launch(cross_dkv_split_kernel<T, BIAS>, cut.groups, lds, s, a);
-    else launch(cross_dkv_kernel<T, BIAS>, cut.groups, lds, s, a);
+    if (cut.split) launch(cross_dkv_split_kernel<T, BIAS>, cut.grid(), lds, s, a);
+    else launch(cross_dkv_kernel<T, BIAS>, cut.grid(), lds, s, a);
 }
 
 bool cross_attention_backward(hipStream_t s, const vh_cross *c, const CrossBuffers &b, KernelTimer *t) {

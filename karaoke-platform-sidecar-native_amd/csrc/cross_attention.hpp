@@ -205,6 +205,76 @@ VH_DEVICE Frag<float> tile_col(const unsigned char *tile, int st, int t, int lan
     return f;
 }
 
+// Which (sequence, head) pair and which of its tiles a workgroup takes.  The pairs
+// are dealt out to the 8 XCDs in turn (workgroup i runs on XCD i % 8), so that a
+// pair's tiles find their keys in one L2 and a batch's long and short sequences are
+// spread evenly; where that leaves the XCDs unequal (few pairs, not a multiple of
+// 8), workgroups are taken as they come.  False: none (the last round of pairs).
+constexpr bool pairs_by_xcd(int64_t pairs) { return pairs % 8 == 0 || pairs >= 64; }
+VH_DEVICE bool pair_task(int pairs, int tiles, int &pair, int &tile) {
+    int i = (int)blockIdx.x;
+    pair = i / tiles;
+    tile = i % tiles;
+    if (!pairs_by_xcd(pairs)) return true;
+    const int xcd = i % 8;
+    i /= 8;
+    pair = i / tiles * 8 + xcd;
+    tile = i % tiles;
+    return pair < pairs;
+}
+
+// Where a product's operands come from.  A streamed tile: in LDS, or (fp32) as it
+// lies in global memory, rows past `last` (the tile's own count) read as row `last`.
+template <typename T>
+struct LdsTile {
+    const unsigned char *p;
+    VH_DEVICE Frag<T> row(int g, int lane) const { return tile_row(p, lane & 31, g, lane >> 5, T()); }
+    VH_DEVICE Frag<T> col(int st, int t, int lane) const { return tile_col(p, st, t, lane, T()); }
+};
+struct GlobalTile {
+    const char *p;  // row 0 of the tile, the same in every lane
+    uint32_t row_bytes;
+    int last;
+    VH_DEVICE uint32_t at(int r) const { return (uint32_t)min(r, last) * row_bytes; }
+    VH_DEVICE Frag<float> row(int g, int lane) const {
+        return frag_load(reinterpret_cast<const float *>(p + (at(lane & 31) + 64u * g + 32u * (lane >> 5))));
+    }
+    VH_DEVICE Frag<float> col(int st, int t, int lane) const {
+        Frag<float> f;
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            f.v[e >> 2][e & 3] = *reinterpret_cast<const float *>(
+                p + (at(16 * st + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) + 128u * t + 4u * (lane & 31)));
+        return f;
+    }
+};
+// The operand that stays: 32 rows in registers, or in a tile of LDS.
+template <typename T>
+struct RegRows {
+    Frag<T> f[4];
+    VH_DEVICE const Frag<T> &get(int g, int) const { return f[g]; }
+};
+template <typename T>
+struct LdsRows {
+    const unsigned char *p;
+    VH_DEVICE Frag<T> get(int g, int lane) const { return tile_row(p, lane & 31, g, lane >> 5, T()); }
+};
+// Dims 16 g + 8 lh .. + 7 of row li into a tile.
+VH_DEVICE void put_row(unsigned char *t, int g, int lane, const Frag<float> &f) {
+    using L = Tile<float>;
+    unsigned char *p = t + (lane & 31) * L::ROW;
+    const int c = 4 * g + 2 * (lane >> 5), z = L::swz(lane & 31);
+    *reinterpret_cast<floatx4 *>(p + 16 * (c ^ z)) = f.v[0];
+    *reinterpret_cast<floatx4 *>(p + 16 * ((c + 1) ^ z)) = f.v[1];
+}
+
+// The same pointer, in scalar registers: the wave's lanes all have it.
+VH_DEVICE const char *uniform(const void *from) {
+    const uint64_t p = (uint64_t)from;
+    return reinterpret_cast<const char *>((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32 |
+                                          (uint32_t)__builtin_amdgcn_readfirstlane((int)p));
+}
+
 // Copies rows row0 .. row0 + 31 of a tensor's sequence and head (base: its row 0)
 // into a tile, 1 KB a load, the loads dealt out to WAVES waves.  Rows past `last`
 // are copies of row `last`: what lies behind the valid rows is never read.
@@ -212,7 +282,8 @@ template <typename T, int WAVES>
 VH_DEVICE void tile_issue(const char *base, int64_t row_bytes, int row0, int last, uint32_t tile_lds, int wave,
                           int lane) {
     using L = Tile<T>;
-    const char *sbase = base + (int64_t)row0 * row_bytes;
+    const char *sbase = uniform(base + (int64_t)row0 * row_bytes);
+    tile_lds = (uint32_t)__builtin_amdgcn_readfirstlane((int)tile_lds);
     constexpr int LOADS = CA_TILE / L::DMA_ROWS / WAVES;
 #pragma unroll
     for (int i = 0; i < LOADS; i++) {
@@ -240,11 +311,11 @@ VH_DEVICE void wave_order() {
 constexpr float CA_LOG2E = 1.4426950408889634f;
 
 VH_DEVICE int cross_length(const int *lengths, int s, int most) {
-    return lengths ? max(0, min(lengths[s], most)) : most;
+    return lengths ? max(0, min(__builtin_amdgcn_readfirstlane(lengths[s]), most)) : most;
 }
 // Positions further out than any length act alike.
 VH_DEVICE int cross_start(const CrossArgs &a, int s) {
-    return a.query_start ? max(-(1 << 30), min(a.query_start[s], 1 << 30)) : 0;
+    return a.query_start ? max(-(1 << 30), min(__builtin_amdgcn_readfirstlane(a.query_start[s]), 1 << 30)) : 0;
 }
 
 // The bias by relative position -max_distance - 63 .. max_distance + 63 (beyond
@@ -298,6 +369,25 @@ struct RowState {
     VH_DEVICE float top() const { return m == -INFINITY ? m : mc; }  // the maximum in powers of two
 };
 
+// q's fragment g, of the scale's sign.
+template <typename T>
+VH_DEVICE Frag<T> load_query(const CrossArgs &a, const char *row, int g, int lh) {
+    Frag<T> f = frag_load(reinterpret_cast<const T *>(row) + 16 * g + 8 * lh);
+    if (a.scale < 0.0f) frag_negate(f);
+    return f;
+}
+// rows of the streamed tile x the held rows, over the head's 64 dims, added to x
+template <typename Tile, typename Held>
+VH_DEVICE void dot_tile(floatx16 &x, const Tile &tile, const Held &held, int lane) {
+#pragma unroll
+    for (int g = 0; g < 4; g++) frag_mfma(x, tile.row(g, lane), held.get(g, lane));
+}
+template <typename Tile, typename Held>
+VH_DEVICE void scores(floatx16 &x, const Tile &tile, const Held &held, int lane) {
+    zero16(x);
+    dot_tile(x, tile, held, lane);
+}
+
 // One tile of keys: x holds its scores on entry; seen: rows of the tile that the
 // lane's query sees, -inf past them where mask says that a lane has fewer than 32.
 // The maximum is raised only when a tile exceeds it by more than 2^8, which fp32
@@ -334,15 +424,15 @@ VH_DEVICE void softmax_tile(RowState &st, floatx16 &x, float c, bool mask, int s
     }
 }
 // out^T += V^T P^T.
-template <typename T, bool BIAS, bool KEEP>
-VH_DEVICE void values_tile(RowState &st, floatx16 &x, const unsigned char *Vs, int lane) {
+template <typename T, bool BIAS, bool KEEP, typename Tile>
+VH_DEVICE void values_tile(RowState &st, floatx16 &x, const Tile &v, int lane) {
 #pragma unroll
     for (int g = 0; g < 2; g++) {
         Frag<T> pb, vf[2];
         frag_from(pb, x, g);
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            vf[t] = tile_col(Vs, g, t, lane, T());
+            vf[t] = v.col(g, t, lane);
             frag_mfma(st.o[t], vf[t], pb);
         }
         if constexpr (KEEP && sizeof(T) == 2) {
@@ -384,8 +474,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) void cross_forward_ker
     float *window = reinterpret_cast<float *>(smem + 4 * Tile<T>::BYTES);
 
     const int qtiles = (a.Lq + 127) / 128;
-    const int task = xcd_swizzle((int)blockIdx.x, (int)gridDim.x);
-    const int qt = task % qtiles, h = task / qtiles % a.H, s = task / qtiles / a.H;
+    int pair, qt;
+    if (!pair_task(a.S * a.H, qtiles, pair, qt)) return;
+    const int h = pair % a.H, s = pair / a.H;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 31, lh = lane >> 5;
     const int kh = h / (a.H / a.KV);
@@ -406,14 +497,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) void cross_forward_ker
     };
     if (keys > 0) issue(0);
     if constexpr (BIAS) fill_bias_window(a, h, window, tid);  // read after the loop's first barrier
-    Frag<T> qf[4];
+    RegRows<T> w;
     if (active) {
         const char *qp = a.q.p + s * a.q.seq + (int64_t)min(q, qlen - 1) * a.q.row + h * a.q.head;
 #pragma unroll
-        for (int g = 0; g < 4; g++) {
-            qf[g] = frag_load(reinterpret_cast<const T *>(qp) + 16 * g + 8 * lh);
-            if (a.scale < 0.0f) frag_negate(qf[g]);
-        }
+        for (int g = 0; g < 4; g++) w.f[g] = load_query<T>(a, qp, g, lh);
     }
     RowState st;
     st.clear();
@@ -425,16 +513,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) void cross_forward_ker
         wait_vmcnt<0>();
         __syncthreads();  // this tile is there, and the last one has been read
         if (k0 + CA_TILE < keys) issue(k0 + CA_TILE);
-        const unsigned char *Ks = smem + (k0 / CA_TILE & 1) * 2 * Tile<T>::BYTES;
+        const LdsTile<T> K{smem + (k0 / CA_TILE & 1) * 2 * Tile<T>::BYTES}, V{K.p + Tile<T>::BYTES};
         floatx16 x;
-        zero16(x);
-#pragma unroll
-        for (int g = 0; g < 4; g++) frag_mfma(x, tile_row(Ks, li, g, lh, T()), qf[g]);
+        scores(x, K, w, lane);
         const int lo = k0 - (start + q0 + 31), hi = k0 + 31 - (start + q0);
         if constexpr (BIAS) add_bias(a, x, window, lo, hi, k0 - (start + q), 1, lh);
         softmax_tile<BIAS>(st, x, a.scale2, k0 + 32 > klen || (a.causal && hi > 0),
                            (a.causal ? min(klen, start + q + 1) : klen) - k0, lh);
-        values_tile<T, BIAS, KEEP>(st, x, Ks + Tile<T>::BYTES, lane);
+        values_tile<T, BIAS, KEEP>(st, x, V, lane);
     }
     for (; k0 < keys; k0 += CA_TILE) {
         wait_vmcnt<0>();
@@ -465,13 +551,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) void cross_forward_ker
 // a tile's rows are the queries' heads that share the key head, head by head
 // within a query, so that single tokens of shared heads fill it.  A wave has one
 // place for either tile and starts the next one's copies as soon as it has read the
-// last: half the LDS of two places (8 x 801 rows over 1723 keys 54 -> 48 us).
-template <typename T>
+// last: half the LDS of two places (8 x 801 rows over 1723 keys 54 -> 48 us).  fp32's
+// forward (DIRECT), whose matrix instructions take most of the time, reads the
+// streamed operands from global memory as it goes, and keeps in LDS what the waves
+// share, so that registers and LDS leave room for four waves on a SIMD.
+template <typename T, bool D = false>
 struct SplitLds {
+    static constexpr bool DIRECT = D;
     static constexpr int WAVE = 2 * Tile<T>::BYTES;
+    static constexpr int TILES = DIRECT ? 2 * Tile<T>::BYTES : 4 * WAVE;
     static constexpr int PITCH = CA_D + 4;
     static constexpr int RESULTS = 4 * 32 * PITCH * 4 + 4 * 32 * 8;  // the waves' [32][CA_D] and (m, l), over the tiles
-    static constexpr int BYTES = 4 * WAVE > RESULTS ? 4 * WAVE : RESULTS;
+    static constexpr int BYTES = TILES > RESULTS ? TILES : RESULTS;
     static constexpr int LOADS = CA_TILE / Tile<T>::DMA_ROWS;  // copies of a tile
 };
 // Waits until at most the newest N copies are still under way; none where there is
@@ -504,15 +595,15 @@ VH_DEVICE void scores_packed(const CrossArgs &a, floatx16 &x, const PackedBias &
 }
 
 template <typename T, bool BIAS, bool KEEP, bool PACK>
-__global__ __launch_bounds__(256, 2) void cross_forward_split_kernel(CrossArgs a) {
-    using L = SplitLds<T>;
+__global__ __launch_bounds__(256, sizeof(T) == 4 ? 4 : 2) void cross_forward_split_kernel(CrossArgs a) {
+    using L = SplitLds<T, sizeof(T) == 4>;
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     float *window = reinterpret_cast<float *>(smem + L::BYTES);
     const int G = a.H / a.KV, per = PACK ? G : 1, HH = a.H / per;
     const int rtiles = (int)(((int64_t)a.Lq * per + 31) / 32);
-    const int task = xcd_swizzle((int)blockIdx.x, (int)gridDim.x);
-    const int rt = task % rtiles, part = task / rtiles % a.parts;
-    const int hh = task / rtiles / a.parts % HH, s = task / rtiles / a.parts / HH;
+    int pair, tile;
+    if (!pair_task(a.S * HH, rtiles * a.parts, pair, tile)) return;
+    const int rt = tile % rtiles, part = tile / rtiles, hh = pair % HH, s = pair / HH;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 31, lh = lane >> 5;
     const int kh = PACK ? hh : hh / G;
@@ -537,47 +628,57 @@ __global__ __launch_bounds__(256, 2) void cross_forward_split_kernel(CrossArgs a
         }
         __syncthreads();
     }
-    Frag<T> qf[4];
-    if (active) {
-        const char *qp = a.q.p + s * a.q.seq + (int64_t)min(q, qlen - 1) * a.q.row + head * a.q.head;
-#pragma unroll
-        for (int g = 0; g < 4; g++) {
-            qf[g] = frag_load(reinterpret_cast<const T *>(qp) + 16 * g + 8 * lh);
-            if (a.scale < 0.0f) frag_negate(qf[g]);
-        }
-    }
+    const char *qp = a.q.p + s * a.q.seq + (int64_t)min(q, qlen - 1) * a.q.row + head * a.q.head;
     RowState st;
     st.clear();
     const char *kp = a.k.p + s * a.k.seq + kh * a.k.head, *vp = a.v.p + s * a.v.seq + kh * a.v.head;
-    unsigned char *tile = smem + wave * L::WAVE;
-    const uint32_t lds = (uint32_t)(uintptr_t)tile;
-    const unsigned char *Ks = tile, *Vs = tile + Tile<T>::BYTES;
-    auto issue_k = [&](int t) { tile_issue<T, 1>(kp, a.k.row, 32 * t, klen - 1, lds, 0, lane); };
-    auto issue_v = [&](int t) { tile_issue<T, 1>(vp, a.v.row, 32 * t, klen - 1, lds + Tile<T>::BYTES, 0, lane); };
-    int t = first + wave;
-    if (t < last) {
-        issue_k(t);
-        issue_v(t);
-    }
-    for (; t < last; t += 4) {
-        const bool next = t + 4 < last;
-        const int k0 = 32 * t;
-        floatx16 x;
-        zero16(x);
-        wait_vmcnt<L::LOADS>();  // K is there, V may be under way
-#pragma unroll
-        for (int g = 0; g < 4; g++) frag_mfma(x, tile_row(Ks, li, g, lh, T()), qf[g]);
-        wait_lds();
-        if (next) issue_k(t + 4);
+    const float c = a.scale2;
+    auto weigh = [&](floatx16 &x, int k0) {
         const int lo = k0 - (start + q_hi), hi = k0 + 31 - (start + q_lo);
         if constexpr (BIAS && PACK) scores_packed(a, x, pb, lo, hi, k0 - (start + q), head - kh * G, lh);
         else if constexpr (BIAS) add_bias(a, x, window, lo, hi, k0 - (start + q), 1, lh);
-        softmax_tile<BIAS>(st, x, a.scale2, k0 + 32 > klen || (a.causal && hi > 0),
+        softmax_tile<BIAS>(st, x, c, k0 + 32 > klen || (a.causal && hi > 0),
                            (a.causal ? min(klen, start + q + 1) : klen) - k0, lh);
-        wait_tile<L::LOADS>(next);
-        values_tile<T, BIAS, KEEP>(st, x, Vs, lane);
-        wait_lds();
-        if (next) issue_v(t + 4);
+    };
+    int t = first + wave;
+    if constexpr (L::DIRECT) {
+        if (active) put_row(smem, wave, lane, load_query<T>(a, qp, wave, lh));
+        __syncthreads();
+        const LdsRows<T> w{smem};
+        for (; t < last; t += 4) {
+            const int64_t k0 = 32 * t;
+            floatx16 x;
+            scores(x, GlobalTile{kp + k0 * a.k.row, (uint32_t)a.k.row, klen - 1 - 32 * t}, w, lane);
+            weigh(x, 32 * t);
+            values_tile<T, BIAS, KEEP>(st, x, GlobalTile{vp + k0 * a.v.row, (uint32_t)a.v.row, klen - 1 - 32 * t}, lane);
+        }
+    } else {
+        RegRows<T> w;
+        if (active) {
+#pragma unroll
+            for (int g = 0; g < 4; g++) w.f[g] = load_query<T>(a, qp, g, lh);
+        }
+        const LdsTile<T> K{smem + wave * L::WAVE}, V{K.p + Tile<T>::BYTES};
+        const uint32_t lds = (uint32_t)(uintptr_t)smem + (uint32_t)(wave * L::WAVE);
+        auto issue_k = [&](int t) { tile_issue<T, 1>(kp, a.k.row, 32 * t, klen - 1, lds, 0, lane); };
+        auto issue_v = [&](int t) { tile_issue<T, 1>(vp, a.v.row, 32 * t, klen - 1, lds + Tile<T>::BYTES, 0, lane); };
+        if (t < last) {
+            issue_k(t);
+            issue_v(t);
+        }
+        for (; t < last; t += 4) {
+            const bool next = t + 4 < last;
+            floatx16 x;
+            wait_vmcnt<L::LOADS>();  // K is there, V may be under way
+            scores(x, K, w, lane);
+            wait_lds();
+            if (next) issue_k(t + 4);
+            weigh(x, 32 * t);
+            wait_tile<L::LOADS>(next);
+            values_tile<T, BIAS, KEEP>(st, x, V, lane);
+            wait_lds();
+            if (next) issue_v(t + 4);
+        }
     }
 
     // the four waves' results joined: row tid / 8, dims 8 (tid % 8) .. + 7
@@ -651,7 +752,7 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
         l += v.y * c;
         y += ld4(a.part_o + (p * rows + row) * CA_D + d) * c;
     }
-    const bool seen = q < cross_length(a.query_lengths, s, a.Lq) && (l > 0.0f || l != l);
+    const bool seen = q < (a.query_lengths ? a.query_lengths[s] : a.Lq) && (l > 0.0f || l != l);
     const float inv = seen ? 1.0f / l : 0.0f;
     if (KEEP && d == 0) a.stats[row] = row_stats(BIAS, seen, m, l);
 #pragma unroll
@@ -674,19 +775,16 @@ VH_DEVICE RowStats *row_tile(const CrossArgs &a, int s, int h, int t) {
 
 // Copies a tile's into LDS: 24 lanes of a wave, 16 bytes each.
 VH_DEVICE void row_tile_issue(const RowStats *from, uint32_t lds, int lane) {
-    const uint64_t p = (uint64_t)from;
-    const uint64_t base = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32 |
-                          (uint32_t)__builtin_amdgcn_readfirstlane((int)p);
+    const char *base = uniform(from);
     lds = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds);
-    if (lane < 24) lds_dma16s(16u * (uint32_t)lane, reinterpret_cast<const void *>(base), lds);
+    if (lane < 24) lds_dma16s(16u * (uint32_t)lane, base, lds);
 }
 
 // What a wave's 32 query rows need as columns, besides their tiles.
 template <typename T>
 struct QueryRows {
-    Frag<T> q[4], dout[4];
-    floatx16 delta;  // -delta, dP's product's initial value
-    float m, n;
+    RegRows<T> q, dout;
+    float delta, m, n;  // delta: its negative
 };
 // Rows q (clamped into qlen) of head h; their statistics are also left where `leave`.
 template <typename T, bool BIAS>
@@ -700,23 +798,22 @@ VH_DEVICE void load_rows(const CrossArgs &a, QueryRows<T> &w, int s, int h, int 
 #pragma unroll
     for (int g = 0; g < 4; g++) {
         const int d = 16 * g + 8 * lh;
-        w.q[g] = frag_load(qp + d);
-        if (a.scale < 0.0f) frag_negate(w.q[g]);
-        w.dout[g] = frag_load(dp + d);
+        w.q.f[g] = load_query<T>(a, reinterpret_cast<const char *>(qp), g, lh);
+        w.dout.f[g] = frag_load(dp + d);
         const Frag<T> of = frag_load(op + d);
         if constexpr (sizeof(T) == 2) {
             if constexpr (BIAS) {
                 const Frag<float> rf = frag_load(static_cast<const float *>(a.rest) + row * CA_D + d);
 #pragma unroll
-                for (int e = 0; e < 8; e++) delta += (float)w.dout[g].v[e] * ((float)of.v[e] + rf.v[e >> 2][e & 3]);
+                for (int e = 0; e < 8; e++) delta += (float)w.dout.f[g].v[e] * ((float)of.v[e] + rf.v[e >> 2][e & 3]);
             } else {
                 const Frag<bf16> rf = frag_load(static_cast<const bf16 *>(a.rest) + row * CA_D + d);
 #pragma unroll
-                for (int e = 0; e < 8; e++) delta += (float)w.dout[g].v[e] * ((float)of.v[e] + (float)rf.v[e]);
+                for (int e = 0; e < 8; e++) delta += (float)w.dout.f[g].v[e] * ((float)of.v[e] + (float)rf.v[e]);
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) delta += w.dout[g].v[e >> 2][e & 3] * of.v[e >> 2][e & 3];
+            for (int e = 0; e < 8; e++) delta += w.dout.f[g].v[e >> 2][e & 3] * of.v[e >> 2][e & 3];
         }
     }
     delta = -(delta + __shfl_xor(delta, 32, 64));
@@ -727,8 +824,7 @@ VH_DEVICE void load_rows(const CrossArgs &a, QueryRows<T> &w, int s, int h, int 
     }
     w.m = st.x;
     w.n = st.y;
-#pragma unroll
-    for (int r = 0; r < 16; r++) w.delta[r] = delta;
+    w.delta = delta;
     if (leave && lh == 0) {
         RowStats *to = row_tile(a, s, h, q / CA_TILE);
         to->m[lane] = st.x;
@@ -828,21 +924,18 @@ struct Dbias {
     }
 };
 
-// One tile of keys: dq^T += K^T dS^T, and the table's gradient.  have_k() is called
-// before K is read, had_v() when V has been.
-template <typename T, bool BIAS, typename HaveK, typename HadV>
-VH_DEVICE void dq_tile(const CrossArgs &a, const QueryRows<T> &w, floatx16 (&acc)[2], Dbias &db, const float *window,
-                       const unsigned char *Ks, const unsigned char *Vs, int k0, int pos, int pos_lo, int klen, int wave,
-                       int lane, HaveK have_k, HadV had_v) {
-    const int li = lane & 31, lh = lane >> 5;
-    floatx16 x, dp = w.delta;
-    zero16(x);
-#pragma unroll
-    for (int g = 0; g < 4; g++) frag_mfma(dp, tile_row(Vs, li, g, lh, T()), w.dout[g]);
+// One tile of keys: dq^T += K^T dS^T, and the table's gradient.  dp: -delta, where
+// dP's product begins; have_k() is called before K is read, had_v() when V has been.
+template <typename T, bool BIAS, typename Tile, typename Held, typename HaveK, typename HadV>
+VH_DEVICE void dq_tile(const CrossArgs &a, const QueryRows<T> &w, const Held &q, const Held &dout, floatx16 dp,
+                       floatx16 (&acc)[2], Dbias &db, const float *window, const Tile &K, const Tile &V, int k0, int pos,
+                       int pos_lo, int klen, int wave, int lane, HaveK have_k, HadV had_v) {
+    const int lh = lane >> 5;
+    floatx16 x;
+    dot_tile(dp, V, dout, lane);
     had_v();
     have_k();
-#pragma unroll
-    for (int g = 0; g < 4; g++) frag_mfma(x, tile_row(Ks, li, g, lh, T()), w.q[g]);
+    scores(x, K, q, lane);
     const int lo = k0 - (pos_lo + 31), hi = k0 + 31 - pos_lo;
     const int seen = (a.causal ? min(klen, pos + 1) : klen) - k0;  // rows of the tile that the lane's query sees
     const bool mask = k0 + 32 > klen || (a.causal && hi > 0);
@@ -863,7 +956,7 @@ VH_DEVICE void dq_tile(const CrossArgs &a, const QueryRows<T> &w, floatx16 (&acc
         Frag<T> sb;
         frag_from(sb, x, g);
 #pragma unroll
-        for (int t = 0; t < 2; t++) frag_mfma(acc[t], tile_col(Ks, g, t, lane, T()), sb);
+        for (int t = 0; t < 2; t++) frag_mfma(acc[t], K.col(g, t, lane), sb);
     }
 }
 
@@ -876,8 +969,9 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(CrossArgs a) {
     db.lay(a, smem + 4 * Tile<T>::BYTES, window);
 
     const int qtiles = (a.Lq + 127) / 128;
-    const int task = xcd_swizzle((int)blockIdx.x, (int)gridDim.x);
-    const int qt = task % qtiles, h = task / qtiles % a.H, s = task / qtiles / a.H;
+    int pair, qt;
+    if (!pair_task(a.S * a.H, qtiles, pair, qt)) return;
+    const int h = pair % a.H, s = pair / a.H;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 31, lh = lane >> 5;
     const int kh = h / (a.H / a.KV);
@@ -903,6 +997,9 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(CrossArgs a) {
     }
     QueryRows<T> w;
     if (active) load_rows<T, BIAS>(a, w, s, h, q, qlen, true, lane);
+    floatx16 delta;
+#pragma unroll
+    for (int r = 0; r < 16; r++) delta[r] = w.delta;
     floatx16 acc[2];
     zero16(acc[0]);
     zero16(acc[1]);
@@ -912,9 +1009,9 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(CrossArgs a) {
         wait_vmcnt<0>();
         __syncthreads();
         if (k0 + CA_TILE < keys) issue(k0 + CA_TILE);
-        const unsigned char *Ks = smem + (k0 / CA_TILE & 1) * 2 * Tile<T>::BYTES;
+        const LdsTile<T> K{smem + (k0 / CA_TILE & 1) * 2 * Tile<T>::BYTES}, V{K.p + Tile<T>::BYTES};
         dq_tile<T, BIAS>(
-            a, w, acc, db, window, Ks, Ks + Tile<T>::BYTES, k0, start + q, start + q0, klen, wave, lane, [] {}, [] {});
+            a, w, w.q, w.dout, delta, acc, db, window, K, V, k0, start + q, start + q0, klen, wave, lane, [] {}, [] {});
     }
     for (; k0 < keys; k0 += CA_TILE) {
         wait_vmcnt<0>();
@@ -971,9 +1068,9 @@ __global__ __launch_bounds__(256, 2) void cross_dq_split_kernel(CrossArgs a) {
     db.lay(a, smem + L::BYTES, window);
 
     const int rtiles = (a.Lq + 31) / 32;
-    const int task = xcd_swizzle((int)blockIdx.x, (int)gridDim.x);
-    const int rt = task % rtiles, part = task / rtiles % a.parts;
-    const int h = task / rtiles / a.parts % a.H, s = task / rtiles / a.parts / a.H;
+    int pair, tile;
+    if (!pair_task(a.S * a.H, rtiles * a.parts, pair, tile)) return;
+    const int rt = tile % rtiles, part = tile / rtiles, h = pair % a.H, s = pair / a.H;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int kh = h / (a.H / a.KV);
     const int start = cross_start(a, s);
@@ -991,31 +1088,35 @@ __global__ __launch_bounds__(256, 2) void cross_dq_split_kernel(CrossArgs a) {
     }
     QueryRows<T> w;
     if (q0 < qlen) load_rows<T, BIAS>(a, w, s, h, q, qlen, part == 0 && wave == 0, lane);
-    floatx16 acc[2];
+    floatx16 delta, acc[2];
+#pragma unroll
+    for (int r = 0; r < 16; r++) delta[r] = w.delta;
     zero16(acc[0]);
     zero16(acc[1]);
     const char *kp = a.k.p + s * a.k.seq + kh * a.k.head, *vp = a.v.p + s * a.v.seq + kh * a.v.head;
-    unsigned char *tile = smem + wave * L::WAVE;
-    const uint32_t lds = (uint32_t)(uintptr_t)tile;
-    auto issue_k = [&](int t) { tile_issue<T, 1>(kp, a.k.row, 32 * t, klen - 1, lds, 0, lane); };
-    auto issue_v = [&](int t) { tile_issue<T, 1>(vp, a.v.row, 32 * t, klen - 1, lds + Tile<T>::BYTES, 0, lane); };
     int t = first + wave;
-    if (t < last) {
-        issue_v(t);
-        issue_k(t);
-    }
-    for (; t < last; t += 4) {
-        const bool next = t + 4 < last;
-        wait_vmcnt<L::LOADS>();  // V is there, K may be under way
-        dq_tile<T, BIAS>(
-            a, w, acc, db, window, tile, tile + Tile<T>::BYTES, 32 * t, start + q, start + q0, klen, wave, lane,
-            [&] { wait_tile<L::LOADS>(next); },
-            [&] {
-                wait_lds();
-                if (next) issue_v(t + 4);
-            });
-        wait_lds();
-        if (next) issue_k(t + 4);
+    {
+        const LdsTile<T> K{smem + wave * L::WAVE}, V{K.p + Tile<T>::BYTES};
+        const uint32_t lds = (uint32_t)(uintptr_t)smem + (uint32_t)(wave * L::WAVE);
+        auto issue_k = [&](int t) { tile_issue<T, 1>(kp, a.k.row, 32 * t, klen - 1, lds, 0, lane); };
+        auto issue_v = [&](int t) { tile_issue<T, 1>(vp, a.v.row, 32 * t, klen - 1, lds + Tile<T>::BYTES, 0, lane); };
+        if (t < last) {
+            issue_v(t);
+            issue_k(t);
+        }
+        for (; t < last; t += 4) {
+            const bool next = t + 4 < last;
+            wait_vmcnt<L::LOADS>();  // V is there, K may be under way
+            dq_tile<T, BIAS>(
+                a, w, w.q, w.dout, delta, acc, db, window, K, V, 32 * t, start + q, start + q0, klen, wave, lane,
+                [&] { wait_tile<L::LOADS>(next); },
+                [&] {
+                    wait_lds();
+                    if (next) issue_v(t + 4);
+                });
+            wait_lds();
+            if (next) issue_k(t + 4);
+        }
     }
     if constexpr (BIAS) {
         if (a.dbias_part) db.finish(a, h, (s * rtiles + rt) * a.parts + part, tid);
@@ -1039,47 +1140,49 @@ __global__ __launch_bounds__(256, 2) void cross_dq_split_kernel(CrossArgs a) {
     st4(out + 4, y[1]);
 }
 
-// A wave's 32 keys as columns, and their gradients' sums.
+// A wave's 32 keys as columns: fragments g of k (of the scale's sign) and of v, and
+// their gradients' sums.
 template <typename T>
 struct KeyRows {
-    Frag<T> k[4], v[4];
+    RegRows<T> k, v;
+};
+struct KeySums {
     floatx16 dk[2], dv[2];
+    VH_DEVICE void clear() {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            zero16(dk[t]);
+            zero16(dv[t]);
+        }
+    }
 };
 template <typename T>
 VH_DEVICE void load_keys(const CrossArgs &a, KeyRows<T> &w, int s, int kh, int key, int klen, int lh) {
-#pragma unroll
-    for (int t = 0; t < 2; t++) {
-        zero16(w.dk[t]);
-        zero16(w.dv[t]);
-    }
     if (klen <= 0) return;
     const int64_t kr = min(key, klen - 1);
     const T *kp = reinterpret_cast<const T *>(a.k.p + s * a.k.seq + kr * a.k.row + kh * a.k.head);
     const T *vp = reinterpret_cast<const T *>(a.v.p + s * a.v.seq + kr * a.v.row + kh * a.v.head);
 #pragma unroll
     for (int g = 0; g < 4; g++) {
-        w.k[g] = frag_load(kp + 16 * g + 8 * lh);
-        if (a.scale < 0.0f) frag_negate(w.k[g]);
-        w.v[g] = frag_load(vp + 16 * g + 8 * lh);
+        w.k.f[g] = load_query<T>(a, reinterpret_cast<const char *>(kp), g, lh);
+        w.v.f[g] = frag_load(vp + 16 * g + 8 * lh);
     }
 }
+
 // One tile of queries: S = Q K^T with the keys as columns, so that P and dS are B
 // operands of dv^T += dout^T P and dk^T += Q^T dS as they are.  have_q() is called
 // before Q is read, had_dout() when dout and the statistics have been.
-template <typename T, bool BIAS, typename HaveQ, typename HadDout>
-VH_DEVICE void dkv_tile(const CrossArgs &a, KeyRows<T> &w, const float *window, const unsigned char *Qs,
-                        const unsigned char *Ds, const RowStats *rs, int q0, int start, int key, int k0, int lane,
-                        HaveQ have_q, HadDout had_dout) {
-    const int li = lane & 31, lh = lane >> 5;
+template <typename T, bool BIAS, typename Tile, typename Held, typename HaveQ, typename HadDout>
+VH_DEVICE void dkv_tile(const CrossArgs &a, const Held &k, const Held &v, KeySums &w, const float *window, const Tile &Q,
+                        const Tile &D, const RowStats *rs, int q0, int start, int key, int k0, int lane, HaveQ have_q,
+                        HadDout had_dout) {
+    const int lh = lane >> 5;
     floatx16 x, dp;
-    zero16(x);
 #pragma unroll
     for (int r = 0; r < 16; r++) dp[r] = rs->delta[row_of(r, lh)];
-#pragma unroll
-    for (int g = 0; g < 4; g++) frag_mfma(dp, tile_row(Ds, li, g, lh, T()), w.v[g]);
+    dot_tile(dp, D, v, lane);
     have_q();
-#pragma unroll
-    for (int g = 0; g < 4; g++) frag_mfma(x, tile_row(Qs, li, g, lh, T()), w.k[g]);
+    scores(x, Q, k, lane);
     const int lo = k0 - (start + q0 + 31), hi = k0 + 31 - (start + q0);
     if constexpr (BIAS) add_bias(a, x, window, lo, hi, key - (start + q0), -1, lh);
 #pragma unroll
@@ -1099,7 +1202,7 @@ VH_DEVICE void dkv_tile(const CrossArgs &a, KeyRows<T> &w, const float *window, 
         Frag<T> pb;
         frag_from(pb, x, g);
 #pragma unroll
-        for (int t = 0; t < 2; t++) frag_mfma(w.dv[t], tile_col(Ds, g, t, lane, T()), pb);
+        for (int t = 0; t < 2; t++) frag_mfma(w.dv[t], D.col(g, t, lane), pb);
     }
     had_dout();
 #pragma unroll
@@ -1107,7 +1210,7 @@ VH_DEVICE void dkv_tile(const CrossArgs &a, KeyRows<T> &w, const float *window, 
         Frag<T> sb;
         frag_from(sb, dp, g);
 #pragma unroll
-        for (int t = 0; t < 2; t++) frag_mfma(w.dk[t], tile_col(Qs, g, t, lane, T()), sb);
+        for (int t = 0; t < 2; t++) frag_mfma(w.dk[t], Q.col(g, t, lane), sb);
     }
 }
 
@@ -1120,8 +1223,9 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(CrossArgs a) {
     float *window = reinterpret_cast<float *>(rs + 2);                       // [2]: of two heads in turn
 
     const int ktiles = (a.Lk + 127) / 128;
-    const int task = xcd_swizzle((int)blockIdx.x, (int)gridDim.x);
-    const int kt = task % ktiles, kh = task / ktiles % a.KV, s = task / ktiles / a.KV;
+    int pair, kt;
+    if (!pair_task(a.S * a.KV, ktiles, pair, kt)) return;
+    const int kh = pair % a.KV, s = pair / a.KV;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 31, lh = lane >> 5;
     const int start = cross_start(a, s);
@@ -1148,6 +1252,8 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(CrossArgs a) {
     if (first < qlen) issue(kh * G, first, 0);
     KeyRows<T> w;
     load_keys(a, w, s, kh, key, klen, lh);
+    KeySums sums;
+    sums.clear();
     int buf = 0;
     for (int g = 0; g < G; g++) {
         // the window before last is free: its head's tiles ended a barrier ago
@@ -1163,9 +1269,9 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(CrossArgs a) {
         for (; q0 < mine; q0 += CA_TILE, buf ^= 1) begin(q0);
         for (; q0 < qlen; q0 += CA_TILE, buf ^= 1) {
             begin(q0);
-            const unsigned char *Qs = smem + buf * 2 * Tile<T>::BYTES;
+            const LdsTile<T> Q{smem + buf * 2 * Tile<T>::BYTES}, D{Q.p + Tile<T>::BYTES};
             dkv_tile<T, BIAS>(
-                a, w, bias, Qs, Qs + Tile<T>::BYTES, rs + buf, q0, start, key, k0, lane, [] {}, [] {});
+                a, w.k, w.v, sums, bias, Q, D, rs + buf, q0, start, key, k0, lane, [] {}, [] {});
         }
     }
     if (key >= a.Lk) return;
@@ -1178,8 +1284,8 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(CrossArgs a) {
             floatx4 y, z;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                y[r] = key < klen ? w.dk[t][4 * rq + r] * a.scale : 0.0f;
-                z[r] = key < klen ? w.dv[t][4 * rq + r] : 0.0f;
+                y[r] = key < klen ? sums.dk[t][4 * rq + r] * a.scale : 0.0f;
+                z[r] = key < klen ? sums.dv[t][4 * rq + r] : 0.0f;
             }
             st4(pk + 32 * t + 8 * rq + 4 * lh, y);
             st4(pv + 32 * t + 8 * rq + 4 * lh, z);
@@ -1197,9 +1303,9 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_split_kernel(CrossArgs a) {
     float *window = reinterpret_cast<float *>(stats + 4);
 
     const int ktiles = (a.Lk + 31) / 32, G = a.H / a.KV;
-    const int task = xcd_swizzle((int)blockIdx.x, (int)gridDim.x);
-    const int kt = task % ktiles, part = task / ktiles % a.kv_parts;
-    const int h = task / ktiles / a.kv_parts % a.H, s = task / ktiles / a.kv_parts / a.H;
+    int pair, tile;
+    if (!pair_task(a.S * a.H, ktiles * a.kv_parts, pair, tile)) return;
+    const int kt = tile % ktiles, part = tile / ktiles, h = pair % a.H, s = pair / a.H;
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lh = lane >> 5, kh = h / G;
     const int start = cross_start(a, s);
@@ -1214,37 +1320,41 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_split_kernel(CrossArgs a) {
         fill_bias_window(a, h, window, tid);
         __syncthreads();
     }
-    KeyRows<T> w;
-    load_keys(a, w, s, kh, key, klen, lh);
+    KeySums sums;
+    sums.clear();
     const char *qp = a.q.p + s * a.q.seq + h * a.q.head, *dp = a.dout.p + s * a.dout.seq + h * a.dout.head;
-    unsigned char *tile = smem + wave * L::WAVE;
-    const uint32_t lds = (uint32_t)(uintptr_t)tile;
-    RowStats *rs = stats + wave;
-    auto issue_q = [&](int t) { tile_issue<T, 1>(qp, a.q.row, 32 * t, qlen - 1, lds, 0, lane); };
-    auto issue_dout = [&](int t) {
-        tile_issue<T, 1>(dp, a.dout.row, 32 * t, qlen - 1, lds + Tile<T>::BYTES, 0, lane);
-        row_tile_issue(row_tile(a, s, h, t), (uint32_t)(uintptr_t)rs, lane);
-    };
     int t = first + wave;
-    if (t < last) {
-        issue_dout(t);
-        issue_q(t);
-    }
-    for (; t < last; t += 4) {
-        const bool next = t + 4 < last;
-        wait_vmcnt<L::LOADS>();  // dout is there, Q may be under way
-        dkv_tile<T, BIAS>(
-            a, w, window, tile, tile + Tile<T>::BYTES, rs, 32 * t, start, key, k0, lane, [&] { wait_vmcnt<0>(); },
-            [&] {
-                wait_lds();
-                if (next) issue_dout(t + 4);
-            });
-        wait_lds();
-        if (next) issue_q(t + 4);
+    {
+        KeyRows<T> w;
+        load_keys(a, w, s, kh, key, klen, lh);
+        const LdsTile<T> Q{smem + wave * L::WAVE}, D{Q.p + Tile<T>::BYTES};
+        const uint32_t lds = (uint32_t)(uintptr_t)smem + (uint32_t)(wave * L::WAVE);
+        RowStats *rs = stats + wave;
+        auto issue_q = [&](int t) { tile_issue<T, 1>(qp, a.q.row, 32 * t, qlen - 1, lds, 0, lane); };
+        auto issue_dout = [&](int t) {
+            tile_issue<T, 1>(dp, a.dout.row, 32 * t, qlen - 1, lds + Tile<T>::BYTES, 0, lane);
+            row_tile_issue(row_tile(a, s, h, t), (uint32_t)(uintptr_t)rs, lane);
+        };
+        if (t < last) {
+            issue_dout(t);
+            issue_q(t);
+        }
+        for (; t < last; t += 4) {
+            const bool next = t + 4 < last;
+            wait_vmcnt<L::LOADS>();  // dout is there, Q may be under way
+            dkv_tile<T, BIAS>(
+                a, w.k, w.v, sums, window, Q, D, rs, 32 * t, start, key, k0, lane, [&] { wait_vmcnt<0>(); },
+                [&] {
+                    wait_lds();
+                    if (next) issue_dout(t + 4);
+                });
+            wait_lds();
+            if (next) issue_q(t + 4);
+        }
     }
     floatx4 y[2], z[2];
-    waves_sum<T>(reinterpret_cast<float *>(smem), w.dk, tid, y);
-    waves_sum<T>(reinterpret_cast<float *>(smem), w.dv, tid, z);
+    waves_sum<T>(reinterpret_cast<float *>(smem), sums.dk, tid, y);
+    waves_sum<T>(reinterpret_cast<float *>(smem), sums.dv, tid, z);
     const int ok = k0 + (tid >> 3), d = 8 * (tid & 7);
     if (ok >= a.Lk) return;
 #pragma unroll
