@@ -9,9 +9,12 @@
 //   (dk and dv summed over the query heads that share the key head), and
 //   dtable[b][h] = sum of dS over the pairs whose bucket is b.
 //
-// T is the type of the tensors, fp32 or bf16.  Every product runs on the matrix
-// cores in 32 x 32 tiles with fp32 accumulation, the statistics, the
-// exponentials and dS are fp32.  bf16 operands are the tensors as they are;
+// T is the type of the tensors, fp32 or bf16.  Every product runs on the bf16 matrix
+// cores in 32 x 32 tiles with fp32 accumulation; the statistics, the exponentials
+// and dS are fp32.  fp32 operands are the exact sums of three bf16 pieces each
+// (gemm_split.hpp), multiplied in the six products of pieces that reach 2^-24 of
+// the whole: six instructions of 32 cycles where the fp32 one takes eight of 64,
+// beside 5.5 others a value to split it.  bf16 operands are the tensors as they are;
 // P and dS are rounded to bf16 (by up to 2^-8 of themselves, as the outputs are)
 // where they enter a product, and nowhere else: scale, bias, statistics and the
 // table's gradient see the fp32 values.  delta stands for the sum of P dP, and out
@@ -27,18 +30,17 @@
 // score (a negative scale turns q's, or k's, sign instead); with a bias as s c + b
 // log2(e), where a finite b stays finite.
 //
-// Operand order (both types).  v_mfma_f32_32x32x16_bf16 takes 8 values of the
-// summed index per lane: lane (li = l % 32, lh = l / 32) holds row or column li
-// and indexes 8 lh + e of a group of 16.  fp32 runs the same group as eight
-// v_mfma_f32_32x32x2_f32, the e-th on every lane's e-th value: the groups' terms
-// come in another order, so fragments are loaded alike for both types.  A result
-// holds column li and rows 8 (r / 4) + 4 lh + r % 4; its registers 8 st .. 8 st + 7
-// are therefore a B operand over rows {16 st + 4 lh + 0..3, 16 st + 8 + 4 lh +
-// 0..3}, and the A operand beside it is read from LDS transposed in that order.
+// Operand order.  v_mfma_f32_32x32x16_bf16 takes 8 values of the summed index per
+// lane: lane (li = l % 32, lh = l / 32) holds row or column li and indexes 8 lh + e
+// of a group of 16.  A result holds column li and rows 8 (r / 4) + 4 lh + r % 4; its
+// registers 8 st .. 8 st + 7 are therefore a B operand over rows {16 st + 4 lh +
+// 0..3, 16 st + 8 + 4 lh + 0..3}, and the A operand beside it is read transposed in
+// that order.
 #pragma once
 
 #include "attention.hpp"
 #include "gemm_bf16.hpp"
+#include "gemm_split.hpp"
 
 namespace vh {
 
@@ -109,11 +111,31 @@ struct Frag<float> {
 VH_DEVICE void frag_mfma(floatx16 &acc, const Frag<bf16> &a, const Frag<bf16> &b) {
     acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, acc, 0, 0, 0);
 }
-VH_DEVICE void frag_mfma(floatx16 &acc, const Frag<float> &a, const Frag<float> &b) {
+// fp32's in three bf16 pieces, the largest first.
+struct Pieces {
+    bf16x8 p[3];
+};
+VH_DEVICE void frag_mfma(floatx16 &acc, const Pieces &a, const Pieces &b) {
+    constexpr int ia[6] = {2, 0, 1, 1, 0, 0}, ib[6] = {0, 2, 1, 0, 1, 0};  // small products first
 #pragma unroll
-    for (int e = 0; e < 8; e++)
-        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[e >> 2][e & 3], b.v[e >> 2][e & 3], acc, 0, 0, 0);
+    for (int i = 0; i < 6; i++)
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[ia[i]], b.p[ib[i]], acc, 0, 0, 0);
 }
+// What a product takes for a fragment.
+VH_DEVICE const Frag<bf16> &operand(const Frag<bf16> &f) { return f; }
+VH_DEVICE Pieces operand(const Frag<float> &f) {
+    Pieces o;
+    split8(f.v[0], f.v[1], o.p[0], o.p[1], o.p[2]);
+    return o;
+}
+template <typename T>
+struct Operand {
+    typedef Frag<bf16> type;
+};
+template <>
+struct Operand<float> {
+    typedef Pieces type;
+};
 
 // 8 consecutive elements of global memory.
 VH_DEVICE Frag<bf16> frag_load(const bf16 *p) { return {*reinterpret_cast<const bf16x8 *>(p)}; }
@@ -251,21 +273,24 @@ struct GlobalTile {
 // The operand that stays: 32 rows in registers, or in a tile of LDS.
 template <typename T>
 struct RegRows {
-    Frag<T> f[4];
-    VH_DEVICE const Frag<T> &get(int g, int) const { return f[g]; }
+    typename Operand<T>::type f[4];
+    VH_DEVICE const typename Operand<T>::type &get(int g, int) const { return f[g]; }
 };
-template <typename T>
-struct LdsRows {
-    const unsigned char *p;
-    VH_DEVICE Frag<T> get(int g, int lane) const { return tile_row(p, lane & 31, g, lane >> 5, T()); }
+struct LdsPieces {
+    const unsigned char *p;  // three bf16 tiles
+    VH_DEVICE Pieces get(int g, int lane) const {
+        Pieces o;
+#pragma unroll
+        for (int i = 0; i < 3; i++) o.p[i] = tile_row(p + i * Tile<bf16>::BYTES, lane & 31, g, lane >> 5, bf16()).v;
+        return o;
+    }
 };
-// Dims 16 g + 8 lh .. + 7 of row li into a tile.
-VH_DEVICE void put_row(unsigned char *t, int g, int lane, const Frag<float> &f) {
-    using L = Tile<float>;
-    unsigned char *p = t + (lane & 31) * L::ROW;
-    const int c = 4 * g + 2 * (lane >> 5), z = L::swz(lane & 31);
-    *reinterpret_cast<floatx4 *>(p + 16 * (c ^ z)) = f.v[0];
-    *reinterpret_cast<floatx4 *>(p + 16 * ((c + 1) ^ z)) = f.v[1];
+// Dims 16 g + 8 lh .. + 7 of row li into them.
+VH_DEVICE void put_row(unsigned char *t, int g, int lane, const Pieces &o) {
+    using L = Tile<bf16>;
+    unsigned char *p = t + (lane & 31) * L::ROW + 16 * ((2 * g + (lane >> 5)) ^ L::swz(lane & 31));
+#pragma unroll
+    for (int i = 0; i < 3; i++) *reinterpret_cast<bf16x8 *>(p + i * L::BYTES) = o.p[i];
 }
 
 // The same pointer, in scalar registers: the wave's lanes all have it.
@@ -380,7 +405,7 @@ VH_DEVICE Frag<T> load_query(const CrossArgs &a, const char *row, int g, int lh)
 template <typename Tile, typename Held>
 VH_DEVICE void dot_tile(floatx16 &x, const Tile &tile, const Held &held, int lane) {
 #pragma unroll
-    for (int g = 0; g < 4; g++) frag_mfma(x, tile.row(g, lane), held.get(g, lane));
+    for (int g = 0; g < 4; g++) frag_mfma(x, operand(tile.row(g, lane)), held.get(g, lane));
 }
 template <typename Tile, typename Held>
 VH_DEVICE void scores(floatx16 &x, const Tile &tile, const Held &held, int lane) {
@@ -428,12 +453,14 @@ template <typename T, bool BIAS, bool KEEP, typename Tile>
 VH_DEVICE void values_tile(RowState &st, floatx16 &x, const Tile &v, int lane) {
 #pragma unroll
     for (int g = 0; g < 2; g++) {
-        Frag<T> pb, vf[2];
+        Frag<T> pb;
         frag_from(pb, x, g);
+        typename Operand<T>::type vf[2];
+        const auto po = operand(pb);
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            vf[t] = v.col(g, t, lane);
-            frag_mfma(st.o[t], vf[t], pb);
+            vf[t] = operand(v.col(g, t, lane));
+            frag_mfma(st.o[t], vf[t], po);
         }
         if constexpr (KEEP && sizeof(T) == 2) {
 #pragma unroll
@@ -501,7 +528,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) void cross_forward_ker
     if (active) {
         const char *qp = a.q.p + s * a.q.seq + (int64_t)min(q, qlen - 1) * a.q.row + h * a.q.head;
 #pragma unroll
-        for (int g = 0; g < 4; g++) w.f[g] = load_query<T>(a, qp, g, lh);
+        for (int g = 0; g < 4; g++) w.f[g] = operand(load_query<T>(a, qp, g, lh));
     }
     RowState st;
     st.clear();
@@ -552,14 +579,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) void cross_forward_ker
 // within a query, so that single tokens of shared heads fill it.  A wave has one
 // place for either tile and starts the next one's copies as soon as it has read the
 // last: half the LDS of two places (8 x 801 rows over 1723 keys 54 -> 48 us).  fp32's
-// forward (DIRECT), whose matrix instructions take most of the time, reads the
-// streamed operands from global memory as it goes, and keeps in LDS what the waves
-// share, so that registers and LDS leave room for four waves on a SIMD.
+// forward (DIRECT) reads the streamed operands from global memory as it goes, and
+// keeps in LDS the pieces of q, which the waves share, so that registers and LDS
+// leave room for four waves on a SIMD.
 template <typename T, bool D = false>
 struct SplitLds {
     static constexpr bool DIRECT = D;
     static constexpr int WAVE = 2 * Tile<T>::BYTES;
-    static constexpr int TILES = DIRECT ? 2 * Tile<T>::BYTES : 4 * WAVE;
+    static constexpr int TILES = DIRECT ? 3 * Tile<bf16>::BYTES : 4 * WAVE;
     static constexpr int PITCH = CA_D + 4;
     static constexpr int RESULTS = 4 * 32 * PITCH * 4 + 4 * 32 * 8;  // the waves' [32][CA_D] and (m, l), over the tiles
     static constexpr int BYTES = TILES > RESULTS ? TILES : RESULTS;
@@ -642,9 +669,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 4 : 2) void cross_forward_spl
     };
     int t = first + wave;
     if constexpr (L::DIRECT) {
-        if (active) put_row(smem, wave, lane, load_query<T>(a, qp, wave, lh));
+        if (active) put_row(smem, wave, lane, operand(load_query<T>(a, qp, wave, lh)));
         __syncthreads();
-        const LdsRows<T> w{smem};
+        const LdsPieces w{smem};
         for (; t < last; t += 4) {
             const int64_t k0 = 32 * t;
             floatx16 x;
@@ -656,7 +683,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 4 : 2) void cross_forward_spl
         RegRows<T> w;
         if (active) {
 #pragma unroll
-            for (int g = 0; g < 4; g++) w.f[g] = load_query<T>(a, qp, g, lh);
+            for (int g = 0; g < 4; g++) w.f[g] = operand(load_query<T>(a, qp, g, lh));
         }
         const LdsTile<T> K{smem + wave * L::WAVE}, V{K.p + Tile<T>::BYTES};
         const uint32_t lds = (uint32_t)(uintptr_t)smem + (uint32_t)(wave * L::WAVE);
@@ -798,22 +825,23 @@ VH_DEVICE void load_rows(const CrossArgs &a, QueryRows<T> &w, int s, int h, int 
 #pragma unroll
     for (int g = 0; g < 4; g++) {
         const int d = 16 * g + 8 * lh;
-        w.q.f[g] = load_query<T>(a, reinterpret_cast<const char *>(qp), g, lh);
-        w.dout.f[g] = frag_load(dp + d);
+        w.q.f[g] = operand(load_query<T>(a, reinterpret_cast<const char *>(qp), g, lh));
+        const Frag<T> df = frag_load(dp + d);
+        w.dout.f[g] = operand(df);
         const Frag<T> of = frag_load(op + d);
         if constexpr (sizeof(T) == 2) {
             if constexpr (BIAS) {
                 const Frag<float> rf = frag_load(static_cast<const float *>(a.rest) + row * CA_D + d);
 #pragma unroll
-                for (int e = 0; e < 8; e++) delta += (float)w.dout.f[g].v[e] * ((float)of.v[e] + rf.v[e >> 2][e & 3]);
+                for (int e = 0; e < 8; e++) delta += (float)df.v[e] * ((float)of.v[e] + rf.v[e >> 2][e & 3]);
             } else {
                 const Frag<bf16> rf = frag_load(static_cast<const bf16 *>(a.rest) + row * CA_D + d);
 #pragma unroll
-                for (int e = 0; e < 8; e++) delta += (float)w.dout.f[g].v[e] * ((float)of.v[e] + (float)rf.v[e]);
+                for (int e = 0; e < 8; e++) delta += (float)df.v[e] * ((float)of.v[e] + (float)rf.v[e]);
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) delta += w.dout.f[g].v[e >> 2][e & 3] * of.v[e >> 2][e & 3];
+            for (int e = 0; e < 8; e++) delta += df.v[e >> 2][e & 3] * of.v[e >> 2][e & 3];
         }
     }
     delta = -(delta + __shfl_xor(delta, 32, 64));
@@ -955,8 +983,9 @@ VH_DEVICE void dq_tile(const CrossArgs &a, const QueryRows<T> &w, const Held &q,
     for (int g = 0; g < 2; g++) {
         Frag<T> sb;
         frag_from(sb, x, g);
+        const auto so = operand(sb);
 #pragma unroll
-        for (int t = 0; t < 2; t++) frag_mfma(acc[t], K.col(g, t, lane), sb);
+        for (int t = 0; t < 2; t++) frag_mfma(acc[t], operand(K.col(g, t, lane)), so);
     }
 }
 
@@ -1164,8 +1193,8 @@ VH_DEVICE void load_keys(const CrossArgs &a, KeyRows<T> &w, int s, int kh, int k
     const T *vp = reinterpret_cast<const T *>(a.v.p + s * a.v.seq + kr * a.v.row + kh * a.v.head);
 #pragma unroll
     for (int g = 0; g < 4; g++) {
-        w.k.f[g] = load_query<T>(a, reinterpret_cast<const char *>(kp), g, lh);
-        w.v.f[g] = frag_load(vp + 16 * g + 8 * lh);
+        w.k.f[g] = operand(load_query<T>(a, reinterpret_cast<const char *>(kp), g, lh));
+        w.v.f[g] = operand(frag_load(vp + 16 * g + 8 * lh));
     }
 }
 
@@ -1201,16 +1230,18 @@ VH_DEVICE void dkv_tile(const CrossArgs &a, const Held &k, const Held &v, KeySum
     for (int g = 0; g < 2; g++) {
         Frag<T> pb;
         frag_from(pb, x, g);
+        const auto po = operand(pb);
 #pragma unroll
-        for (int t = 0; t < 2; t++) frag_mfma(w.dv[t], D.col(g, t, lane), pb);
+        for (int t = 0; t < 2; t++) frag_mfma(w.dv[t], operand(D.col(g, t, lane)), po);
     }
     had_dout();
 #pragma unroll
     for (int g = 0; g < 2; g++) {
         Frag<T> sb;
         frag_from(sb, dp, g);
+        const auto so = operand(sb);
 #pragma unroll
-        for (int t = 0; t < 2; t++) frag_mfma(w.dk[t], Q.col(g, t, lane), sb);
+        for (int t = 0; t < 2; t++) frag_mfma(w.dk[t], operand(Q.col(g, t, lane)), so);
     }
 }
 
