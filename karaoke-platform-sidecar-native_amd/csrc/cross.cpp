@@ -16,10 +16,24 @@ namespace vh {
 
 // --------------------------------------------------------------- layer norm
 constexpr int LN_MAX_DIM = 16384;
-// Workgroups of the backward pass: each keeps its rows' weight gradients, so
-// more of them are more sums to add up afterwards.
+// A row's lanes.  Forward: 16 of a wave while 32 elements of bf16, 16 of fp32, a lane
+// hold the row (four rows share a reduction; 49662 x 384 bf16 17 us against a wave's
+// 19, 16000 x 256 5.5 against 7.7); backward, whose sums for the weights fill the
+// registers, up to 128 columns (49662 x 384 bf16 61 us against 51).  A wave up to
+// 2048 columns, 256 up to 8192 (2400 of them bf16 75 us against 1024 lanes' 91),
+// then 1024; the next more where rows of these are too few to fill the chip (800 x
+// 1500 bf16 16 us against 19).
+static int layernorm_lanes(int type, int64_t rows, int dim, bool backward) {
+    const bool few = rows < 4096;
+    if (dim <= 16 || (dim <= (backward ? 128 : type == VH_TYPE_BF16 ? 512 : 256) && !few)) return 16;
+    if (dim <= 512 || (dim <= 2048 && !few)) return 64;
+    return dim <= 8192 ? 256 : 1024;
+}
+// Workgroups of the backward pass: each keeps its rows' weight gradients, so more
+// of them are more sums to add up afterwards.
 static int layernorm_parts(int64_t rows, int dim) {
-    return (int)std::min<int64_t>(dim <= 1024 ? (rows + 7) / 8 : rows, 512);
+    const int lanes = layernorm_lanes(VH_TYPE_FP32, rows, dim, true), per = lanes > 64 ? 1 : 512 / lanes;
+    return (int)std::min<int64_t>((rows + per - 1) / per, 512);
 }
 
 static bool layernorm_ok(const char *what, int type, int64_t rows, int dim, std::initializer_list<int64_t> pitches) {
@@ -43,25 +57,41 @@ size_t layernorm_workspace_bytes(int64_t rows, int dim) {
 
 template <typename T, int LANES, int N, int NV>
 static void layernorm_launch(hipStream_t s, const NormArgs &a, bool backward, int parts) {
-    using S = NormShape<LANES>;
+    using S = NormShape<LANES, N, NV>;
     if (backward)
         hipLaunchKernelGGL((layernorm_backward_kernel<T, LANES, N, NV>), dim3((unsigned)parts), dim3(S::THREADS), 0, s, a);
     else
         hipLaunchKernelGGL((layernorm_kernel<T, LANES, N, NV>), dim3((unsigned)((a.rows + S::ROWS - 1) / S::ROWS)),
                            dim3(S::THREADS), 0, s, a);
 }
-
-// 16 bytes a lane and load (8 where a row is short), a wave a row up to 1024.
+// E: the lane's elements, in loads of 16 bytes.
+template <typename T, int LANES, int E>
+static void layernorm_elements(hipStream_t s, const NormArgs &a, bool backward, int parts) {
+    constexpr int N = 16 / sizeof(T);
+    layernorm_launch<T, LANES, N, E / N>(s, a, backward, parts);
+}
 template <typename T>
 static void layernorm_dispatch(hipStream_t s, const NormArgs &a, bool backward, int parts) {
-    constexpr int N = 16 / sizeof(T);
-    const int d = a.dim;
-    if (d <= 256) layernorm_launch<T, 64, 4, 1>(s, a, backward, parts);
-    else if (d <= 512) layernorm_launch<T, 64, N, 8 / N>(s, a, backward, parts);
-    else if (d <= 1024) layernorm_launch<T, 64, N, 16 / N>(s, a, backward, parts);
-    else if (d <= 2048) layernorm_launch<T, 256, N, 8 / N>(s, a, backward, parts);
-    else if (d <= 4096) layernorm_launch<T, 256, N, 16 / N>(s, a, backward, parts);
-    else layernorm_launch<T, 1024, N, 16 / N>(s, a, backward, parts);
+    const int type = sizeof(T) == 2 ? VH_TYPE_BF16 : VH_TYPE_FP32;
+    const int d = a.dim, lanes = layernorm_lanes(type, a.rows, d, backward), e = (d + lanes - 1) / lanes;
+    if (d < (int)(16 / sizeof(T))) layernorm_launch<T, 16, 1, 1>(s, a, backward, parts);
+    else if (lanes == 16) {
+        if (e <= 8) layernorm_elements<T, 16, 8>(s, a, backward, parts);
+        else if (e <= 16) layernorm_elements<T, 16, 16>(s, a, backward, parts);
+        else if (e <= 24) layernorm_elements<T, 16, 24>(s, a, backward, parts);
+        else layernorm_elements<T, 16, 32>(s, a, backward, parts);
+    } else if (lanes == 64) {
+        if (e <= 8) layernorm_elements<T, 64, 8>(s, a, backward, parts);
+        else if (e <= 16) layernorm_elements<T, 64, 16>(s, a, backward, parts);
+        else if (e <= 24) layernorm_elements<T, 64, 24>(s, a, backward, parts);
+        else layernorm_elements<T, 64, 32>(s, a, backward, parts);
+    } else if (lanes == 256) {
+        if (e <= 8) layernorm_elements<T, 256, 8>(s, a, backward, parts);
+        else if (e <= 16) layernorm_elements<T, 256, 16>(s, a, backward, parts);
+        else layernorm_elements<T, 256, 32>(s, a, backward, parts);
+    } else {
+        layernorm_elements<T, 1024, 16>(s, a, backward, parts);
+    }
 }
 
 bool layernorm(hipStream_t s, const LayerNorm &n, KernelTimer *t) {
