@@ -178,6 +178,7 @@ static void bias_args(CrossArgs &a, int buckets, int max_distance, int bidirecti
     a.side = bidirectional ? buckets / 2 : buckets;
     a.near = a.side / 2;
     a.edges = bucket_edges(a.side, a.near, max_distance, a.edge);
+    a.per_octave = (float)a.edges / log2f((float)max_distance / (float)a.near);
 }
 
 int relative_bucket(int rel, int buckets, int max_distance, int bidirectional) {

@@ -82,17 +82,23 @@ struct CrossArgs {
     float *dbias;       // [buckets][H]
     // far buckets of one side: bucket near + i begins at distance edge[i]
     int side, near, edges;
+    float per_octave;  // far buckets in a doubling of the distance
     int edge[CA_MAX_BUCKETS];
 };
 
+// Bucket of a distance on its side: its place among the edges, guessed by their
+// logarithm and put right by the edges themselves.
+VH_HOST_DEVICE inline int side_bucket(const CrossArgs &a, int n) {
+    if (n < a.near) return n;
+    int i = (int)(log2f((float)n / (float)a.near) * a.per_octave);
+    i = i < 0 ? 0 : i > a.edges - 1 ? a.edges - 1 : i;
+    while (i > 0 && n < a.edge[i]) i--;
+    while (i + 1 < a.edges && n >= a.edge[i + 1]) i++;
+    return a.near + i;
+}
 // Bucket of a relative position (key's minus query's).
 VH_HOST_DEVICE inline int cross_bucket(const CrossArgs &a, int rel) {
-    const int n = rel < 0 ? -rel : a.bidirectional ? rel : 0;
-    int b = n;
-    if (n >= a.near) {
-        b = a.near - 1;
-        for (int i = 0; i < a.edges; i++) b += n >= a.edge[i] ? 1 : 0;
-    }
+    const int b = side_bucket(a, rel < 0 ? -rel : a.bidirectional ? rel : 0);
     return a.bidirectional && rel > 0 ? b + a.side : b;
 }
 
@@ -351,13 +357,21 @@ VH_DEVICE float bias_log2(float b) {
     const float y = b * CA_LOG2E;
     return __builtin_isinf(y) && !__builtin_isinf(b) ? __builtin_copysignf(3.402823466e38f, b) : y;
 }
+// bias(i, bucket): place i of the window, both sides of every distance at once.
+template <typename Fill>
+VH_DEVICE void fill_window(const CrossArgs &a, int tid, Fill fill) {
+    const int zero = a.max_distance + CA_PAD;
+    for (int n = tid; n <= zero; n += 256) {
+        const int b = side_bucket(a, n);
+        fill(zero - n, b);
+        if (n) fill(zero + n, a.bidirectional ? b + a.side : 0);
+    }
+}
 VH_DEVICE void fill_bias_window(const CrossArgs &a, int h, float *window, int tid) {
-    for (int i = tid; i < cross_window(a); i += 256)
-        window[i] = bias_log2(a.table[(int64_t)cross_bucket(a, i - a.max_distance - CA_PAD) * a.H + h]);
+    fill_window(a, tid, [&](int i, int b) { window[i] = bias_log2(a.table[(int64_t)b * a.H + h]); });
 }
 VH_DEVICE void fill_bucket_window(const CrossArgs &a, unsigned char *window, int tid) {
-    for (int i = tid; i < cross_window(a); i += 256)
-        window[i] = (unsigned char)cross_bucket(a, i - a.max_distance - CA_PAD);
+    fill_window(a, tid, [&](int i, int b) { window[i] = (unsigned char)b; });
 }
 
 // Scores of a tile with the bias.  rel0: the relative position of register row 0
@@ -886,8 +900,9 @@ struct Dbias {
         bucket = reinterpret_cast<unsigned char *>(window + cross_window(a));
     }
     VH_DEVICE void clear(const CrossArgs &a, int tid) {
-        for (int i = tid; i < 128 * a.buckets; i += 256) slots[i] = 0.0f;
-        for (int i = tid; i < 4 * 48 * CA_DIAG; i += 256) (&db->diag[0][0])[i] = 0.0f;
+        const floatx4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = tid; i < 32 * a.buckets; i += 256) st4(slots + 4 * i, zero);
+        for (int i = tid; i < 48 * CA_DIAG; i += 256) st4(&db->diag[0][0] + 4 * i, zero);
         fill_bucket_window(a, bucket, tid);
     }
     // x: dS of a tile whose pairs have the relative positions tile_lo .. tile_hi
@@ -940,14 +955,23 @@ struct Dbias {
             db->far[wave][1] = hi;
         }
         __syncthreads();
-        for (int b = tid; b < a.buckets; b += 256) {
-            float sum = 0.0f;
+        // wave w's 32 slots of a bucket, a thread each; then the four waves'
+        float *sums = &db->diag[0][0];
+        for (int i = tid; i < 4 * a.buckets; i += 256) {
+            floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < 8; j++) v += ld4(slots + 32 * i + 4 * ((i + j) & 7));
+            sums[i] = (v[0] + v[1]) + (v[2] + v[3]);
+        }
+        __syncthreads();
+        if (tid < a.buckets) {
+            float sum = (sums[tid] + sums[a.buckets + tid]) + (sums[2 * a.buckets + tid] + sums[3 * a.buckets + tid]);
+            const int zero = a.max_distance + CA_PAD;
             for (int w = 0; w < 4; w++) {
-                for (int i = 0; i < 32; i++) sum += slots[(w * a.buckets + b) * 32 + (i + b) % 32];
-                if (b == cross_bucket(a, -a.max_distance)) sum += db->far[w][0];
-                if (b == cross_bucket(a, a.max_distance)) sum += db->far[w][1];
+                if (tid == bucket[CA_PAD]) sum += db->far[w][0];
+                if (tid == bucket[zero + a.max_distance]) sum += db->far[w][1];
             }
-            a.dbias_part[((int64_t)h * a.dbias_parts + at) * a.buckets + b] = sum;
+            a.dbias_part[((int64_t)h * a.dbias_parts + at) * a.buckets + tid] = sum;
         }
     }
 };
