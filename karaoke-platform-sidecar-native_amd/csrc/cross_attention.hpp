@@ -783,10 +783,12 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
     const int d = 4 * ((int)threadIdx.x & 15);
     const int q = (int)(row % a.Lq), h = (int)(row / a.Lq % a.H), s = (int)(row / a.Lq / a.H);
     float m = -INFINITY;
+#pragma unroll 8
     for (int p = 0; p < a.parts; p++) m = fmaxf(m, a.part_ml[p * rows + row].x);
     const float base = m == -INFINITY ? 0.0f : m;
     float l = 0.0f;
     floatx4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
     for (int p = 0; p < a.parts; p++) {
         const float2 v = a.part_ml[p * rows + row];
         const float c = __builtin_amdgcn_exp2f(v.x - base);
@@ -1448,6 +1450,7 @@ VH_DEVICE void sum_parts(const float *part, int parts, int64_t rows, int64_t row
     if (row >= rows) return;
     const int d = 4 * ((int)threadIdx.x & 15);
     floatx4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
     for (int p = 0; p < parts; p++) y += ld4(part + (p * rows + row) * CA_D + d);
     const int64_t i = row % len, h = row / len % heads, s = row / len / heads;
     st4(reinterpret_cast<T *>(to.p + s * to.seq + i * to.row + h * to.head) + d, y);
@@ -1471,8 +1474,11 @@ __global__ __launch_bounds__(256) void cross_finish_kernel(CrossArgs a, FinishAr
     const int h = (int)(block - 2 * f.dkv), lanes = 256 / a.buckets;  // threads that share a bucket
     const int b = tid % a.buckets, l = tid / a.buckets;
     float sum = 0.0f;
-    if (l < lanes)
-        for (int i = l; i < a.dbias_parts; i += lanes) sum += a.dbias_part[((int64_t)h * a.dbias_parts + i) * a.buckets + b];
+    if (l < lanes) {
+#pragma unroll 16
+        for (int i = l; i < a.dbias_parts; i += lanes)
+            sum += a.dbias_part[((int64_t)h * a.dbias_parts + i) * a.buckets + b];
+    }
     sums[tid] = sum;
     __syncthreads();
     if (tid >= a.buckets) return;
