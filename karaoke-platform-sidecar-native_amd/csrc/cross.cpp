@@ -146,16 +146,12 @@ bool layernorm_backward(hipStream_t s, const LayerNorm &n, KernelTimer *t) {
 // ---------------------------------------------------------- cross attention
 // Distances from which the far buckets of a side begin.  Bucket near + i is
 // reached at the first whole n with n^far >= max_distance^i near^(far - i), far
-// = side - near: in logarithms, with a difference within their rounding taken
-// as equal (whole numbers that meet the border exactly).
+// = side - near: the next whole number from near (max_distance / near)^(i / far) on,
+// which is taken as whole where it is within a double's roundings.
 static int bucket_edges(int side, int near, int max_distance, int *edge) {
     const int far = side - near;
-    const long double step = logl((long double)max_distance / near) / far;
-    int n = near;
-    for (int i = 0; i < far; i++) {
-        while (logl((long double)n / near) < step * i - 1e-13L) n++;
-        edge[i] = n;
-    }
+    const double step = log((double)max_distance / near) / far;
+    for (int i = 0; i < far; i++) edge[i] = (int)ceil(near * exp(step * i) * (1.0 - 1e-12));
     return far;
 }
 
@@ -273,16 +269,22 @@ constexpr size_t CA_LDS = 160 * 1024;  // of a workgroup
 static size_t window_bytes(const vh_cross *c) {
     return c->bias_table ? (size_t)(2 * (c->max_distance + CA_PAD) + 1) * sizeof(float) : 0;
 }
-static size_t tiles_lds(const vh_cross *c, bool split, bool forward = false) {
-    if (c->type == VH_TYPE_BF16) return split ? SplitLds<bf16>::BYTES : 4 * Tile<bf16>::BYTES;
-    return !split ? 4 * Tile<float>::BYTES : forward ? SplitLds<float, true>::BYTES : SplitLds<float>::BYTES;
+// split: the kernels whose four waves share 32 rows; else those of 128 rows in one
+// group of waves, or 64 in two.
+template <typename T>
+static size_t tiles_bytes(bool split, int groups, bool forward) {
+    if (!split) return groups == 2 ? SharedLds<T, 2>::BYTES : SharedLds<T, 1>::BYTES;
+    return forward && sizeof(T) == 4 ? SplitLds<T, true>::BYTES : SplitLds<T>::BYTES;
+}
+static size_t tiles_lds(const vh_cross *c, bool split, int groups, bool forward) {
+    return c->type == VH_TYPE_BF16 ? tiles_bytes<bf16>(split, groups, forward) : tiles_bytes<float>(split, groups, forward);
 }
 static size_t dq_lds(const vh_cross *c, bool split) {
-    if (!c->bias_table) return tiles_lds(c, split);
-    return tiles_lds(c, split) + window_bytes(c) + sizeof(DbiasLds) + 128 * sizeof(float) * c->buckets + window_bytes(c) / sizeof(float);
+    if (!c->bias_table) return tiles_lds(c, split, 1, false);
+    return tiles_lds(c, split, 1, false) + window_bytes(c) + sizeof(DbiasLds) + 128 * sizeof(float) * c->buckets + window_bytes(c) / sizeof(float);
 }
 static size_t pack_lds(const vh_cross *c) {
-    return tiles_lds(c, true, true) +
+    return tiles_lds(c, true, 1, true) +
            (c->bias_table ? sizeof(float) * c->buckets * (c->heads / c->kv_heads) + window_bytes(c) / sizeof(float) : 0);
 }
 
@@ -290,19 +292,26 @@ static size_t pack_lds(const vh_cross *c) {
 // rows, in `parts` pieces; else those of 128 rows.
 struct CrossCut {
     bool split = false, pack = false;
-    int parts = 1;
+    int parts = 1, heads = 1, waves = 1;  // heads: that a workgroup of dk and dv takes, waves: groups of them in a workgroup
     int64_t pairs = 0, tiles = 0;  // (sequence, head) pairs, and workgroups of each
     int64_t groups() const { return pairs * tiles; }
     int64_t grid() const { return (pairs_by_xcd(pairs) ? (pairs + 7) / 8 * 8 : pairs) * tiles; }
 };
 // From 1.5 128-row workgroups per CU on, their sharing of tiles wins over even work
 // (8 x 801 rows over 1723 keys, 448 of them: 42 us against 48; 4 x 1000 rows over
-// 1200 in fp32, 256: 101 against 94).  Below, pieces of at least 8 tiles (two a
-// wave) until there are about two workgroups per CU.
-constexpr int64_t CA_ENOUGH = 384, CA_PIECES = 512;
-static int pieces(int64_t groups, int across) {
-    const int tiles = (across + 31) / 32;
-    return groups > 0 ? (int)std::max<int64_t>(1, std::min<int64_t>({CA_PIECES / groups, tiles / 8, 64})) : 1;
+// 1200 in fp32, 256: 101 against 94); the forward's are of 64 rows in two groups up to
+// four per CU (30 against 34 us for the same 448; backward no gain).  Below, pieces
+// of at least 8 tiles (two a wave) until there are about two workgroups per CU, for
+// single tokens of 32 until there are four (16 x 32 of them over 8192 keys 42 us
+// against 44; 2 x 3841 rows over 3278 so cut 120 against 107).
+constexpr int64_t CA_ENOUGH = 384, CA_PAIRED = 1024, CA_PIECES = 512, CA_ONE = 256;
+constexpr size_t CA_WINDOWS = 16 * 1024;
+static int pieces(int64_t groups, int across, bool few) {
+    const int64_t tiles = (across + 31) / 32;
+    if (groups <= 0) return 1;
+    int64_t n = std::min(CA_PIECES / groups, tiles / 8);
+    if (few) n = std::max(n, std::min(2 * CA_PIECES / groups, tiles / 32));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(n, 64));
 }
 static CrossCut cross_cut(int64_t pairs, int rows, int pack, int across, bool fits) {
     CrossCut cut;
@@ -313,14 +322,19 @@ static CrossCut cross_cut(int64_t pairs, int rows, int pack, int across, bool fi
     cut.pack = pack > 1 && rows < 32;
     if (cut.pack) cut.pairs /= pack;
     cut.tiles = ((int64_t)rows * (cut.pack ? pack : 1) + 31) / 32;
-    cut.parts = pieces(cut.groups(), across);
+    cut.parts = pieces(cut.groups(), across, rows < 32);
     cut.tiles *= cut.parts;
     return cut;
 }
 static CrossCut forward_cut(const vh_cross *c, bool keep) {
     const int shared = c->heads / c->kv_heads;
     const bool pack = !keep && (!c->bias_table || pack_lds(c) <= CA_LDS);
-    return cross_cut((int64_t)c->sequences * c->heads, c->query_length, pack ? shared : 1, c->key_length, true);
+    CrossCut cut = cross_cut((int64_t)c->sequences * c->heads, c->query_length, pack ? shared : 1, c->key_length, true);
+    if (!cut.split && cut.groups() < CA_PAIRED) {
+        cut.waves = 2;
+        cut.tiles = (c->query_length + 63) / 64;
+    }
+    return cut;
 }
 static CrossCut dq_cut(const vh_cross *c) {
     return cross_cut((int64_t)c->sequences * c->heads, c->query_length, 1, c->key_length, dq_lds(c, true) <= CA_LDS);
@@ -328,10 +342,17 @@ static CrossCut dq_cut(const vh_cross *c) {
 static CrossCut dkv_cut(const vh_cross *c) {
     CrossCut cut = cross_cut((int64_t)c->sequences * c->kv_heads, c->key_length, 1, c->query_length, true);
     if (!cut.split) return cut;
-    // the heads that share the keys are pairs of their own, their sums pieces
-    cut.pairs = (int64_t)c->sequences * c->heads;
+    // a workgroup takes all heads that share its keys, where their bias windows fit
+    // beside its tiles; else, or where that makes less than one workgroup per CU, the
+    // heads are pairs of their own and their sums pieces
+    const int shared = c->heads / c->kv_heads;
     cut.tiles = (c->key_length + 31) / 32;
-    cut.parts = pieces(cut.groups(), c->query_length);
+    cut.heads = shared;
+    if (cut.groups() < CA_ONE || shared * window_bytes(c) > CA_WINDOWS || (int64_t)shared * c->query_length > CA_MAX_LENGTH) {
+        cut.pairs *= shared;
+        cut.heads = 1;
+    }
+    cut.parts = pieces(cut.groups(), c->query_length, false);
     cut.tiles *= cut.parts;
     return cut;
 }
@@ -357,7 +378,7 @@ static CrossWork forward_work(const vh_cross *c, bool keep) {
     }
     return w;
 }
-static int kv_pieces(const vh_cross *c, const CrossCut &cut) { return cut.split ? c->heads / c->kv_heads * cut.parts : 1; }
+static int kv_pieces(const vh_cross *c, const CrossCut &cut) { return cut.split ? c->heads / c->kv_heads / cut.heads * cut.parts : 1; }
 static CrossWork backward_work(const vh_cross *c) {
     CrossWork w;
     w.rows = dq_cut(c);
@@ -425,13 +446,18 @@ static void launch(F kernel, int64_t groups, size_t lds, hipStream_t s, const Cr
     hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), lds, s, a);
 }
 
+template <typename T, bool BIAS, int KW>
+static void forward_shared(hipStream_t s, const CrossArgs &a, int64_t grid, size_t lds) {
+    if (a.stats) launch(cross_forward_kernel<T, BIAS, true, KW>, grid, lds, s, a);
+    else launch(cross_forward_kernel<T, BIAS, false, KW>, grid, lds, s, a);
+}
 template <typename T, bool BIAS>
 static void forward_launch(hipStream_t s, const vh_cross *c, const CrossArgs &a, const CrossCut &cut) {
     const bool keep = a.stats != nullptr;
-    const size_t lds = tiles_lds(c, cut.split, true) + window_bytes(c);
+    const size_t lds = tiles_lds(c, cut.split, cut.waves, true) + window_bytes(c);
     if (!cut.split) {
-        if (keep) launch(cross_forward_kernel<T, BIAS, true>, cut.grid(), lds, s, a);
-        else launch(cross_forward_kernel<T, BIAS, false>, cut.grid(), lds, s, a);
+        if (cut.waves == 2) forward_shared<T, BIAS, 2>(s, a, cut.grid(), lds);
+        else forward_shared<T, BIAS, 1>(s, a, cut.grid(), lds);
         return;
     }
     if (cut.pack) {
@@ -480,7 +506,7 @@ static void dq_launch(hipStream_t s, const vh_cross *c, const CrossArgs &a, cons
 
 template <typename T, bool BIAS>
 static void dkv_launch(hipStream_t s, const vh_cross *c, const CrossArgs &a, const CrossCut &cut) {
-    const size_t lds = tiles_lds(c, cut.split) + (cut.split ? 4 * sizeof(RowStats) + window_bytes(c)
+    const size_t lds = tiles_lds(c, cut.split, 1, false) + (cut.split ? 4 * sizeof(RowStats) + cut.heads * window_bytes(c)
                                                         : 2 * sizeof(RowStats) + 2 * window_bytes(c));
     if (cut.split) launch(cross_dkv_split_kernel<T, BIAS>, cut.grid(), lds, s, a);
     else launch(cross_dkv_kernel<T, BIAS>, cut.grid(), lds, s, a);
@@ -509,6 +535,7 @@ bool cross_attention_backward(hipStream_t s, const vh_cross *c, const CrossBuffe
     a.rows = at(w.stats);
     a.parts = w.rows.parts;
     a.kv_parts = w.keys.parts;
+    a.kv_heads = w.keys.heads;
     a.part_o = at(w.part_o);
     a.part_dk = at(w.part_dk);
     a.part_dv = at(w.part_dv);

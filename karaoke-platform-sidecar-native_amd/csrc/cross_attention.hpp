@@ -72,8 +72,8 @@ struct CrossArgs {
     // Sums over a part of the keys (forward, dq) or queries (dk, dv), when a row
     // tile's work is split: parts pieces, [part][S][H][Lq][64] and their (m, l);
     // [part][S][KV][Lk][64] for dk, dv, part = head among those that share the
-    // keys * kv_parts + piece
-    int parts, kv_parts;
+    // keys / kv_heads * kv_parts + piece, a workgroup taking kv_heads of them
+    int parts, kv_parts, kv_heads;
     float *part_o;
     float2 *part_ml;
     float *part_dk, *part_dv;
@@ -505,16 +505,42 @@ VH_DEVICE float2 row_stats(bool bias, bool seen, float m, float l) {
     return make_float2(bias ? m : m + n, -n);
 }
 
-// Workgroup: 4 waves x 32 queries of one head, tiles of 32 keys that they share,
+// A workgroup's four waves are KW groups that take the same ROWS rows and every
+// KW-th tile of the other side: twice the workgroups, of half the work, where those
+// of 128 rows are few.  A group's RW waves share its tiles, [2] places of two each.
+template <typename T, int KW>
+struct SharedLds {
+    static constexpr int RW = 4 / KW, ROWS = 32 * RW;
+    static constexpr int GROUP = 4 * Tile<T>::BYTES;
+    static constexpr int RESULTS = KW > 1 ? RW * 64 * (32 * 4 + 8) : 0;  // a group's accumulators, over the tiles
+    static constexpr int BYTES = KW * GROUP > RESULTS ? KW * GROUP : RESULTS;
+};
+// A group's tiles: it takes t = group, group + KW, ... while 32 t < end.
+template <int KW>
+VH_DEVICE int group_tiles(int end, int group) {
+    return max(0, ((max(end, 0) + CA_TILE - 1) / CA_TILE - group + KW - 1) / KW);
+}
+// Accumulators of the second group's waves for the first's: lane by lane.
+VH_DEVICE void give(float *res, int i, int rw, int lane, const floatx16 &x) {
+#pragma unroll
+    for (int r = 0; r < 16; r++) res[(rw * 32 + 16 * i + r) * 64 + lane] = x[r];
+}
+VH_DEVICE void take(const float *res, int i, int rw, int lane, floatx16 &x) {
+#pragma unroll
+    for (int r = 0; r < 16; r++) x[r] += res[(rw * 32 + 16 * i + r) * 64 + lane];
+}
+
+// Workgroup: RW waves x 32 queries of one head (KW times), tiles of 32 keys that they share,
 // the next one's copies in flight while one is worked on.  Per wave and tile S^T =
 // K Q^T, so that a lane holds 16 scores of one query, the online softmax, and out^T
 // += V^T P^T from the same registers.  KEEP: statistics, rest, and P in two pieces.
-template <typename T, bool BIAS, bool KEEP>
+template <typename T, bool BIAS, bool KEEP, int KW>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) void cross_forward_kernel(CrossArgs a) {
-    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];  // [2] K and V tiles
-    float *window = reinterpret_cast<float *>(smem + 4 * Tile<T>::BYTES);
+    using L = SharedLds<T, KW>;
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
+    float *window = reinterpret_cast<float *>(smem + L::BYTES);
 
-    const int qtiles = (a.Lq + 127) / 128;
+    const int qtiles = (a.Lq + L::ROWS - 1) / L::ROWS;
     int pair, qt;
     if (!pair_task(a.S * a.H, qtiles, pair, qt)) return;
     const int h = pair % a.H, s = pair / a.H;
@@ -523,20 +549,24 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) void cross_forward_ker
     const int kh = h / (a.H / a.KV);
     const int start = cross_start(a, s);
     const int qlen = cross_length(a.query_lengths, s, a.Lq), klen = cross_length(a.key_lengths, s, a.Lk);
-    const int q0 = 128 * qt + 32 * wave, q = q0 + li;
+    const int group = wave / L::RW, rw = wave % L::RW;
+    const int q0 = L::ROWS * qt + 32 * rw, q = q0 + li;
     const bool active = q0 < qlen;
     int keys = klen;  // that any row of the workgroup sees
-    if (a.causal) keys = min(keys, start + min(128 * qt + 128, qlen));
-    if (128 * qt >= qlen) keys = 0;
+    if (a.causal) keys = min(keys, start + min(L::ROWS * (qt + 1), qlen));
+    if (L::ROWS * qt >= qlen) keys = 0;
 
     const char *kp = a.k.p + s * a.k.seq + kh * a.k.head, *vp = a.v.p + s * a.v.seq + kh * a.v.head;
-    const uint32_t lds = (uint32_t)(uintptr_t)smem;
-    auto issue = [&](int k0) {
-        const uint32_t at = lds + (uint32_t)(k0 / CA_TILE & 1) * 2 * Tile<T>::BYTES;
-        tile_issue<T, 4>(kp, a.k.row, k0, klen - 1, at, wave, lane);
-        tile_issue<T, 4>(vp, a.v.row, k0, klen - 1, at + Tile<T>::BYTES, wave, lane);
+    const unsigned char *tiles = smem + group * L::GROUP;
+    const uint32_t lds = (uint32_t)(uintptr_t)smem + (uint32_t)(group * L::GROUP);
+    auto issue = [&](int i) {  // the group's i-th tile, if there is one
+        const int k0 = CA_TILE * (KW * i + group);
+        const uint32_t at = lds + (uint32_t)(i & 1) * 2 * Tile<T>::BYTES;
+        if (k0 >= keys) return;
+        tile_issue<T, L::RW>(kp, a.k.row, k0, klen - 1, at, rw, lane);
+        tile_issue<T, L::RW>(vp, a.v.row, k0, klen - 1, at + Tile<T>::BYTES, rw, lane);
     };
-    if (keys > 0) issue(0);
+    issue(0);
     if constexpr (BIAS) fill_bias_window(a, h, window, tid);  // read after the loop's first barrier
     RegRows<T> w;
     if (active) {
@@ -548,13 +578,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) void cross_forward_ker
     st.clear();
     // the tiles of which the wave sees something, then the others' only for the rest
     // of the workgroup (a branch in the loop would copy every accumulator each time)
-    const int mine = !active ? 0 : a.causal ? min(keys, start + q0 + 32) : keys;
-    int k0 = 0;
-    for (; k0 < mine; k0 += CA_TILE) {
+    const int steps = group_tiles<KW>(keys, 0);
+    const int mine = group_tiles<KW>(!active ? 0 : a.causal ? min(keys, start + q0 + 32) : keys, group);
+    int i = 0;
+    for (; i < mine; i++) {
         wait_vmcnt<0>();
         __syncthreads();  // this tile is there, and the last one has been read
-        if (k0 + CA_TILE < keys) issue(k0 + CA_TILE);
-        const LdsTile<T> K{smem + (k0 / CA_TILE & 1) * 2 * Tile<T>::BYTES}, V{K.p + Tile<T>::BYTES};
+        issue(i + 1);
+        const int k0 = CA_TILE * (KW * i + group);
+        const LdsTile<T> K{tiles + (i & 1) * 2 * Tile<T>::BYTES}, V{K.p + Tile<T>::BYTES};
         floatx16 x;
         scores(x, K, w, lane);
         const int lo = k0 - (start + q0 + 31), hi = k0 + 31 - (start + q0);
@@ -563,10 +595,36 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) void cross_forward_ker
                            (a.causal ? min(klen, start + q + 1) : klen) - k0, lh);
         values_tile<T, BIAS, KEEP>(st, x, V, lane);
     }
-    for (; k0 < keys; k0 += CA_TILE) {
+    for (; i < steps; i++) {
         wait_vmcnt<0>();
         __syncthreads();
-        if (k0 + CA_TILE < keys) issue(k0 + CA_TILE);
+        issue(i + 1);
+    }
+    if constexpr (KW == 2) {  // the second group's results joined to the first's
+        float *res = reinterpret_cast<float *>(smem);
+        float2 *ml = reinterpret_cast<float2 *>(res + L::RW * 32 * 64) + rw * 64 + lane;
+        __syncthreads();
+        if (group) {
+            const float top = st.top();
+            give(res, 0, rw, lane, st.o[0]);
+            give(res, 1, rw, lane, st.o[1]);
+            *ml = make_float2(top, st.l);
+        }
+        __syncthreads();
+        if (group) return;
+        const float2 other = *ml;
+        const float top = fmaxf(st.top(), other.x), base = top == -INFINITY ? 0.0f : top;
+        const float f = __builtin_amdgcn_exp2f(st.top() - base), g = __builtin_amdgcn_exp2f(other.x - base);
+        st.l = st.l * f + other.y * g;
+        st.mc = base;
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            floatx16 o;
+            zero16(o);
+            take(res, t, rw, lane, o);
+#pragma unroll
+            for (int r = 0; r < 16; r++) st.o[t][r] = st.o[t][r] * f + o[r] * g;
+        }
     }
     if (q >= a.Lq) return;
     const float l = st.l + __shfl_xor(st.l, 32, 64);
@@ -1350,8 +1408,9 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(CrossArgs a) {
 }
 
 // The same in too few workgroups: 4 waves take the same 32 keys and every fourth
-// tile of one head's queries; the heads that share the keys, and a.kv_parts pieces
-// of their queries, are workgroups of their own.
+// tile of the queries of all heads that share them, one head after the other; or,
+// where there are too few such workgroups, each head and a.kv_parts pieces of its
+// queries are workgroups of their own.
 template <typename T, bool BIAS>
 __global__ __launch_bounds__(256, 2) void cross_dkv_split_kernel(CrossArgs a) {
     using L = SplitLds<T>;
@@ -1359,10 +1418,10 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_split_kernel(CrossArgs a) {
     RowStats *stats = reinterpret_cast<RowStats *>(smem + L::BYTES);  // [4]
     float *window = reinterpret_cast<float *>(stats + 4);
 
-    const int ktiles = (a.Lk + 31) / 32, G = a.H / a.KV;
+    const int ktiles = (a.Lk + 31) / 32, G = a.H / a.KV, HH = a.H / a.kv_heads;
     int pair, tile;
-    if (!pair_task(a.S * a.H, ktiles * a.kv_parts, pair, tile)) return;
-    const int kt = tile % ktiles, part = tile / ktiles, h = pair % a.H, s = pair / a.H;
+    if (!pair_task(a.S * HH, ktiles * a.kv_parts, pair, tile)) return;
+    const int kt = tile % ktiles, part = tile / ktiles, h = pair % HH * a.kv_heads, s = pair / HH;  // h: the first head
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lh = lane >> 5, kh = h / G;
     const int start = cross_start(a, s);
@@ -1370,16 +1429,16 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_split_kernel(CrossArgs a) {
     const int k0 = 32 * kt, key = k0 + (lane & 31);
     int begin = 0, tiles = k0 < klen ? (qlen + 31) / 32 : 0;
     if (a.causal) begin = min(tiles, max(0, min(k0 - start, qlen)) / 32);
-    const int first = begin + (int)((int64_t)(tiles - begin) * part / a.kv_parts);
-    const int last = begin + (int)((int64_t)(tiles - begin) * (part + 1) / a.kv_parts);
+    const int each = tiles - begin;  // of a head, the workgroup's numbered head by head
+    const int64_t all = (int64_t)each * a.kv_heads;
+    const int first = (int)(all * part / a.kv_parts), last = (int)(all * (part + 1) / a.kv_parts);
 
     if constexpr (BIAS) {
-        fill_bias_window(a, h, window, tid);
+        for (int g = 0; g < a.kv_heads; g++) fill_bias_window(a, h + g, window + g * cross_window(a), tid);
         __syncthreads();
     }
     KeySums sums;
     sums.clear();
-    const char *qp = a.q.p + s * a.q.seq + h * a.q.head, *dp = a.dout.p + s * a.dout.seq + h * a.dout.head;
     int t = first + wave;
     {
         KeyRows<T> w;
@@ -1387,10 +1446,14 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_split_kernel(CrossArgs a) {
         const LdsTile<T> Q{smem + wave * L::WAVE}, D{Q.p + Tile<T>::BYTES};
         const uint32_t lds = (uint32_t)(uintptr_t)smem + (uint32_t)(wave * L::WAVE);
         RowStats *rs = stats + wave;
-        auto issue_q = [&](int t) { tile_issue<T, 1>(qp, a.q.row, 32 * t, qlen - 1, lds, 0, lane); };
+        auto issue_q = [&](int t) {
+            const char *qp = a.q.p + s * a.q.seq + (h + t / each) * a.q.head;
+            tile_issue<T, 1>(qp, a.q.row, 32 * (begin + t % each), qlen - 1, lds, 0, lane);
+        };
         auto issue_dout = [&](int t) {
-            tile_issue<T, 1>(dp, a.dout.row, 32 * t, qlen - 1, lds + Tile<T>::BYTES, 0, lane);
-            row_tile_issue(row_tile(a, s, h, t), (uint32_t)(uintptr_t)rs, lane);
+            const char *dp = a.dout.p + s * a.dout.seq + (h + t / each) * a.dout.head;
+            tile_issue<T, 1>(dp, a.dout.row, 32 * (begin + t % each), qlen - 1, lds + Tile<T>::BYTES, 0, lane);
+            row_tile_issue(row_tile(a, s, h + t / each, begin + t % each), (uint32_t)(uintptr_t)rs, lane);
         };
         if (t < last) {
             issue_dout(t);
@@ -1400,7 +1463,8 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_split_kernel(CrossArgs a) {
             const bool next = t + 4 < last;
             wait_vmcnt<L::LOADS>();  // dout is there, Q may be under way
             dkv_tile<T, BIAS>(
-                a, w.k, w.v, sums, window, Q, D, rs, 32 * t, start, key, k0, lane, [&] { wait_vmcnt<0>(); },
+                a, w.k, w.v, sums, BIAS ? window + t / each * cross_window(a) : nullptr, Q, D, rs,
+                32 * (begin + t % each), start, key, k0, lane, [&] { wait_vmcnt<0>(); },
                 [&] {
                     wait_lds();
                     if (next) issue_dout(t + 4);
@@ -1421,8 +1485,8 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_split_kernel(CrossArgs a) {
             y[e][r] = ok < klen ? y[e][r] * a.scale : 0.0f;
             z[e][r] = ok < klen ? z[e][r] : 0.0f;
         }
-    if (G * a.kv_parts > 1) {
-        const int64_t at = ((((int64_t)(h % G) * a.kv_parts + part) * a.S + s) * a.KV + kh) * a.Lk + ok;
+    if (G / a.kv_heads * a.kv_parts > 1) {
+        const int64_t at = ((((int64_t)(h % G) / a.kv_heads * a.kv_parts + part) * a.S + s) * a.KV + kh) * a.Lk + ok;
 #pragma unroll
         for (int e = 0; e < 2; e++) {
             st4(a.part_dk + at * CA_D + d + 4 * e, y[e]);
@@ -1467,7 +1531,7 @@ __global__ __launch_bounds__(256) void cross_finish_kernel(CrossArgs a, FinishAr
     block -= f.dq;
     if (block < 2 * f.dkv) {
         const bool v = block >= f.dkv;
-        sum_parts<T>(v ? a.part_dv : a.part_dk, a.H / a.KV * a.kv_parts, (int64_t)a.S * a.KV * a.Lk,
+        sum_parts<T>(v ? a.part_dv : a.part_dk, a.H / a.KV / a.kv_heads * a.kv_parts, (int64_t)a.S * a.KV * a.Lk,
                      (block - (v ? f.dkv : 0)) * 16 + sub, a.Lk, a.KV, v ? a.dv : a.dk);
         return;
     }
