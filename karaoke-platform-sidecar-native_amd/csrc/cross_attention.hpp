@@ -942,16 +942,22 @@ VH_DEVICE void load_rows(const CrossArgs &a, QueryRows<T> &w, int s, int h, int 
 // long).  Each diagonal is then added to its bucket's slot of that lane: the order
 // of every sum is fixed.  Tiles wholly beyond max_distance have one bucket and are
 // summed in registers.
+// A row's dS add up to 0, and the far buckets hold most of its keys: there an error
+// of delta, dP or P counts as often as there are keys, while the sum itself is only
+// what the near buckets leave.  So what a row's dS add up to, r, is taken out of the
+// far buckets by their part of the row's probability, r P(far).
 constexpr int CA_DIAG = 20;  // pitch: 16-byte reads, and stores of 32 lanes in 32 banks
 struct DbiasLds {
     float diag[4][48 * CA_DIAG];
     float far[4][2];
+    float rows[4][CA_TILE];
 };
 struct Dbias {
     DbiasLds *db;
     float *slots;           // [4][buckets][32]
     unsigned char *bucket;  // by relative position, as the bias window
-    float lo = 0.0f, hi = 0.0f;
+    float lo = 0.0f, hi = 0.0f, near = 0.0f;  // the lane's row's dS
+    float p_lo = 0.0f, p_hi = 0.0f;           // its probability in the far buckets
     // behind the tiles: where the gradient is wanted the sums, and the bias window
     VH_DEVICE void lay(const CrossArgs &a, unsigned char *at, float *&window) {
         db = reinterpret_cast<DbiasLds *>(at);
@@ -965,17 +971,37 @@ struct Dbias {
         for (int i = tid; i < 48 * CA_DIAG; i += 256) st4(&db->diag[0][0] + 4 * i, zero);
         fill_bucket_window(a, bucket, tid);
     }
+    VH_DEVICE static float sum16(const floatx16 &x) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; r++) sum += x[r];
+        return sum;
+    }
+    // p: the probabilities of a tile of relative positions tile_lo .. tile_hi, of
+    // which rows `seen` and up are masked
+    VH_DEVICE void mass(const CrossArgs &a, const floatx16 &p, int tile_lo, int tile_hi, bool mask, int seen, int lh) {
+        const bool below = tile_hi <= -a.max_distance;
+        if (!below && tile_lo < a.max_distance) return;
+        float sum = 0.0f;
+        if (mask) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) sum += row_of(r, lh) < seen ? p[r] : 0.0f;
+        } else {
+            sum = sum16(p);
+        }
+        if (below) p_lo += sum;
+        else p_hi += sum;
+    }
     // x: dS of a tile whose pairs have the relative positions tile_lo .. tile_hi
     VH_DEVICE void add(const CrossArgs &a, const floatx16 &x, int tile_lo, int tile_hi, int wave, int lane) {
         const int md = a.max_distance, li = lane & 31, lh = lane >> 5;
         if (tile_hi <= -md || tile_lo >= md) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int r = 0; r < 16; r++) sum += x[r];
+            const float sum = sum16(x);
             if (tile_hi <= -md) lo += sum;
             else hi += sum;
             return;
         }
+        near += sum16(x);
         float *diag = &db->diag[wave][0];
         float sum[2];
 #pragma unroll
@@ -1004,11 +1030,21 @@ struct Dbias {
         }
         wave_order();
     }
-    // the workgroup's sums into part `at` of head h
-    VH_DEVICE void finish(const CrossArgs &a, int h, int at, int tid) {
+    // the workgroup's sums into part `at` of head h; split: its waves share their rows.
+    // Rows whose keys are shared by several workgroups are left as they are.
+    VH_DEVICE void finish(const CrossArgs &a, int h, int at, int tid, bool split) {
         const int wave = tid >> 6;
-        lo = wave_sum(lo);
-        hi = wave_sum(hi);
+        float rest = near + (lo + hi);
+        rest += __shfl_xor(rest, 32, 64);
+        if (split) {
+            if ((tid & 63) < 32) db->rows[wave][tid & 31] = rest;
+            __syncthreads();
+            rest = 0.0f;
+            if (a.parts == 1)
+                rest = (db->rows[0][tid & 31] + db->rows[1][tid & 31]) + (db->rows[2][tid & 31] + db->rows[3][tid & 31]);
+        }
+        lo = wave_sum(__builtin_fmaf(-rest, p_lo, lo));
+        hi = wave_sum(__builtin_fmaf(-rest, p_hi, hi));
         __syncthreads();  // cleared, where no tile was worked on
         if ((tid & 63) == 0) {
             db->far[wave][0] = lo;
@@ -1054,7 +1090,12 @@ VH_DEVICE void dq_tile(const CrossArgs &a, const QueryRows<T> &w, const Held &q,
     if constexpr (BIAS) add_bias(a, x, window, lo, hi, k0 - pos, 1, lh);
 #pragma unroll
     for (int r = 0; r < 16; r++)
-        x[r] = __builtin_amdgcn_exp2f(BIAS ? (x[r] - w.m) + w.n : __builtin_fmaf(x[r], a.scale2, -w.m)) * dp[r];
+        x[r] = __builtin_amdgcn_exp2f(BIAS ? (x[r] - w.m) + w.n : __builtin_fmaf(x[r], a.scale2, -w.m));
+    if constexpr (BIAS) {
+        if (a.dbias_part) db.mass(a, x, lo, hi, mask, seen, lh);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; r++) x[r] *= dp[r];
     if (mask) {
 #pragma unroll
         for (int r = 0; r < 16; r++)
@@ -1132,7 +1173,7 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(CrossArgs a) {
         if (k0 + CA_TILE < keys) issue(k0 + CA_TILE);
     }
     if constexpr (BIAS) {
-        if (a.dbias_part) db.finish(a, h, s * qtiles + qt, tid);
+        if (a.dbias_part) db.finish(a, h, s * qtiles + qt, tid, false);
     }
     if (q >= a.Lq) return;
     T *out = reinterpret_cast<T *>(a.dq.p + s * a.dq.seq + (int64_t)q * a.dq.row + h * a.dq.head);
@@ -1232,7 +1273,7 @@ __global__ __launch_bounds__(256, 2) void cross_dq_split_kernel(CrossArgs a) {
         }
     }
     if constexpr (BIAS) {
-        if (a.dbias_part) db.finish(a, h, (s * rtiles + rt) * a.parts + part, tid);
+        if (a.dbias_part) db.finish(a, h, (s * rtiles + rt) * a.parts + part, tid, true);
     }
     floatx4 y[2];
     waves_sum<T>(reinterpret_cast<float *>(smem), acc, tid, y);
