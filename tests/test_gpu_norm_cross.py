@@ -97,6 +97,14 @@ def test_layernorm_many_rows(ctx, rows, dim, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [1, 7, 20, 72, 130, 200, 300, 384, 500, 512, 513, 700, 1023, 1024, 1500, 2047])
+def test_layernorm_more_rows(ctx, dim, dtype):
+    """Enough rows for several to a wave, at each number of a row's lanes and of a lane's elements."""
+    check_norm(ctx, randn(1, 4160, dim, dtype=dtype), 1 + 0.1 * randn(2, dim), randn(3, dim),
+               randn(4, 4160, dim, dtype=dtype), f"4160x{dim}")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("dim,pitch", [(384, 400), (384, 385), (65, 128), (1028, 1030), (5000, 5004)])
 def test_layernorm_pitch(ctx, dim, pitch, dtype):
     """Rows with gaps between them, which are neither read nor written."""
@@ -312,6 +320,54 @@ def test_bias(ctx, size, buckets, max_distance, bidirectional, start, causal, dt
           max_distance=max_distance, bidirectional=bidirectional, scale=0.1)
 
 
+# many rows, sequences and heads: workgroups of 128 rows (forward: of 64 below 1024 of them), dk and dv of all heads
+# that share their keys in one workgroup or each head's on its own
+MANY = [(13, 16, 16, 600, 97), (5, 16, 16, 600, 600), (10, 16, 8, 300, 600), (32, 12, 12, 64, 70), (8, 16, 8, 200, 130),
+        (6, 16, 2, 260, 300), (70, 16, 16, 40, 33)]
+
+
+def few(bound, n):
+    return [int(bound * (i % n) / (n - 1)) for i in range(n)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", MANY, ids=str)
+def test_many(ctx, size, dtype):
+    q, k, v, dout = make(*size, dtype)
+    check(ctx, q, k, v, dout, str(size))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal,buckets", [(True, 0), (False, 32), (True, 32)])
+@pytest.mark.parametrize("size", MANY, ids=str)
+def test_many_ragged(ctx, size, causal, buckets, dtype):
+    """Lengths from none to all, NaN behind them; equal calls give equal bits."""
+    S, H, KV, Lq, Lk = size
+    qlens, klens = few(Lq, S), few(Lk, S)[::-1]
+    klens[S // 2] = Lk
+    q, k, v, dout = make(*size, dtype)
+    for s in range(S):
+        q[s, qlens[s]:], dout[s, qlens[s]:], k[s, klens[s]:], v[s, klens[s]:] = NAN, math.inf, math.inf, NAN
+    kw = dict(causal=causal, query_lengths=qlens, key_lengths=klens, query_start=[Lk - Lq + 40 * (s % 3 - 1) for s in range(S)])
+    if buckets:
+        kw.update(bias_table=randn(9, buckets, H), max_distance=128, bidirectional=not causal)
+    got = check(ctx, q, k, v, dout, str(size), **kw)
+    again = attend(ctx, q, k, v, dout, **kw)
+    assert all(torch.equal(got[n], again[n]) for n in got)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("size,start", [((2, 8, 2, 1, 5000), [4999, 1300]), ((1, 4, 1, 9, 4100), [4000]),
+                                        ((2, 4, 2, 40, 2500), [2460, -7]), ((1, 2, 2, 1300, 64), [0]),
+                                        ((1, 4, 2, 100, 100), [2 ** 31 - 1]), ((1, 4, 2, 100, 100), [-2 ** 31])], ids=str)
+def test_bias_in_pieces(ctx, size, start, causal, dtype):
+    """Few rows over many keys, and few keys under many rows, whose sums are joined; starts out of reach."""
+    q, k, v, dout = make(*size, dtype)
+    check(ctx, q, k, v, dout, str(size), causal=causal, query_start=start, bias_table=randn(9, 32, size[1]),
+          key_lengths=[size[4] - 30 * s for s in range(size[0])])
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_bias_that_hides(ctx, dtype):
     """Buckets at -inf hide their pairs, some rows' all of them (0, and no gradient); buckets at the type's lowest value
@@ -335,6 +391,17 @@ def test_bias_that_hides(ctx, dtype):
     hidden[15] = -math.inf
     a, b = (attend(ctx, q, k, v, bias_table=t)["out"][0, :100] for t in (table, hidden))
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("causal", [False, True])
+def test_bias_that_hides_many(ctx, causal, dtype):
+    """The same in workgroups of 128 rows; scores of hundreds there."""
+    q, k, v, dout = make(8, 16, 16, 400, 33, dtype, size=20.0)
+    table = randn(9, 32, 16)
+    table[15] = -math.inf
+    got = check(ctx, q, k, v, dout, "-inf", bias_table=table, causal=causal)
+    assert not bool(got["out"][:, 170:].any()) and not bool(got["dq"][:, 170:].any())
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
