@@ -211,7 +211,7 @@ int vh_attention_noalloc(vh_context *ctx, int sequences, int length, int heads, 
    Device x[rows][ldx], y[rows][ldy] of `type`, gamma[dim], beta[dim] (may be
    null: 0); stats[rows][2] (may be null) receives (mean, rstd) for the backward
    pass.  dim 1 to 16384, any pitch from dim up, any alignment, rows from 0; y may
-   be x.  Issues one kernel: no allocation, no synchronisation, fit for stream
+   be x at the same pitch.  Issues kernels only: no allocation, no synchronisation, fit for stream
    capture. */
 int vh_layernorm(vh_context *ctx, int type, int64_t rows, int dim, const void *x, int64_t ldx, const float *gamma,
                  const float *beta, float eps, void *y, int64_t ldy, float *stats);
@@ -222,7 +222,7 @@ int vh_layernorm(vh_context *ctx, int type, int64_t rows, int dim, const void *x
    summed in a fixed order: equal calls give equal bits.  They need `workspace`,
    vh_layernorm_workspace_bytes(rows, dim) bytes of device memory, 16-byte
    aligned, the caller's: it is free again when the call's work is done, and two
-   captured graphs that may run at once need one each.  dx may be dy or x.  With
+   captured graphs that may run at once need one each.  dx may be dy or x at the same pitch.  With
    0 rows dgamma and dbeta are 0.  Issues kernels only. */
 int vh_layernorm_backward(vh_context *ctx, int type, int64_t rows, int dim, const void *dy, int64_t lddy, const void *x,
                           int64_t ldx, const float *gamma, const float *stats, void *dx, int64_t lddx, float *dgamma,
@@ -261,12 +261,16 @@ typedef struct {
 } vh_cross;
 /* out = softmax(scale q k^T + bias) v over the keys a row sees.  A row that sees
    none (no keys, causal before the first one, or a bias of -inf at all of them)
-   is 0.  The products run on the matrix cores (bf16 operands as they are, P
-   rounded to bf16; fp32 in fp32), scores, softmax and sums in fp32.
+   is 0.  The products run on the bf16 matrix cores: bf16 operands as they are, P
+   rounded to bf16; fp32 operands as three bf16 values each, whose products keep 24
+   bits (infinities in them give NaN); scores, softmax and sums are fp32.
+   A key that no row sees is never read.  A NaN or infinity in a value that a row's
+   neighbours see and it does not, causal, may reach it (0 times it is NaN).
    saved (may be null): vh_cross_saved_bytes bytes for the backward pass (the
-   rows' softmax statistics and, for bf16, what rounding took from out).
-   workspace: vh_cross_workspace_bytes(c, 0) bytes.  Tensors, saved and workspace
-   16-byte aligned device memory.  Issues kernels only, without allocation or
+   rows' softmax statistics and, for bf16, what rounding took from out: bf16, with
+   a bias table fp32).  workspace: vh_cross_workspace_bytes(c, 0) bytes.  Tensors,
+   saved and workspace are 16-byte aligned device memory; out, saved and workspace
+   overlap nothing else.  Issues kernels only, without allocation or
    synchronisation, so it may be captured; workspace is free again when the
    call's work is done, and graphs that may run at once need one each. */
 int vh_cross_attention(vh_context *ctx, const vh_cross *c, const void *q, const void *k, const void *v, void *out,

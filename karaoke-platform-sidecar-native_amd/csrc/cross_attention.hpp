@@ -308,7 +308,8 @@ VH_DEVICE const char *uniform(const void *from) {
 
 // Copies rows row0 .. row0 + 31 of a tensor's sequence and head (base: its row 0)
 // into a tile, 1 KB a load, the loads dealt out to WAVES waves.  Rows past `last`
-// are copies of row `last`: what lies behind the valid rows is never read.
+// are copies of row `last`: what lies behind the rows that count is never read (a
+// probability of 0 would not hide a NaN there).
 template <typename T, int WAVES>
 VH_DEVICE void tile_issue(const char *base, int64_t row_bytes, int row0, int last, uint32_t tile_lds, int wave,
                           int lane) {
@@ -563,8 +564,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) void cross_forward_ker
         const int k0 = CA_TILE * (KW * i + group);
         const uint32_t at = lds + (uint32_t)(i & 1) * 2 * Tile<T>::BYTES;
         if (k0 >= keys) return;
-        tile_issue<T, L::RW>(kp, a.k.row, k0, klen - 1, at, rw, lane);
-        tile_issue<T, L::RW>(vp, a.v.row, k0, klen - 1, at + Tile<T>::BYTES, rw, lane);
+        tile_issue<T, L::RW>(kp, a.k.row, k0, keys - 1, at, rw, lane);
+        tile_issue<T, L::RW>(vp, a.v.row, k0, keys - 1, at + Tile<T>::BYTES, rw, lane);
     };
     issue(0);
     if constexpr (BIAS) fill_bias_window(a, h, window, tid);  // read after the loop's first barrier
@@ -747,9 +748,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 4 : 2) void cross_forward_spl
         for (; t < last; t += 4) {
             const int64_t k0 = 32 * t;
             floatx16 x;
-            scores(x, GlobalTile{kp + k0 * a.k.row, (uint32_t)a.k.row, klen - 1 - 32 * t}, w, lane);
+            scores(x, GlobalTile{kp + k0 * a.k.row, (uint32_t)a.k.row, keys - 1 - 32 * t}, w, lane);
             weigh(x, 32 * t);
-            values_tile<T, BIAS, KEEP>(st, x, GlobalTile{vp + k0 * a.v.row, (uint32_t)a.v.row, klen - 1 - 32 * t}, lane);
+            values_tile<T, BIAS, KEEP>(st, x, GlobalTile{vp + k0 * a.v.row, (uint32_t)a.v.row, keys - 1 - 32 * t}, lane);
         }
     } else {
         RegRows<T> w;
@@ -759,8 +760,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 4 : 2) void cross_forward_spl
         }
         const LdsTile<T> K{smem + wave * L::WAVE}, V{K.p + Tile<T>::BYTES};
         const uint32_t lds = (uint32_t)(uintptr_t)smem + (uint32_t)(wave * L::WAVE);
-        auto issue_k = [&](int t) { tile_issue<T, 1>(kp, a.k.row, 32 * t, klen - 1, lds, 0, lane); };
-        auto issue_v = [&](int t) { tile_issue<T, 1>(vp, a.v.row, 32 * t, klen - 1, lds + Tile<T>::BYTES, 0, lane); };
+        auto issue_k = [&](int t) { tile_issue<T, 1>(kp, a.k.row, 32 * t, keys - 1, lds, 0, lane); };
+        auto issue_v = [&](int t) { tile_issue<T, 1>(vp, a.v.row, 32 * t, keys - 1, lds + Tile<T>::BYTES, 0, lane); };
         if (t < last) {
             issue_k(t);
             issue_v(t);
@@ -1141,8 +1142,8 @@ __global__ __launch_bounds__(256, 2) void cross_dq_kernel(CrossArgs a) {
     const uint32_t lds = (uint32_t)(uintptr_t)smem;
     auto issue = [&](int k0) {
         const uint32_t at = lds + (uint32_t)(k0 / CA_TILE & 1) * 2 * Tile<T>::BYTES;
-        tile_issue<T, 4>(kp, a.k.row, k0, klen - 1, at, wave, lane);
-        tile_issue<T, 4>(vp, a.v.row, k0, klen - 1, at + Tile<T>::BYTES, wave, lane);
+        tile_issue<T, 4>(kp, a.k.row, k0, keys - 1, at, wave, lane);
+        tile_issue<T, 4>(vp, a.v.row, k0, keys - 1, at + Tile<T>::BYTES, wave, lane);
     };
     if (keys > 0) issue(0);
     if constexpr (BIAS) {  // read after the loop's first barrier
@@ -1252,8 +1253,8 @@ __global__ __launch_bounds__(256, 2) void cross_dq_split_kernel(CrossArgs a) {
     {
         const LdsTile<T> K{smem + wave * L::WAVE}, V{K.p + Tile<T>::BYTES};
         const uint32_t lds = (uint32_t)(uintptr_t)smem + (uint32_t)(wave * L::WAVE);
-        auto issue_k = [&](int t) { tile_issue<T, 1>(kp, a.k.row, 32 * t, klen - 1, lds, 0, lane); };
-        auto issue_v = [&](int t) { tile_issue<T, 1>(vp, a.v.row, 32 * t, klen - 1, lds + Tile<T>::BYTES, 0, lane); };
+        auto issue_k = [&](int t) { tile_issue<T, 1>(kp, a.k.row, 32 * t, keys - 1, lds, 0, lane); };
+        auto issue_v = [&](int t) { tile_issue<T, 1>(vp, a.v.row, 32 * t, keys - 1, lds + Tile<T>::BYTES, 0, lane); };
         if (t < last) {
             issue_v(t);
             issue_k(t);
@@ -1310,10 +1311,17 @@ struct KeySums {
         }
     }
 };
+// The first row of the first tile of queries that sees key k0 (qlen: none does).
+VH_DEVICE int first_query(const CrossArgs &a, int k0, int start, int qlen) {
+    const int q = a.causal ? max(0, k0 - start) : 0;
+    return q < qlen ? q / CA_TILE * CA_TILE : qlen;
+}
+// Keys that no query sees are copies of the last one that some does.
 template <typename T>
-VH_DEVICE void load_keys(const CrossArgs &a, KeyRows<T> &w, int s, int kh, int key, int klen, int lh) {
-    if (klen <= 0) return;
-    const int64_t kr = min(key, klen - 1);
+VH_DEVICE void load_keys(const CrossArgs &a, KeyRows<T> &w, int s, int kh, int key, int start, int qlen, int klen, int lh) {
+    const int end = a.causal ? min(klen, start + qlen) : klen;
+    if (end <= 0) return;
+    const int64_t kr = min(key, end - 1);
     const T *kp = reinterpret_cast<const T *>(a.k.p + s * a.k.seq + kr * a.k.row + kh * a.k.head);
     const T *vp = reinterpret_cast<const T *>(a.v.p + s * a.v.seq + kr * a.v.row + kh * a.v.head);
 #pragma unroll
@@ -1389,12 +1397,9 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(CrossArgs a) {
     const int k0 = 128 * kt + 32 * wave, key = k0 + li;
     const bool active = k0 < klen;
     // the first query that sees a key of the workgroup
-    int first = 0;
-    if (a.causal) first = max(0, min(128 * kt - start, qlen)) / CA_TILE * CA_TILE;
-    if (128 * kt >= klen) first = qlen;
+    const int first = 128 * kt < klen ? first_query(a, 128 * kt, start, qlen) : qlen;
     // and one of the wave's own: the tiles before it are the other waves' (as in the forward)
-    int mine = active ? first : qlen;
-    if (active && a.causal) mine = max(first, max(0, min(k0 - start, qlen)) / CA_TILE * CA_TILE);
+    const int mine = active ? first_query(a, k0, start, qlen) : qlen;
 
     const uint32_t lds = (uint32_t)(uintptr_t)smem, rs_lds = (uint32_t)(uintptr_t)rs;
     const int G = a.H / a.KV;
@@ -1407,7 +1412,7 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(CrossArgs a) {
     };
     if (first < qlen) issue(kh * G, first, 0);
     KeyRows<T> w;
-    load_keys(a, w, s, kh, key, klen, lh);
+    load_keys(a, w, s, kh, key, start, qlen, klen, lh);
     KeySums sums;
     sums.clear();
     int buf = 0;
@@ -1468,8 +1473,8 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_split_kernel(CrossArgs a) {
     const int start = cross_start(a, s);
     const int qlen = cross_length(a.query_lengths, s, a.Lq), klen = cross_length(a.key_lengths, s, a.Lk);
     const int k0 = 32 * kt, key = k0 + (lane & 31);
-    int begin = 0, tiles = k0 < klen ? (qlen + 31) / 32 : 0;
-    if (a.causal) begin = min(tiles, max(0, min(k0 - start, qlen)) / 32);
+    const int tiles = k0 < klen ? (qlen + 31) / 32 : 0;
+    const int begin = min(tiles, (first_query(a, k0, start, qlen) + 31) / 32);
     const int each = tiles - begin;  // of a head, the workgroup's numbered head by head
     const int64_t all = (int64_t)each * a.kv_heads;
     const int first = (int)(all * part / a.kv_parts), last = (int)(all * (part + 1) / a.kv_parts);
@@ -1483,7 +1488,7 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_split_kernel(CrossArgs a) {
     int t = first + wave;
     {
         KeyRows<T> w;
-        load_keys(a, w, s, kh, key, klen, lh);
+        load_keys(a, w, s, kh, key, start, qlen, klen, lh);
         const LdsTile<T> Q{smem + wave * L::WAVE}, D{Q.p + Tile<T>::BYTES};
         const uint32_t lds = (uint32_t)(uintptr_t)smem + (uint32_t)(wave * L::WAVE);
         RowStats *rs = stats + wave;

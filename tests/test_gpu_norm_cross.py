@@ -307,6 +307,29 @@ def test_causal(ctx, size, start, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("buckets", [0, 32])
+@pytest.mark.parametrize("size,start", [((2, 8, 2, 1, 300), [100, 17]), ((2, 4, 4, 5, 90), [60, 0]),
+                                        ((2, 4, 2, 70, 400), [200, 3]), ((5, 16, 16, 600, 700), [40, 0, -20, 77, 99])],
+                         ids=str)
+def test_causal_cache_not_yet_filled(ctx, size, start, buckets, dtype):
+    """Keys that come after every query hold NaN and infinity, as memory that a cache has not written: nobody sees
+    them."""
+    S, H, KV, Lq, Lk = size
+    q, k, v, dout = make(*size, dtype)
+    kw = dict(causal=True, query_start=start)
+    if buckets:
+        kw.update(bias_table=randn(9, buckets, H), bidirectional=False)
+    val, tol = R.attention(q, k, v, dout=dout, **kw)
+    for s in range(S):
+        end = start[s] + Lq
+        k[s, end::2], k[s, end + 1::2], v[s, end::2], v[s, end + 1::2] = NAN, math.inf, -math.inf, NAN
+    got = attend(ctx, q, k, v, dout, **kw)
+    for n in got:
+        R.assert_within(got[n], val[n], tol[n], f"{size} {n}")
+    R.assert_within(attend(ctx, q, k, v, **kw)["out"], val["out"], tol["out"], f"{size} out alone")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("size,buckets,max_distance,bidirectional,start", [
     ((1, 2, 2, 1, 1), 32, 128, True, None), ((2, 4, 4, 70, 70), 32, 128, True, None),
