@@ -222,8 +222,8 @@ int vh_layernorm(vh_context *ctx, int type, int64_t rows, int dim, const void *x
    summed in a fixed order: equal calls give equal bits.  They need `workspace`,
    vh_layernorm_workspace_bytes(rows, dim) bytes of device memory, 16-byte
    aligned, the caller's: it is free again when the call's work is done, and two
-   captured graphs that may run at once need one each.  dx may be dy or x at the same pitch.  With
-   0 rows dgamma and dbeta are 0.  Issues kernels only. */
+   captured graphs that may run at once need one each.  dx may be dy or x, at the
+   same pitch.  With 0 rows dgamma and dbeta are 0.  Issues kernels only. */
 int vh_layernorm_backward(vh_context *ctx, int type, int64_t rows, int dim, const void *dy, int64_t lddy, const void *x,
                           int64_t ldx, const float *gamma, const float *stats, void *dx, int64_t lddx, float *dgamma,
                           float *dbeta, void *workspace);

@@ -524,7 +524,7 @@ bool cross_attention_backward(hipStream_t s, const vh_cross *c, const CrossBuffe
         return false;
     }
     const bool rows = cross_rows(c) > 0, keys = (int64_t)c->sequences * c->key_length > 0;
-    if ((rows && (!b.q || !b.out || !b.saved || !b.dout || !b.dq)) || (rows && keys && (!b.k || !b.v)) || !b.workspace) {
+    if ((rows && (!b.q || !b.out || !b.saved || !b.dout || !b.dq)) || ((rows || b.dk) && keys && (!b.k || !b.v)) || !b.workspace) {
         set_error("%s: null q, k, v, out, saved, dout, dq or workspace", what);
         return false;
     }

@@ -540,6 +540,21 @@ def test_refusals(ctx):
     assert bool((out == 5.0).all())
 
 
+def test_keys_without_rows(ctx):
+    """No query rows: dk and dv are 0, and null keys are refused there too."""
+    q, k, v, dout = make(2, 2, 2, 0, 5, F32)
+    p = native.CrossAttention(ctx, q, k, v, q)
+    dk, dv, ws = torch.full_like(k, NAN), torch.full_like(k, NAN), buf(p.workspace_bytes(True))
+    null = lambda t: None if not t.numel() else t.data_ptr()  # noqa: E731
+    call = lambda k: native.lib().vh_cross_attention_backward(  # noqa: E731
+        ctx.h, p._ref, null(q), k, v.data_ptr(), null(q), ws.data_ptr(), null(dout), null(q), dk.data_ptr(),
+        dv.data_ptr(), None, ws.data_ptr())
+    assert not call(None) and "null" in native.last_error()
+    assert call(k.data_ptr())
+    torch.cuda.synchronize()
+    assert not bool(dk.any()) and not bool(dv.any())
+
+
 @pytest.mark.parametrize("causal", [False, True])
 def test_gradients_by_differences(ctx, causal):
     """dq, dk, dv and dbias against central differences of the forward pass in a random direction."""
