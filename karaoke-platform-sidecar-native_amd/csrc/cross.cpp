@@ -14,6 +14,8 @@
 
 namespace vh {
 
+constexpr int64_t MAX_THREADS = UINT32_MAX;  // of a launch
+
 // --------------------------------------------------------------- layer norm
 constexpr int LN_MAX_DIM = 16384;
 // A row's lanes.  Forward: 16 of a wave while 32 elements of bf16, 16 of fp32, a lane
@@ -58,11 +60,20 @@ size_t layernorm_workspace_bytes(int64_t rows, int dim) {
 template <typename T, int LANES, int N, int NV>
 static void layernorm_launch(hipStream_t s, const NormArgs &a, bool backward, int parts) {
     using S = NormShape<LANES, N, NV>;
-    if (backward)
+    if (backward) {
         hipLaunchKernelGGL((layernorm_backward_kernel<T, LANES, N, NV>), dim3((unsigned)parts), dim3(S::THREADS), 0, s, a);
-    else
-        hipLaunchKernelGGL((layernorm_kernel<T, LANES, N, NV>), dim3((unsigned)((a.rows + S::ROWS - 1) / S::ROWS)),
-                           dim3(S::THREADS), 0, s, a);
+        return;
+    }
+    constexpr int64_t MOST = MAX_THREADS / S::THREADS * S::ROWS;  // rows of a launch
+    for (int64_t row = 0; row < a.rows; row += MOST) {
+        NormArgs b = a;
+        b.rows = std::min(MOST, a.rows - row);
+        b.x = static_cast<const T *>(a.x) + row * a.ldx;
+        b.y = static_cast<T *>(a.y) + row * a.ldy;
+        if (a.stats) b.stats = a.stats + row;
+        hipLaunchKernelGGL((layernorm_kernel<T, LANES, N, NV>), dim3((unsigned)((b.rows + S::ROWS - 1) / S::ROWS)),
+                           dim3(S::THREADS), 0, s, b);
+    }
 }
 // E: the lane's elements, in loads of 16 bytes.
 template <typename T, int LANES, int E>
@@ -229,13 +240,14 @@ static bool cross_ok(const char *what, const vh_cross *c, bool backward) {
                    {"v", c->v_strides, c->key_length, c->kv_heads, backward},
                    {"out", c->out_strides, c->query_length, c->heads, true}};
     for (const auto &t : tensors) {
+        const int64_t counts[3] = {c->sequences, t.rows, t.heads};  // of one of them the stride counts for nothing
         for (int i = 0; i < 3; i++)
-            if (t.strides[i] < 0 || t.strides[i] * size % 16 || t.strides[i] > ((int64_t)1 << 46)) {
+            if (counts[i] > 1 && (t.strides[i] < 0 || t.strides[i] * size % 16 || t.strides[i] > ((int64_t)1 << 46))) {
                 set_error("%s: %s's strides %lld, %lld, %lld: none negative, whole multiples of 16 bytes", what, t.name,
                           (long long)t.strides[0], (long long)t.strides[1], (long long)t.strides[2]);
                 return false;
             }
-        if (t.strides[1] * size > CA_MAX_ROW) {
+        if (t.rows > 1 && t.strides[1] * size > CA_MAX_ROW) {
             set_error("%s: %s's row stride of %lld is over %lld bytes", what, t.name, (long long)t.strides[1],
                       (long long)CA_MAX_ROW);
             return false;
@@ -398,10 +410,32 @@ static CrossWork backward_work(const vh_cross *c) {
     return w;
 }
 
+// Workgroups of the joining kernels: 16 rows each.
+static int64_t join_groups(int64_t rows) { return (rows + 15) / 16; }
+static int64_t key_rows(const vh_cross *c) { return (int64_t)c->sequences * c->kv_heads * c->key_length; }
+
+// Whether a call's launches are within the device's.
+static bool launches_ok(const char *what, const vh_cross *c, const CrossWork &w, bool backward) {
+    int64_t most = std::max(w.rows.grid(), w.rows.parts > 1 ? join_groups(cross_rows(c)) : 0);
+    if (backward) {
+        most = std::max(most, w.keys.grid());
+        most = std::max(most, (w.rows.parts > 1 ? join_groups(cross_rows(c)) : 0) +
+                                  (kv_pieces(c, w.keys) > 1 ? 2 * join_groups(key_rows(c)) : 0) + c->heads);
+    }
+    if (most <= MAX_THREADS / 256) return true;
+    set_error("%s: %lld workgroups", what, (long long)most);
+    return false;
+}
+
 size_t cross_workspace_bytes(const vh_cross *c, bool backward) {
-    if (!cross_ok("vh_cross_workspace_bytes", c, backward)) return 0;
-    if (backward) return std::max<size_t>(16, backward_work(c).bytes);
-    return std::max<size_t>({16, forward_work(c, false).bytes, forward_work(c, true).bytes});
+    const char *what = "vh_cross_workspace_bytes";
+    if (!cross_ok(what, c, backward)) return 0;
+    if (backward) {
+        const CrossWork w = backward_work(c);
+        return launches_ok(what, c, w, true) ? std::max<size_t>(16, w.bytes) : 0;
+    }
+    const CrossWork w = forward_work(c, false), keep = forward_work(c, true);
+    return launches_ok(what, c, w, false) && launches_ok(what, c, keep, false) ? std::max<size_t>({16, w.bytes, keep.bytes}) : 0;
 }
 
 static CrossTensor cross_tensor(const void *p, const int64_t *strides, int64_t size) {
@@ -484,6 +518,7 @@ bool cross_attention(hipStream_t s, const vh_cross *c, const CrossBuffers &b, Ke
     if (!aligned(what, {b.q, b.k, b.v, b.out, b.saved, b.workspace})) return false;
     CrossArgs a = cross_args(c, b);
     const CrossWork w = forward_work(c, a.stats != nullptr);
+    if (!launches_ok(what, c, w, false)) return false;
     if (w.bytes && !b.workspace) {
         set_error("%s: null workspace (vh_cross_workspace_bytes)", what);
         return false;
@@ -531,6 +566,7 @@ bool cross_attention_backward(hipStream_t s, const vh_cross *c, const CrossBuffe
     if (!aligned(what, {b.q, b.k, b.v, b.out, b.saved, b.workspace, b.dout, b.dq, b.dk, b.dv})) return false;
     CrossArgs a = cross_args(c, b);
     const CrossWork w = backward_work(c);
+    if (!launches_ok(what, c, w, true)) return false;
     auto at = [&](size_t n) { return reinterpret_cast<float *>(static_cast<char *>(b.workspace) + n); };
     a.rows = at(w.stats);
     a.parts = w.rows.parts;
@@ -557,8 +593,8 @@ bool cross_attention_backward(hipStream_t s, const vh_cross *c, const CrossBuffe
         if (!sync_debug(s, "cross_dkv_kernel")) return false;
     }
     FinishArgs f{};
-    if (rows && w.rows.split && w.rows.parts > 1) f.dq = (cross_rows(c) + 15) / 16;
-    if (dkv && kv_pieces(c, w.keys) > 1) f.dkv = ((int64_t)c->sequences * c->kv_heads * c->key_length + 15) / 16;
+    if (rows && w.rows.split && w.rows.parts > 1) f.dq = join_groups(cross_rows(c));
+    if (dkv && kv_pieces(c, w.keys) > 1) f.dkv = join_groups(key_rows(c));
     const int64_t groups = f.dq + 2 * f.dkv + (b.dbias ? c->heads : 0);
     if (!groups) return true;
     Scope sc(t, s, "cross_attention_sums");

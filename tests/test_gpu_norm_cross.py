@@ -121,6 +121,20 @@ def test_layernorm_unaligned(ctx, dtype):
     check_norm(ctx, x, gamma, beta, dy, "unaligned")
 
 
+def test_layernorm_beyond_one_launch(ctx):
+    """More rows than one launch has places for, at single-column pitch: (a, b) has the norm (+-1, -+1) where a != b."""
+    rows = (1 << 28) + 5
+    x = torch.zeros(rows, 2, dtype=BF16, device=DEV)
+    x[:, 0] = 1
+    x[-7:] = torch.tensor([0, 1], dtype=BF16, device=DEV)
+    gamma = torch.tensor([2.0, 4.0], device=DEV)
+    st = torch.full((rows, 2), NAN, device=DEV)
+    ctx.layernorm(x, gamma, None, x, rows, 2, eps=0.0, stats=st, bf16=True)
+    want = torch.tensor([2.0, -4.0], dtype=BF16, device=DEV)
+    assert bool((x[:-7] == want).all()) and bool((x[-7:] == -want).all())
+    assert bool((st == torch.tensor([0.5, 2.0], device=DEV)).all())
+
+
 def test_layernorm_values(ctx):
     """Rows far from 0 (the variance is taken about the mean), constant rows (variance 0, only eps), eps 0, tiny and
     huge rows; no weights' gradients wanted."""
@@ -435,6 +449,15 @@ def test_strides(ctx, strides, dtype):
     check(ctx, q, k, v, dout, str(strides), bias_table=randn(9, 32, 4), key_lengths=[45, 20])
     q1, k1, v1, dout1 = make(2, 4, 2, 1, 300, dtype, strides=strides)
     check(ctx, q1, k1, v1, dout1, str(strides), key_lengths=[300, 20])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_strides_of_single_ones(ctx, dtype):
+    """One row, one head, one sequence: whatever their strides are."""
+    for size in ((1, 1, 1, 1, 40), (1, 2, 2, 1, 1), (3, 1, 1, 1, 1), (1, 1, 1, 50, 40)):
+        q, k, v, dout = make(*size, dtype)
+        odd = lambda t: t.as_strided(t.shape, [n if m > 1 else 77 for m, n in zip(t.shape[:3], t.stride())] + [1])  # noqa: E731
+        check(ctx, odd(q), odd(k), odd(v), dout, str(size))
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

@@ -50,6 +50,29 @@ def test_layout_refused(change, text):
     assert refused(layout(**change), 0, text)
 
 
+@pytest.mark.parametrize("change,backward", [
+    # single rows of 2^24 (sequence, head) pairs, a workgroup each; more key tiles than that beside single queries
+    ({"sequences": 1 << 20, "heads": 16, "kv_heads": 16, "query_length": 1, "key_length": 1}, 0),
+    ({"sequences": 1 << 21, "heads": 1, "kv_heads": 1, "query_length": 1, "key_length": 1025}, 1),
+])
+def test_launches_beyond_the_device(change, backward):
+    heads = change["heads"] * 64
+    rows = (change["query_length"] * heads, heads, 64)
+    c = layout(**change, q_strides=rows, out_strides=rows, k_strides=(change["key_length"] * heads, heads, 64),
+               v_strides=(change["key_length"] * heads, heads, 64))
+    assert refused(c, backward, "workgroups")
+    c.sequences //= 2
+    assert native.lib().vh_cross_workspace_bytes(ctypes.byref(c), backward) > 0, native.last_error()
+
+
+def test_strides_of_single_ones():
+    """Where there is one sequence, row or head, its stride counts for nothing."""
+    odd = (7, -3, 1 << 60)
+    c = layout(sequences=1, heads=1, kv_heads=1, query_length=1, key_length=1, q_strides=odd, k_strides=odd, v_strides=odd,
+               out_strides=odd)
+    assert native.lib().vh_cross_workspace_bytes(ctypes.byref(c), 1) > 0, native.last_error()
+
+
 def test_broadcast_inputs_have_no_gradient():
     """Keys that all sequences share, or heads on one place: fine to read, refused where a gradient goes there."""
     for name, strides in (("k_strides", (0, 256, 64)), ("v_strides", (1792, 0, 64)), ("q_strides", (2560, 512, 0))):
