@@ -335,8 +335,9 @@ class Context:
 class CrossAttention:
     """The layout of an attention over another sequence's states (vh_cross), for tensors q [S][Lq][H][64], k and v
     [S][Lk][KV heads][64] and out as q, of any strides that vh_cross takes.  Later calls may pass other tensors of the
-    same layout.  query_lengths, key_lengths, query_start: int32 device tensors [S]; bias_table: fp32 [buckets][H].
-    Shapes, types and devices are checked here; strides and sizes by the library."""
+    same layout (dq, dk, dv as q, k, v and dout as out).  query_lengths, key_lengths, query_start: int32 device tensors
+    [S]; bias_table: fp32 [buckets][H].  Shapes, types, devices and the buffers' sizes are checked here; what the library
+    takes of strides and sizes by it."""
 
     def __init__(self, ctx: Context, q, k, v, out, *, causal: bool = False, scale: float = 0.125, query_lengths=None,
                  key_lengths=None, query_start=None, bias_table=None, max_distance: int = 128,
@@ -349,6 +350,9 @@ class CrossAttention:
             raise NativeError("CrossAttention: q and out [S][Lq][H][64], k and v [S][Lk][KV][64], all fp32 or all bf16")
         if any(t.stride(3) != 1 for t in (q, k, v, out)):
             raise NativeError("CrossAttention: a head's 64 elements are consecutive")
+        if any(t is not None and t.device != q.device
+               for t in (k, v, out, query_lengths, key_lengths, query_start, bias_table)):
+            raise NativeError("CrossAttention: tensors on different devices")
         for t in (query_lengths, key_lengths, query_start):
             if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (S,) or not t.is_contiguous()):
                 raise NativeError("CrossAttention: lengths and starts are contiguous int32 [S]")
@@ -366,6 +370,31 @@ class CrossAttention:
             self.c.buckets, self.c.max_distance = bias_table.shape[0], max_distance
             self.c.bidirectional = int(bidirectional)
         self._ref = ctypes.byref(self.c)
+        self._like = {n: (t.dtype, t.shape, t.stride(), t.device)
+                      for n, t in (("q", q), ("k", k), ("v", v), ("out", out))}
+        self._packed = {"q": q.is_contiguous(), "k": k.is_contiguous(), "v": v.is_contiguous(), "out": out.is_contiguous()}
+        self._bytes = {}
+
+    def _tensor(self, name, like, t):
+        """t's address; laid out as `like` was, or (of contiguous ones) any view of as many elements."""
+        dtype, shape, stride, device = self._like[like]
+        if t.shape == shape:
+            same = t.stride() == stride or not t.numel() or \
+                all(n == 1 or a == b for n, a, b in zip(shape, t.stride(), stride))
+        else:
+            same = t.is_contiguous() and self._packed[like] and t.numel() == shape.numel()
+        if not same or t.dtype != dtype or t.device != device:
+            raise NativeError(f"CrossAttention: {name} is not laid out as {like} was")
+        return t.data_ptr()
+
+    def _buffer(self, name, t, size, *key):
+        if t is None:
+            return None
+        if key not in self._bytes:
+            self._bytes[key] = size(*key[1:])
+        if t.numel() * t.element_size() < self._bytes[key] or t.device != self._like["q"][3]:
+            raise NativeError(f"CrossAttention: {name} has fewer than {self._bytes[key]} bytes, or is on another device")
+        return t.data_ptr()
 
     def saved_bytes(self) -> int:
         n = int(lib().vh_cross_saved_bytes(self._ref))
@@ -378,13 +407,24 @@ class CrossAttention:
         return n
 
     def forward(self, q, k, v, out, saved=None, workspace=None):
-        _ok(lib().vh_cross_attention(self.ctx.h, self._ref, ptr(q), ptr(k), ptr(v), ptr(out), _opt(saved),
-                                     _opt(workspace)), "vh_cross_attention")
+        f = self._tensor
+        args = (f("q", "q", q), f("k", "k", k), f("v", "v", v), f("out", "out", out),
+                self._buffer("saved", saved, self.saved_bytes, "saved"),
+                self._buffer("workspace", workspace, self.workspace_bytes, "workspace", False))
+        _ok(lib().vh_cross_attention(self.ctx.h, self._ref, *args), "vh_cross_attention")
 
     def backward(self, q, k, v, out, saved, dout, dq, dk=None, dv=None, dbias=None, workspace=None):
-        _ok(lib().vh_cross_attention_backward(self.ctx.h, self._ref, ptr(q), ptr(k), ptr(v), ptr(out), ptr(saved),
-                                              ptr(dout), ptr(dq), _opt(dk), _opt(dv), _opt(dbias), _opt(workspace)),
-            "vh_cross_attention_backward")
+        f = self._tensor
+        table = self._kept[3]
+        if dbias is not None and table is not None and \
+                ((dbias.dtype, dbias.shape, dbias.device) != (table.dtype, table.shape, table.device) or
+                 not dbias.is_contiguous()):
+            raise NativeError("CrossAttention: dbias is not laid out as the bias table")
+        args = (f("q", "q", q), f("k", "k", k), f("v", "v", v), f("out", "out", out),
+                self._buffer("saved", saved, self.saved_bytes, "saved"), f("dout", "out", dout), f("dq", "q", dq),
+                f("dk", "k", dk) if dk is not None else None, f("dv", "v", dv) if dv is not None else None, _opt(dbias),
+                self._buffer("workspace", workspace, self.workspace_bytes, "workspace", True))
+        _ok(lib().vh_cross_attention_backward(self.ctx.h, self._ref, *args), "vh_cross_attention_backward")
 
 
 class Model:

@@ -156,3 +156,27 @@ def test_binding_checks_shapes():
     c = native.CrossAttention(None, **good, bias_table=table).c
     assert (c.sequences, c.heads, c.kv_heads, c.query_length, c.key_length, c.buckets) == (2, 8, 4, 5, 7, 32)
     assert list(c.k_strides) == [7 * 256, 256, 64]
+
+
+def test_binding_checks_calls():
+    """Tensors of a later call that the layout does not describe, and buffers that are too small, are refused before the
+    library sees them."""
+    q, k = torch.zeros(2, 5, 8, 64), torch.zeros(2, 7, 4, 64)
+    table = torch.zeros(32, 8)
+    p = native.CrossAttention(None, q, k, k, q, bias_table=table)
+    saved, ws = torch.zeros(p.saved_bytes(), dtype=torch.uint8), torch.zeros(p.workspace_bytes(True), dtype=torch.uint8)
+    good = dict(q=q, k=k, v=k, out=q, saved=saved, workspace=ws)
+    more = dict(dout=q, dq=q, dk=k, dv=k, dbias=table)
+    turned = q.transpose(1, 2).contiguous().transpose(1, 2)
+    for bad, text in (({"q": turned}, "q is not"), ({"k": k.bfloat16()}, "k is not"), ({"v": k[:, :5]}, "v is not"),
+                      ({"out": turned}, "out is not"), ({"saved": saved[:-1]}, "saved"), ({"workspace": ws[:15]}, "workspace")):
+        with pytest.raises(native.NativeError, match=text):
+            p.forward(**{**good, **bad})
+    for bad, text in (({"dout": q[:1, :1].expand_as(q)}, "dout is not"), ({"dq": turned}, "dq is not"),
+                      ({"dk": k[:1]}, "dk is not"), ({"dv": k.double()}, "dv is not"), ({"workspace": ws[:-1]}, "workspace"),
+                      ({"saved": saved[:-1]}, "saved"), ({"dbias": table[:16]}, "dbias"), ({"dbias": table.t()}, "dbias"),
+                      ({"dbias": table.bfloat16()}, "dbias")):
+        with pytest.raises(native.NativeError, match=text):
+            p.backward(**{**good, **more, **bad})
+    with pytest.raises(native.NativeError, match="devices"):
+        native.CrossAttention(None, q, k, k, q, bias_table=table.to("meta"))
