@@ -149,7 +149,7 @@ bool layernorm_backward(hipStream_t s, const LayerNorm &n, KernelTimer *t) {
         if (!sync_debug(s, "layernorm_backward_kernel")) return false;
     }
     if (!weights) return true;
-    hipLaunchKernelGGL(layernorm_columns_kernel, dim3((unsigned)(2 * n.dim + 63) / 64), dim3(1024), 0, s,
+    hipLaunchKernelGGL(layernorm_columns_kernel, dim3((unsigned)(2 * n.dim + 15) / 16), dim3(1024), 0, s,
                        static_cast<const float *>(n.workspace), parts, n.dim, n.dgamma, n.dbeta);
     return sync_debug(s, "layernorm_columns_kernel");
 }

@@ -244,20 +244,22 @@ static __global__ __launch_bounds__((NormShape<LANES, N, NV>::THREADS)) void lay
     }
 }
 
-// Column sums of the workgroups' parts [parts][2 dim]: 64 columns x 16 rows a
-// workgroup.  out: dgamma, then dbeta (either may be null).
+// Column sums of the workgroups' parts [parts][2 dim]: 16 columns x 64 rows a
+// workgroup, so that a thread's loads (8 of 512 parts) are all under way at once.
 static __global__ __launch_bounds__(1024) void layernorm_columns_kernel(const float *part, int parts, int dim,
                                                                          float *dgamma, float *dbeta) {
-    __shared__ float sums[16][64];
-    const int i = (int)threadIdx.x & 63, c = (int)blockIdx.x * 64 + i, w = (int)threadIdx.x >> 6;
+    __shared__ float sums[16][16];
+    const int tid = (int)threadIdx.x, i = tid & 15, c = (int)blockIdx.x * 16 + i;
     float sum = 0.0f;
     if (c < 2 * dim) {
 #pragma unroll 8
-        for (int p = w; p < parts; p += 16) sum += part[(int64_t)p * 2 * dim + c];
+        for (int p = tid >> 4; p < parts; p += 64) sum += part[(int64_t)p * 2 * dim + c];
     }
-    sums[w][i] = sum;
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if ((tid & 63) < 16) sums[tid >> 6][i] = sum;
     __syncthreads();
-    if (w || c >= 2 * dim) return;
+    if (tid >= 16 || c >= 2 * dim) return;
 #pragma unroll
     for (int k = 1; k < 16; k++) sum += sums[k][i];
     float *out = c < dim ? dgamma : dbeta;
