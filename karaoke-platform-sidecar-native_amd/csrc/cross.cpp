@@ -295,6 +295,11 @@ static size_t dq_lds(const vh_cross *c, bool split) {
     if (!c->bias_table) return tiles_lds(c, split, 1, false);
     return tiles_lds(c, split, 1, false) + window_bytes(c) + sizeof(DbiasLds) + 128 * sizeof(float) * c->buckets + window_bytes(c) / sizeof(float);
 }
+// heads: that a workgroup takes, one after the other
+static size_t dkv_lds(const vh_cross *c, bool split, int heads) {
+    return tiles_lds(c, split, 1, false) + (split ? 4 * sizeof(RowStats) + heads * window_bytes(c)
+                                                  : 2 * (sizeof(RowStats) + window_bytes(c)));
+}
 static size_t pack_lds(const vh_cross *c) {
     return tiles_lds(c, true, 1, true) +
            (c->bias_table ? sizeof(float) * c->buckets * (c->heads / c->kv_heads) + window_bytes(c) / sizeof(float) : 0);
@@ -317,7 +322,6 @@ struct CrossCut {
 // single tokens of 32 until there are four (16 x 32 of them over 8192 keys 42 us
 // against 44; 2 x 3841 rows over 3278 so cut 120 against 107).
 constexpr int64_t CA_ENOUGH = 384, CA_PAIRED = 1024, CA_PIECES = 512, CA_ONE = 256;
-constexpr size_t CA_WINDOWS = 16 * 1024;
 static int pieces(int64_t groups, int across, bool few) {
     const int64_t tiles = (across + 31) / 32;
     if (groups <= 0) return 1;
@@ -354,13 +358,15 @@ static CrossCut dq_cut(const vh_cross *c) {
 static CrossCut dkv_cut(const vh_cross *c) {
     CrossCut cut = cross_cut((int64_t)c->sequences * c->kv_heads, c->key_length, 1, c->query_length, true);
     if (!cut.split) return cut;
-    // a workgroup takes all heads that share its keys, where their bias windows fit
-    // beside its tiles; else, or where that makes less than one workgroup per CU, the
-    // heads are pairs of their own and their sums pieces
+    // a workgroup takes all heads that share its keys, where their bias windows leave
+    // room for two workgroups on a CU (four windows of 800 positions 140 us against
+    // 143); else, or where that makes less than one workgroup per CU, the heads are
+    // pairs of their own and their sums pieces (56 workgroups: 37 us against 42; 320:
+    // together 84 against 89)
     const int shared = c->heads / c->kv_heads;
     cut.tiles = (c->key_length + 31) / 32;
     cut.heads = shared;
-    if (cut.groups() < CA_ONE || shared * window_bytes(c) > CA_WINDOWS || (int64_t)shared * c->query_length > CA_MAX_LENGTH) {
+    if (cut.groups() < CA_ONE || dkv_lds(c, true, shared) > CA_LDS / 2 || (int64_t)shared * c->query_length > CA_MAX_LENGTH) {
         cut.pairs *= shared;
         cut.heads = 1;
     }
@@ -541,8 +547,7 @@ static void dq_launch(hipStream_t s, const vh_cross *c, const CrossArgs &a, cons
 
 template <typename T, bool BIAS>
 static void dkv_launch(hipStream_t s, const vh_cross *c, const CrossArgs &a, const CrossCut &cut) {
-    const size_t lds = tiles_lds(c, cut.split, 1, false) + (cut.split ? 4 * sizeof(RowStats) + cut.heads * window_bytes(c)
-                                                        : 2 * sizeof(RowStats) + 2 * window_bytes(c));
+    const size_t lds = dkv_lds(c, cut.split, cut.heads);
     if (cut.split) launch(cross_dkv_split_kernel<T, BIAS>, cut.grid(), lds, s, a);
     else launch(cross_dkv_kernel<T, BIAS>, cut.grid(), lds, s, a);
 }

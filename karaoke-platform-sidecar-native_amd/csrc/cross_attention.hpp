@@ -531,10 +531,14 @@ VH_DEVICE void take(const float *res, int i, int rw, int lane, floatx16 &x) {
     for (int r = 0; r < 16; r++) x[r] += res[(rw * 32 + 16 * i + r) * 64 + lane];
 }
 
-// Workgroup: RW waves x 32 queries of one head (KW times), tiles of 32 keys that they share,
-// the next one's copies in flight while one is worked on.  Per wave and tile S^T =
-// K Q^T, so that a lane holds 16 scores of one query, the online softmax, and out^T
-// += V^T P^T from the same registers.  KEEP: statistics, rest, and P in two pieces.
+// Workgroup: RW waves x 32 queries of one head (KW times), tiles of 32 keys that they
+// share, the next one's copies in flight while one is worked on.  Per wave and tile
+// S^T = K Q^T, so that a lane holds 16 scores of one query, the online softmax, and
+// out^T += V^T P^T from the same registers.  KEEP: statistics, rest, and P in pieces.
+// Bound by the VALU (exponentials take four issues each) beside the matrix cores
+// where the chip is full: 4 x 16 heads x 4096 rows over 4096 with a bias 351 us, 0.78
+// PFLOP/s; below, by how evenly the workgroups fill it: 8 x 8 x 801 rows over 1723,
+// ragged, 28 us, 0.53.
 template <typename T, bool BIAS, bool KEEP, int KW>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) void cross_forward_kernel(CrossArgs a) {
     using L = SharedLds<T, KW>;
@@ -834,7 +838,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 ? 4 : 2) void cross_forward_spl
     }
 }
 
-// The pieces of every row joined: 16 lanes a row, 4 dims each.
+// The pieces of every row joined: 16 lanes a row, 4 dims each, the pieces' loads
+// under way together (512 rows of 4 pieces: 4.8 us, most of it the launch).
 template <typename T, bool BIAS, bool KEEP>
 __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
     const int64_t rows = (int64_t)a.S * a.H * a.Lq, row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
@@ -1115,7 +1120,11 @@ VH_DEVICE void dq_tile(const CrossArgs &a, const QueryRows<T> &w, const Held &q,
     }
 }
 
-// dq, delta and the table's gradient: workgroup and tiles as the forward's.
+// dq, delta and the table's gradient: workgroup and tiles as the forward's.  Three
+// products a tile; 8 x 8 heads x 1023 rows over 862 keys, ragged, bf16: 28 us, 0.51
+// PFLOP/s, at two waves on a SIMD.  Two tiles a step (half the barriers, the second
+// one's products beside the first one's exponentials): 27.5 us, and 50.5 for 50 with a
+// bias; two groups of two waves: no gain.  Neither is kept.
 template <typename T, bool BIAS>
 __global__ __launch_bounds__(256, 2) void cross_dq_kernel(CrossArgs a) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];  // [2] K and V tiles
@@ -1379,7 +1388,8 @@ VH_DEVICE void dkv_tile(const CrossArgs &a, const Held &k, const Held &v, KeySum
 }
 
 // dk and dv: workgroup of 4 waves x 32 keys of one key head, tiles of 32 queries
-// of every query head that shares it.
+// of every query head that shares it.  Four products a tile; 4 x 12 heads x 1025
+// rows over 1025 keys, ragged, with a bias: 51 us, as many as dq's with the table.
 template <typename T, bool BIAS>
 __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(CrossArgs a) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];  // [2] Q and dout tiles
@@ -1456,7 +1466,8 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_kernel(CrossArgs a) {
 // The same in too few workgroups: 4 waves take the same 32 keys and every fourth
 // tile of the queries of all heads that share them, one head after the other; or,
 // where there are too few such workgroups, each head and a.kv_parts pieces of its
-// queries are workgroups of their own.
+// queries are workgroups of their own.  8 x 8 heads over 4 x 862 keys, 1023 rows,
+// bf16: 36 us.
 template <typename T, bool BIAS>
 __global__ __launch_bounds__(256, 2) void cross_dkv_split_kernel(CrossArgs a) {
     using L = SplitLds<T>;
