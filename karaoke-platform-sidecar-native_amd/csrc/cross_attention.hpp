@@ -536,8 +536,8 @@ VH_DEVICE void take(const float *res, int i, int rw, int lane, floatx16 &x) {
 // S^T = K Q^T, so that a lane holds 16 scores of one query, the online softmax, and
 // out^T += V^T P^T from the same registers.  KEEP: statistics, rest, and P in pieces.
 // Bound by the VALU (exponentials take four issues each) beside the matrix cores
-// where the chip is full: 4 x 16 heads x 4096 rows over 4096 with a bias 351 us, 0.78
-// PFLOP/s; below, by how evenly the workgroups fill it: 8 x 8 x 801 rows over 1723,
+// where the chip is full: 4 x 16 heads x 4096 rows over 4096 with a bias 347 to 367 us,
+// 0.75 to 0.79 PFLOP/s (VALU 83% busy, matrix cores 39%); below, by how evenly the workgroups fill it: 8 x 8 x 801 rows over 1723,
 // ragged, 28 us, 0.53.
 template <typename T, bool BIAS, bool KEEP, int KW>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) void cross_forward_kernel(CrossArgs a) {
