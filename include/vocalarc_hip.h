@@ -263,7 +263,7 @@ typedef struct {
    none (no keys, causal before the first one, or a bias of -inf at all of them)
    is 0.  The products run on the bf16 matrix cores: bf16 operands as they are, P
    rounded to bf16; fp32 operands as three bf16 values each, whose products keep 24
-   bits (infinities in them give NaN); scores, softmax and sums are fp32.
+   bits (infinities in them, and what bf16 would round to one, give NaN); scores, softmax and sums are fp32.
    A key that no row sees is never read.  A NaN or infinity in a value that a row's
    neighbours see and it does not, causal, may reach it (0 times it is NaN).
    saved (may be null): vh_cross_saved_bytes bytes for the backward pass (the
