@@ -320,7 +320,8 @@ struct CrossCut {
 // four per CU (30 against 34 us for the same 448; backward no gain).  Below, pieces
 // of at least 8 tiles (two a wave) until there are about two workgroups per CU, for
 // single tokens of 32 until there are four (16 x 32 of them over 8192 keys 42 us
-// against 44; 2 x 3841 rows over 3278 so cut 120 against 107).
+// against 44; 2 x 3841 rows over 3278 so cut 120 against 107; dk and dv of 416
+// workgroups in two pieces, 4 x 8 x 801 rows fp32, 130 against 120).
 constexpr int64_t CA_ENOUGH = 384, CA_PAIRED = 1024, CA_PIECES = 512, CA_ONE = 256;
 static int pieces(int64_t groups, int across, bool few) {
     const int64_t tiles = (across + 31) / 32;

@@ -1259,28 +1259,26 @@ __global__ __launch_bounds__(256, 2) void cross_dq_split_kernel(CrossArgs a) {
     zero16(acc[1]);
     const char *kp = a.k.p + s * a.k.seq + kh * a.k.head, *vp = a.v.p + s * a.v.seq + kh * a.v.head;
     int t = first + wave;
-    {
-        const LdsTile<T> K{smem + wave * L::WAVE}, V{K.p + Tile<T>::BYTES};
-        const uint32_t lds = (uint32_t)(uintptr_t)smem + (uint32_t)(wave * L::WAVE);
-        auto issue_k = [&](int t) { tile_issue<T, 1>(kp, a.k.row, 32 * t, keys - 1, lds, 0, lane); };
-        auto issue_v = [&](int t) { tile_issue<T, 1>(vp, a.v.row, 32 * t, keys - 1, lds + Tile<T>::BYTES, 0, lane); };
-        if (t < last) {
-            issue_v(t);
-            issue_k(t);
-        }
-        for (; t < last; t += 4) {
-            const bool next = t + 4 < last;
-            wait_vmcnt<L::LOADS>();  // V is there, K may be under way
-            dq_tile<T, BIAS>(
-                a, w, w.q, w.dout, delta, acc, db, window, K, V, 32 * t, start + q, start + q0, klen, wave, lane,
-                [&] { wait_tile<L::LOADS>(next); },
-                [&] {
-                    wait_lds();
-                    if (next) issue_v(t + 4);
-                });
-            wait_lds();
-            if (next) issue_k(t + 4);
-        }
+    const LdsTile<T> K{smem + wave * L::WAVE}, V{K.p + Tile<T>::BYTES};
+    const uint32_t lds = (uint32_t)(uintptr_t)smem + (uint32_t)(wave * L::WAVE);
+    auto issue_k = [&](int t) { tile_issue<T, 1>(kp, a.k.row, 32 * t, keys - 1, lds, 0, lane); };
+    auto issue_v = [&](int t) { tile_issue<T, 1>(vp, a.v.row, 32 * t, keys - 1, lds + Tile<T>::BYTES, 0, lane); };
+    if (t < last) {
+        issue_v(t);
+        issue_k(t);
+    }
+    for (; t < last; t += 4) {
+        const bool next = t + 4 < last;
+        wait_vmcnt<L::LOADS>();  // V is there, K may be under way
+        dq_tile<T, BIAS>(
+            a, w, w.q, w.dout, delta, acc, db, window, K, V, 32 * t, start + q, start + q0, klen, wave, lane,
+            [&] { wait_tile<L::LOADS>(next); },
+            [&] {
+                wait_lds();
+                if (next) issue_v(t + 4);
+            });
+        wait_lds();
+        if (next) issue_k(t + 4);
     }
     if constexpr (BIAS) {
         if (a.dbias_part) db.finish(a, h, (s * rtiles + rt) * a.parts + part, tid, true);
@@ -1497,38 +1495,36 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_split_kernel(CrossArgs a) {
     KeySums sums;
     sums.clear();
     int t = first + wave;
-    {
-        KeyRows<T> w;
-        load_keys(a, w, s, kh, key, start, qlen, klen, lh);
-        const LdsTile<T> Q{smem + wave * L::WAVE}, D{Q.p + Tile<T>::BYTES};
-        const uint32_t lds = (uint32_t)(uintptr_t)smem + (uint32_t)(wave * L::WAVE);
-        RowStats *rs = stats + wave;
-        auto issue_q = [&](int t) {
-            const char *qp = a.q.p + s * a.q.seq + (h + t / each) * a.q.head;
-            tile_issue<T, 1>(qp, a.q.row, 32 * (begin + t % each), qlen - 1, lds, 0, lane);
-        };
-        auto issue_dout = [&](int t) {
-            const char *dp = a.dout.p + s * a.dout.seq + (h + t / each) * a.dout.head;
-            tile_issue<T, 1>(dp, a.dout.row, 32 * (begin + t % each), qlen - 1, lds + Tile<T>::BYTES, 0, lane);
-            row_tile_issue(row_tile(a, s, h + t / each, begin + t % each), (uint32_t)(uintptr_t)rs, lane);
-        };
-        if (t < last) {
-            issue_dout(t);
-            issue_q(t);
-        }
-        for (; t < last; t += 4) {
-            const bool next = t + 4 < last;
-            wait_vmcnt<L::LOADS>();  // dout is there, Q may be under way
-            dkv_tile<T, BIAS>(
-                a, w.k, w.v, sums, BIAS ? window + t / each * cross_window(a) : nullptr, Q, D, rs,
-                32 * (begin + t % each), start, key, k0, lane, [&] { wait_vmcnt<0>(); },
-                [&] {
-                    wait_lds();
-                    if (next) issue_dout(t + 4);
-                });
-            wait_lds();
-            if (next) issue_q(t + 4);
-        }
+    KeyRows<T> w;
+    load_keys(a, w, s, kh, key, start, qlen, klen, lh);
+    const LdsTile<T> Q{smem + wave * L::WAVE}, D{Q.p + Tile<T>::BYTES};
+    const uint32_t lds = (uint32_t)(uintptr_t)smem + (uint32_t)(wave * L::WAVE);
+    RowStats *rs = stats + wave;
+    auto issue_q = [&](int t) {
+        const char *qp = a.q.p + s * a.q.seq + (h + t / each) * a.q.head;
+        tile_issue<T, 1>(qp, a.q.row, 32 * (begin + t % each), qlen - 1, lds, 0, lane);
+    };
+    auto issue_dout = [&](int t) {
+        const char *dp = a.dout.p + s * a.dout.seq + (h + t / each) * a.dout.head;
+        tile_issue<T, 1>(dp, a.dout.row, 32 * (begin + t % each), qlen - 1, lds + Tile<T>::BYTES, 0, lane);
+        row_tile_issue(row_tile(a, s, h + t / each, begin + t % each), (uint32_t)(uintptr_t)rs, lane);
+    };
+    if (t < last) {
+        issue_dout(t);
+        issue_q(t);
+    }
+    for (; t < last; t += 4) {
+        const bool next = t + 4 < last;
+        wait_vmcnt<L::LOADS>();  // dout is there, Q may be under way
+        dkv_tile<T, BIAS>(
+            a, w.k, w.v, sums, BIAS ? window + t / each * cross_window(a) : nullptr, Q, D, rs,
+            32 * (begin + t % each), start, key, k0, lane, [&] { wait_vmcnt<0>(); },
+            [&] {
+                wait_lds();
+                if (next) issue_dout(t + 4);
+            });
+        wait_lds();
+        if (next) issue_q(t + 4);
     }
     floatx4 y[2], z[2];
     waves_sum<T>(reinterpret_cast<float *>(smem), sums.dk, tid, y);
