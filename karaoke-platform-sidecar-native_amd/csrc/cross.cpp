@@ -379,7 +379,7 @@ static CrossCut dkv_cut(const vh_cross *c) {
 // The workspace's sections, in bytes from its start.
 struct CrossWork {
     CrossCut rows, keys;  // backward: of dq, of dk and dv
-    size_t stats = 0, part_o = 0, part_ml = 0, part_dk = 0, part_dv = 0, dbias = 0, bytes = 0;
+    size_t stats = 0, part_o = 0, part_ml = 0, part_dk = 0, part_dv = 0, dbias = 0, dbias_rows = 0, bytes = 0;
     int dbias_parts = 0;
     size_t take(size_t n) {
         const size_t at = bytes;
@@ -413,6 +413,7 @@ static CrossWork backward_work(const vh_cross *c) {
     if (c->bias_table) {
         w.dbias_parts = (int)(w.rows.groups() / c->heads);
         w.dbias = w.take((size_t)w.rows.groups() * c->buckets * sizeof(float));
+        if (w.rows.parts > 1) w.dbias_rows = w.take((size_t)w.rows.groups() * CA_TILE * sizeof(floatx4));
     }
     return w;
 }
@@ -584,6 +585,7 @@ bool cross_attention_backward(hipStream_t s, const vh_cross *c, const CrossBuffe
     a.dbias = b.dbias;
     a.dbias_part = b.dbias ? at(w.dbias) : nullptr;
     a.dbias_parts = w.dbias_parts;
+    a.dbias_rows = reinterpret_cast<floatx4 *>(at(w.dbias_rows));
     const bool is_bf16 = c->type == VH_TYPE_BF16;
     if (rows) {
         Scope sc(t, s, "cross_attention_dq");
@@ -601,7 +603,8 @@ bool cross_attention_backward(hipStream_t s, const vh_cross *c, const CrossBuffe
     FinishArgs f{};
     if (rows && w.rows.split && w.rows.parts > 1) f.dq = join_groups(cross_rows(c));
     if (dkv && kv_pieces(c, w.keys) > 1) f.dkv = join_groups(key_rows(c));
-    const int64_t groups = f.dq + 2 * f.dkv + (b.dbias ? c->heads : 0);
+    f.heads = b.dbias ? c->heads : 0;
+    const int64_t groups = f.heads + f.dq + 2 * f.dkv;
     if (!groups) return true;
     Scope sc(t, s, "cross_attention_sums");
     if (is_bf16) hipLaunchKernelGGL(cross_finish_kernel<bf16>, dim3((unsigned)groups), dim3(256), 0, s, a, f);

@@ -79,6 +79,7 @@ struct CrossArgs {
     float *part_dk, *part_dv;
     float *dbias_part;  // [H][dbias_parts][buckets]
     int dbias_parts;    // per head: sequences x row tiles x pieces
+    floatx4 *dbias_rows;  // pieces: [H][dbias_parts][32] rows' (sum of dS, probability in either side's far buckets, -)
     float *dbias;       // [buckets][H]
     // far buckets of one side: bucket near + i begins at distance edge[i]
     int side, near, edges;
@@ -956,7 +957,6 @@ constexpr int CA_DIAG = 20;  // pitch: 16-byte reads, and stores of 32 lanes in 
 struct DbiasLds {
     float diag[4][48 * CA_DIAG];
     float far[4][2];
-    float rows[4][CA_TILE];
 };
 struct Dbias {
     DbiasLds *db;
@@ -1036,18 +1036,22 @@ struct Dbias {
         }
         wave_order();
     }
-    // the workgroup's sums into part `at` of head h; split: its waves share their rows.
-    // Rows whose keys are shared by several workgroups are left as they are.
+    // the workgroup's sums into part `at` of head h; split: its waves share their
+    // rows.  Where several workgroups do, each leaves its part of a row's sum and
+    // probabilities, and cross_finish_kernel takes the far buckets' part out.
     VH_DEVICE void finish(const CrossArgs &a, int h, int at, int tid, bool split) {
         const int wave = tid >> 6;
         float rest = near + (lo + hi);
         rest += __shfl_xor(rest, 32, 64);
         if (split) {
-            if ((tid & 63) < 32) db->rows[wave][tid & 31] = rest;
+            const float low = p_lo + __shfl_xor(p_lo, 32, 64), high = p_hi + __shfl_xor(p_hi, 32, 64);
+            wave_order();  // the wave's diagonals are read; rows of (rest, low, high) in their place
+            float *row = &db->diag[0][0] + 4 * (tid & 31);
+            if ((tid & 63) < 32) st4(row + wave * 48 * CA_DIAG, floatx4{rest, low, high, 0.0f});
             __syncthreads();
-            rest = 0.0f;
-            if (a.parts == 1)
-                rest = (db->rows[0][tid & 31] + db->rows[1][tid & 31]) + (db->rows[2][tid & 31] + db->rows[3][tid & 31]);
+            const floatx4 v = (ld4(row) + ld4(row + 48 * CA_DIAG)) + (ld4(row + 96 * CA_DIAG) + ld4(row + 144 * CA_DIAG));
+            rest = a.parts == 1 ? v[0] : 0.0f;
+            if (a.parts > 1 && tid < 32) a.dbias_rows[((int64_t)h * a.dbias_parts + at) * 32 + tid] = v;
         }
         lo = wave_sum(__builtin_fmaf(-rest, p_lo, lo));
         hi = wave_sum(__builtin_fmaf(-rest, p_hi, hi));
@@ -1556,10 +1560,10 @@ __global__ __launch_bounds__(256, 2) void cross_dkv_split_kernel(CrossArgs a) {
     }
 }
 
-// The pieces added up, in their order: workgroups of 16 rows of dq, then of dk and
-// of dv, then one for each head's bias.
+// The pieces added up, in their order: workgroups of one head's bias each, which take
+// the longest, then of 16 rows of dq, of dk and of dv.
 struct FinishArgs {
-    int64_t dq, dkv;  // workgroups of dq; of dk (and as many of dv)
+    int64_t heads, dq, dkv;  // workgroups of the bias; of dq; of dk (and as many of dv)
 };
 template <typename T>
 VH_DEVICE void sum_parts(const float *part, int parts, int64_t rows, int64_t row, int len, int heads,
@@ -1574,21 +1578,21 @@ VH_DEVICE void sum_parts(const float *part, int parts, int64_t rows, int64_t row
 }
 template <typename T>
 __global__ __launch_bounds__(256) void cross_finish_kernel(CrossArgs a, FinishArgs f) {
-    __shared__ float sums[256];
-    int64_t block = blockIdx.x;
+    __shared__ float sums[256], far[4][2];
     const int tid = (int)threadIdx.x, sub = tid >> 4;
-    if (block < f.dq) {
-        sum_parts<T>(a.part_o, a.parts, (int64_t)a.S * a.H * a.Lq, block * 16 + sub, a.Lq, a.H, a.dq);
-        return;
-    }
-    block -= f.dq;
-    if (block < 2 * f.dkv) {
+    if (blockIdx.x >= f.heads) {
+        int64_t block = blockIdx.x - f.heads;
+        if (block < f.dq) {
+            sum_parts<T>(a.part_o, a.parts, (int64_t)a.S * a.H * a.Lq, block * 16 + sub, a.Lq, a.H, a.dq);
+            return;
+        }
+        block -= f.dq;
         const bool v = block >= f.dkv;
         sum_parts<T>(v ? a.part_dv : a.part_dk, a.H / a.KV / a.kv_heads * a.kv_parts, (int64_t)a.S * a.KV * a.Lk,
                      (block - (v ? f.dkv : 0)) * 16 + sub, a.Lk, a.KV, v ? a.dv : a.dk);
         return;
     }
-    const int h = (int)(block - 2 * f.dkv), lanes = 256 / a.buckets;  // threads that share a bucket
+    const int h = (int)blockIdx.x, lanes = 256 / a.buckets;  // threads that share a bucket
     const int b = tid % a.buckets, l = tid / a.buckets;
     float sum = 0.0f;
     if (l < lanes) {
@@ -1597,9 +1601,40 @@ __global__ __launch_bounds__(256) void cross_finish_kernel(CrossArgs a, FinishAr
             sum += a.dbias_part[((int64_t)h * a.dbias_parts + i) * a.buckets + b];
     }
     sums[tid] = sum;
+    if (a.parts > 1) {
+        // the rows' pieces joined, 8 row tiles at a time and four such loads under way
+        // (those past the last are its own, and count for nothing), and what a row's dS
+        // add up to times its probability in the far buckets
+        const floatx4 *rows = a.dbias_rows + (int64_t)h * a.dbias_parts * 32 + (tid & 31);
+        const int tiles = a.dbias_parts / a.parts;
+        float lo = 0.0f, hi = 0.0f;
+        for (int t0 = tid >> 5; t0 < tiles; t0 += 32) {
+            floatx4 v[4] = {};
+#pragma unroll 4
+            for (int i = 0; i < a.parts; i++)
+#pragma unroll
+                for (int u = 0; u < 4; u++) v[u] += rows[((int64_t)min(t0 + 8 * u, tiles - 1) * a.parts + i) * 32];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const float rest = t0 + 8 * u < tiles ? v[u][0] : 0.0f;
+                lo = __builtin_fmaf(rest, v[u][1], lo);
+                hi = __builtin_fmaf(rest, v[u][2], hi);
+            }
+        }
+        lo = wave_sum(lo);
+        hi = wave_sum(hi);
+        if ((tid & 63) == 0) {
+            far[tid >> 6][0] = lo;
+            far[tid >> 6][1] = hi;
+        }
+    }
     __syncthreads();
     if (tid >= a.buckets) return;
     for (int i = 1; i < lanes; i++) sum += sums[i * a.buckets + b];
+    if (a.parts > 1) {
+        if (b == cross_bucket(a, -a.max_distance)) sum -= (far[0][0] + far[1][0]) + (far[2][0] + far[3][0]);
+        if (b == cross_bucket(a, a.max_distance)) sum -= (far[0][1] + far[1][1]) + (far[2][1] + far[3][1]);
+    }
     a.dbias[(int64_t)b * a.H + h] = sum;
 }
 
