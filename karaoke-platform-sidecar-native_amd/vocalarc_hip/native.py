@@ -332,12 +332,30 @@ class Context:
         return ms.value, n.value
 
 
+def _reshapes(shape, like) -> bool:
+    """Whether a contiguous tensor of `shape` has the elements of a contiguous one of `like` in the same places for a
+    reader of either: each dimension joins or splits neighbours of the other's, in their order (dimensions of 1 aside)."""
+    a, b = [n for n in shape if n != 1], [n for n in like if n != 1]
+    if 0 in a or 0 in b:
+        return 0 in a and 0 in b
+    while a and b:
+        n, m = a.pop(0), b.pop(0)
+        many = b if n > m else a  # whose dimensions are joined to the wider one
+        wide, joined = max(n, m), min(n, m)
+        while joined < wide and many:
+            joined *= many.pop(0)
+        if joined != wide:
+            return False
+    return not a and not b
+
+
 class CrossAttention:
     """The layout of an attention over another sequence's states (vh_cross), for tensors q [S][Lq][H][64], k and v
     [S][Lk][KV heads][64] and out as q, of any strides that vh_cross takes.  Later calls may pass other tensors of the
-    same layout (dq, dk, dv as q, k, v and dout as out).  query_lengths, key_lengths, query_start: int32 device tensors
-    [S]; bias_table: fp32 [buckets][H].  Shapes, types, devices and the buffers' sizes are checked here; what the library
-    takes of strides and sizes by it."""
+    same layout (dq, dk, dv as q, k, v and dout as out); contiguous ones also in a shape that joins or splits neighbouring
+    dimensions ([S * Lq][H * 64]).  query_lengths, key_lengths, query_start: int32 device tensors [S]; bias_table: fp32
+    [buckets][H].  Shapes, types, devices and the buffers' sizes are checked here; what the library takes of strides and
+    sizes by it."""
 
     def __init__(self, ctx: Context, q, k, v, out, *, causal: bool = False, scale: float = 0.125, query_lengths=None,
                  key_lengths=None, query_start=None, bias_table=None, max_distance: int = 128,
@@ -376,13 +394,13 @@ class CrossAttention:
         self._bytes = {}
 
     def _tensor(self, name, like, t):
-        """t's address; laid out as `like` was, or (of contiguous ones) any view of as many elements."""
+        """t's address; laid out as `like` was, or (of contiguous ones) a shape that joins or splits its dimensions."""
         dtype, shape, stride, device = self._like[like]
         if t.shape == shape:
             same = t.stride() == stride or not t.numel() or \
                 all(n == 1 or a == b for n, a, b in zip(shape, t.stride(), stride))
         else:
-            same = t.is_contiguous() and self._packed[like] and t.numel() == shape.numel()
+            same = t.is_contiguous() and self._packed[like] and _reshapes(t.shape, shape)
         if not same or t.dtype != dtype or t.device != device:
             raise NativeError(f"CrossAttention: {name} is not laid out as {like} was")
         return t.data_ptr()

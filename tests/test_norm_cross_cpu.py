@@ -180,3 +180,23 @@ def test_binding_checks_calls():
             p.backward(**{**good, **more, **bad})
     with pytest.raises(native.NativeError, match="devices"):
         native.CrossAttention(None, q, k, k, q, bias_table=table.to("meta"))
+
+
+def test_binding_refuses_reordered_tensors():
+    """Contiguous tensors of as many elements are taken where their shape joins or splits neighbouring dimensions, not
+    where it has them in another order (heads before rows)."""
+    q, k = torch.zeros(2, 5, 8, 64), torch.zeros(2, 7, 4, 64)
+    p = native.CrossAttention(None, q, k, k, q)
+    for shape in ((10, 512), (2, 5, 512), (10, 8, 64), (5120,), (1, 10, 512), (2, 5, 4, 2, 64), (2, 5, 8, 2, 32), (2, 40, 2, 32)):
+        assert p._tensor("q", "q", torch.zeros(shape)), shape
+    for shape in ((2, 8, 5, 64), (16, 5, 64), (16, 320), (2, 8, 320), (5, 2, 8, 64), (2, 5, 64, 8), (8, 2, 5, 64), (40, 128),
+                  (4, 20, 64), (2, 10, 4, 64)):
+        with pytest.raises(native.NativeError, match="q is not"):
+            p._tensor("q", "q", torch.zeros(shape))
+    with pytest.raises(native.NativeError, match="k is not"):
+        p.forward(q, torch.zeros(2, 4, 7, 64), k, q)
+    with pytest.raises(native.NativeError, match="dv is not"):
+        saved, ws = torch.zeros(p.saved_bytes(), dtype=torch.uint8), torch.zeros(p.workspace_bytes(True), dtype=torch.uint8)
+        p.backward(q, k, k, q, saved, q, q, k, torch.zeros(2, 4, 7, 64), workspace=ws)
+    empty = native.CrossAttention(None, q[:0], k[:0], k[:0], q[:0])
+    empty._tensor("q", "q", torch.zeros(0, 8, 5, 64))
