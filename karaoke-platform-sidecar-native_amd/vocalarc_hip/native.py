@@ -410,8 +410,9 @@ class CrossAttention:
             return None
         if key not in self._bytes:
             self._bytes[key] = size(*key[1:])
-        if t.numel() * t.element_size() < self._bytes[key] or t.device != self._like["q"][3]:
-            raise NativeError(f"CrossAttention: {name} has fewer than {self._bytes[key]} bytes, or is on another device")
+        if t.numel() * t.element_size() < self._bytes[key] or not t.is_contiguous() or t.device != self._like["q"][3]:
+            raise NativeError(f"CrossAttention: {name} has fewer than {self._bytes[key]} bytes in a row, or is on another "
+                              "device")
         return t.data_ptr()
 
     def saved_bytes(self) -> int:

@@ -200,3 +200,18 @@ def test_binding_refuses_reordered_tensors():
         p.backward(q, k, k, q, saved, q, q, k, torch.zeros(2, 4, 7, 64), workspace=ws)
     empty = native.CrossAttention(None, q[:0], k[:0], k[:0], q[:0])
     empty._tensor("q", "q", torch.zeros(0, 8, 5, 64))
+
+
+def test_binding_refuses_buffers_in_pieces():
+    """A buffer's elements are counted only where they lie one behind the other."""
+    q, k = torch.zeros(2, 5, 8, 64), torch.zeros(2, 7, 4, 64)
+    p = native.CrossAttention(None, q, k, k, q)
+    n, w = p.saved_bytes(), p.workspace_bytes(True)
+    byte = torch.zeros(1, dtype=torch.uint8)
+    for bad in (byte.expand(n), torch.zeros(2 * n, dtype=torch.uint8)[::2]):
+        with pytest.raises(native.NativeError, match="saved"):
+            p.forward(q, k, k, q, saved=bad)
+    with pytest.raises(native.NativeError, match="workspace"):
+        p.forward(q, k, k, q, workspace=byte.expand(w))
+    with pytest.raises(native.NativeError, match="workspace"):
+        p.backward(q, k, k, q, torch.zeros(n, dtype=torch.uint8), q, q, workspace=byte.expand(w))
