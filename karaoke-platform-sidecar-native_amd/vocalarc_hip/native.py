@@ -415,6 +415,11 @@ class CrossAttention:
                               "device")
         return t.data_ptr()
 
+    def _on_gpu(self):
+        device = self._like["q"][3]
+        if device.type != "cuda" or device.index != 0:  # the GPU of every context
+            raise NativeError(f"CrossAttention: the tensors are on {device}, the context's work runs on cuda:0")
+
     def saved_bytes(self) -> int:
         n = int(lib().vh_cross_saved_bytes(self._ref))
         _ok(n, "vh_cross_saved_bytes")
@@ -430,6 +435,7 @@ class CrossAttention:
         args = (f("q", "q", q), f("k", "k", k), f("v", "v", v), f("out", "out", out),
                 self._buffer("saved", saved, self.saved_bytes, "saved"),
                 self._buffer("workspace", workspace, self.workspace_bytes, "workspace", False))
+        self._on_gpu()
         _ok(lib().vh_cross_attention(self.ctx.h, self._ref, *args), "vh_cross_attention")
 
     def backward(self, q, k, v, out, saved, dout, dq, dk=None, dv=None, dbias=None, workspace=None):
@@ -443,6 +449,7 @@ class CrossAttention:
                 self._buffer("saved", saved, self.saved_bytes, "saved"), f("dout", "out", dout), f("dq", "q", dq),
                 f("dk", "k", dk) if dk is not None else None, f("dv", "v", dv) if dv is not None else None, _opt(dbias),
                 self._buffer("workspace", workspace, self.workspace_bytes, "workspace", True))
+        self._on_gpu()
         _ok(lib().vh_cross_attention_backward(self.ctx.h, self._ref, *args), "vh_cross_attention_backward")
 
 

@@ -215,3 +215,14 @@ def test_binding_refuses_buffers_in_pieces():
         p.forward(q, k, k, q, workspace=byte.expand(w))
     with pytest.raises(native.NativeError, match="workspace"):
         p.backward(q, k, k, q, torch.zeros(n, dtype=torch.uint8), q, q, workspace=byte.expand(w))
+
+
+def test_binding_refuses_other_devices():
+    """Calls whose tensors the context's GPU cannot read: host memory, another GPU's."""
+    q, k = torch.zeros(2, 5, 8, 64), torch.zeros(2, 7, 4, 64)
+    p = native.CrossAttention(None, q, k, k, q)
+    saved, ws = torch.zeros(p.saved_bytes(), dtype=torch.uint8), torch.zeros(p.workspace_bytes(True), dtype=torch.uint8)
+    with pytest.raises(native.NativeError, match="cpu"):
+        p.forward(q, k, k, q, workspace=ws)
+    with pytest.raises(native.NativeError, match="cpu"):
+        p.backward(q, k, k, q, saved, q, q, k, k, workspace=ws)
