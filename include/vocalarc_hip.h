@@ -281,7 +281,9 @@ int vh_cross_attention(vh_context *ctx, const vh_cross *c, const void *q, const 
    receive the sum over their query heads; a bias table shared by several calls
    and inputs that several sequences share are summed by the caller.  Every sum
    has a fixed order: equal calls give equal bits.  workspace:
-   vh_cross_workspace_bytes(c, 1) bytes. */
+   vh_cross_workspace_bytes(c, 1) bytes.  dq, dk, dv, dbias and workspace overlap
+   nothing else (dk and dv may be slices of one tensor); both calls refuse one
+   that begins where another tensor does. */
 int vh_cross_attention_backward(vh_context *ctx, const vh_cross *c, const void *q, const void *k, const void *v,
                                 const void *out, const void *saved, const void *dout, void *dq, void *dk, void *dv,
                                 float *dbias, void *workspace);

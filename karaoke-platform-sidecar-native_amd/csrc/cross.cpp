@@ -483,6 +483,17 @@ static bool aligned(const char *what, std::initializer_list<const void *> pointe
     return true;
 }
 
+// Whether what is written begins where nothing else does.
+static bool written_apart(const char *what, std::initializer_list<const void *> written,
+                          std::initializer_list<const void *> read) {
+    for (const void *const *w = written.begin(); w != written.end(); w++)
+        if (*w && (std::find(read.begin(), read.end(), *w) != read.end() || std::find(w + 1, written.end(), *w) != written.end())) {
+            set_error("%s: an output, saved or workspace is at the address of another tensor", what);
+            return false;
+        }
+    return true;
+}
+
 template <typename F>
 static void launch(F kernel, int64_t groups, size_t lds, hipStream_t s, const CrossArgs &a) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), lds, s, a);
@@ -531,6 +542,9 @@ bool cross_attention(hipStream_t s, const vh_cross *c, const CrossBuffers &b, Ke
         set_error("%s: null workspace (vh_cross_workspace_bytes)", what);
         return false;
     }
+    if (!written_apart(what, {b.out, b.saved, w.bytes ? b.workspace : nullptr},
+                       {b.q, c->key_length ? b.k : nullptr, c->key_length ? b.v : nullptr, c->bias_table}))
+        return false;
     a.parts = w.rows.parts;
     a.part_o = reinterpret_cast<float *>(static_cast<char *>(b.workspace) + w.part_o);
     a.part_ml = reinterpret_cast<float2 *>(static_cast<char *>(b.workspace) + w.part_ml);
@@ -574,6 +588,13 @@ bool cross_attention_backward(hipStream_t s, const vh_cross *c, const CrossBuffe
     CrossArgs a = cross_args(c, b);
     const CrossWork w = backward_work(c);
     if (!launches_ok(what, c, w, true)) return false;
+    // a tensor of no rows has no address
+    auto if_rows = [&](const void *p) { return rows ? p : nullptr; };
+    auto if_keys = [&](const void *p) { return keys ? p : nullptr; };
+    if (!written_apart(what, {if_rows(b.dq), if_keys(b.dk), if_keys(b.dv), b.dbias, b.workspace},
+                       {if_rows(b.q), if_keys(b.k), if_keys(b.v), if_rows(b.out), if_rows(b.saved), if_rows(b.dout),
+                        c->bias_table}))
+        return false;
     auto at = [&](size_t n) { return reinterpret_cast<float *>(static_cast<char *>(b.workspace) + n); };
     a.rows = at(w.stats);
     a.parts = w.rows.parts;

@@ -1,0 +1,58 @@
+"""Layer norm and cross attention on the GPU: calls that are refused, and cuts of the work that other tests do not take."""
+
+import pytest
+import torch
+
+import norm_cross_ref as R
+from helpers import gpu_available
+
+pytestmark = pytest.mark.gpu
+
+if gpu_available():
+    from vocalarc_hip import native
+
+DEV = "cuda:0"
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = native.Context()
+    yield c
+    c.close()
+
+
+def buffer(n):
+    return torch.empty(max(int(n), 16), dtype=torch.uint8, device=DEV).fill_(0xff)
+
+
+def make(S, H, KV, Lq, Lk, dtype=F32):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(S + Lq)
+    return [torch.randn(S, n, h, 64, device=DEV, generator=g).to(dtype) for n, h in ((Lq, H), (Lk, KV), (Lk, KV), (Lq, H))]
+
+
+def test_outputs_on_inputs_refused(ctx):
+    """An output that begins where another tensor does; self attention's q, k and v in one place are read only."""
+    q, k, v, dout = make(2, 4, 4, 40, 40)
+    out, table = torch.empty_like(q), torch.randn(32, 4, device=DEV)
+    p = native.CrossAttention(ctx, q, k, v, out, bias_table=table)
+    saved, ws = buffer(p.saved_bytes()), buffer(max(p.workspace_bytes(False), p.workspace_bytes(True)))
+    before = [t.clone() for t in (q, k, v, dout)]
+    for bad in (q, k, v):
+        with pytest.raises(native.NativeError, match="address"):
+            p.forward(q, k, v, bad, saved=saved, workspace=ws)
+    p.forward(q, q, q, out, saved=saved, workspace=ws)
+    good = dict(dq=torch.empty_like(q), dk=torch.empty_like(k), dv=torch.empty_like(v), dbias=torch.empty_like(table))
+    for bad in (dict(dq=q), dict(dq=dout), dict(dq=out), dict(dk=k), dict(dv=v), dict(dk=good["dv"]), dict(dk=q), dict(dv=dout),
+                dict(dq=good["dk"]), dict(dbias=table)):
+        with pytest.raises(native.NativeError, match="address"):
+            p.backward(q, k, v, out, saved, dout, workspace=ws, **{**good, **bad})
+    if p.saved_bytes() >= p.workspace_bytes(True):
+        with pytest.raises(native.NativeError, match="address"):
+            p.backward(q, k, v, out, saved, dout, workspace=saved, **good)
+    big = buffer(p.saved_bytes() + p.workspace_bytes(True))
+    with pytest.raises(native.NativeError, match="address"):
+        p.backward(q, k, v, out, big, dout, workspace=big, **good)
+    p.backward(q, q, q, out, saved, dout, workspace=ws, **good)
+    assert all(torch.equal(a, b) for a, b in zip((q, k, v, dout), before))
