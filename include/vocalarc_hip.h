@@ -211,7 +211,7 @@ int vh_attention_noalloc(vh_context *ctx, int sequences, int length, int heads, 
    Device x[rows][ldx], y[rows][ldy] of `type`, gamma[dim], beta[dim] (may be
    null: 0); stats[rows][2] (may be null) receives (mean, rstd) for the backward
    pass.  dim 1 to 16384, any pitch from dim up, any alignment, rows from 0; y may
-   be x at the same pitch.  Issues kernels only: no allocation, no synchronisation, fit for stream
+   be x at the same pitch (at another it is refused).  Issues kernels only: no allocation, no synchronisation, fit for stream
    capture. */
 int vh_layernorm(vh_context *ctx, int type, int64_t rows, int dim, const void *x, int64_t ldx, const float *gamma,
                  const float *beta, float eps, void *y, int64_t ldy, float *stats);

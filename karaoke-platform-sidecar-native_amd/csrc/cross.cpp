@@ -105,12 +105,21 @@ static void layernorm_dispatch(hipStream_t s, const NormArgs &a, bool backward, 
     }
 }
 
+// In place: row for row.
+static bool in_place_ok(const char *what, int64_t rows, const void *to, int64_t ld, const void *from, int64_t ldf) {
+    if (to != from || ld == ldf || rows <= 1) return true;
+    set_error("%s: in place at pitches of %lld and %lld: rows would be written before they are read", what, (long long)ld,
+              (long long)ldf);
+    return false;
+}
+
 bool layernorm(hipStream_t s, const LayerNorm &n, KernelTimer *t) {
     if (!layernorm_ok("vh_layernorm", n.type, n.rows, n.dim, {n.ldx, n.ldy})) return false;
     if (!(n.eps >= 0.0f) || isinf(n.eps) || !n.gamma || (n.rows && (!n.x || !n.y))) {
         set_error("vh_layernorm: null x, gamma or y, or an eps that is no number from 0 up");
         return false;
     }
+    if (!in_place_ok("vh_layernorm", n.rows, n.y, n.ldy, n.x, n.ldx)) return false;
     if (!n.rows) return true;
     NormArgs a{};
     a.x = n.x; a.y = n.y; a.ldx = n.ldx; a.ldy = n.ldy;
@@ -129,6 +138,9 @@ bool layernorm_backward(hipStream_t s, const LayerNorm &n, KernelTimer *t) {
         set_error("vh_layernorm_backward: null dy, x, gamma, stats or dx");
         return false;
     }
+    if (!in_place_ok("vh_layernorm_backward", n.rows, n.dx, n.lddx, n.x, n.ldx) ||
+        !in_place_ok("vh_layernorm_backward", n.rows, n.dx, n.lddx, n.dy, n.ldy))
+        return false;
     const bool weights = n.dgamma || n.dbeta;
     if (weights && (!n.workspace || ((uintptr_t)n.workspace & 15))) {
         set_error("vh_layernorm_backward: the weights' gradients need a 16-byte aligned workspace "

@@ -56,3 +56,16 @@ def test_outputs_on_inputs_refused(ctx):
         p.backward(q, k, v, out, big, dout, workspace=big, **good)
     p.backward(q, q, q, out, saved, dout, workspace=ws, **good)
     assert all(torch.equal(a, b) for a, b in zip((q, k, v, dout), before))
+
+
+def test_layernorm_in_place_at_another_pitch_refused(ctx):
+    x, gamma = torch.randn(6, 16, device=DEV), torch.ones(8, device=DEV)
+    stats = torch.empty(6, 2, device=DEV)
+    with pytest.raises(native.NativeError, match="pitches"):
+        ctx.layernorm(x, gamma, None, x, 6, 8, ldx=16, ldy=12)
+    dy, ws = torch.randn(6, 16, device=DEV), buffer(1024)
+    for a, b in ((dy, x), (x, dy)):
+        with pytest.raises(native.NativeError, match="pitches"):
+            ctx.layernorm_backward(a, b, gamma, stats, x, 6, 8, lddy=16, ldx=16, lddx=8, workspace=ws)
+    ctx.layernorm(x, gamma, None, x, 1, 8, ldx=16, ldy=8)  # one row has no pitch
+    ctx.layernorm(x, gamma, None, x, 6, 8, ldx=16, ldy=16, stats=stats)
