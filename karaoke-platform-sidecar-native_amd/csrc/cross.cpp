@@ -212,11 +212,11 @@ int relative_bucket(int rel, int buckets, int max_distance, int bidirectional) {
 static bool apart(const int64_t *strides, int64_t seqs, int64_t rows, int64_t heads) {
     std::pair<int64_t, int64_t> d[3] = {{strides[0], seqs}, {strides[1], rows}, {strides[2], heads}};
     std::sort(d, d + 3);
-    int64_t span = CA_D;
+    int64_t span = CA_D, stretch;
     for (const auto &[stride, n] : d) {
         if (n <= 1) continue;
         if (stride < span) return false;
-        span = stride * (n - 1) + span;
+        if (__builtin_mul_overflow(stride, n - 1, &stretch) || __builtin_add_overflow(span, stretch, &span)) span = INT64_MAX;
     }
     return true;
 }
@@ -271,8 +271,10 @@ static bool cross_ok(const char *what, const vh_cross *c, bool backward) {
             return false;
         }
     }
-    const int64_t tasks = (int64_t)c->sequences * c->heads * ((std::max(c->query_length, c->key_length) + 127) / 128 + 1);
-    if (tasks > INT32_MAX / 8) {
+    constexpr int64_t MOST = INT32_MAX / 8;
+    const int64_t pairs = (int64_t)c->sequences * c->heads;  // below 2^47
+    const int64_t tasks = std::min(pairs, MOST + 1) * ((std::max(c->query_length, c->key_length) + 127) / 128 + 1);
+    if (tasks > MOST) {
         set_error("%s: %lld workgroups", what, (long long)tasks);
         return false;
     }

@@ -226,3 +226,15 @@ def test_binding_refuses_other_devices():
         p.forward(q, k, k, q, workspace=ws)
     with pytest.raises(native.NativeError, match="cpu"):
         p.backward(q, k, k, q, saved, q, q, k, k, workspace=ws)
+
+
+def test_sizes_whose_products_pass_64_bits():
+    """2^30 sequences x 2^16 heads x 2^18 tiles are 2^64 workgroups, which is none in 64 bits; 2^45 elements between 2^20
+    heads leave no room for a second sequence 2^46 behind the first."""
+    c = layout(sequences=1 << 30, heads=1 << 16, kv_heads=1, query_length=1, key_length=((1 << 18) - 1) * 128,
+               q_strides=(1 << 22, 64, 64), out_strides=(1 << 22, 64, 64), k_strides=(0, 64, 64), v_strides=(0, 64, 64))
+    assert native.lib().vh_cross_saved_bytes(ctypes.byref(c)) == 0 and "workgroups" in native.last_error()
+    c = layout(sequences=2, heads=1 << 16, kv_heads=1, query_length=1, out_strides=(1 << 46, 64, 1 << 45))
+    assert native.lib().vh_cross_saved_bytes(ctypes.byref(c)) == 0 and "overlap" in native.last_error()
+    c = layout(sequences=1 << 20, heads=2, kv_heads=1, query_length=1, out_strides=(1 << 45, 64, 1 << 46))
+    assert native.lib().vh_cross_saved_bytes(ctypes.byref(c)) == 0 and "overlap" in native.last_error()
