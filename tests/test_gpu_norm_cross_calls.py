@@ -69,3 +69,53 @@ def test_layernorm_in_place_at_another_pitch_refused(ctx):
             ctx.layernorm_backward(a, b, gamma, stats, x, 6, 8, lddy=16, ldx=16, lddx=8, workspace=ws)
     ctx.layernorm(x, gamma, None, x, 1, 8, ldx=16, ldy=8)  # one row has no pitch
     ctx.layernorm(x, gamma, None, x, 6, 8, ldx=16, ldy=16, stats=stats)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("buckets", [0, 32])
+@pytest.mark.parametrize("form", ["plain", "causal", "ragged"])
+@pytest.mark.parametrize("size", [(8, 8, 4, 600, 256), (4, 24, 8, 1100, 250)], ids=str)
+def test_shared_heads_in_pieces(ctx, size, form, buckets, dtype):
+    """dk and dv of several heads in one workgroup whose queries are cut in two as well: 256 workgroups of 32 keys and from
+    16 tiles of queries on, where a piece ends within one head and the next begins there."""
+    S, H, KV, Lq, Lk = size
+    q, k, v, dout = make(*size, dtype)
+    kw = dict(causal=form == "causal")
+    if form == "ragged":
+        kw.update(query_lengths=[Lq - 67 * s for s in range(S)], key_lengths=[Lk - 30 * s for s in range(S)])
+    if form == "causal":
+        kw.update(query_start=[Lk - Lq + 9 * s for s in range(S)])
+    if buckets:
+        kw.update(bias_table=torch.randn(buckets, H, device=DEV), bidirectional=form != "causal")
+    val, tol = R.attention(q, k, v, dout=dout, **kw)
+    for n in ("query_lengths", "key_lengths", "query_start"):
+        if n in kw:
+            kw[n] = torch.tensor(kw[n], dtype=torch.int32, device=DEV)
+    got = {"out": torch.empty_like(q)}
+    p = native.CrossAttention(ctx, q, k, v, got["out"], **kw)
+    saved, ws = buffer(p.saved_bytes()), buffer(max(p.workspace_bytes(False), p.workspace_bytes(True)))
+    p.forward(q, k, v, got["out"], saved=saved, workspace=ws)
+    got.update(dq=torch.empty_like(q), dk=torch.empty_like(k), dv=torch.empty_like(v))
+    if buckets:
+        got["dbias"] = torch.empty_like(kw["bias_table"])
+    ws.fill_(0xff)
+    p.backward(q, k, v, got["out"], saved, dout, got["dq"], got["dk"], got["dv"], dbias=got.get("dbias"), workspace=ws)
+    for n in got:
+        R.assert_within(got[n], val[n], tol[n], f"{size} {form} {n}")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", [(1, 4, 2, 100, 3000), (2, 4, 2, 70, 90), (4, 12, 12, 1030, 64)], ids=str)
+def test_table_without_gradient(ctx, size, dtype):
+    """A table whose gradient is not wanted, also where it would be joined from pieces: the other gradients keep their bits."""
+    q, k, v, dout = make(*size, dtype)
+    table, out = torch.randn(32, size[1], device=DEV), torch.empty_like(q)
+    p = native.CrossAttention(ctx, q, k, v, out, bias_table=table)
+    saved, ws = buffer(p.saved_bytes()), buffer(max(p.workspace_bytes(False), p.workspace_bytes(True)))
+    p.forward(q, k, v, out, saved=saved, workspace=ws)
+    r = []
+    for dbias in (torch.empty_like(table), None):
+        g = [torch.empty_like(t) for t in (q, k, v)]
+        p.backward(q, k, v, out, saved, dout, *g, dbias=dbias, workspace=ws)
+        r.append(g)
+    assert all(torch.equal(a, b) for a, b in zip(*r)) and all(bool(t.isfinite().all()) for t in r[0])
