@@ -255,20 +255,24 @@ typedef struct {
     const int32_t *query_start;
     /* learned relative position bias, null for none: device fp32
        [buckets][heads], added to the scaled scores at bucket(j - (query_start +
-       i)), vh_relative_bucket's */
+       i)), vh_relative_bucket's; finite values that pass fp32's range when times
+       log2(e), from 2.36e38 on, count as its end */
     const float *bias_table;
     int buckets, max_distance, bidirectional;
 } vh_cross;
 /* out = softmax(scale q k^T + bias) v over the keys a row sees.  A row that sees
    none (no keys, causal before the first one, or a bias of -inf at all of them)
    is 0.  The products run on the bf16 matrix cores: bf16 operands as they are, P
-   rounded to bf16; fp32 operands as three bf16 values each, whose products keep 24
-   bits (infinities in them, and what bf16 would round to one, give NaN); scores, softmax and sums are fp32.
+   rounded to bf16; fp32 operands as three bf16 values each, whose products are
+   left out below 2^-23 of the whole (infinities in them, and what bf16 would round
+   to one, give NaN); scores, softmax and sums are fp32.
    A key that no row sees is never read.  A NaN or infinity in a value that a row's
    neighbours see and it does not, causal, may reach it (0 times it is NaN).
    saved (may be null): vh_cross_saved_bytes bytes for the backward pass (the
    rows' softmax statistics and, for bf16, what rounding took from out: bf16, with
-   a bias table fp32).  workspace: vh_cross_workspace_bytes(c, 0) bytes.  Tensors,
+   a bias table fp32).  With saved, bf16's P enters the product in two or three
+   bf16 values instead of one: out then is closer to exact than without, not the
+   same bits.  workspace: vh_cross_workspace_bytes(c, 0) bytes.  Tensors,
    saved and workspace are 16-byte aligned device memory; out, saved and workspace
    overlap nothing else.  Issues kernels only, without allocation or
    synchronisation, so it may be captured; workspace is free again when the
