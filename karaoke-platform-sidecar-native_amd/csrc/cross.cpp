@@ -328,14 +328,20 @@ struct CrossCut {
     int64_t groups() const { return pairs * tiles; }
     int64_t grid() const { return (pairs_by_xcd(pairs) ? (pairs + 7) / 8 * 8 : pairs) * tiles; }
 };
-// From 1.5 128-row workgroups per CU on, their sharing of tiles wins over even work
-// (8 x 801 rows over 1723 keys, 448 of them: 42 us against 48; 4 x 1000 rows over
-// 1200 in fp32, 256: 101 against 94); the forward's are of 64 rows in two groups up to
-// four per CU (30 against 34 us for the same 448; backward no gain).  Below, pieces
-// of at least 8 tiles (two a wave) until there are about two workgroups per CU, for
-// single tokens of 32 until there are four (16 x 32 of them over 8192 keys 42 us
-// against 44; 2 x 3841 rows over 3278 so cut 120 against 107; dk and dv of 416
-// workgroups in two pieces, 4 x 8 x 801 rows fp32, 130 against 120).
+// From 1.5 128-row workgroups per CU on, their sharing of tiles wins over even work.
+// Both sides in turn, shared against split (8 heads each): forward of 8 x 801 rows over
+// 1723 keys, 448 of them, 46 us against 55, fp32 181 against 195; a training step of 6 x
+// 1000 over 1000, 384 of them, 103 against 110, but fp32 440 against 419.  At 256 of
+// them, 4 x 1000 over 1000, a step in fp32 298 against 283, but bf16 74 against 81, and
+// the forward alone, whose 64-row workgroups double their number, 21 against 26 (fp32 71
+// against 86): one border for all passes and types costs a fifth there.  The forward's
+// are of 64 rows in two groups up to four 128-row ones per CU: 33 us against 36 for 8 x
+// 801 ragged rows, even 46 both, 672 of them 58 against 57; backward no gain.  Below, pieces
+// of at least 8 tiles (two a wave) until there are about two workgroups per CU (a step
+// of 4 x 8 x 801 rows over 389 keys in fp32, 416 workgroups of dk and dv: in one piece
+// 124 us, in two 137); for single tokens of 32 tiles until there are four (16 x 32 of
+// them over 8192 keys 37.6 us against 37.3 until there are two; many rows so cut, 2 x
+// 3841 over 3278, 24.7 against 23.2).
 constexpr int64_t CA_ENOUGH = 384, CA_PAIRED = 1024, CA_PIECES = 512, CA_ONE = 256;
 static int pieces(int64_t groups, int across, bool few) {
     const int64_t tiles = (across + 31) / 32;
@@ -374,10 +380,11 @@ static CrossCut dkv_cut(const vh_cross *c) {
     CrossCut cut = cross_cut((int64_t)c->sequences * c->kv_heads, c->key_length, 1, c->query_length, true);
     if (!cut.split) return cut;
     // a workgroup takes all heads that share its keys, where their bias windows leave
-    // room for two workgroups on a CU (four windows of 800 positions 140 us against
-    // 143); else, or where that makes less than one workgroup per CU, the heads are
-    // pairs of their own and their sums pieces (56 workgroups: 37 us against 42; 320:
-    // together 84 against 89)
+    // room for two workgroups on a CU (a step with four windows of 800 positions 140 us
+    // against 142); else, or where that makes less than one workgroup per CU, the heads
+    // are pairs of their own and their sums pieces (56 workgroups: a step 38 us, together
+    // 40; 320: together 82 against 88, with a bias 125 against 129, but fp32 276 against
+    // 263)
     const int shared = c->heads / c->kv_heads;
     cut.tiles = (c->key_length + 31) / 32;
     cut.heads = shared;
