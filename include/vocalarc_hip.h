@@ -286,8 +286,10 @@ int vh_cross_attention(vh_context *ctx, const vh_cross *c, const void *q, const 
    and inputs that several sequences share are summed by the caller.  Every sum
    has a fixed order: equal calls give equal bits.  workspace:
    vh_cross_workspace_bytes(c, 1) bytes.  dq, dk, dv, dbias and workspace overlap
-   nothing else (dk and dv may be slices of one tensor); both calls refuse one
-   that begins where another tensor does. */
+   nothing else (dk and dv may be slices of one tensor), but for a gradient in the
+   place of what only its own rows need: dk on k, dv on v, dq on an out of q's
+   strides, and without dk and dv dq on q or on such a dout.  Both calls refuse one
+   that begins where it would overwrite what is still read. */
 int vh_cross_attention_backward(vh_context *ctx, const vh_cross *c, const void *q, const void *k, const void *v,
                                 const void *out, const void *saved, const void *dout, void *dq, void *dk, void *dv,
                                 float *dbias, void *workspace);

@@ -504,7 +504,8 @@ static bool aligned(const char *what, std::initializer_list<const void *> pointe
     return true;
 }
 
-// Whether what is written begins where nothing else does.
+// Whether each of what is written begins where none of the others and none of what
+// is still read does.
 static bool written_apart(const char *what, std::initializer_list<const void *> written,
                           std::initializer_list<const void *> read) {
     for (const void *const *w = written.begin(); w != written.end(); w++)
@@ -513,6 +514,9 @@ static bool written_apart(const char *what, std::initializer_list<const void *> 
             return false;
         }
     return true;
+}
+static bool same_layout(const int64_t *a, const int64_t *b, int64_t seqs, int64_t rows, int64_t heads) {
+    return (seqs <= 1 || a[0] == b[0]) && (rows <= 1 || a[1] == b[1]) && (heads <= 1 || a[2] == b[2]);
 }
 
 template <typename F>
@@ -563,8 +567,11 @@ bool cross_attention(hipStream_t s, const vh_cross *c, const CrossBuffers &b, Ke
         set_error("%s: null workspace (vh_cross_workspace_bytes)", what);
         return false;
     }
-    if (!written_apart(what, {b.out, b.saved, w.bytes ? b.workspace : nullptr},
-                       {b.q, c->key_length ? b.k : nullptr, c->key_length ? b.v : nullptr, c->bias_table}))
+    // a row of q is read by the workgroups that write its out, before they do
+    const bool as_q = same_layout(c->out_strides, c->q_strides, c->sequences, c->query_length, c->heads);
+    const void *ws = w.bytes ? b.workspace : nullptr, *k = c->key_length ? b.k : nullptr, *v = c->key_length ? b.v : nullptr;
+    if (!written_apart(what, {b.out, b.saved, ws}, {k, v, c->bias_table}) ||
+        !written_apart(what, {b.saved, ws, as_q ? nullptr : b.out}, {b.q}))
         return false;
     a.parts = w.rows.parts;
     a.part_o = reinterpret_cast<float *>(static_cast<char *>(b.workspace) + w.part_o);
@@ -609,12 +616,19 @@ bool cross_attention_backward(hipStream_t s, const vh_cross *c, const CrossBuffe
     CrossArgs a = cross_args(c, b);
     const CrossWork w = backward_work(c);
     if (!launches_ok(what, c, w, true)) return false;
-    // a tensor of no rows has no address
+    // Tensors without rows have no address.  dq's kernel reads k and v anywhere, and of q,
+    // dout and out a row where it writes it; dk's and dv's read q and dout anywhere, and of k
+    // and v a row where they write it: there a gradient may take its input's place.
     auto if_rows = [&](const void *p) { return rows ? p : nullptr; };
     auto if_keys = [&](const void *p) { return keys ? p : nullptr; };
-    if (!written_apart(what, {if_rows(b.dq), if_keys(b.dk), if_keys(b.dv), b.dbias, b.workspace},
-                       {if_rows(b.q), if_keys(b.k), if_keys(b.v), if_rows(b.out), if_rows(b.saved), if_rows(b.dout),
-                        c->bias_table}))
+    const bool as_out = same_layout(c->q_strides, c->out_strides, c->sequences, c->query_length, c->heads);
+    const bool as_v = same_layout(c->k_strides, c->v_strides, c->sequences, c->key_length, c->kv_heads);
+    const void *q = if_rows(b.q), *k = if_keys(b.k), *v = if_keys(b.v), *out = if_rows(b.out), *dout = if_rows(b.dout);
+    const void *saved = if_rows(b.saved), *dq = if_rows(b.dq), *dk = if_keys(b.dk), *dv = if_keys(b.dv);
+    if (!written_apart(what, {dq, dk, dv, b.dbias, b.workspace}, {saved}) ||
+        !written_apart(what, {b.workspace}, {q, k, v, out, dout, c->bias_table}) ||
+        !written_apart(what, {dq}, {k, v, c->bias_table, as_out ? nullptr : out, dk || !as_out ? dout : nullptr, dk ? q : nullptr}) ||
+        !written_apart(what, {dk, dv}, {q, dout, c->bias_table}) || (!as_v && (!written_apart(what, {dk}, {v}) || !written_apart(what, {dv}, {k}))))
         return false;
     auto at = [&](size_t n) { return reinterpret_cast<float *>(static_cast<char *>(b.workspace) + n); };
     a.rows = at(w.stats);

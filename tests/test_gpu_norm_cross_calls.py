@@ -33,29 +33,61 @@ def make(S, H, KV, Lq, Lk, dtype=F32):
 
 
 def test_outputs_on_inputs_refused(ctx):
-    """An output that begins where another tensor does; self attention's q, k and v in one place are read only."""
+    """An output that begins where another tensor does, which is read after it is written; self attention's q, k and v in
+    one place are read only."""
     q, k, v, dout = make(2, 4, 4, 40, 40)
     out, table = torch.empty_like(q), torch.randn(32, 4, device=DEV)
     p = native.CrossAttention(ctx, q, k, v, out, bias_table=table)
     saved, ws = buffer(p.saved_bytes()), buffer(max(p.workspace_bytes(False), p.workspace_bytes(True)))
     before = [t.clone() for t in (q, k, v, dout)]
-    for bad in (q, k, v):
+    for bad in (k, v):
         with pytest.raises(native.NativeError, match="address"):
             p.forward(q, k, v, bad, saved=saved, workspace=ws)
     p.forward(q, q, q, out, saved=saved, workspace=ws)
     good = dict(dq=torch.empty_like(q), dk=torch.empty_like(k), dv=torch.empty_like(v), dbias=torch.empty_like(table))
-    for bad in (dict(dq=q), dict(dq=dout), dict(dq=out), dict(dk=k), dict(dv=v), dict(dk=good["dv"]), dict(dk=q), dict(dv=dout),
-                dict(dq=good["dk"]), dict(dbias=table)):
+    for bad in (dict(dq=q), dict(dq=dout), dict(dq=k), dict(dq=v), dict(dk=good["dv"]), dict(dk=q), dict(dv=dout), dict(dk=dout),
+                dict(dq=good["dk"]), dict(dq=k, dk=None, dv=None)):
         with pytest.raises(native.NativeError, match="address"):
             p.backward(q, k, v, out, saved, dout, workspace=ws, **{**good, **bad})
-    if p.saved_bytes() >= p.workspace_bytes(True):
-        with pytest.raises(native.NativeError, match="address"):
-            p.backward(q, k, v, out, saved, dout, workspace=saved, **good)
+    with pytest.raises(native.NativeError, match="address"):  # k is q
+        p.backward(q, q, q, out, saved, dout, dq=q, workspace=ws)
     big = buffer(p.saved_bytes() + p.workspace_bytes(True))
     with pytest.raises(native.NativeError, match="address"):
         p.backward(q, k, v, out, big, dout, workspace=big, **good)
+    # q before heads, out after them: in the place of out's rows are others of dq's
+    turned = torch.empty(2, 4, 40, 64, device=DEV).transpose(1, 2)
+    p2 = native.CrossAttention(ctx, turned.copy_(q), k, v, out)
+    with pytest.raises(native.NativeError, match="address"):
+        native._ok(native.lib().vh_cross_attention(ctx.h, p2._ref, turned.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                                   turned.data_ptr(), None, ws.data_ptr()), "vh_cross_attention")
     p.backward(q, q, q, out, saved, dout, workspace=ws, **good)
     assert all(torch.equal(a, b) for a, b in zip((q, k, v, dout), before))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", [(2, 4, 2, 70, 90), (1, 4, 4, 60, 2000), (8, 16, 16, 400, 400), (1, 2, 2, 1500, 40)], ids=str)
+def test_gradients_in_place(ctx, size, dtype):
+    """dk on k, dv on v and dq on out; without dk and dv, dq on q or on dout; out on q: the bits of places of their own."""
+    q, k, v, dout = make(*size, dtype)
+    out, table = torch.empty_like(q), torch.randn(32, size[1], device=DEV)
+    p = native.CrossAttention(ctx, q, k, v, out, bias_table=table, key_lengths=torch.tensor(
+        [size[4] - 5 * s for s in range(size[0])], dtype=torch.int32, device=DEV), causal=size[3] == size[4])
+    saved, ws = buffer(p.saved_bytes()), buffer(max(p.workspace_bytes(False), p.workspace_bytes(True)))
+    p.forward(q, k, v, out, saved=saved, workspace=ws)
+    want = [torch.empty_like(t) for t in (q, k, v)]
+    p.backward(q, k, v, out, saved, dout, *want, workspace=ws)
+    place = [t.clone() for t in (out, k, v)]
+    p.backward(q, place[1], place[2], place[0], saved, dout, *place, workspace=ws)
+    assert all(torch.equal(a, b) for a, b in zip(place, want))
+    for i in (0, 1):
+        t = [q.clone(), dout.clone()]
+        p.backward(t[0], k, v, out, saved, t[1], t[i], workspace=ws)
+        assert torch.equal(t[i], want[0])
+    alone = torch.empty_like(q)
+    p.forward(q, k, v, alone, workspace=ws)
+    on_q = q.clone()
+    p.forward(on_q, k, v, on_q, workspace=ws)
+    assert torch.equal(on_q, alone)
 
 
 def test_layernorm_in_place_at_another_pitch_refused(ctx):
