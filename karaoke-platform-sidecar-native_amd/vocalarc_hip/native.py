@@ -390,6 +390,7 @@ class CrossAttention:
         self._ref = ctypes.byref(self.c)
         self._like = {n: (t.dtype, t.shape, t.stride(), t.device)
                       for n, t in (("q", q), ("k", k), ("v", v), ("out", out))}
+        self._elsewhere = None if q.device == torch.device("cuda:0") else q.device  # every context's GPU is the first
         self._packed = {"q": q.is_contiguous(), "k": k.is_contiguous(), "v": v.is_contiguous(), "out": out.is_contiguous()}
         self._bytes = {}
 
@@ -416,9 +417,8 @@ class CrossAttention:
         return t.data_ptr()
 
     def _on_gpu(self):
-        device = self._like["q"][3]
-        if device.type != "cuda" or device.index != 0:  # the GPU of every context
-            raise NativeError(f"CrossAttention: the tensors are on {device}, the context's work runs on cuda:0")
+        if self._elsewhere is not None:
+            raise NativeError(f"CrossAttention: the tensors are on {self._elsewhere}, the context's work runs on cuda:0")
 
     def saved_bytes(self) -> int:
         n = int(lib().vh_cross_saved_bytes(self._ref))
