@@ -304,6 +304,165 @@ size_t vh_cross_workspace_bytes(const vh_cross *c, int backward);
    (bidirectional: even, from 4), near < max_distance <= 4096.  -1: refused. */
 int vh_relative_bucket(int rel, int buckets, int max_distance, int bidirectional);
 
+/* ---- rotary positions ------------------------------------------------------ */
+/* Beside vh_rope_bhld (pairs of neighbours, a whole head of 64, base 10000, in
+   place): either pairing, a part of the head, angles of any base, scaled for
+   contexts longer than a model was trained on; and the gradient. */
+typedef struct {
+    double base;   /* theta_i = base^(-2 i / dim), base > 1 */
+    /* from factor > 1 on angles are scaled: theta_i (keep + (1 - keep) / factor),
+       with original > 0 keep = (turns - low) / (high - low) within [0, 1] and turns
+       = original theta_i / 2 pi, those of the pair in `original` positions; with
+       original 0 keep is 0 */
+    double factor; /* at least 1 */
+    int original;
+    double low, high;
+    double magnitude; /* of the rotation, cos and sin are multiplied by it: 1 */
+} vh_rotary_angles;
+/* A rotation, given to the calls that turn what they read: x's pair (a, b) at
+   position p becomes (a c - b s, a s + b c) with (c, s) = table[p][pair], products
+   and sums rounded to fp32 one by one.  Positions that the table has not give NaN. */
+typedef struct {
+    int dim;            /* the head's leading dims that turn: even, 2 to 256; the others stay */
+    int interleaved;    /* 1: pair i is dims 2 i and 2 i + 1; 0: dims i and i + dim / 2 */
+    int positions;      /* rows of the table, from 1 */
+    const float *table; /* device [positions][dim / 2][2], 16-byte aligned */
+} vh_rotary;
+/* Fills a table (device, the caller's): cosines and sines of p theta_i in 64 bits,
+   rounded once. */
+int vh_rotary_table(vh_context *ctx, const vh_rotary_angles *angles, int dim, int positions, float *table);
+typedef struct {
+    int type;                                /* VH_TYPE_* of x and y */
+    int sequences, length, heads, head_dim;  /* head_dim from the rotation's dim to 1024 */
+    /* elements between sequences, rows and heads (a head's dims are consecutive),
+       none negative; any alignment of an element */
+    int64_t x_strides[3], y_strides[3];
+    const int32_t *start; /* device [sequences], the position of row 0; null: 0 */
+} vh_rotary_rows;
+/* y = x with every row's heads turned.  y may be x (with its strides).  backward: by
+   the transpose, (a c + b s, b c - a s), which takes y's gradient to x's.  Issues
+   kernels only: no allocation, no synchronisation, fit for stream capture. */
+int vh_rotary_apply(vh_context *ctx, const vh_rotary *r, const vh_rotary_rows *rows, const void *x, void *y,
+                    int backward);
+
+/* ---- paged cache of keys and values, and attention over it ------------------- */
+/* A pool of pages, each with the keys and values of page_tokens tokens of all
+   kv_heads; a sequence's token t is in page table[sequence][t / page_tokens].  Which
+   pages a sequence has is the caller's: sequences may share pages that none of them
+   writes.  An entry that is no page of the pool stands for tokens that are not there:
+   they are not appended, read as 0, and no query sees them.
+     VH_CACHE_BF16  values rounded to bf16
+     VH_CACHE_INT8  8 bits with a fp32 scale for every 16 tokens (VH_CACHE_BLOCK: from
+                    a multiple of 16 on) of a head, of keys and of values each.  A call
+                    that appends to a block takes scale = max(max |x| / 127 of its new
+                    tokens, 2^-100), and not less than the block had if it holds
+                    earlier ones; x is held as the whole number next to x (1 / scale)
+                    and stands for that times scale, earlier ones as the whole number
+                    next to old (old scale (1 / scale)), all in fp32.  A NaN or infinity
+                    makes the scale NaN, and with it all that the block stands for.
+   The layout within a page is the library's (vh_cache_read gives rows). */
+#define VH_CACHE_BF16 0
+#define VH_CACHE_INT8 1
+#define VH_CACHE_BLOCK 16
+typedef struct {
+    int type;                /* VH_CACHE_* */
+    int kv_heads, head_dim;  /* up to 4096 heads of 64 or 128 */
+    int page_tokens;         /* a multiple of 16, up to 4096 */
+    int pages;               /* of the pool, from 1 */
+    int sequences;           /* rows of the table */
+    int table_pages;         /* entries of a row; times page_tokens at most 2^29 */
+    void *pool;              /* device, vh_cache_bytes(c) bytes, 256-byte aligned, the caller's */
+    const int32_t *table;    /* device [sequences][table_pages] */
+} vh_cache;
+size_t vh_cache_bytes(const vh_cache *c); /* 0: refused (vh_last_error) */
+/* Rows of keys and values [sequences][length][kv_heads][head_dim]. */
+typedef struct {
+    int type, length; /* VH_TYPE_* */
+    /* elements between sequences, rows and heads; whole multiples of 16 bytes, none
+       negative, rows at most 2^26 bytes apart */
+    int64_t k_strides[3], v_strides[3];
+    const int32_t *start;   /* device [sequences], the position of row 0 in its sequence; null: 0 */
+    const int32_t *lengths; /* device [sequences], rows that count; null: length */
+    /* Starts below 0 act as 0, lengths beyond 0 and `length` as those.  Rows beyond
+       what the table has room for are not appended, and read as 0. */
+} vh_cache_rows;
+/* Puts rows into the cache, keys turned by `rotary` (may be null; its dim a multiple
+   of 16 and at most head_dim) at their positions.  A sequence's tokens from start +
+   length to the end of that block are lost, others stay.  Pages that a call writes
+   belong to one sequence each.  k and v: 16-byte aligned device memory that the pool
+   does not overlap.  Issues kernels only. */
+int vh_cache_append(vh_context *ctx, const vh_cache *c, const vh_cache_rows *rows, const vh_rotary *rotary,
+                    const void *k, const void *v);
+/* The values that the cache holds at those rows' positions (keys turned, as they are);
+   rows from a sequence's length on become 0.  k or v may be null.  Issues kernels only. */
+int vh_cache_read(vh_context *ctx, const vh_cache *c, const vh_cache_rows *rows, void *k, void *v);
+/* Queries [sequences][length][heads][head_dim] over the cache, heads a multiple of
+   kv_heads (query head h reads key head h / (heads / kv_heads)). */
+typedef struct {
+    int type, heads, length;  /* VH_TYPE_* of q and out */
+    int causal;               /* 1: query i of sequence s sees keys j <= start[s] + i */
+    int most_keys;            /* keys beyond are not read; the work is divided by it */
+    float scale;              /* of the scores q.k, e.g. 0.125 */
+    int64_t q_strides[3], out_strides[3]; /* as vh_cache_rows' */
+    /* device [sequences], each may be null.  Rows from a sequence's query length on are
+       padding: their out is 0.  Lengths beyond 0 and length, most_keys or what the
+       table has room for act as those. */
+    const int32_t *query_lengths, *key_lengths;
+    const int32_t *start;     /* position of row 0, for causal and the rotation; null: 0 */
+} vh_cache_queries;
+/* out = softmax(scale q' k^T) v over the keys that a row sees, q' = q turned by
+   `rotary` (may be null; as vh_cache_append's).  A row that sees none is 0.  Keys from
+   a sequence's length on and behind the last that a row may see are not read beyond
+   their block of 16, and change nothing (int8: but for a block's NaN); NaN in what a
+   row's neighbours see and it does not, causal, may reach it (0 times it is NaN).
+   Products run on the matrix cores: over int8 pages, whose whole numbers fp16 holds,
+   q' and the probabilities are fp16 times a power of two each (fp32 out: two fp16, 22
+   bits), over bf16 pages bf16 (fp32 out: three bf16, 24 bits); the rest is fp32.
+   workspace: vh_cache_workspace_bytes(c, q) bytes of device memory, 16-byte aligned,
+   free again when the call's work is done; graphs that may run at once need one each.
+   q and out: 16-byte aligned; out may be q (with its strides), else overlaps nothing.
+   Issues kernels only. */
+int vh_cache_attention(vh_context *ctx, const vh_cache *c, const vh_cache_queries *queries, const vh_rotary *rotary,
+                       const void *q, void *out, void *workspace);
+size_t vh_cache_workspace_bytes(const vh_cache *c, const vh_cache_queries *queries); /* 0: refused */
+/* The rows of the table in another order, for beams: c's sequences are groups of
+   `beams` rows, all rows of a group with the same number of tokens, lengths[group],
+   and each with a last page (where that is not full) of its own.  Row r goes on from
+   its group's row parents[r] (0 to beams - 1; else from itself): table_out[r] has the
+   parent's full pages, and r's own entries behind them; where the parent is another,
+   the parent's last page is copied into page spare[r], which takes the place of r's
+   own, and spare_out[r] is that one, free for the next call (else spare[r]).  Layers
+   with pools of their own and one table call with the same arguments each.
+   parents, spare, spare_out: device [sequences]; lengths: [sequences / beams];
+   table_out: [sequences][table_pages], not c's table.  Issues kernels only. */
+int vh_cache_reorder(vh_context *ctx, const vh_cache *c, int beams, const int32_t *parents, const int32_t *lengths,
+                     const int32_t *spare, int32_t *table_out, int32_t *spare_out);
+
+/* ---- beam search -------------------------------------------------------------- */
+typedef struct {
+    int type;             /* VH_TYPE_* of the logits */
+    int sequences, beams; /* 1 to 64 beams */
+    int vocab;            /* 1 to 2^24 */
+    int picks;            /* 1 to 64, at most beams vocab */
+    int end_token;        /* -1: none */
+    int64_t strides[2];   /* elements between sequences and beams of the logits */
+} vh_beam;
+/* One step: of all sequences' candidates (beam b, token t) with the scores scores[b] +
+   log softmax(logits[b])[t] the best `picks`, best first: beams' numbers to parents,
+   tokens, scores rounded to fp32, and whether the beam has ended to new_ended (may be
+   null).  Scores are compared before they are rounded, in 64 bits; of equal ones the
+   lower beam is first, within a beam the larger logit, then the lower token.
+   scores: device fp32 [sequences][beams]; a beam whose score is not finite, or whose
+   logits have a NaN, +inf or nothing but -inf, has candidates of -inf only, lowest
+   token first.  ended (may be null; needs an end token): device int32
+   [sequences][beams], where it is not 0 the end token goes on with the score as it is
+   and the others are -inf; such a beam's logits are not read.  outputs: device
+   [sequences][picks].  workspace: vh_beam_workspace_bytes(b) bytes, 16-byte aligned.
+   Issues kernels only. */
+int vh_beam_select(vh_context *ctx, const vh_beam *b, const void *logits, const float *scores, const int32_t *ended,
+                   int32_t *tokens, int32_t *parents, float *new_scores, int32_t *new_ended, void *workspace);
+size_t vh_beam_workspace_bytes(const vh_beam *b); /* 0: refused */
+
 /* ---- model -------------------------------------------------------------- */
 /* Upload a VSCNAT01 pack (native/vocalarc_separation.c:528-589) laid out for
    `dims` from host memory.  Returns NULL on a malformed pack. */

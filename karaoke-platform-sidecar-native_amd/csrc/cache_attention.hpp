@@ -1,0 +1,515 @@
+// Attention over a paged cache.
+//
+//   x_ij = scale q'_i.k_j,  P = softmax over the keys that row i sees,  out_i = sum_j P_ij v_j
+//
+// with q' = q turned to its position, and out_i = 0 where row i sees no key.  The rows
+// of a key head are those of all query heads that share it, token by token: a decoding
+// step's single tokens fill a matrix tile with their heads.
+//
+// A wave has RG groups of 16 rows as columns and walks over the keys in steps of KB
+// blocks of 16, each read once, as the page holds it, into registers: S^T = K Q^T and
+// O^T = V^T P^T in 16 x 16 x 32 instructions, whose results' lanes (column l % 16, rows
+// 4 (l / 16) + 0 .. 3) are where the second product wants P, so nothing passes through
+// LDS.  One pass, with the running maximum and sum of the softmax.
+//
+// Over int8 pages keys and values are whole numbers, exact in fp16 (from the byte by a
+// permute and an addition: 0x6400 + u is 1024 + u); a row of q' enters as fp16 times a
+// power of two (its largest just below 2^14, so 2^-25 of that is what a small one is
+// off by), the block's scale of keys as a factor of the scores.  P enters times the
+// block's scale of values over the largest one so far, times 2^14.  fp32 out: q' and P
+// in two fp16 values each.  Over bf16 pages: bf16, fp32 out: three bf16 values each.
+//
+// Bound by HBM for single tokens: the cache is read once.
+#pragma once
+
+#include "h2.hpp"
+#include "paged_cache.hpp"
+
+namespace vh {
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+struct CacheAttentionArgs {
+    PagedArgs p;
+    Rotation r;
+    const char *q;
+    char *out;
+    int64_t qs[3], os[3];  // bytes
+    const int *query_lengths, *key_lengths, *start;
+    int S, H, group, Lq;   // group: query heads of a key head
+    int most, causal;
+    float scale2;          // scale log2(e)
+    int tiles;             // workgroups of a (sequence, key head)'s rows
+    int parts, piece;      // pieces of the keys, and blocks of one
+    float *part_o;         // [parts][S][Lq][H][D]
+    float2 *part_ml;       // [parts][S][Lq][H]
+    Divisor heads;         // group
+};
+
+// Operands: I8 pages fp16, else bf16; N of them a value of q' or P.
+template <bool I8>
+struct Operand16 {
+    typedef halfx8 type;
+    VH_DEVICE static floatx4 mfma(halfx8 a, halfx8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    VH_DEVICE static halfx8 round(const float (&x)[8]) {
+        halfx8 h;
+#pragma unroll
+        for (int e = 0; e < 8; e++) h[e] = (_Float16)x[e];
+        return h;
+    }
+};
+template <>
+struct Operand16<false> {
+    typedef bf16x8 type;
+    VH_DEVICE static floatx4 mfma(bf16x8 a, bf16x8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    VH_DEVICE static bf16x8 round(const float (&x)[8]) {
+        bf16x8 h;
+#pragma unroll
+        for (int e = 0; e < 8; e++) h[e] = (bf16)x[e];
+        return h;
+    }
+};
+// x as the sum of N operands, the largest first.
+template <bool I8, int N>
+VH_DEVICE void split_n(float (&x)[8], typename Operand16<I8>::type (&o)[N]) {
+    // the value rounded to fp32 is what is split: a product that the compiler joins with
+    // the conversion, but not with the subtraction, is another one in rare cases, and an
+    // fp16 step too large
+    if constexpr (N > 1)
+#pragma unroll
+        for (int e = 0; e < 8; e++) asm("" : "+v"(x[e]));
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        o[n] = Operand16<I8>::round(x);
+        if (n + 1 < N)
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] -= (float)o[n][e];
+    }
+}
+
+// Four bytes (numbers plus 128) as fp16.
+VH_DEVICE void bytes_to_half(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+    const halfx2 bias = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+    lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(halfx2, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) + bias);
+    hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(halfx2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) + bias);
+}
+template <bool I8>
+VH_DEVICE typename Operand16<I8>::type operand_of(u32x2 a, u32x2 b) {
+    return __builtin_bit_cast(typename Operand16<I8>::type, (u32x4){a[0], a[1], b[0], b[1]});
+}
+
+// A step's keys or values in registers, as the page holds them.
+template <int D, bool I8, int KB>
+struct RawBlocks {
+    using B = BlockShape<D, I8>;
+    u32x4 w[KB][B::UNITS];
+    // keys' operand m: dims 32 m .. of block b's
+    VH_DEVICE typename Operand16<I8>::type key(int b, int m) const {
+        if constexpr (I8) {
+            u32x4 o;
+            uint32_t lo, hi;
+            bytes_to_half(w[b][m / 2][2 * (m % 2)], lo, hi);
+            o[0] = lo;
+            o[1] = hi;
+            bytes_to_half(w[b][m / 2][2 * (m % 2) + 1], lo, hi);
+            o[2] = lo;
+            o[3] = hi;
+            return __builtin_bit_cast(halfx8, o);
+        } else {
+            return __builtin_bit_cast(bf16x8, w[b][m]);
+        }
+    }
+    // values' operand for dims DT i + t, of blocks 2 c and 2 c + 1
+    VH_DEVICE typename Operand16<I8>::type value(int c, int t) const {
+        u32x4 o;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            if constexpr (I8) {
+                uint32_t lo, hi;
+                bytes_to_half(w[2 * c + h][t / 4][t % 4], lo, hi);
+                o[2 * h] = lo;
+                o[2 * h + 1] = hi;
+            } else {
+                o[2 * h] = w[2 * c + h][t / 2][2 * (t % 2)];
+                o[2 * h + 1] = w[2 * c + h][t / 2][2 * (t % 2) + 1];
+            }
+        }
+        return __builtin_bit_cast(typename Operand16<I8>::type, o);
+    }
+};
+
+// 8 dims of a query from d on, turned to its position.
+template <typename T>
+VH_DEVICE void load_query8(const Rotation &r, const T *q, const float *cs, int d, float (&x)[8]) {
+    load_n<8>(q + d, x);
+    if (!r.table || d >= r.dim) return;
+    if (!cs) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = __builtin_nanf("");
+        return;
+    }
+    if (r.interleaved) {
+        float c[8];
+        load_n<8>(cs + d, c);
+#pragma unroll
+        for (int e = 0; e < 4; e++) turn_pair(x[2 * e], x[2 * e + 1], c[2 * e], c[2 * e + 1]);
+        return;
+    }
+    const int half = r.dim / 2;
+    const bool second = d >= half;
+    const int pair = second ? d - half : d;
+    float c[16], y[8];
+    load_n<16>(cs + 2 * pair, c);
+    load_n<8>(q + (second ? pair : d + half), y);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        if (second) turn_pair(y[e], x[e], c[2 * e], c[2 * e + 1]);
+        else turn_pair(x[e], y[e], c[2 * e], c[2 * e + 1]);
+    }
+}
+
+VH_DEVICE float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// SPLIT: a workgroup's four waves share the rows, each every fourth step of the keys,
+// and join; else each wave has rows of its own.
+template <typename T, int D, bool I8, int RG, int KB, bool SPLIT>
+static __global__ __launch_bounds__(256) void cache_attention_kernel(CacheAttentionArgs a) {
+    using B = BlockShape<D, I8>;
+    using Op = Operand16<I8>;
+    constexpr int DT = B::DT, QS = D / 32, N = sizeof(T) == 2 ? 1 : I8 ? 2 : 3;
+    constexpr int WAVES = SPLIT ? 4 : 1, ROWS = 16 * RG * (SPLIT ? 1 : 4);
+    constexpr int PER_FETCH = 64 / KB;
+    constexpr float P_SCALE = I8 ? 0x1p14f : 1.0f;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int i = lane & 15, g = lane >> 4;
+    int pair, task;
+    if (!pair_task(a.S * a.p.kv, a.tiles * a.parts, pair, task)) return;
+    const int s = pair / a.p.kv, head = pair % a.p.kv;
+    // causal: a sequence's last rows, which see most, first
+    const int tile = a.tiles - 1 - task / a.parts, part = task % a.parts;
+    const int rows = a.Lq * a.group, row0 = tile * ROWS + (SPLIT ? 0 : wave * 16 * RG);
+    const int qlen = a.query_lengths ? max(0, min(__builtin_amdgcn_readfirstlane(a.query_lengths[s]), a.Lq)) : a.Lq;
+    const int keys = a.key_lengths ? max(0, min(__builtin_amdgcn_readfirstlane(a.key_lengths[s]), a.most)) : a.most;
+    const int64_t start = a.start ? __builtin_amdgcn_readfirstlane(a.start[s]) : 0;
+    auto sees = [&](int token) {  // keys that a row sees
+        return a.causal ? (int)max((int64_t)0, min((int64_t)keys, start + token + 1)) : keys;
+    };
+    const int last_row = min(row0 + 16 * RG, rows) - 1;
+    const int last_token = min(last_row / a.group, qlen - 1);  // -1: none, or (no rows) less
+    const bool any = row0 < rows && row0 / a.group < qlen;
+    const int upto = any ? sees(last_token) : 0, all_see = any ? sees(row0 / a.group) : 0;
+
+    // the wave's rows as columns
+    typename Op::type qf[RG][QS][N];
+    float factor[RG];  // of the scores, in powers of two
+    int limit[RG];     // keys that the lane's row sees
+#pragma unroll
+    for (int rg = 0; rg < RG; rg++) {
+        const int row = min(row0 + 16 * rg + i, rows - 1), token = row / a.heads;
+        const T *q = reinterpret_cast<const T *>(a.q + s * a.qs[0] + token * a.qs[1] +
+                                                 (head * a.group + row - token * a.group) * a.qs[2]);
+        const float *cs = a.r.table ? rotation_row(a.r, start + token) : nullptr;
+        limit[rg] = sees(token);
+        float x[QS][8];
+        float top = 0.0f;
+#pragma unroll
+        for (int m = 0; m < QS; m++) {
+            load_query8(a.r, q, cs, 64 * (m / 2) + 16 * g + 8 * (m % 2), x[m]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[m][e]));
+        }
+        factor[rg] = a.scale2;
+        if constexpr (I8) {
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const int e2 = h2_exponent(top);
+#pragma unroll
+            for (int m = 0; m < QS; m++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[m][e] = __builtin_ldexpf(x[m][e], e2);
+            factor[rg] = __builtin_ldexpf(a.scale2, -e2);
+        }
+#pragma unroll
+        for (int m = 0; m < QS; m++) split_n<I8, N>(x[m], qf[rg][m]);
+    }
+
+    floatx4 o[RG][DT];
+    float m_run[RG], l_run[RG];
+#pragma unroll
+    for (int rg = 0; rg < RG; rg++) {
+#pragma unroll
+        for (int t = 0; t < DT; t++) o[rg][t] = (floatx4){0, 0, 0, 0};
+        m_run[rg] = -INFINITY;
+        l_run[rg] = 0.0f;
+    }
+    float v_top = 0x1p-100f;  // the largest scale of values so far
+
+    const int block0 = part * a.piece;
+    const int block1 = min(block0 + a.piece, (upto + PC_BLOCK - 1) / PC_BLOCK);
+    const int steps_all = max(0, (block1 - block0 + KB - 1) / KB);
+    const int steps = SPLIT ? max(0, (steps_all - wave + 3) / 4) : steps_all;
+    auto block_of = [&](int step) { return block0 + (SPLIT ? wave + 4 * step : step) * KB; };
+
+    // Lane l holds where block l % KB of step fetched + l / KB is, and its scales.
+    uint32_t at_lo = 0, at_hi = 0;
+    float sk = 0.0f, sv = 0.0f;
+    uint64_t there = 0;
+    auto fetch = [&](int step) {
+        const int block = block_of(step + lane / KB) + lane % KB;
+        int page = -1;
+        uint32_t column = 0;
+        if (block < block1) {
+            column = (uint32_t)block / a.p.blocks;
+            page = page_of(a.p, s, column);
+        }
+        const int slot = page >= 0 ? block - (int)(column * a.p.blocks.d) : 0;
+        const char *p = block_at(a.p, max(page, 0), head, slot, B::BYTES);
+        at_lo = (uint32_t)(uint64_t)p;
+        at_hi = (uint32_t)((uint64_t)p >> 32);
+        if constexpr (I8) {
+            const float2 sc = *reinterpret_cast<const float2 *>(scale_at(a.p, max(page, 0), head, slot));
+            sk = page >= 0 ? sc.x : 0.0f;
+            sv = page >= 0 ? sc.y : 0.0f;
+        }
+        there = __ballot(page >= 0);
+    };
+    auto read_lane = [](uint32_t v, int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
+
+    struct Step {
+        RawBlocks<D, I8, KB> k, v;
+        float sk[KB], sv[KB];
+        uint32_t there;
+    };
+    auto load = [&](Step &st, int step) {
+        const int at = step % PER_FETCH * KB;
+        if (at == 0) fetch(step);
+        st.there = (uint32_t)(there >> at) & ((1u << KB) - 1);
+#pragma unroll
+        for (int b = 0; b < KB; b++) {
+            const char *p = reinterpret_cast<const char *>((uint64_t)read_lane(at_hi, at + b) << 32 | read_lane(at_lo, at + b));
+            const char *from = p + 16 * lane;
+#pragma unroll
+            for (int u = 0; u < B::UNITS; u++) st.k.w[b][u] = *reinterpret_cast<const u32x4 *>(from + 1024 * u);
+#pragma unroll
+            for (int u = 0; u < B::UNITS; u++) st.v.w[b][u] = *reinterpret_cast<const u32x4 *>(from + B::PART + 1024 * u);
+            if constexpr (I8) {
+                st.sk[b] = __uint_as_float(read_lane(__float_as_uint(sk), at + b));
+                st.sv[b] = __uint_as_float(read_lane(__float_as_uint(sv), at + b));
+            }
+        }
+    };
+
+    auto compute = [&](Step &st, int step) {
+        const int first = block_of(step) * PC_BLOCK;
+        const bool whole = first + KB * PC_BLOCK <= all_see && st.there == (1u << KB) - 1;
+        floatx4 x[RG][KB];
+#pragma unroll
+        for (int rg = 0; rg < RG; rg++)
+#pragma unroll
+            for (int b = 0; b < KB; b++) x[rg][b] = (floatx4){0, 0, 0, 0};
+#pragma unroll
+        for (int b = 0; b < KB; b++)
+#pragma unroll
+            for (int m = 0; m < QS; m++) {
+                const typename Op::type k = st.k.key(b, m);
+#pragma unroll
+                for (int rg = 0; rg < RG; rg++)
+#pragma unroll
+                    for (int n = N - 1; n >= 0; n--) x[rg][b] = Op::mfma(k, qf[rg][m][n], x[rg][b]);
+            }
+        // bf16: what lies behind the keys may be no number, which a probability of 0 does not hide
+        if (!I8 && !whole) {
+#pragma unroll
+            for (int b = 0; b < KB; b++)
+#pragma unroll
+                for (int u = 0; u < B::UNITS; u++)
+#pragma unroll
+                    for (int d = 0; d < 4; d++) {
+                        // a word holds tokens 4 g + 2 (d % 2) and the next
+                        const int key = first + 16 * b + 4 * g + 2 * (d % 2);
+                        uint32_t keep = (st.there >> b & 1) == 0 || key >= upto ? 0u : key + 1 >= upto ? 0xffffu : ~0u;
+                        st.v.w[b][u][d] &= keep;
+                    }
+        }
+        float v_new = v_top;
+        float sv[KB];
+        if constexpr (I8) {
+#pragma unroll
+            for (int b = 0; b < KB; b++) v_new = fmaxf(v_new, st.sv[b]);
+            const float inv = P_SCALE / v_new;
+#pragma unroll
+            for (int b = 0; b < KB; b++) sv[b] = st.sv[b] * inv;
+        }
+        const float shrink = I8 ? v_top / v_new : 1.0f;
+        v_top = v_new;
+        typename Op::type pf[RG][KB / 2][N];
+#pragma unroll
+        for (int rg = 0; rg < RG; rg++) {
+            float top = m_run[rg];
+#pragma unroll
+            for (int b = 0; b < KB; b++) {
+                const float f = I8 ? factor[rg] * st.sk[b] : factor[rg];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    x[rg][b][r] *= f;
+                    if (!whole && ((st.there >> b & 1) == 0 || first + 16 * b + 4 * g + r >= limit[rg])) x[rg][b][r] = -INFINITY;
+                    top = fmaxf(top, x[rg][b][r]);
+                }
+            }
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float base = top == -INFINITY ? 0.0f : top;  // -inf - -inf is no number
+            const float alpha = exp2_of(m_run[rg] - base);
+            m_run[rg] = top;
+            float sum = 0.0f;
+#pragma unroll
+            for (int c = 0; c < KB / 2; c++) {
+                float p[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int b = 2 * c + e / 4;
+                    p[e] = exp2_of(x[rg][b][e % 4] - base);
+                    sum += p[e];
+                    if constexpr (I8) p[e] *= sv[b];
+                }
+                split_n<I8, N>(p, pf[rg][c]);
+            }
+            l_run[rg] = l_run[rg] * alpha + sum;
+            const float rescale = alpha * shrink;
+#pragma unroll
+            for (int t = 0; t < DT; t++) o[rg][t] *= rescale;
+        }
+#pragma unroll
+        for (int c = 0; c < KB / 2; c++)
+#pragma unroll
+            for (int t = 0; t < DT; t++) {
+                const typename Op::type v = st.v.value(c, t);
+#pragma unroll
+                for (int rg = 0; rg < RG; rg++)
+#pragma unroll
+                    for (int n = N - 1; n >= 0; n--) o[rg][t] = Op::mfma(v, pf[rg][c][n], o[rg][t]);
+            }
+    };
+
+    Step st;
+    for (int step = 0; step < steps; step++) {
+        load(st, step);
+        compute(st, step);
+    }
+
+    // in the values' own units
+    const float unit = I8 ? v_top / P_SCALE : 1.0f;
+#pragma unroll
+    for (int rg = 0; rg < RG; rg++) {
+        l_run[rg] += __shfl_xor(l_run[rg], 16, 64);
+        l_run[rg] += __shfl_xor(l_run[rg], 32, 64);
+#pragma unroll
+        for (int t = 0; t < DT; t++) o[rg][t] *= unit;
+    }
+    // a row's D / 4 dims from d on, with its maximum and sum
+    auto put = [&](int row, int d, const float (&v)[4 * DT / (SPLIT ? 4 : 1)], float m, float l) {
+        constexpr int NV = 4 * DT / (SPLIT ? 4 : 1);
+        const int token = (int)((uint32_t)row / a.heads), h = head * a.group + row - token * a.group;
+        if (a.parts > 1) {
+            const int64_t at = (((int64_t)part * a.S + s) * a.Lq + token) * a.H + h;
+            if (l > 0.0f || l != l)
+                store_n<NV>(a.part_o + at * D + d, v);
+            if (d == 0) a.part_ml[at] = {m, l};
+            return;
+        }
+        float y[NV];
+        const float inv = l == 0.0f || token >= qlen ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int e = 0; e < NV; e++) y[e] = inv == 0.0f ? 0.0f : v[e] * inv;
+        store_n<NV>(reinterpret_cast<T *>(a.out + s * a.os[0] + token * a.os[1] + h * a.os[2]) + d, y);
+    };
+    if constexpr (!SPLIT) {
+#pragma unroll
+        for (int rg = 0; rg < RG; rg++) {
+            const int row = row0 + 16 * rg + i;
+            if (row >= rows) continue;
+            float v[4 * DT];
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int t = 0; t < DT; t++) v[DT * r + t] = o[rg][t][r];
+            put(row, 4 * DT * g, v, m_run[rg], l_run[rg]);
+        }
+    } else {
+        constexpr int LROW = D + 4;
+        __shared__ __align__(16) float lo[4][16 * RG * LROW];
+        __shared__ float2 ml[4][16 * RG];
+#pragma unroll
+        for (int rg = 0; rg < RG; rg++) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                float v[DT];
+#pragma unroll
+                for (int t = 0; t < DT; t++) v[t] = o[rg][t][r];
+                store_lds<DT>(&lo[wave][(16 * rg + i) * LROW + DT * (4 * g + r)], v);
+            }
+            if (g == 0) ml[wave][16 * rg + i] = {m_run[rg], l_run[rg]};
+        }
+        __syncthreads();
+        // DT dims of a row a thread
+        for (int n = threadIdx.x; n < 16 * RG * 16; n += 256) {
+            const int r = n / 16, d = n % 16 * DT, row = row0 + r;
+            if (row >= rows) continue;
+            float m = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) m = fmaxf(m, ml[w][r].x);
+            float v[DT], l = 0.0f;
+#pragma unroll
+            for (int e = 0; e < DT; e++) v[e] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) {
+                const float f = ml[w][r].x == -INFINITY ? 0.0f : exp2_of(ml[w][r].x - m);
+                l += ml[w][r].y * f;
+                float x[DT];
+                load_lds<DT>(&lo[w][r * LROW + d], x);
+#pragma unroll
+                for (int e = 0; e < DT; e++) v[e] += x[e] * f;
+            }
+            put(row, d, v, m, l);
+        }
+    }
+}
+
+// Joins the pieces of the keys: DT dims of a row a thread.
+template <typename T, int D>
+static __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttentionArgs a) {
+    constexpr int DT = D / 16;
+    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x, row = n / 16;
+    const int64_t rows = (int64_t)a.S * a.Lq * a.H;
+    if (row >= rows) return;
+    const int d = (int)(n % 16) * DT;
+    const int s = (int)(row / ((int64_t)a.Lq * a.H)), in = (int)(row - (int64_t)s * a.Lq * a.H);
+    const int token = in / a.H, h = in % a.H;
+    const int qlen = a.query_lengths ? max(0, min(a.query_lengths[s], a.Lq)) : a.Lq;
+    const int keys = a.key_lengths ? max(0, min(a.key_lengths[s], a.most)) : a.most;
+    int64_t seen = token < qlen ? keys : 0;
+    if (a.causal) seen = max((int64_t)0, min(seen, (a.start ? a.start[s] : 0) + (int64_t)token + 1));
+    const int parts = (int)((seen + (int64_t)a.piece * PC_BLOCK - 1) / ((int64_t)a.piece * PC_BLOCK));
+    float m = -INFINITY;
+    for (int p = 0; p < parts; p++) m = fmaxf(m, a.part_ml[p * rows + row].x);
+    float v[DT], l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < DT; e++) v[e] = 0.0f;
+    for (int p = 0; p < parts; p++) {
+        const float2 ml = a.part_ml[p * rows + row];
+        if (ml.y == 0.0f) continue;  // nothing was written for it
+        const float f = exp2_of(ml.x - m);
+        l += ml.y * f;
+        float x[DT];
+        load_n<DT>(a.part_o + (p * rows + row) * D + d, x);
+#pragma unroll
+        for (int e = 0; e < DT; e++) v[e] += x[e] * f;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int e = 0; e < DT; e++) v[e] = inv == 0.0f ? 0.0f : v[e] * inv;
+    store_n<DT>(reinterpret_cast<T *>(a.out + s * a.os[0] + token * a.os[1] + h * a.os[2]) + d, v);
+}
+
+}  // namespace vh

@@ -209,10 +209,10 @@ int relative_bucket(int rel, int buckets, int max_distance, int bidirectional) {
 
 // Whether different (sequence, row, head) have different places: each stride, in
 // ascending order, at least what the smaller ones span.
-static bool apart(const int64_t *strides, int64_t seqs, int64_t rows, int64_t heads) {
+bool strides_apart(const int64_t *strides, int64_t seqs, int64_t rows, int64_t heads, int width) {
     std::pair<int64_t, int64_t> d[3] = {{strides[0], seqs}, {strides[1], rows}, {strides[2], heads}};
     std::sort(d, d + 3);
-    int64_t span = CA_D, stretch;
+    int64_t span = width, stretch;
     for (const auto &[stride, n] : d) {
         if (n <= 1) continue;
         if (stride < span) return false;
@@ -264,7 +264,7 @@ static bool cross_ok(const char *what, const vh_cross *c, bool backward) {
                       (long long)CA_MAX_ROW);
             return false;
         }
-        if (t.written && !apart(t.strides, c->sequences, t.rows, t.heads)) {
+        if (t.written && !strides_apart(t.strides, c->sequences, t.rows, t.heads, CA_D)) {
             set_error("%s: %s's strides %lld, %lld, %lld let rows overlap, and %s is written", what, t.name,
                       (long long)t.strides[0], (long long)t.strides[1], (long long)t.strides[2],
                       t.name[0] == 'o' ? "out" : "its gradient");

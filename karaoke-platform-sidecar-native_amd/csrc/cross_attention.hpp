@@ -234,24 +234,6 @@ VH_DEVICE Frag<float> tile_col(const unsigned char *tile, int st, int t, int lan
     return f;
 }
 
-// Which (sequence, head) pair and which of its tiles a workgroup takes.  The pairs
-// are dealt out to the 8 XCDs in turn (workgroup i runs on XCD i % 8), so that a
-// pair's tiles find their keys in one L2 and a batch's long and short sequences are
-// spread evenly; where that leaves the XCDs unequal (few pairs, not a multiple of
-// 8), workgroups are taken as they come.  False: none (the last round of pairs).
-constexpr bool pairs_by_xcd(int64_t pairs) { return pairs % 8 == 0 || pairs >= 64; }
-VH_DEVICE bool pair_task(int pairs, int tiles, int &pair, int &tile) {
-    int i = (int)blockIdx.x;
-    pair = i / tiles;
-    tile = i % tiles;
-    if (!pairs_by_xcd(pairs)) return true;
-    const int xcd = i % 8;
-    i /= 8;
-    pair = i / tiles * 8 + xcd;
-    tile = i % tiles;
-    return pair < pairs;
-}
-
 // Where a product's operands come from.  A streamed tile: in LDS, or (fp32) as it
 // lies in global memory, rows past `last` (the tile's own count) read as row `last`.
 template <typename T>

@@ -318,6 +318,29 @@ size_t cross_workspace_bytes(const vh_cross *c, bool backward);
 // Bucket of a relative position; -1 where the buckets are none.
 int relative_bucket(int rel, int buckets, int max_distance, int bidirectional);
 
+// Whether different (sequence, row, head) of `width` consecutive elements have
+// different places.
+bool strides_apart(const int64_t *strides, int64_t seqs, int64_t rows, int64_t heads, int width);
+
+// Rotary positions, the paged cache with the attention over it, beam search (rotary.hpp,
+// paged_cache.hpp, cache_attention.hpp, beam_search.hpp).
+bool rotary_table(hipStream_t s, const vh_rotary_angles *a, int dim, int positions, float *table, KernelTimer *t = nullptr);
+bool rotary_apply(hipStream_t s, const vh_rotary *r, const vh_rotary_rows *rows, const void *x, void *y, bool backward,
+                  KernelTimer *t = nullptr);
+size_t cache_bytes(const vh_cache *c);
+bool cache_append(hipStream_t s, const vh_cache *c, const vh_cache_rows *r, const vh_rotary *rotary, const void *k, const void *v,
+                  KernelTimer *t = nullptr);
+bool cache_read(hipStream_t s, const vh_cache *c, const vh_cache_rows *r, void *k, void *v, KernelTimer *t = nullptr);
+bool cache_reorder(hipStream_t s, const vh_cache *c, int beams, const int32_t *parents, const int32_t *lengths,
+                   const int32_t *spare, int32_t *table_out, int32_t *spare_out, KernelTimer *t = nullptr);
+bool cache_attention(hipStream_t s, const vh_cache *c, const vh_cache_queries *q, const vh_rotary *rotary, const void *qp,
+                     void *out, void *workspace, KernelTimer *t = nullptr);
+size_t cache_workspace_bytes(const vh_cache *c, const vh_cache_queries *q);
+bool beam_select(hipStream_t s, const vh_beam *b, const void *logits, const float *scores, const int32_t *ended,
+                 int32_t *tokens, int32_t *parents, float *new_scores, int32_t *new_ended, void *workspace,
+                 KernelTimer *t = nullptr);
+size_t beam_workspace_bytes(const vh_beam *b);
+
 // ------------------------------------------------------------------- dims
 struct Dims {
     int dim, depth, bands, heads, dim_head, ff_dim, ffn_glu, gated, mask_hidden, n_fft, hop, channels;

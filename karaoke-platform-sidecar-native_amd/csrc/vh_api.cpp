@@ -493,6 +493,64 @@ extern "C" int vh_relative_bucket(int rel, int buckets, int max_distance, int bi
     return relative_bucket(rel, buckets, max_distance, bidirectional);
 }
 
+// ------------------------------- rotary positions, paged cache, beam search
+extern "C" int vh_rotary_table(vh_context *ctx, const vh_rotary_angles *angles, int dim, int positions, float *table) {
+    if (!have_context(ctx, "vh_rotary_table")) return 0;
+    const OnDevice on(ctx);
+    return on.ok && rotary_table(ctx->stream, angles, dim, positions, table, &ctx->timer);
+}
+
+extern "C" int vh_rotary_apply(vh_context *ctx, const vh_rotary *r, const vh_rotary_rows *rows, const void *x, void *y,
+                               int backward) {
+    if (!have_context(ctx, "vh_rotary_apply")) return 0;
+    const OnDevice on(ctx);
+    return on.ok && rotary_apply(ctx->stream, r, rows, x, y, backward != 0, &ctx->timer);
+}
+
+extern "C" size_t vh_cache_bytes(const vh_cache *c) { return cache_bytes(c); }
+
+extern "C" int vh_cache_append(vh_context *ctx, const vh_cache *c, const vh_cache_rows *rows, const vh_rotary *rotary,
+                               const void *k, const void *v) {
+    if (!have_context(ctx, "vh_cache_append")) return 0;
+    const OnDevice on(ctx);
+    return on.ok && cache_append(ctx->stream, c, rows, rotary, k, v, &ctx->timer);
+}
+
+extern "C" int vh_cache_read(vh_context *ctx, const vh_cache *c, const vh_cache_rows *rows, void *k, void *v) {
+    if (!have_context(ctx, "vh_cache_read")) return 0;
+    const OnDevice on(ctx);
+    return on.ok && cache_read(ctx->stream, c, rows, k, v, &ctx->timer);
+}
+
+extern "C" int vh_cache_attention(vh_context *ctx, const vh_cache *c, const vh_cache_queries *queries,
+                                  const vh_rotary *rotary, const void *q, void *out, void *workspace) {
+    if (!have_context(ctx, "vh_cache_attention")) return 0;
+    const OnDevice on(ctx);
+    return on.ok && cache_attention(ctx->stream, c, queries, rotary, q, out, workspace, &ctx->timer);
+}
+
+extern "C" size_t vh_cache_workspace_bytes(const vh_cache *c, const vh_cache_queries *queries) {
+    return cache_workspace_bytes(c, queries);
+}
+
+extern "C" int vh_cache_reorder(vh_context *ctx, const vh_cache *c, int beams, const int32_t *parents,
+                                const int32_t *lengths, const int32_t *spare, int32_t *table_out, int32_t *spare_out) {
+    if (!have_context(ctx, "vh_cache_reorder")) return 0;
+    const OnDevice on(ctx);
+    return on.ok && cache_reorder(ctx->stream, c, beams, parents, lengths, spare, table_out, spare_out, &ctx->timer);
+}
+
+extern "C" int vh_beam_select(vh_context *ctx, const vh_beam *b, const void *logits, const float *scores,
+                              const int32_t *ended, int32_t *tokens, int32_t *parents, float *new_scores,
+                              int32_t *new_ended, void *workspace) {
+    if (!have_context(ctx, "vh_beam_select")) return 0;
+    const OnDevice on(ctx);
+    return on.ok && beam_select(ctx->stream, b, logits, scores, ended, tokens, parents, new_scores, new_ended, workspace,
+                                &ctx->timer);
+}
+
+extern "C" size_t vh_beam_workspace_bytes(const vh_beam *b) { return beam_workspace_bytes(b); }
+
 // -------------------------------------------------------------------- model
 namespace {
 

@@ -25,6 +25,7 @@ BF16_A, BF16_C, BF16_STAGED = 1, 2, 4  # vh_gemm_bf16 operand flags; STAGED forc
 ATT_OUT_BF16, ATT_BF16, ATT_SPLIT, ATT_H2, ATT_OUT_H2 = 1, 2, 4, 8, 16  # vh_attention flags
 NOALLOC_MAX_LENGTH = 4096  # VH_NOALLOC_MAX_LENGTH
 TYPE_FP32, TYPE_BF16 = 0, 1  # VH_TYPE_*
+CACHE_BF16, CACHE_INT8, CACHE_BLOCK = 0, 1, 16  # VH_CACHE_*
 SPEC_REFERENCE, SPEC_FRAME_MAJOR = 0, 1  # spectrum layouts: [F][C][T][2] / [C][T][F][2]
 
 _P = ctypes.c_void_p
@@ -40,6 +41,46 @@ class CCross(ctypes.Structure):
                 [(n, _I64 * 3) for n in ("q_strides", "k_strides", "v_strides", "out_strides")] +
                 [(n, _P) for n in ("query_lengths", "key_lengths", "query_start", "bias_table")] +
                 [(n, _I) for n in ("buckets", "max_distance", "bidirectional")])
+
+
+class CRotaryAngles(ctypes.Structure):
+    """vh_rotary_angles"""
+    _fields_ = [("base", ctypes.c_double), ("factor", ctypes.c_double), ("original", _I), ("low", ctypes.c_double),
+                ("high", ctypes.c_double), ("magnitude", ctypes.c_double)]
+
+
+class CRotary(ctypes.Structure):
+    """vh_rotary"""
+    _fields_ = [("dim", _I), ("interleaved", _I), ("positions", _I), ("table", _P)]
+
+
+class CRotaryRows(ctypes.Structure):
+    """vh_rotary_rows"""
+    _fields_ = ([(n, _I) for n in ("type", "sequences", "length", "heads", "head_dim")] +
+                [("x_strides", _I64 * 3), ("y_strides", _I64 * 3), ("start", _P)])
+
+
+class CCache(ctypes.Structure):
+    """vh_cache"""
+    _fields_ = ([(n, _I) for n in ("type", "kv_heads", "head_dim", "page_tokens", "pages", "sequences", "table_pages")] +
+                [("pool", _P), ("table", _P)])
+
+
+class CCacheRows(ctypes.Structure):
+    """vh_cache_rows"""
+    _fields_ = [("type", _I), ("length", _I), ("k_strides", _I64 * 3), ("v_strides", _I64 * 3), ("start", _P), ("lengths", _P)]
+
+
+class CCacheQueries(ctypes.Structure):
+    """vh_cache_queries"""
+    _fields_ = ([(n, _I) for n in ("type", "heads", "length", "causal", "most_keys")] + [("scale", ctypes.c_float)] +
+                [("q_strides", _I64 * 3), ("out_strides", _I64 * 3)] +
+                [(n, _P) for n in ("query_lengths", "key_lengths", "start")])
+
+
+class CBeam(ctypes.Structure):
+    """vh_beam"""
+    _fields_ = ([(n, _I) for n in ("type", "sequences", "beams", "vocab", "picks", "end_token")] + [("strides", _I64 * 2)])
 
 
 # Signatures (result, arguments) of every entry point declared in
@@ -74,6 +115,16 @@ SIGNATURES = {
     "vh_cross_saved_bytes": (ctypes.c_size_t, [ctypes.POINTER(CCross)]),
     "vh_cross_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(CCross), _I]),
     "vh_relative_bucket": (_I, [_I, _I, _I, _I]),
+    "vh_rotary_table": (_I, [_P, ctypes.POINTER(CRotaryAngles), _I, _I, _P]),
+    "vh_rotary_apply": (_I, [_P, ctypes.POINTER(CRotary), ctypes.POINTER(CRotaryRows), _P, _P, _I]),
+    "vh_cache_bytes": (ctypes.c_size_t, [ctypes.POINTER(CCache)]),
+    "vh_cache_append": (_I, [_P, ctypes.POINTER(CCache), ctypes.POINTER(CCacheRows), ctypes.POINTER(CRotary), _P, _P]),
+    "vh_cache_read": (_I, [_P, ctypes.POINTER(CCache), ctypes.POINTER(CCacheRows), _P, _P]),
+    "vh_cache_attention": (_I, [_P, ctypes.POINTER(CCache), ctypes.POINTER(CCacheQueries), ctypes.POINTER(CRotary), _P, _P, _P]),
+    "vh_cache_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(CCache), ctypes.POINTER(CCacheQueries)]),
+    "vh_cache_reorder": (_I, [_P, ctypes.POINTER(CCache), _I] + [_P] * 5),
+    "vh_beam_select": (_I, [_P, ctypes.POINTER(CBeam)] + [_P] * 8),
+    "vh_beam_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(CBeam)]),
     "vh_model_load": (_P, [_P, ctypes.POINTER(CDims), _P, ctypes.c_size_t]),
     "vh_model_free": (None, [_P]), "vh_model_set_precision": (_I, [_P, _I]),
     "vh_transformer": (_I, [_P, _P, _I, _I, _P, _I, _I]),
@@ -451,6 +502,270 @@ class CrossAttention:
                 self._buffer("workspace", workspace, self.workspace_bytes, "workspace", True))
         self._on_gpu()
         _ok(lib().vh_cross_attention_backward(self.ctx.h, self._ref, *args), "vh_cross_attention_backward")
+
+
+class _Plan:
+    """What the bindings below share: later calls' tensors and buffers are checked against the ones that a layout was made
+    of, before the library sees them."""
+
+    what = ""
+
+    def _keep(self, **tensors):
+        self._like = {n: (t.dtype, t.shape, t.stride(), t.device) for n, t in tensors.items()}
+
+    def _refuse(self, text):
+        raise NativeError(f"{self.what}: {text}")
+
+    def _same_device(self, tensors):
+        devices = {t.device for t in tensors if t is not None}
+        if len(devices) > 1:
+            self._refuse("tensors on different devices")
+
+    def _ints(self, name, t, *shape):
+        import torch
+        if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous()):
+            self._refuse(f"{name} is a contiguous int32 tensor {list(shape)}")
+
+    def _activations(self, **tensors):
+        import torch
+        if any(t.dtype not in (torch.float32, torch.bfloat16) for t in tensors.values()) or \
+                len({t.dtype for t in tensors.values()}) != 1:
+            self._refuse(f"{', '.join(tensors)}: all fp32 or all bf16")
+        if any(t.shape[-1] > 1 and t.stride(-1) != 1 for t in tensors.values()):
+            self._refuse("a row's elements are consecutive")
+
+    def _tensor(self, name, like, t):
+        """t's address, where it is laid out as `like` was."""
+        dtype, shape, stride, device = self._like[like]
+        if t.dtype != dtype or t.shape != shape or t.device != device or \
+                (t.stride() != stride and t.numel() and any(n > 1 and a != b for n, a, b in zip(shape, t.stride(), stride))):
+            self._refuse(f"{name} is not laid out as {like} was")
+        return t.data_ptr()
+
+    def _buffer(self, name, t, nbytes, device):
+        if t is None:
+            return None
+        if t.numel() * t.element_size() < nbytes or not t.is_contiguous() or t.device != device:
+            self._refuse(f"{name} has fewer than {nbytes} bytes in a row, or is on another device")
+        return t.data_ptr()
+
+    def _on_gpu(self, device):
+        if device.type != "cuda" or device.index:  # every context's GPU is the first
+            self._refuse(f"the tensors are on {device}, the context's work runs on cuda:0")
+
+
+def _rotary_ref(r):
+    return r._ref if r is not None else None
+
+
+class Rotary(_Plan):
+    """A rotation (vh_rotary) with its table of `positions` rows, on the context's GPU.  dim: the head's leading dims that
+    turn; interleaved: pairs of neighbours, else of the halves; with a factor over 1 the angles are scaled (see
+    vh_rotary_angles)."""
+
+    what = "Rotary"
+
+    def __init__(self, ctx: Context, positions: int, dim: int, *, interleaved: bool = False, base: float = 10000.0,
+                 factor: float = 1.0, original: int = 0, low: float = 1.0, high: float = 32.0, magnitude: float = 1.0):
+        import torch
+        if positions < 1 or dim < 2 or dim > 256 or dim % 2:
+            self._refuse(f"{positions} positions (from 1) of {dim} dims (even, 2 to 256)")
+        self.ctx = ctx
+        self.table = torch.empty(positions, dim // 2, 2, device="cuda:0")
+        self.c = CRotary(dim, int(interleaved), positions, ptr(self.table))
+        self._ref = ctypes.byref(self.c)
+        angles = CRotaryAngles(base, factor, original, low, high, magnitude)
+        _ok(lib().vh_rotary_table(ctx.h, ctypes.byref(angles), dim, positions, ptr(self.table)), "vh_rotary_table")
+        self._rows = {}
+
+    def apply(self, x, y, start=None, backward: bool = False):
+        """y [S][L][H][D] = x turned from position start[s] (int32 device tensor [S], None: 0) on; y may be x.  backward:
+        by the transpose, which takes y's gradient to x's."""
+        key = (x.dtype, x.shape, x.stride(), y.dtype, y.stride())
+        rows = self._rows.get(key)
+        if rows is None:
+            if x.dim() != 4 or x.shape[3] < self.c.dim:
+                self._refuse(f"x and y are [S][L][H][D] with D from {self.c.dim}")
+            self._activations(x=x, y=y)
+            S, L, H, D = x.shape
+            rows = CRotaryRows(int(x.element_size() == 2), S, L, H, D, (_I64 * 3)(*x.stride()[:3]), (_I64 * 3)(*y.stride()[:3]))
+            self._rows = {**(self._rows if len(self._rows) < 64 else {}), key: rows}
+        if y.shape != x.shape:
+            self._refuse("y is not of x's shape")
+        if start is not None:
+            self._ints("start", start, x.shape[0])
+        self._same_device((x, y, start))
+        self._on_gpu(x.device)
+        rows.start = _opt(start)
+        _ok(lib().vh_rotary_apply(self.ctx.h, self._ref, ctypes.byref(rows), x.data_ptr(), y.data_ptr(), int(backward)),
+            "vh_rotary_apply")
+
+
+class PagedCache(_Plan):
+    """A pool of pages of keys and values (vh_cache): kind "bf16", or "int8" with a scale for every 16 tokens and head.
+    Tables [sequences][pages of one], int32, say which pages a sequence has, and are the caller's."""
+
+    what = "PagedCache"
+
+    def __init__(self, ctx: Context, kind: str, *, kv_heads: int, head_dim: int, page_tokens: int, pages: int,
+                 device: str = "cuda:0"):
+        import torch
+        if kind not in ("bf16", "int8"):
+            self._refuse(f"a cache of {kind!r}: bf16 or int8")
+        self.ctx = ctx
+        self.c = CCache(CACHE_INT8 if kind == "int8" else CACHE_BF16, kv_heads, head_dim, page_tokens, pages)
+        n = int(lib().vh_cache_bytes(ctypes.byref(self.c)))
+        _ok(n, "vh_cache_bytes")
+        self.pool = torch.empty(n, dtype=torch.uint8, device=device)
+        self.c.pool = ptr(self.pool)
+
+    def _with(self, table):
+        """The cache seen through a table."""
+        import torch
+        if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
+            self._refuse("the table is a contiguous int32 tensor [sequences][pages]")
+        self._same_device((self.pool, table))
+        c = CCache.from_buffer_copy(self.c)
+        c.sequences, c.table_pages, c.table = table.shape[0], table.shape[1], ptr(table)
+        return c
+
+    def tokens(self, table, k, v, *, start=None, lengths=None, rotary: Rotary | None = None) -> "CacheTokens":
+        """Rows k and v [sequences][length][kv_heads][head_dim] to append, or to read into."""
+        return CacheTokens(self, table, k, v, start, lengths, rotary)
+
+    def queries(self, table, q, out, *, most_keys: int, causal: bool = False, scale: float = 0.125, query_lengths=None,
+                key_lengths=None, query_start=None, rotary: Rotary | None = None) -> "CacheQueries":
+        """Queries q and out [sequences][length][heads][head_dim] over the cache."""
+        return CacheQueries(self, table, q, out, most_keys, causal, scale, query_lengths, key_lengths, query_start, rotary)
+
+    def reorder(self, table, parents, lengths, spare, table_out, spare_out, *, beams: int):
+        """The table's rows in the order of their parents (see vh_cache_reorder)."""
+        c = self._with(table)
+        S = c.sequences
+        if beams < 1 or S % beams:
+            self._refuse(f"{S} sequences in groups of {beams} beams")
+        for name, t, shape in (("parents", parents, (S,)), ("lengths", lengths, (S // beams,)), ("spare", spare, (S,)),
+                               ("table_out", table_out, tuple(table.shape)), ("spare_out", spare_out, (S,))):
+            self._ints(name, t, *shape)
+        self._same_device((table, parents, lengths, spare, table_out, spare_out))
+        self._on_gpu(table.device)
+        _ok(lib().vh_cache_reorder(self.ctx.h, ctypes.byref(c), beams, ptr(parents), ptr(lengths), ptr(spare), ptr(table_out),
+                                   ptr(spare_out)), "vh_cache_reorder")
+
+
+class CacheTokens(_Plan):
+    """The layout of rows of keys and values and where they are in a paged cache.  Later calls may pass other tensors of the
+    same layout; table, start and lengths are read when a call's work runs."""
+
+    what = "CacheTokens"
+
+    def __init__(self, cache: PagedCache, table, k, v, start, lengths, rotary):
+        self.ctx, self.c = cache.ctx, cache._with(table)
+        if k.dim() != 4 or k.shape[0] != table.shape[0] or tuple(k.shape[2:]) != (self.c.kv_heads, self.c.head_dim) or \
+                v.shape != k.shape:
+            self._refuse("k and v are [sequences][length][kv_heads][head_dim]")
+        self._activations(k=k, v=v)
+        self._ints("start", start, k.shape[0])
+        self._ints("lengths", lengths, k.shape[0])
+        self._same_device((cache.pool, k, v, start, lengths))
+        self._kept = (cache, table, start, lengths, rotary)
+        self._keep(k=k, v=v)
+        self.rows = CCacheRows(int(k.element_size() == 2), k.shape[1], (_I64 * 3)(*k.stride()[:3]), (_I64 * 3)(*v.stride()[:3]),
+                               _opt(start), _opt(lengths))
+        self._refs = (ctypes.byref(self.c), ctypes.byref(self.rows))
+        self._rotary = _rotary_ref(rotary)
+        self._device = k.device
+
+    def append(self, k, v):
+        """Puts the rows into the cache, keys turned."""
+        args = self._tensor("k", "k", k), self._tensor("v", "v", v)
+        self._on_gpu(self._device)
+        _ok(lib().vh_cache_append(self.ctx.h, *self._refs, self._rotary, *args), "vh_cache_append")
+
+    def read(self, k=None, v=None):
+        """What the cache holds at the rows' positions, as it is there, into k and v (either may be None)."""
+        args = [self._tensor(n, n, t) if t is not None else None for n, t in (("k", k), ("v", v))]
+        self._on_gpu(self._device)
+        _ok(lib().vh_cache_read(self.ctx.h, *self._refs, *args), "vh_cache_read")
+
+
+class CacheQueries(_Plan):
+    """The layout of an attention over a paged cache (vh_cache_queries).  Later calls may pass other tensors of the same
+    layout; table, lengths and starts are read when a call's work runs, so a captured call follows them."""
+
+    what = "CacheQueries"
+
+    def __init__(self, cache: PagedCache, table, q, out, most_keys, causal, scale, query_lengths, key_lengths, query_start, rotary):
+        self.ctx, self.c = cache.ctx, cache._with(table)
+        if q.dim() != 4 or q.shape[0] != table.shape[0] or q.shape[3] != self.c.head_dim or out.shape != q.shape:
+            self._refuse("q and out are [sequences][length][heads][head_dim]")
+        self._activations(q=q, out=out)
+        for name, t in (("query_lengths", query_lengths), ("key_lengths", key_lengths), ("query_start", query_start)):
+            self._ints(name, t, q.shape[0])
+        self._same_device((cache.pool, q, out, query_lengths, key_lengths, query_start))
+        self._kept = (cache, table, query_lengths, key_lengths, query_start, rotary)
+        self._keep(q=q, out=out)
+        self.q = CCacheQueries(int(q.element_size() == 2), q.shape[2], q.shape[1], int(causal), most_keys, scale,
+                               (_I64 * 3)(*q.stride()[:3]), (_I64 * 3)(*out.stride()[:3]), _opt(query_lengths),
+                               _opt(key_lengths), _opt(query_start))
+        self._refs = (ctypes.byref(self.c), ctypes.byref(self.q))
+        self._rotary = _rotary_ref(rotary)
+        self._device, self._bytes = q.device, None
+
+    def workspace_bytes(self) -> int:
+        if self._bytes is None:
+            n = int(lib().vh_cache_workspace_bytes(*self._refs))
+            _ok(n, "vh_cache_workspace_bytes")
+            self._bytes = n
+        return self._bytes
+
+    def forward(self, q, out, workspace=None):
+        args = (self._tensor("q", "q", q), self._tensor("out", "out", out),
+                self._buffer("workspace", workspace, self.workspace_bytes(), self._device))
+        self._on_gpu(self._device)
+        _ok(lib().vh_cache_attention(self.ctx.h, *self._refs, self._rotary, *args), "vh_cache_attention")
+
+
+class BeamSearch(_Plan):
+    """One step of beam search (vh_beam) for logits [sequences][beams][vocab], fp32 or bf16."""
+
+    what = "BeamSearch"
+
+    def __init__(self, ctx: Context, logits, *, picks: int | None = None, end_token: int = -1):
+        if logits.dim() != 3:
+            self._refuse("logits are [sequences][beams][vocab]")
+        self._activations(logits=logits)
+        S, B, V = logits.shape
+        self.ctx, self.picks = ctx, B if picks is None else picks
+        self._keep(logits=logits)
+        self.c = CBeam(int(logits.element_size() == 2), S, B, V, self.picks, end_token, (_I64 * 2)(*logits.stride()[:2]))
+        self._ref = ctypes.byref(self.c)
+        self._device, self._bytes = logits.device, None
+
+    def workspace_bytes(self) -> int:
+        if self._bytes is None:
+            n = int(lib().vh_beam_workspace_bytes(self._ref))
+            _ok(n, "vh_beam_workspace_bytes")
+            self._bytes = n
+        return self._bytes
+
+    def select(self, logits, scores, tokens, parents, new_scores, *, ended=None, new_ended=None, workspace):
+        """The best `picks` of each sequence: tokens and parents (int32), new_scores (fp32) and new_ended (int32), all
+        [sequences][picks]; scores (fp32) and ended (int32) are the beams' [sequences][beams]."""
+        import torch
+        S, B = self.c.sequences, self.c.beams
+        address = self._tensor("logits", "logits", logits)
+        for name, t, shape in (("scores", scores, (S, B)), ("new_scores", new_scores, (S, self.picks))):
+            if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous():
+                self._refuse(f"{name} is a contiguous fp32 tensor {list(shape)}")
+        for name, t, n in (("ended", ended, B), ("tokens", tokens, self.picks), ("parents", parents, self.picks),
+                           ("new_ended", new_ended, self.picks)):
+            self._ints(name, t, S, n)
+        self._same_device((logits, scores, ended, tokens, parents, new_scores, new_ended))
+        ws = self._buffer("workspace", workspace, self.workspace_bytes(), self._device)
+        self._on_gpu(self._device)
+        _ok(lib().vh_beam_select(self.ctx.h, self._ref, address, ptr(scores), _opt(ended), ptr(tokens), ptr(parents),
+                                 ptr(new_scores), _opt(new_ended), ws), "vh_beam_select")
 
 
 class Model:
