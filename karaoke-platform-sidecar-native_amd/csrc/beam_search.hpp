@@ -13,7 +13,7 @@
 
 namespace vh {
 
-constexpr int BS_THREADS = 1024, BS_WAVES = 16;
+constexpr int BS_THREADS = 256, BS_WAVES = 4;
 constexpr int BS_MAX_PICKS = 64, BS_MAX_BEAMS = 64;
 constexpr int BS_LIST = 256;  // a wave's candidates
 
@@ -55,30 +55,45 @@ template <>
 struct Logits<bf16> {
     uint32_t w[4];
     VH_DEVICE float get(int e) const { return __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16); }
+    VH_DEVICE float pick(int e) const {  // e not known at compile time
+        const uint32_t a = e & 4 ? w[2] : w[0], b = e & 4 ? w[3] : w[1], u = e & 2 ? b : a;
+        return __uint_as_float(e & 1 ? u & 0xffff0000u : u << 16);
+    }
     VH_DEVICE void load(const bf16 *p) {
         const Elements<uint16_t, 8>::type a = *reinterpret_cast<const Elements<uint16_t, 8>::type *>(p);
 #pragma unroll
         for (int e = 0; e < 4; e++) w[e] = (uint32_t)a[2 * e] | (uint32_t)a[2 * e + 1] << 16;
     }
-    VH_DEVICE void load(const bf16 *p, int n) {
+    VH_DEVICE void load_few(const bf16 *p, int n) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) w[e] = 0xff80ff80u;
+        for (int e = 0; e < 4; e++)
+            w[e] = (uint32_t)__builtin_bit_cast(uint16_t, p[max(0, 2 * e - 8 + n)]) |
+                   (uint32_t)__builtin_bit_cast(uint16_t, p[max(0, 2 * e - 7 + n)]) << 16;
+    }
+    // the first n as -inf
+    VH_DEVICE void leave_out(int n) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            if (e >= n) continue;
-            const uint32_t v = __builtin_bit_cast(uint16_t, p[e]);
-            w[e / 2] = e & 1 ? (w[e / 2] & 0xffffu) | v << 16 : (w[e / 2] & 0xffff0000u) | v;
-        }
+        for (int e = 0; e < 8; e++)
+            if (e < n) w[e / 2] = e & 1 ? (w[e / 2] & 0xffffu) | 0xff800000u : (w[e / 2] & 0xffff0000u) | 0xff80u;
     }
 };
 template <>
 struct Logits<float> {
     float w[8];
     VH_DEVICE float get(int e) const { return w[e]; }
+    VH_DEVICE float pick(int e) const {
+        const float a = e & 4 ? w[4] : w[0], b = e & 4 ? w[5] : w[1], c = e & 4 ? w[6] : w[2], d = e & 4 ? w[7] : w[3];
+        return e & 2 ? (e & 1 ? d : c) : (e & 1 ? b : a);
+    }
     VH_DEVICE void load(const float *p) { load_n<8>(p, w); }
-    VH_DEVICE void load(const float *p, int n) {
+    VH_DEVICE void load_few(const float *p, int n) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) w[e] = e < n ? p[e] : -INFINITY;
+        for (int e = 0; e < 8; e++) w[e] = p[max(0, e - 8 + n)];
+    }
+    VH_DEVICE void leave_out(int n) {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (e < n) w[e] = -INFINITY;
     }
 };
 
@@ -88,35 +103,60 @@ VH_DEVICE double wave_sum_double(double v) {
     return v;
 }
 
-// Keeps the compiler from holding what it made of the logits up to here.
-template <typename T, int NV>
-VH_DEVICE void anew(Logits<T> (&x)[NV]) {
-#pragma unroll
-    for (int j = 0; j < NV; j++)
-#pragma unroll
-        for (auto &w : x[j].w) asm volatile("" : "+v"(w));
+// LDS accesses of the wave's lanes before and after stay in that order (the hardware
+// keeps a wave's; this keeps the compiler's).
+VH_DEVICE void beam_wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
-// A wave's best `most` of NV * 8 logits a lane into list, unordered; how many.
-// Lane l's vector j covers the stretch's elements (j * BS_THREADS + thread) * 8 .. + 7,
-// `valid` (of the stretch) of them there.  floor: a value that `most` of them reach,
-// or -inf.
+// Keeps the compiler from holding what it made of the logits up to here, and from
+// taking up more of them than a vector at a time: else it unpacks all of a thread's
+// logits at once, and spills.
+template <typename T>
+VH_DEVICE void anew(Logits<T> &x) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (auto &w : x.w) asm volatile("" : "+v"(w));
+}
+
+// A thread's vector j covers the stretch's logits (j * BS_THREADS + thread) * 8 .. + 7.
+// One that reaches beyond the `valid` of the stretch is moved back to end with them, so
+// that no load is partial; its first `skip` logits are the vector's before it (8: all of
+// it is beyond).  Of a vocabulary of n < 8 the last n are it, the others its first once more.
+struct BeamPlace {
+    int at, skip;
+    VH_DEVICE BeamPlace(int j, int thread, int valid) {
+        const int own = (j * BS_THREADS + thread) * 8;
+        at = min(own, valid - 8);
+        skip = min(own - at, 8);
+    }
+};
+
+// A wave's best `most` of NV * 8 logits a lane into list, unordered; how many.  floor: a
+// value that `most` of them reach, or -inf.
 template <typename T, int NV>
 VH_DEVICE int collect(Logits<T> (&x)[NV], int thread, int valid, float floor, int most, BeamPick *list) {
-    const uint64_t below = ((uint64_t)1 << (threadIdx.x & 63)) - 1;
-    auto at = [&](int j) { return (j * BS_THREADS + thread) * 8; };
+    const int lane = threadIdx.x & 63;
+    const uint64_t below = ((uint64_t)1 << lane) - 1;
     int n = 0;
 #pragma unroll
-    for (int j = 0; j < NV; j++)
+    for (int j = 0; j < NV; j++) {
+        anew(x[j]);
+        const BeamPlace place(j, thread, valid);
+        // the lane's logits of this vector that reach the floor, as bits
+        uint32_t mine = 0;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float v = x[j].get(e);
-            const uint64_t m = __ballot(v >= floor && at(j) + e < valid);
-            if (!m) continue;
-            const int k = n + __popcll(m & below);
-            if ((m >> (threadIdx.x & 63) & 1) && k < BS_LIST) list[k] = {v, at(j) + e};
+        for (int e = 0; e < 8; e++) mine |= x[j].get(e) >= floor ? 1u << e : 0u;
+        mine &= 0xffu << place.skip;
+        while (__ballot(mine != 0)) {  // one of each lane's at a time
+            const uint64_t m = __ballot(mine != 0);
+            const int e = __ffs((int)mine) - 1, k = n + __popcll(m & below);
+            if (mine && k < BS_LIST) list[k] = {x[j].pick(e), place.at + e};
+            mine &= mine - 1;
             n += __popcll(m);
         }
+    }
     if (n <= BS_LIST) return n;
     // Too many (many logits alike, or those of one lane all larger than others'): the
     // value that the most-th best has, bit by bit; those above it, and of its own the
@@ -125,51 +165,47 @@ VH_DEVICE int collect(Logits<T> (&x)[NV], int thread, int valid, float floor, in
     for (int bit = 31; bit >= 0; bit--) {
         const uint32_t trial = best | 1u << bit;
         int count = 0;
-        anew(x);
 #pragma unroll
-        for (int j = 0; j < NV; j++)
+        for (int j = 0; j < NV; j++) {
+            anew(x[j]);
+            const BeamPlace place(j, thread, valid);
+            int mine = 0;
 #pragma unroll
             for (int e = 0; e < 8; e++)
-                count += __popcll(__ballot(x[j].get(e) == x[j].get(e) && ordered(x[j].get(e)) >= trial && at(j) + e < valid));
+                mine += x[j].get(e) == x[j].get(e) && ordered(x[j].get(e)) >= trial && e >= place.skip ? 1 : 0;
+            count += mine;
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) count += __shfl_xor(count, o, 64);
         if (count >= most) best = trial;
     }
     const float limit = from_ordered(best);
     n = 0;
-    anew(x);
 #pragma unroll
-    for (int j = 0; j < NV; j++)
+    for (int pass = 0; pass < 2; pass++) {  // above the limit, then at it while there is room
+        const int room = pass ? most : BS_LIST;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float v = x[j].get(e);
-            const uint64_t m = __ballot(v > limit && at(j) + e < valid);
-            if (!m) continue;
-            if (m >> (threadIdx.x & 63) & 1) list[n + __popcll(m & below)] = {v, at(j) + e};
-            n += __popcll(m);
-        }
-    int room = most - n;
-    anew(x);
+        for (int j = 0; j < NV; j++) {
+            anew(x[j]);
+            const BeamPlace place(j, thread, valid);
+            int mine = 0;
 #pragma unroll
-    for (int j = 0; j < NV; j++) {
-        if (room <= 0) break;
-        int mine = 0;
+            for (int e = 0; e < 8; e++) mine += (pass ? x[j].get(e) == limit : x[j].get(e) > limit) && e >= place.skip ? 1 : 0;
+            int upto = mine;
 #pragma unroll
-        for (int e = 0; e < 8; e++) mine += x[j].get(e) == limit && at(j) + e < valid ? 1 : 0;
-        int upto = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int v = __shfl_up(upto, o, 64);
-            if ((int)(threadIdx.x & 63) >= o) upto += v;
-        }
-        int k = upto - mine;
-        const int all = __shfl(upto, 63, 64);
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-            if (x[j].get(e) == limit && at(j) + e < valid) {
-                if (k < room) list[n + k] = {x[j].get(e), at(j) + e};
-                k++;
+            for (int o = 1; o < 64; o <<= 1) {
+                const int v = __shfl_up(upto, o, 64);
+                if (lane >= o) upto += v;
             }
-        n += min(all, room);
-        room -= all;
+            int k = n + upto - mine;
+            n = min(n + __shfl(upto, 63, 64), room);
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if ((pass ? x[j].get(e) == limit : x[j].get(e) > limit) && e >= place.skip) {
+                    if (k < room) list[k] = {x[j].get(e), place.at + e};
+                    k++;
+                }
+        }
     }
     return n;
 }
@@ -189,24 +225,32 @@ static __global__ __launch_bounds__(BS_THREADS) void beam_stretch_kernel(BeamArg
     Logits<T> x[NV];
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-        const int at = (j * BS_THREADS + (int)threadIdx.x) * 8;
-        if (at + 8 <= valid) x[j].load(p + at);
-        else x[j].load(p + at, max(0, valid - at));
+        const BeamPlace place(j, (int)threadIdx.x, valid);
+        if (NV > 1 || a.V >= 8) x[j].load(p + place.at);
+        else x[j].load_few(p, valid);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const BeamPlace place(j, (int)threadIdx.x, valid);
+        if (place.skip) x[j].leave_out(place.skip);
     }
     // the lane's largest, the wave's, and the sum of exponentials (a NaN stays one)
     float top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < NV; j++)
+    for (int j = 0; j < NV; j++) {
+        anew(x[j]);
 #pragma unroll
         for (int e = 0; e < 8; e++) top = fmaxf(top, x[j].get(e));
+    }
     const float wtop = wave_max(top);
     const float c = 1.4426950408889634f, base = wtop == -INFINITY ? 0.0f : wtop;
     float sum = 0.0f;
-    anew(x);
 #pragma unroll
-    for (int j = 0; j < NV; j++)
+    for (int j = 0; j < NV; j++) {
+        anew(x[j]);
 #pragma unroll
         for (int e = 0; e < 8; e++) sum += __builtin_amdgcn_exp2f((x[j].get(e) - base) * c);
+    }
     const double wsum = wave_sum_double((double)sum);
 
     // a value that at least `most` of the wave's lanes' largest reach
@@ -220,9 +264,8 @@ static __global__ __launch_bounds__(BS_THREADS) void beam_stretch_kernel(BeamArg
         if (n >= most) floor = trial;
         if (n == most) break;
     }
-    anew(x);
     int n = collect<T, NV>(x, (int)threadIdx.x, valid, floor ? from_ordered(floor) : -INFINITY, most, lists[wave]);
-    cache_wave_order();
+    beam_wave_order();
     for (int i = lane; i < n; i += 64) {
         const BeamPick mine = lists[wave][i];
         int rank = 0;
@@ -287,77 +330,137 @@ VH_DEVICE double score_of(uint64_t a) {
     return __longlong_as_double((int64_t)(u & 0x8000000000000000ull ? u ^ 0x8000000000000000ull : ~u));
 }
 
-constexpr int BS_JOIN = 1024;  // candidates sorted at once
+// What the join knows of a beam: 0 as it is, 1 no candidate but -inf, 2 ended.
+struct BeamState {
+    double lse;
+    int state;
+};
+// Beam b's candidate `in` of its stretches' lists; (-1, -1): none.
+VH_DEVICE BeamKey candidate(const BeamArgs &a, int s, int beam, int in, const BeamState &st) {
+    const BeamKey none{~0ull, ~0ull};
+    const int row = s * a.B + beam;
+    const double score = (double)a.scores[row];
+    if (st.state) {  // the end token with the score as it is, then the others in order
+        int token = in;
+        double v = -INFINITY;
+        if (st.state == 2) {
+            token = in == 0 ? a.end_token : in - 1 < a.end_token ? in - 1 : in;
+            if (in == 0) v = score;
+        }
+        if (in >= a.picks || token >= a.V) return none;
+        return {score_down(v), (uint64_t)beam << 56 | (uint64_t)token};
+    }
+    const char *p = a.parts + ((int64_t)row * a.stretches + in / a.picks) * a.part_bytes;
+    const BeamPick pick = reinterpret_cast<const BeamPick *>(p + sizeof(BeamPart))[in % a.picks];
+    if (pick.token < 0) return none;
+    const double v = score + ((double)pick.x - st.lse);
+    const uint32_t down = v == -INFINITY ? 0u : ~ordered(pick.x);
+    return {score_down(v), (uint64_t)beam << 56 | (uint64_t)down << 24 | (uint64_t)pick.token};
+}
+VH_DEVICE void put_pick(const BeamArgs &a, int s, int place, const BeamKey &key) {
+    const int beam = (int)(key.b >> 56), token = (int)(key.b & 0xffffff);
+    const int64_t at = (int64_t)s * a.picks + place;
+    a.tokens[at] = token;
+    a.parents[at] = beam;
+    a.new_scores[at] = (float)score_of(key.a);
+    if (a.new_ended) a.new_ended[at] = (a.ended && a.ended[s * a.B + beam]) || token == a.end_token ? 1 : 0;
+}
 
-// A workgroup joins a sequence's beams: stretch by stretch candidates beside the best
-// so far, sorted.
-static __global__ __launch_bounds__(512) void beam_join_kernel(BeamArgs a) {
-    __shared__ BeamKey keys[BS_JOIN];
-    __shared__ double lse[BS_MAX_BEAMS];
-    __shared__ int state[BS_MAX_BEAMS];  // 0: as it is, 1: no candidate but -inf, 2: ended
+constexpr int BS_JOIN = 1024;    // threads of the join, and candidates that it sorts at once
+constexpr int BS_LISTS = 512;    // lists whose heads are compared with one another
+constexpr int BS_LEFT = 4096;    // candidates that those leave, at most: picks of `picks` lists
+
+// A workgroup joins a sequence's beams.  Every list is in order, so with `need` of the
+// lists' candidates at place r at or before a key, need (r + 1) = picks, only candidates
+// at or before it count: those of at most `need` lists with r = 0, else of fewer lists
+// than picks.  They are ranked by counting.  More lists than BS_LISTS are sorted stretch
+// by stretch beside the best so far.
+static __global__ __launch_bounds__(BS_JOIN) void beam_join_kernel(BeamArgs a) {
+    __shared__ __align__(16) BeamKey keys[BS_LEFT];
+    __shared__ BeamState beams[BS_MAX_BEAMS];
+    __shared__ BeamKey limit;
+    __shared__ int left;
     const int s = (int)blockIdx.x, tid = (int)threadIdx.x;
-    if (tid < a.B) {
-        const int row = s * a.B + tid;
-        const float score = a.scores[row];
+    // a beam's 16 lanes (a beam after the other): the logarithm of its sum
+    if (tid == 0) {
+        left = 0;
+        limit = {~0ull, ~0ull};
+    }
+    for (int b0 = 0; b0 < a.B; b0 += BS_JOIN / 16) {
+        const int b = b0 + tid / 16, lane = tid % 16;
+        if (b >= a.B) break;
+        const int row = s * a.B + b;
         int st = a.ended && a.ended[row] ? 2 : 0;
         double l = 0.0;
         if (!st) {
             const char *p = a.parts + (int64_t)row * a.stretches * a.part_bytes;
             float top = -INFINITY;
-            for (int i = 0; i < a.stretches; i++) top = fmaxf(top, reinterpret_cast<const BeamPart *>(p + (int64_t)i * a.part_bytes)->top);
             double sum = 0.0;
-            for (int i = 0; i < a.stretches; i++) {
-                const BeamPart *h = reinterpret_cast<const BeamPart *>(p + (int64_t)i * a.part_bytes);
-                sum += h->top == -INFINITY ? h->sum : h->sum * exp((double)h->top - (double)top);
+            for (int i = lane; i < a.stretches; i += 16) {
+                const BeamPart h = *reinterpret_cast<const BeamPart *>(p + (int64_t)i * a.part_bytes);
+                const float up = fmaxf(top, h.top);
+                // a stretch of nothing but -inf adds nothing, a NaN stays
+                sum = (top == -INFINITY ? sum : sum * exp((double)top - (double)up)) +
+                      (h.top == -INFINITY ? h.sum : h.sum * exp((double)h.top - (double)up));
+                top = up;
             }
-            l = (double)top + log(sum);
+            float all = top;
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor(all, o, 16));
+            if (top != -INFINITY) sum *= exp((double)top - (double)all);
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 16);
+            l = (double)all + log(sum);
             if (!(fabs(l) < INFINITY)) st = 1;
         }
-        if (!(fabsf(score) < INFINITY)) st = 1;
-        lse[tid] = l;
-        state[tid] = st;
+        if (!(fabsf(a.scores[row]) < INFINITY)) st = 1;
+        if (lane == 0) beams[b] = {l, st};
     }
     __syncthreads();
-    const int per_beam = a.stretches * a.picks;
-    const int all = a.B * per_beam;
+    const int lists = a.B * a.stretches, per_beam = a.stretches * a.picks, all = a.B * per_beam;
+    if (lists <= BS_LISTS) {
+        const int place = (a.picks + lists - 1) / lists - 1, need = (a.picks + place) / (place + 1);
+        if (tid < lists) {
+            const int beam = tid / a.stretches;
+            keys[tid] = candidate(a, s, beam, tid % a.stretches * a.picks + place, beams[beam]);
+        }
+        __syncthreads();
+        if (tid < lists) {
+            const BeamKey mine = keys[tid];
+            int rank = 0;
+            for (int i = 0; i < lists; i++) rank += key_less(keys[i], mine) ? 1 : 0;
+            if (rank == need - 1 && ~mine.a) limit = mine;  // fewer than need: no limit
+        }
+        __syncthreads();
+        const BeamKey most = limit;
+        for (int e = tid; e < all; e += BS_JOIN) {
+            const int beam = e / per_beam;
+            const BeamKey key = candidate(a, s, beam, e - beam * per_beam, beams[beam]);
+            if (~key.a && !key_less(most, key)) keys[atomicAdd(&left, 1)] = key;  // in any order: ranked below
+        }
+        __syncthreads();
+        const int n = left;
+        for (int i = tid; i < n; i += BS_JOIN) {
+            const BeamKey mine = keys[i];
+            int rank = 0;
+            for (int k = 0; k < n; k++) rank += key_less(keys[k], mine) ? 1 : 0;
+            if (rank < a.picks) put_pick(a, s, rank, mine);
+        }
+        return;
+    }
     const BeamKey none{~0ull, ~0ull};
     int held = 0;  // the best so far, in front
     for (int done = 0; done < all;) {
         const int take = min(all - done, BS_JOIN - held);
-        int size = 64;
-        while (size < held + take) size *= 2;
-        for (int i = tid; i < size - held; i += 512) {
-            BeamKey key = none;
-            const int e = done + i;
-            if (i < take) {
-                const int beam = e / per_beam, in = e % per_beam, row = s * a.B + beam;
-                const double score = (double)a.scores[row];
-                if (state[beam]) {
-                    // the end token with the score as it is, then the others in order
-                    int token = in;
-                    double v = -INFINITY;
-                    if (state[beam] == 2) {
-                        token = in == 0 ? a.end_token : in - 1 < a.end_token ? in - 1 : in;
-                        if (in == 0) v = score;
-                    }
-                    if (in < a.picks && token < a.V) key = {score_down(v), (uint64_t)beam << 56 | (uint64_t)token};
-                } else {
-                    const char *p = a.parts + ((int64_t)row * a.stretches + in / a.picks) * a.part_bytes;
-                    const BeamPick pick = reinterpret_cast<const BeamPick *>(p + sizeof(BeamPart))[in % a.picks];
-                    if (pick.token >= 0) {
-                        const double v = score + ((double)pick.x - lse[beam]);
-                        const uint32_t down = v == -INFINITY ? 0u : ~ordered(pick.x);
-                        key = {score_down(v), (uint64_t)beam << 56 | (uint64_t)down << 24 | (uint64_t)pick.token};
-                    }
-                }
-            }
-            keys[held + i] = key;
+        for (int i = tid; i < BS_JOIN - held; i += BS_JOIN) {
+            const int e = done + i, beam = e / per_beam;
+            keys[held + i] = i < take ? candidate(a, s, beam, e - beam * per_beam, beams[beam]) : none;
         }
         __syncthreads();
-        for (int k = 2; k <= size; k *= 2)
+        for (int k = 2; k <= BS_JOIN; k *= 2)
             for (int j = k / 2; j > 0; j /= 2) {
-                for (int i = tid; i < size / 2; i += 512) {
-                    const int lo = i / j * 2 * j + i % j, hi = lo + j;
+                if (tid < BS_JOIN / 2) {
+                    const int lo = tid / j * 2 * j + tid % j, hi = lo + j;
                     const bool up = (lo & k) == 0;
                     const BeamKey x = keys[lo], y = keys[hi];
                     if (key_less(y, x) == up) {
@@ -370,15 +473,7 @@ static __global__ __launch_bounds__(512) void beam_join_kernel(BeamArgs a) {
         done += take;
         held = min(a.picks, held + take);
     }
-    if (tid < a.picks) {
-        const BeamKey key = keys[tid];
-        const int beam = (int)(key.b >> 56), token = (int)(key.b & 0xffffff);
-        const int64_t at = (int64_t)s * a.picks + tid;
-        a.tokens[at] = token;
-        a.parents[at] = beam;
-        a.new_scores[at] = (float)score_of(key.a);
-        if (a.new_ended) a.new_ended[at] = (a.ended && a.ended[s * a.B + beam]) || token == a.end_token ? 1 : 0;
-    }
+    if (tid < a.picks) put_pick(a, s, tid, keys[tid]);
 }
 
 }  // namespace vh

@@ -15,8 +15,8 @@
 // Over int8 pages keys and values are whole numbers, exact in fp16 (from the byte by a
 // permute and an addition: 0x6400 + u is 1024 + u); a row of q' enters as fp16 times a
 // power of two (its largest just below 2^14, so 2^-25 of that is what a small one is
-// off by), the block's scale of keys as a factor of the scores.  P enters times the
-// block's scale of values over the largest one so far, times 2^14.  fp32 out: q' and P
+// off by), the block's scale of keys as a factor of the scores.  P, up to 2^4, enters
+// times the block's scale of values over the largest one so far, times 2^10.  fp32 out: q' and P
 // in two fp16 values each.  Over bf16 pages: bf16, fp32 out: three bf16 values each.
 //
 // Bound by HBM for single tokens: the cache is read once.
@@ -38,7 +38,8 @@ struct CacheAttentionArgs {
     const int *query_lengths, *key_lengths, *start;
     int S, H, group, Lq;   // group: query heads of a key head
     int most, causal;
-    float scale2;          // scale log2(e)
+    float scale2;          // |scale| log2(e), at least the smallest normal number
+    int negative;          // the scale is: q' is turned instead
     int tiles;             // workgroups of a (sequence, key head)'s rows
     int parts, piece;      // pieces of the keys, and blocks of one
     float *part_o;         // [parts][S][Lq][H][D]
@@ -139,48 +140,22 @@ struct RawBlocks {
     }
 };
 
-// 8 dims of a query from d on, turned to its position.
-template <typename T>
-VH_DEVICE void load_query8(const Rotation &r, const T *q, const float *cs, int d, float (&x)[8]) {
-    load_n<8>(q + d, x);
-    if (!r.table || d >= r.dim) return;
-    if (!cs) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = __builtin_nanf("");
-        return;
-    }
-    if (r.interleaved) {
-        float c[8];
-        load_n<8>(cs + d, c);
-#pragma unroll
-        for (int e = 0; e < 4; e++) turn_pair(x[2 * e], x[2 * e + 1], c[2 * e], c[2 * e + 1]);
-        return;
-    }
-    const int half = r.dim / 2;
-    const bool second = d >= half;
-    const int pair = second ? d - half : d;
-    float c[16], y[8];
-    load_n<16>(cs + 2 * pair, c);
-    load_n<8>(q + (second ? pair : d + half), y);
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        if (second) turn_pair(y[e], x[e], c[2 * e], c[2 * e + 1]);
-        else turn_pair(x[e], y[e], c[2 * e], c[2 * e + 1]);
-    }
-}
-
 VH_DEVICE float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+constexpr float FLT_LEAST = 0x1p-126f;
+constexpr float LAZY = 4.0f;  // P up to 2^LAZY: times P_SCALE it is fp16's
 
 // SPLIT: a workgroup's four waves share the rows, each every fourth step of the keys,
 // and join; else each wave has rows of its own.
 template <typename T, int D, bool I8, int RG, int KB, bool SPLIT>
-static __global__ __launch_bounds__(256) void cache_attention_kernel(CacheAttentionArgs a) {
+static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAttentionArgs a) {
     using B = BlockShape<D, I8>;
     using Op = Operand16<I8>;
-    constexpr int DT = B::DT, QS = D / 32, N = sizeof(T) == 2 ? 1 : I8 ? 2 : 3;
+    // of q' and P: bf16 out one operand, but two where the cache's bytes are what takes the
+    // time; fp32 out as many as 22 bits and more take
+    constexpr int DT = B::DT, QS = D / 32, N = sizeof(T) == 2 ? (SPLIT && !I8 ? 2 : 1) : I8 ? 2 : 3;
     constexpr int WAVES = SPLIT ? 4 : 1, ROWS = 16 * RG * (SPLIT ? 1 : 4);
     constexpr int PER_FETCH = 64 / KB;
-    constexpr float P_SCALE = I8 ? 0x1p14f : 1.0f;
+    constexpr float P_SCALE = I8 ? 0x1p10f : 1.0f;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int i = lane & 15, g = lane >> 4;
     int pair, task;
@@ -200,39 +175,46 @@ static __global__ __launch_bounds__(256) void cache_attention_kernel(CacheAttent
     const bool any = row0 < rows && row0 / a.group < qlen;
     const int upto = any ? sees(last_token) : 0, all_see = any ? sees(row0 / a.group) : 0;
 
-    // the wave's rows as columns
+    // the wave's rows as columns, made when the first keys are asked for
     typename Op::type qf[RG][QS][N];
     float factor[RG];  // of the scores, in powers of two
     int limit[RG];     // keys that the lane's row sees
+    auto prepare_rows = [&] {
 #pragma unroll
-    for (int rg = 0; rg < RG; rg++) {
-        const int row = min(row0 + 16 * rg + i, rows - 1), token = row / a.heads;
-        const T *q = reinterpret_cast<const T *>(a.q + s * a.qs[0] + token * a.qs[1] +
-                                                 (head * a.group + row - token * a.group) * a.qs[2]);
-        const float *cs = a.r.table ? rotation_row(a.r, start + token) : nullptr;
-        limit[rg] = sees(token);
-        float x[QS][8];
-        float top = 0.0f;
+        for (int rg = 0; rg < RG; rg++) {
+            const int row = min(row0 + 16 * rg + i, rows - 1), token = row / a.heads;
+            const T *q = reinterpret_cast<const T *>(a.q + s * a.qs[0] + token * a.qs[1] +
+                                                     (head * a.group + row - token * a.group) * a.qs[2]);
+            const float *cs = a.r.table ? rotation_row(a.r, start + token) : nullptr;
+            limit[rg] = sees(token);
+            float x[QS][8];
+            float top = 0.0f;
 #pragma unroll
-        for (int m = 0; m < QS; m++) {
-            load_query8(a.r, q, cs, 64 * (m / 2) + 16 * g + 8 * (m % 2), x[m]);
+            for (int m = 0; m < QS; m++) {
+                load_turned8(a.r, q, cs, 64 * (m / 2) + 16 * g + 8 * (m % 2), x[m]);
 #pragma unroll
-            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[m][e]));
+                for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[m][e]));
+            }
+            factor[rg] = a.scale2;
+            if (a.negative)
+#pragma unroll
+                for (int m = 0; m < QS; m++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[m][e] = -x[m][e];
+            if constexpr (I8) {
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const int e2 = h2_exponent(top);
+#pragma unroll
+                for (int m = 0; m < QS; m++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[m][e] = __builtin_ldexpf(x[m][e], e2);
+                factor[rg] = __builtin_ldexpf(a.scale2, -e2);
+            }
+#pragma unroll
+            for (int m = 0; m < QS; m++) split_n<I8, N>(x[m], qf[rg][m]);
         }
-        factor[rg] = a.scale2;
-        if constexpr (I8) {
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const int e2 = h2_exponent(top);
-#pragma unroll
-            for (int m = 0; m < QS; m++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) x[m][e] = __builtin_ldexpf(x[m][e], e2);
-            factor[rg] = __builtin_ldexpf(a.scale2, -e2);
-        }
-#pragma unroll
-        for (int m = 0; m < QS; m++) split_n<I8, N>(x[m], qf[rg][m]);
-    }
+    };
 
     floatx4 o[RG][DT];
     float m_run[RG], l_run[RG];
@@ -332,36 +314,60 @@ static __global__ __launch_bounds__(256) void cache_attention_kernel(CacheAttent
                         st.v.w[b][u][d] &= keep;
                     }
         }
+        // scores to powers of two, s f; their largest in this lane
+        float f[RG][KB], top[RG];
+        bool over = false;
+#pragma unroll
+        for (int rg = 0; rg < RG; rg++) {
+            top[rg] = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < KB; b++) {
+                f[rg][b] = factor[rg];
+                if constexpr (I8) {
+                    f[rg][b] *= st.sk[b];
+                    if (f[rg][b] < FLT_LEAST) f[rg][b] = FLT_LEAST;  // 0 times -inf is no number; a NaN stays
+                }
+                if (!whole)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if ((st.there >> b & 1) == 0 || first + 16 * b + 4 * g + r >= limit[rg]) x[rg][b][r] = -INFINITY;
+                const float most = fmaxf(fmaxf(x[rg][b][0], x[rg][b][1]), fmaxf(x[rg][b][2], x[rg][b][3]));
+                top[rg] = fmaxf(top[rg], most * f[rg][b]);
+            }
+            over |= top[rg] > m_run[rg] + LAZY;
+        }
         float v_new = v_top;
-        float sv[KB];
-        if constexpr (I8) {
+        if constexpr (I8)
 #pragma unroll
             for (int b = 0; b < KB; b++) v_new = fmaxf(v_new, st.sv[b]);
-            const float inv = P_SCALE / v_new;
+        // The exponents' base follows the maximum only when that is 2^LAZY beyond it, and the
+        // values' unit the largest scale: then all that was summed is rescaled.
+        if (__ballot(over || v_new > v_top)) {
+            const float shrink = I8 ? v_top / v_new : 1.0f;
+            v_top = v_new;
+#pragma unroll
+            for (int rg = 0; rg < RG; rg++) {
+                float m = fmaxf(m_run[rg], top[rg]);
+                m = fmaxf(m, __shfl_xor(m, 16, 64));
+                m = fmaxf(m, __shfl_xor(m, 32, 64));
+                const float alpha = m == -INFINITY ? 0.0f : exp2_of(m_run[rg] - m);  // -inf - -inf is no number
+                m_run[rg] = m;
+                l_run[rg] *= alpha;
+                const float rescale = alpha * shrink;
+#pragma unroll
+                for (int t = 0; t < DT; t++) o[rg][t] *= rescale;
+            }
+        }
+        float sv[KB];
+        if constexpr (I8) {
+            const float inv = P_SCALE / v_top;
 #pragma unroll
             for (int b = 0; b < KB; b++) sv[b] = st.sv[b] * inv;
         }
-        const float shrink = I8 ? v_top / v_new : 1.0f;
-        v_top = v_new;
         typename Op::type pf[RG][KB / 2][N];
 #pragma unroll
         for (int rg = 0; rg < RG; rg++) {
-            float top = m_run[rg];
-#pragma unroll
-            for (int b = 0; b < KB; b++) {
-                const float f = I8 ? factor[rg] * st.sk[b] : factor[rg];
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    x[rg][b][r] *= f;
-                    if (!whole && ((st.there >> b & 1) == 0 || first + 16 * b + 4 * g + r >= limit[rg])) x[rg][b][r] = -INFINITY;
-                    top = fmaxf(top, x[rg][b][r]);
-                }
-            }
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float base = top == -INFINITY ? 0.0f : top;  // -inf - -inf is no number
-            const float alpha = exp2_of(m_run[rg] - base);
-            m_run[rg] = top;
+            const float base = m_run[rg] == -INFINITY ? 0.0f : m_run[rg];
             float sum = 0.0f;
 #pragma unroll
             for (int c = 0; c < KB / 2; c++) {
@@ -369,16 +375,13 @@ static __global__ __launch_bounds__(256) void cache_attention_kernel(CacheAttent
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const int b = 2 * c + e / 4;
-                    p[e] = exp2_of(x[rg][b][e % 4] - base);
+                    p[e] = exp2_of(__builtin_fmaf(x[rg][b][e % 4], f[rg][b], -base));
                     sum += p[e];
                     if constexpr (I8) p[e] *= sv[b];
                 }
                 split_n<I8, N>(p, pf[rg][c]);
             }
-            l_run[rg] = l_run[rg] * alpha + sum;
-            const float rescale = alpha * shrink;
-#pragma unroll
-            for (int t = 0; t < DT; t++) o[rg][t] *= rescale;
+            l_run[rg] += sum;
         }
 #pragma unroll
         for (int c = 0; c < KB / 2; c++)
@@ -392,10 +395,16 @@ static __global__ __launch_bounds__(256) void cache_attention_kernel(CacheAttent
             }
     };
 
-    Step st;
-    for (int step = 0; step < steps; step++) {
-        load(st, step);
-        compute(st, step);
+    // the next step's blocks are on their way while one is computed
+    Step even, odd;
+    if (steps > 0) load(even, 0);
+    prepare_rows();
+    for (int step = 0; step < steps; step += 2) {
+        if (step + 1 < steps) load(odd, step + 1);
+        compute(even, step);
+        if (step + 1 >= steps) break;
+        if (step + 2 < steps) load(even, step + 2);
+        compute(odd, step + 1);
     }
 
     // in the values' own units
@@ -476,40 +485,62 @@ static __global__ __launch_bounds__(256) void cache_attention_kernel(CacheAttent
     }
 }
 
-// Joins the pieces of the keys: DT dims of a row a thread.
+// Joins the pieces of the keys: 16 lanes a row, first for the pieces' statistics, then
+// for D / 16 dims each.
 template <typename T, int D>
 static __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttentionArgs a) {
-    constexpr int DT = D / 16;
-    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x, row = n / 16;
-    const int64_t rows = (int64_t)a.S * a.Lq * a.H;
+    constexpr int DT = D / 16, MOST = 4;  // pieces of a lane: 64 in all
+    const int64_t row = (int64_t)blockIdx.x * 16 + threadIdx.x / 16, rows = (int64_t)a.S * a.Lq * a.H;
     if (row >= rows) return;
-    const int d = (int)(n % 16) * DT;
-    const int s = (int)(row / ((int64_t)a.Lq * a.H)), in = (int)(row - (int64_t)s * a.Lq * a.H);
-    const int token = in / a.H, h = in % a.H;
+    const int lane = threadIdx.x & 15;
+    const uint32_t in_tokens = (uint32_t)(row / a.H);
+    const int h = (int)(row - (int64_t)in_tokens * a.H), s = (int)(in_tokens / (uint32_t)a.Lq), token = (int)(in_tokens % (uint32_t)a.Lq);
     const int qlen = a.query_lengths ? max(0, min(a.query_lengths[s], a.Lq)) : a.Lq;
     const int keys = a.key_lengths ? max(0, min(a.key_lengths[s], a.most)) : a.most;
     int64_t seen = token < qlen ? keys : 0;
     if (a.causal) seen = max((int64_t)0, min(seen, (a.start ? a.start[s] : 0) + (int64_t)token + 1));
-    const int parts = (int)((seen + (int64_t)a.piece * PC_BLOCK - 1) / ((int64_t)a.piece * PC_BLOCK));
+    const int piece = a.piece * PC_BLOCK, parts = (int)((seen + piece - 1) / piece);
+    float2 ml[MOST];
     float m = -INFINITY;
-    for (int p = 0; p < parts; p++) m = fmaxf(m, a.part_ml[p * rows + row].x);
-    float v[DT], l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < MOST; i++) {
+        ml[i] = {-INFINITY, 0.0f};
+        if (lane + 16 * i < parts) ml[i] = a.part_ml[(lane + 16 * i) * rows + row];
+        m = fmaxf(m, ml[i].x);
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 16));
+    float f[MOST], l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < MOST; i++) {
+        // of a piece that nothing was written for the weight is 0, and what is read there left out
+        f[i] = ml[i].y == 0.0f ? 0.0f : exp2_of(ml[i].x - m);
+        l += ml[i].y == 0.0f ? 0.0f : ml[i].y * f[i];
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) l += __shfl_xor(l, o, 16);
+    float v[DT];
 #pragma unroll
     for (int e = 0; e < DT; e++) v[e] = 0.0f;
-    for (int p = 0; p < parts; p++) {
-        const float2 ml = a.part_ml[p * rows + row];
-        if (ml.y == 0.0f) continue;  // nothing was written for it
-        const float f = exp2_of(ml.x - m);
-        l += ml.y * f;
-        float x[DT];
-        load_n<DT>(a.part_o + (p * rows + row) * D + d, x);
+    const float *from = a.part_o + row * D + DT * lane;
 #pragma unroll
-        for (int e = 0; e < DT; e++) v[e] += x[e] * f;
+    for (int i = 0; i < MOST; i++) {
+        for (int p0 = 16 * i; p0 < min(parts, 16 * i + 16); p0 += 4) {
+            float x[4][DT];
+#pragma unroll
+            for (int j = 0; j < 4; j++) load_n<DT>(from + min(p0 + j, parts - 1) * rows * D, x[j]);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float w = __shfl(f[i], p0 + j - 16 * i, 16);  // 0 beyond the pieces
+#pragma unroll
+                for (int e = 0; e < DT; e++) v[e] += w == 0.0f ? 0.0f : x[j][e] * w;
+            }
+        }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int e = 0; e < DT; e++) v[e] = inv == 0.0f ? 0.0f : v[e] * inv;
-    store_n<DT>(reinterpret_cast<T *>(a.out + s * a.os[0] + token * a.os[1] + h * a.os[2]) + d, v);
+    store_n<DT>(reinterpret_cast<T *>(a.out + s * a.os[0] + token * a.os[1] + h * a.os[2]) + DT * lane, v);
 }
 
 }  // namespace vh

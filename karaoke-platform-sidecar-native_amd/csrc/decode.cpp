@@ -258,7 +258,7 @@ static bool cache_rows_ok(const char *what, const vh_cache *c, const vh_cache_ro
 }
 
 static bool cache_rows_args(const char *what, const vh_cache *c, const vh_cache_rows *r, const void *k, const void *v,
-                            CacheRowsArgs &a, int64_t &groups) {
+                            bool append, CacheRowsArgs &a, int64_t &groups) {
     if (!paged_args(what, c, a.p) || !aligned16(what, {k, v})) return false;
     const int64_t size = type_bytes(r->type);
     a.k = const_cast<char *>(static_cast<const char *>(k));
@@ -269,10 +269,17 @@ static bool cache_rows_args(const char *what, const vh_cache *c, const vh_cache_
     a.lengths = r->lengths;
     a.length = r->length;
     // from the first block's last token on at worst
-    a.blocks = (int)(((int64_t)r->length + (r->start ? 2 * PC_BLOCK - 2 : PC_BLOCK - 1)) / PC_BLOCK);
-    a.tasks = (int64_t)c->sequences * a.blocks * 2 * c->kv_heads;
-    groups = (a.tasks + 3) / 4;
-    return groups_ok(what, groups);
+    const int64_t blocks = ((int64_t)r->length + (r->start ? 2 * PC_BLOCK - 2 : PC_BLOCK - 1)) / PC_BLOCK;
+    // a wave of an append takes up to 4 heads, while there are 32 waves a CU
+    a.heads = 1;
+    while (append && a.heads < 4 && a.heads < c->kv_heads && c->sequences * blocks * 2 * c->kv_heads / a.heads > 16384) a.heads *= 2;
+    const int64_t of_block = 2 * ((c->kv_heads + a.heads - 1) / a.heads), each = blocks * of_block, tasks = each * c->sequences;  // below 2^59
+    groups = (tasks + 3) / 4;
+    if (!groups_ok(what, groups)) return false;
+    a.tasks = (int)tasks;
+    a.per_sequence = divisor((uint32_t)each);
+    a.per_block = divisor((uint32_t)of_block);
+    return true;
 }
 
 template <typename T, int D, bool I8>
@@ -299,7 +306,7 @@ bool cache_append(hipStream_t s, const vh_cache *c, const vh_cache_rows *r, cons
         return false;
     }
     int64_t groups;
-    if (!cache_rows_args(what, c, r, k, v, a, groups) ||
+    if (!cache_rows_args(what, c, r, k, v, true, a, groups) ||
         !begins_apart(what, {c->pool}, {k, v, c->table, r->start, r->lengths, a.r.table}))
         return false;
     Scope sc(t, s, "cache_append");
@@ -314,7 +321,7 @@ bool cache_read(hipStream_t s, const vh_cache *c, const vh_cache_rows *r, void *
     if (!c->sequences || !r->length || (!k && !v)) return true;
     CacheRowsArgs a{};
     int64_t groups;
-    if (!cache_rows_args(what, c, r, k, v, a, groups) || !begins_apart(what, {k, v}, {c->pool, c->table, r->start, r->lengths}))
+    if (!cache_rows_args(what, c, r, k, v, false, a, groups) || !begins_apart(what, {k, v}, {c->pool, c->table, r->start, r->lengths}))
         return false;
     Scope sc(t, s, "cache_read");
     if (r->type == VH_TYPE_BF16) rows_dispatch<bf16>(s, c, a, groups, false);
@@ -363,18 +370,19 @@ struct CacheCut {
     int64_t pairs, grid;
 };
 constexpr int CQ_MAX_ROWS = 1 << 30;
-static int wave_groups(const vh_cache *c) { return c->head_dim == 64 ? 4 : 2; }
+constexpr int wave_groups(int type, int head_dim) { return (head_dim == 64 ? 4 : 2) / (type == VH_TYPE_BF16 ? 1 : 2); }
+constexpr int split_groups(int type, int head_dim) { return type == VH_TYPE_FP32 && head_dim == 128 ? 1 : 2; }
 static CacheCut cache_cut(const vh_cache *c, const vh_cache_queries *q) {
     CacheCut cut;
     const int rows = q->length * (q->heads / c->kv_heads);
     cut.split = rows <= 128;
-    cut.groups = cut.split ? (rows <= 16 ? 1 : 2) : wave_groups(c);
+    cut.groups = cut.split ? (rows <= 16 ? 1 : split_groups(q->type, c->head_dim)) : wave_groups(q->type, c->head_dim);
     const int per = 16 * cut.groups * (cut.split ? 1 : 4);
     cut.tiles = (rows + per - 1) / per;
     cut.pairs = (int64_t)c->sequences * c->kv_heads;
     const int64_t base = cut.pairs * cut.tiles;
     const int blocks = std::max<int>(1, (int)((std::min<int64_t>(q->most_keys, capacity(c)) + PC_BLOCK - 1) / PC_BLOCK));
-    const int64_t want = std::min<int64_t>((cut.split ? 1024 : 512) / std::max<int64_t>(base, 1), blocks / 32);
+    const int64_t want = std::min<int64_t>(1024 / std::max<int64_t>(base, 1), blocks / 32);
     const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(want, 64));
     cut.piece = ((blocks + parts - 1) / parts + 15) / 16 * 16;  // whole steps of all waves
     cut.parts = (blocks + cut.piece - 1) / cut.piece;
@@ -417,10 +425,11 @@ size_t cache_workspace_bytes(const vh_cache *c, const vh_cache_queries *q) {
 
 template <typename T, int D, bool I8>
 static void attention_launch(hipStream_t s, const CacheAttentionArgs &a, const CacheCut &cut) {
+    constexpr int TYPE = sizeof(T) == 2 ? VH_TYPE_BF16 : VH_TYPE_FP32;
     const dim3 grid((unsigned)cut.grid);
-    if (!cut.split) hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, D == 64 ? 4 : 2, 2, false>), grid, dim3(256), 0, s, a);
-    else if (cut.groups == 2) hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, 2, 2, true>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, 1, I8 || D == 64 ? 4 : 2, true>), grid, dim3(256), 0, s, a);
+    if (!cut.split) hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, wave_groups(TYPE, D), 2, false>), grid, dim3(256), 0, s, a);
+    else if (cut.groups > 1) hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, split_groups(TYPE, D), 2, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, 1, I8 && D == 64 ? 4 : 2, true>), grid, dim3(256), 0, s, a);
     if (cut.parts == 1) return;
     const int64_t rows = (int64_t)a.S * a.Lq * a.H;
     hipLaunchKernelGGL((cache_join_kernel<T, D>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, a);
@@ -470,7 +479,8 @@ bool cache_attention(hipStream_t s, const vh_cache *c, const vh_cache_queries *q
     a.Lq = q->length;
     a.most = (int)std::min<int64_t>(q->most_keys, capacity(c));
     a.causal = q->causal ? 1 : 0;
-    a.scale2 = q->scale * 1.4426950408889634f;
+    a.scale2 = std::max(fabsf(q->scale) * 1.4426950408889634f, 0x1p-126f);
+    a.negative = q->scale < 0.0f;
     a.tiles = cut.tiles;
     a.parts = cut.parts;
     a.piece = cut.piece;
@@ -484,17 +494,21 @@ bool cache_attention(hipStream_t s, const vh_cache *c, const vh_cache_queries *q
 
 // --------------------------------------------------------------- beam search
 // A stretch of a beam's logits, the vectors of 8 that a thread takes of it (of bf16 up
-// to 8, of fp32 4: the same registers).
+// to 8, of fp32 4: the same registers); shorter stretches while there are fewer than
+// two workgroups a CU.
 struct BeamCut {
     int vectors, stretch, stretches, part_bytes;
 };
+constexpr int64_t BS_ENOUGH = 512;
 static BeamCut beam_cut(const vh_beam *b) {
-    const int most = b->type == VH_TYPE_BF16 ? 8 : 4, one = BS_THREADS * 8;
+    constexpr int ONE = BS_THREADS * 8;
+    const int64_t rows = std::max<int64_t>(1, (int64_t)b->sequences * b->beams);
     BeamCut cut;
-    cut.stretches = (b->vocab + most * one - 1) / (most * one);
-    const int each = (b->vocab + cut.stretches - 1) / cut.stretches;
-    for (cut.vectors = 1; cut.vectors * one < each;) cut.vectors *= 2;
-    cut.stretch = (each + 7) / 8 * 8;
+    cut.vectors = b->type == VH_TYPE_BF16 ? 8 : 4;
+    while (cut.vectors > 1 && b->vocab <= cut.vectors / 2 * ONE) cut.vectors /= 2;
+    while (cut.vectors > 1 && rows * ((b->vocab + cut.vectors * ONE - 1) / (cut.vectors * ONE)) < BS_ENOUGH) cut.vectors /= 2;
+    cut.stretches = (b->vocab + cut.vectors * ONE - 1) / (cut.vectors * ONE);
+    cut.stretch = ((b->vocab + cut.stretches - 1) / cut.stretches + 7) / 8 * 8;
     cut.part_bytes = (int)(sizeof(BeamPart) + (b->picks + 1) / 2 * 2 * sizeof(BeamPick));
     return cut;
 }
@@ -517,7 +531,7 @@ static bool beam_ok(const char *what, const vh_beam *b) {
             set_error("%s: the logits' strides %lld, %lld: none negative", what, (long long)b->strides[0], (long long)b->strides[1]);
             return false;
         }
-    return groups_ok(what, (int64_t)b->sequences * b->beams * beam_cut(b).stretches * (BS_THREADS / 256));
+    return groups_ok(what, (int64_t)b->sequences * b->beams * beam_cut(b).stretches);
 }
 static size_t beam_bytes(const vh_beam *b) {
     const BeamCut cut = beam_cut(b);
@@ -579,7 +593,7 @@ bool beam_select(hipStream_t s, const vh_beam *b, const void *logits, const floa
     if (b->type == VH_TYPE_BF16) beam_launch<bf16>(s, a, cut.vectors, groups);
     else beam_launch<float>(s, a, cut.vectors, groups);
     if (!sync_debug(s, "beam_stretch_kernel")) return false;
-    hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)a.S), dim3(512), 0, s, a);
+    hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)a.S), dim3(BS_JOIN), 0, s, a);
     return sync_debug(s, "beam_join_kernel");
 }
 

@@ -33,8 +33,6 @@ struct BlockShape {
     static constexpr int BYTES = 2 * PART;
     static constexpr int UNITS = PART / 1024;
     static constexpr int DT = D / 16;
-    VH_DEVICE static int key_dim(int u, int g) { return 64 * (u * C / 16) + 16 * g + u * C % 16; }
-    VH_DEVICE static int value_dim(int u, int i) { return DT * i + C / 4 * u; }
 };
 
 // Page of a sequence's block; -1: none.
@@ -58,26 +56,28 @@ struct CacheRowsArgs {
     char *k, *v;
     int64_t ks[3], vs[3];  // bytes
     const int *start, *lengths;
-    int length, blocks;    // rows of a sequence, and blocks that they may touch
-    int64_t tasks;         // sequences * blocks * 2 * kv, a wave each
+    int length, tasks;     // rows of a sequence; waves
+    int heads;             // of a task
+    Divisor per_sequence, per_block;  // tasks of a sequence and of a block, 2 * ceil(kv / heads)
 };
 
-// A wave's task: 16 tokens' keys or values of a head.
+// A wave's task: 16 tokens' keys or values of one or several heads.
 struct CacheTask {
-    int s, head, values;
+    int s, head, heads, values;
     int64_t first, start;  // positions of the block's first token and of row 0
     int rows, page, slot;
-    VH_DEVICE bool take(const CacheRowsArgs &a, int wave) {
-        int64_t t = (int64_t)blockIdx.x * 4 + wave;
-        if (t >= a.tasks) return false;
-        const int64_t b = t / (2 * a.p.kv);
-        const int in = (int)(t - b * 2 * a.p.kv);
-        values = in >= a.p.kv;
-        head = values ? in - a.p.kv : in;
-        s = (int)(b / a.blocks);
+    VH_DEVICE bool take(const CacheRowsArgs &a) {
+        const uint32_t t = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+        if (t >= (uint32_t)a.tasks) return false;
+        const uint32_t sq = t / a.per_sequence, in = t - sq * a.per_sequence.d, block_of_call = in / a.per_block;
+        const int part = (int)(in - block_of_call * a.per_block.d), groups = (int)a.per_block.d / 2;
+        values = part >= groups;
+        head = (values ? part - groups : part) * a.heads;
+        heads = min(a.heads, a.p.kv - head);
+        s = (int)sq;
         start = max(0, a.start ? __builtin_amdgcn_readfirstlane(a.start[s]) : 0);
         rows = a.lengths ? max(0, min(__builtin_amdgcn_readfirstlane(a.lengths[s]), a.length)) : a.length;
-        const uint32_t block = (uint32_t)(start / PC_BLOCK + (b - (int64_t)s * a.blocks));
+        const uint32_t block = (uint32_t)(start / PC_BLOCK) + block_of_call;
         first = (int64_t)block * PC_BLOCK;
         const uint32_t column = block / a.p.blocks;
         slot = (int)(block - column * a.p.blocks.d);
@@ -91,6 +91,27 @@ VH_DEVICE uint32_t wave_umax(uint32_t v) {
     for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
     return v;
 }
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// The whole number next to x f (at most 127 and a half), plus 128, in the low byte: a
+// sum with 3 * 2^22 + 128 is rounded there.
+VH_DEVICE uint32_t number_of(float x, float f) {
+#pragma clang fp contract(off)
+    const float q = x * f;
+    return __float_as_uint(q + 12583040.0f);
+}
+VH_DEVICE uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_amdgcn_perm(b, a, 0x0c0c0400u) | __builtin_amdgcn_perm(d, c, 0x04000c0cu);
+}
+
+// A block's tokens: held before the call, in it, or (after it) none.
+struct TokenRange {
+    int lo, hi;
+    VH_DEVICE bool earlier(int t) const { return t < lo; }
+    VH_DEVICE bool of_call(int t) const { return t >= lo && t < hi; }
+};
+
 // LDS accesses of the wave's lanes before and after stay in that order (the hardware
 // keeps a wave's; this keeps the compiler's).
 VH_DEVICE void cache_wave_order() {
@@ -98,190 +119,211 @@ VH_DEVICE void cache_wave_order() {
     __builtin_amdgcn_wave_barrier();
 }
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
-// How a block's numbers come from its rows.
-struct Quant {
-    float inv, earlier;  // 1 / scale, and what the numbers of earlier tokens are multiplied by
-    VH_DEVICE static uint32_t number(float q) { return (uint32_t)((int)fminf(fmaxf(__builtin_rintf(q), -127.0f), 127.0f) + 128); }
-    VH_DEVICE uint32_t of(float x) const { return number(x * inv); }
-    VH_DEVICE uint32_t again(uint32_t byte) const { return number((float)((int)byte - 128) * earlier); }
-};
-// A block's token: held before the call, in it, or (after it) none.
-struct TokenRange {
-    int lo, hi;
-    VH_DEVICE bool earlier(int t) const { return t < lo; }
-    VH_DEVICE bool of_call(int t) const { return t >= lo && t < hi; }
-};
-
-// Rows into a block.  A wave turns its rows, in units of 16 dims a lane, into a tile
-// of LDS, finds the scale, and writes the block from the tile in the block's order,
-// earlier tokens rescaled in place.
+// Rows into a block.  A wave's lanes take units of 16 dims of its tokens, beside each
+// other in a row, and turn them by a table row's part that stays in registers from head
+// to head; by way of a tile of LDS they take them up in the block's order, and write.
+// The next head's rows are on their way meanwhile.  Earlier tokens of a block that is not
+// new are rescaled in place.
 template <typename T, int D, bool I8>
 static __global__ __launch_bounds__(256) void cache_append_kernel(CacheRowsArgs a) {
     using B = BlockShape<D, I8>;
-    constexpr int ROW = D + 4;  // floats: rows four banks apart
+    constexpr int DT = B::DT, NU = D / 64, ROW = D + 4;  // units of a lane; floats of a tile's row, four banks apart
+    typedef typename Elements<T, 8>::type Raw;
     __shared__ __align__(16) float tiles[4][PC_BLOCK * ROW];
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    float *tile = tiles[threadIdx.x >> 6];
     CacheTask w;
-    if (!w.take(a, wave) || w.page < 0) return;
+    if (!w.take(a) || w.page < 0) return;
     const TokenRange tokens{(int)max(w.start - w.first, (int64_t)0), (int)min(w.start + w.rows - w.first, (int64_t)PC_BLOCK)};
     if (tokens.lo >= tokens.hi) return;
-    float *tile = tiles[wave];
     const int64_t *strides = w.values ? a.vs : a.ks;
     const char *rows = (w.values ? a.v : a.k) + w.s * strides[0] + (w.first - w.start) * strides[1] + w.head * strides[2];
-    const int turned = w.values || !a.r.table ? 0 : a.r.dim / 16;
-    const int half = a.r.dim / 2;
-    uint32_t top = 0;
-#pragma unroll
-    for (int n = 0; n < D / 64; n++) {
-        const int t = (lane + 64 * n) / (D / 16), u = (lane + 64 * n) % (D / 16);
-        if (!tokens.of_call(t)) continue;
-        const T *x = reinterpret_cast<const T *>(rows + t * strides[1]);
-        float lo[8], hi[8];
-        int at = 16 * u, beside = 16 * u + 8;
-        if (u < turned && !a.r.interleaved) {
-            at = 8 * u;
-            beside = half + 8 * u;
-        }
-        load_n<8>(x + at, lo);
-        load_n<8>(x + beside, hi);
-        if (u < turned) {
-            const float *cs = rotation_row(a.r, w.first + t);
-            float c[16];
-            if (cs) load_n<16>(cs + 16 * u, c);
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                if (!cs) lo[e] = hi[e] = __builtin_nanf("");
-                else if (!a.r.interleaved) turn_pair(lo[e], hi[e], c[2 * e], c[2 * e + 1]);
-            }
-            if (cs && a.r.interleaved) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    turn_pair(lo[2 * e], lo[2 * e + 1], c[2 * e], c[2 * e + 1]);
-                    turn_pair(hi[2 * e], hi[2 * e + 1], c[8 + 2 * e], c[8 + 2 * e + 1]);
-                }
-            }
-        }
-        float *to = tile + t * ROW;
-#pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-            st4(to + at + e, (floatx4){lo[e], lo[e + 1], lo[e + 2], lo[e + 3]});
-            st4(to + beside + e, (floatx4){hi[e], hi[e + 1], hi[e + 2], hi[e + 3]});
-        }
-        if constexpr (I8)
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                top = max(top, max(__float_as_uint(lo[e]) & 0x7fffffffu, __float_as_uint(hi[e]) & 0x7fffffffu));
-    }
-    cache_wave_order();
-    Quant q{};
-    if constexpr (I8) {
-        top = wave_umax(top);
-        float *held = scale_at(a.p, w.page, w.head, w.slot) + w.values;
-        const float old = tokens.lo ? *held : 0.0f;
-        float scale = fmaxf(__uint_as_float(top) * (1.0f / 127.0f), 0x1p-100f);
-        if (tokens.lo && !(old <= scale)) scale = old;
-        if (top >= 0x7f800000u) scale = __builtin_nanf("");
-        q.inv = 1.0f / scale;
-        q.earlier = old * q.inv;
-        cache_wave_order();  // every lane has the old one
-        if (lane == 0) *held = scale;
-    }
-    char *block = block_at(a.p, w.page, w.head, w.slot, B::BYTES) + w.values * B::PART + 16 * lane;
-    const int i = lane & 15, g = lane >> 4;
-#pragma unroll
-    for (int u = 0; u < B::UNITS; u++) {
-        u32x4 *place = reinterpret_cast<u32x4 *>(block + 1024 * u);
-        u32x4 old = {0, 0, 0, 0}, now;
-        if (tokens.lo) old = *place;
-        // element e of the lane's 16 bytes: its token and its place in the tile
-        const int d0 = w.values ? B::value_dim(u, i) : B::key_dim(u, g);
-        float x[B::C];
-        if (w.values) {
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                float v[B::C / 4];
-                load_lds<B::C / 4>(tile + (4 * g + r) * ROW + d0, v);
-#pragma unroll
-                for (int e = 0; e < B::C / 4; e++) x[4 * e + r] = v[e];
-            }
-        } else {
-            load_lds<B::C>(tile + i * ROW + d0, x);
-        }
-#pragma unroll
-        for (int d = 0; d < 4; d++) {
-            uint32_t word = 0;
-            constexpr int N = I8 ? 4 : 2, BITS = 32 / N;
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                const int at = N * d + e, t = w.values ? 4 * g + at % 4 : i;
-                const uint32_t before = old[d] >> (BITS * e) & ((1ull << BITS) - 1);
-                uint32_t value;
-                if constexpr (I8)
-                    value = tokens.of_call(t) ? q.of(x[at]) : tokens.earlier(t) ? q.again(before) : 128u;
-                else
-                    value = tokens.of_call(t) ? (uint32_t)__builtin_bit_cast(uint16_t, (bf16)x[at]) : tokens.earlier(t) ? before : 0u;
-                word |= value << (BITS * e);
-            }
-            now[d] = word;
-        }
-        *place = now;
-    }
-}
 
-// A block's rows, by way of the same tile.
-template <typename T, int D, bool I8>
-static __global__ __launch_bounds__(256) void cache_read_kernel(CacheRowsArgs a) {
-    using B = BlockShape<D, I8>;
-    constexpr int ROW = D + 4;
-    __shared__ __align__(16) float tiles[4][PC_BLOCK * ROW];
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
-    CacheTask w;
-    if (!w.take(a, wave)) return;
-    char *out = w.values ? a.v : a.k;
-    if (!out) return;
-    float *tile = tiles[wave];
-    const bool any = w.page >= 0 && w.first < w.start + w.rows;
-    if (any) {
-        const char *block = block_at(a.p, w.page, w.head, w.slot, B::BYTES) + w.values * B::PART + 16 * lane;
-        const float scale = I8 ? scale_at(a.p, w.page, w.head, w.slot)[w.values] : 1.0f;
-        const int i = lane & 15, g = lane >> 4;
+    // the lane's units: which token, and where its two times 8 dims are
+    bool mine[NU], turned[NU], off_table[NU];
+    int at[NU], beside[NU];
+    float cs[NU][16];
+    const T *from[NU];
+#pragma unroll
+    for (int n = 0; n < NU; n++) {
+        const int t = (lane + 64 * n) / (D / 16), u = (lane + 64 * n) % (D / 16);
+        mine[n] = tokens.of_call(t);
+        turned[n] = !w.values && a.r.table && u < a.r.dim / 16;
+        at[n] = 16 * u;
+        beside[n] = 16 * u + 8;
+        if (turned[n] && !a.r.interleaved) {
+            at[n] = 8 * u;
+            beside[n] = a.r.dim / 2 + 8 * u;
+        }
+        from[n] = reinterpret_cast<const T *>(rows + (mine[n] ? t : tokens.lo) * strides[1]);
+        off_table[n] = false;
+        if (turned[n]) {
+            const float *row = rotation_row(a.r, w.first + t);
+            off_table[n] = !row;
+            load_n<16>((row ? row : a.r.table) + 16 * u, cs[n]);
+        }
+    }
+    Raw lo[NU], hi[NU];
+    auto load = [&](int head) {
+#pragma unroll
+        for (int n = 0; n < NU; n++) {
+            const T *x = reinterpret_cast<const T *>(reinterpret_cast<const char *>(from[n]) + head * strides[2]);
+            lo[n] = *reinterpret_cast<const Raw *>(x + at[n]);
+            hi[n] = *reinterpret_cast<const Raw *>(x + beside[n]);
+        }
+    };
+    load(0);
+    const bool whole = tokens.lo == 0 && tokens.hi == PC_BLOCK;
+    for (int h = 0; h < w.heads; h++) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int n = 0; n < NU; n++) {
+            float x[8], y[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = (float)lo[n][e], y[e] = (float)hi[n][e];
+            if (turned[n]) {
+                if (a.r.interleaved) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        turn_pair(x[2 * e], x[2 * e + 1], cs[n][2 * e], cs[n][2 * e + 1]);
+                        turn_pair(y[2 * e], y[2 * e + 1], cs[n][8 + 2 * e], cs[n][9 + 2 * e]);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) turn_pair(x[e], y[e], cs[n][2 * e], cs[n][2 * e + 1]);
+                }
+                if (off_table[n])
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[e] = y[e] = __builtin_nanf("");
+            }
+            if constexpr (I8)
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (mine[n]) top = max(top, max(__float_as_uint(x[e]) & 0x7fffffffu, __float_as_uint(y[e]) & 0x7fffffffu));
+            float *to = tile + (lane + 64 * n) / (D / 16) * ROW;
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                st4(to + at[n] + e, (floatx4){x[e], x[e + 1], x[e + 2], x[e + 3]});
+                st4(to + beside[n] + e, (floatx4){y[e], y[e + 1], y[e + 2], y[e + 3]});
+            }
+        }
+        if (h + 1 < w.heads) load(h + 1);
+        u32x4 *block = reinterpret_cast<u32x4 *>(block_at(a.p, w.page, w.head + h, w.slot, B::BYTES) + w.values * B::PART) + lane;
+        float inv = 0.0f, earlier = 0.0f;
+        if constexpr (I8) {
+            top = wave_umax(top);
+            float *held = scale_at(a.p, w.page, w.head + h, w.slot) + w.values;
+            float scale = fmaxf(__uint_as_float(top) * (1.0f / 127.0f), 0x1p-100f);
+            float old = 0.0f;
+            if (tokens.lo) {
+                old = *held;
+                if (!(old <= scale)) scale = old;
+            }
+            if (top >= 0x7f800000u) scale = __builtin_nanf("");
+            inv = 1.0f / scale;
+            earlier = old * inv;
+            if (lane == 0) *held = scale;
+        }
+        cache_wave_order();
 #pragma unroll
         for (int u = 0; u < B::UNITS; u++) {
-            const u32x4 from = *reinterpret_cast<const u32x4 *>(block + 1024 * u);
             float x[B::C];
-#pragma unroll
-            for (int e = 0; e < B::C; e++) {
-                if constexpr (I8) x[e] = (float)((int)(from[e / 4] >> (8 * (e % 4)) & 0xff) - 128) * scale;
-                else x[e] = __uint_as_float(from[e / 2] >> (16 * (e % 2)) << 16);
-            }
-            const int d0 = w.values ? B::value_dim(u, i) : B::key_dim(u, g);
             if (w.values) {
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     float v[B::C / 4];
+                    load_lds<B::C / 4>(tile + (4 * g + r) * ROW + DT * i + B::C / 4 * u, v);
 #pragma unroll
-                    for (int e = 0; e < B::C / 4; e++) v[e] = x[4 * e + r];
-                    store_lds<B::C / 4>(tile + (4 * g + r) * ROW + d0, v);
+                    for (int e = 0; e < B::C / 4; e++) x[4 * e + r] = v[e];
                 }
             } else {
-                store_lds<B::C>(tile + i * ROW + d0, x);
+                load_lds<B::C>(tile + i * ROW + 64 * (u * B::C / 16) + 16 * g + u * B::C % 16, x);
             }
+            u32x4 now;
+#pragma unroll
+            for (int d = 0; d < 4; d++) {
+                if constexpr (I8) {
+                    const float *q = x + 4 * d;
+                    now[d] = low_bytes(number_of(q[0], inv), number_of(q[1], inv), number_of(q[2], inv), number_of(q[3], inv));
+                } else {
+                    const float *q = x + 2 * d;
+                    now[d] = (uint32_t)__builtin_bit_cast(uint16_t, (bf16)q[0]) | (uint32_t)__builtin_bit_cast(uint16_t, (bf16)q[1]) << 16;
+                }
+            }
+            if (!whole) {
+                u32x4 old = {0, 0, 0, 0};
+                if (tokens.lo) old = block[64 * u];
+#pragma unroll
+                for (int d = 0; d < 4; d++) {
+                    constexpr int N = I8 ? 4 : 2, BITS = 32 / N;
+                    constexpr uint32_t MASK = I8 ? 0xffu : 0xffffu;
+                    uint32_t word = 0;
+#pragma unroll
+                    for (int e = 0; e < N; e++) {
+                        const int t = w.values ? 4 * g + (N * d + e) % 4 : i;
+                        uint32_t before = old[d] >> (BITS * e) & MASK;
+                        if constexpr (I8) before = number_of((float)((int)before - 128), earlier) & MASK;
+                        const uint32_t value = tokens.of_call(t) ? now[d] >> (BITS * e) & MASK : tokens.earlier(t) ? before : I8 ? 128u : 0u;
+                        word |= value << (BITS * e);
+                    }
+                    now[d] = word;
+                }
+            }
+            block[64 * u] = now;
+        }
+        cache_wave_order();
+    }
+}
+
+// A block's rows, one head's: lanes write what they hold in the block's order (of keys a
+// token's 16 dims beside each other, of values D / 16 of four tokens).
+template <typename T, int D, bool I8>
+static __global__ __launch_bounds__(256) void cache_read_kernel(CacheRowsArgs a) {
+    using B = BlockShape<D, I8>;
+    constexpr int DT = B::DT;
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    CacheTask w;
+    if (!w.take(a)) return;
+    char *out = w.values ? a.v : a.k;
+    if (!out) return;
+    float x[4 * DT];
+    const bool any = w.page >= 0 && w.first < w.start + w.rows;
+    const int page = any ? w.page : 0;
+    const u32x4 *block = reinterpret_cast<const u32x4 *>(block_at(a.p, page, w.head, any ? w.slot : 0, B::BYTES) + w.values * B::PART) + lane;
+    const float scale = I8 && any ? scale_at(a.p, page, w.head, w.slot)[w.values] : 1.0f;
+#pragma unroll
+    for (int u = 0; u < B::UNITS; u++) {
+        u32x4 from = {0, 0, 0, 0};
+        if (any) from = block[64 * u];
+#pragma unroll
+        for (int e = 0; e < B::C; e++) {
+            if constexpr (I8) x[B::C * u + e] = (float)((int)(from[e / 4] >> (8 * (e % 4)) & 0xff) - 128) * scale;
+            else x[B::C * u + e] = __uint_as_float(from[e / 2] >> (16 * (e % 2)) << 16);
         }
     }
-    cache_wave_order();
     const int64_t *strides = w.values ? a.vs : a.ks;
+    char *to = out + w.s * strides[0] + w.head * strides[2];
+    auto zero_or = [&](int64_t row, float v) { return any && row < w.rows ? v : 0.0f; };
+    if (w.values) {
 #pragma unroll
-    for (int n = 0; n < D / 64; n++) {
-        const int t = (lane + 64 * n) / (D / 16), u = (lane + 64 * n) % (D / 16);
-        const int64_t row = w.first + t - w.start;
-        if (row < 0 || row >= a.length) continue;
-        float x[16];
+        for (int r = 0; r < 4; r++) {
+            const int64_t row = w.first + 4 * g + r - w.start;
+            if (row < 0 || row >= a.length) continue;
+            float v[DT];
 #pragma unroll
-        for (int e = 0; e < 16; e++) x[e] = 0.0f;
-        if (any && row < w.rows) load_lds<16>(tile + t * ROW + 16 * u, x);
-        store_n<16>(reinterpret_cast<T *>(out + w.s * strides[0] + row * strides[1] + w.head * strides[2]) + 16 * u, x);
+            for (int e = 0; e < DT; e++) v[e] = zero_or(row, x[4 * e + r]);
+            store_n<DT>(reinterpret_cast<T *>(to + row * strides[1]) + DT * i, v);
+        }
+    } else {
+        const int64_t row = w.first + i - w.start;
+        if (row < 0 || row >= a.length) return;
+#pragma unroll
+        for (int n = 0; n < D / 64; n++) {
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; e++) v[e] = zero_or(row, x[16 * n + e]);
+            store_n<16>(reinterpret_cast<T *>(to + row * strides[1]) + 64 * n + 16 * g, v);
+        }
     }
 }
 

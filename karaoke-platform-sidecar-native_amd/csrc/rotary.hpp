@@ -85,6 +85,37 @@ VH_DEVICE void store_lds(float *p, const float (&v)[N]) {
     }
 }
 
+// 8 dims of a head from d on (a multiple of 8), turned by the table's row cs (null: NaN).
+// The rotation's dim is a multiple of 16, so they are of one half.
+template <typename T>
+VH_DEVICE void load_turned8(const Rotation &r, const T *x0, const float *cs, int d, float (&x)[8]) {
+    load_n<8>(x0 + d, x);
+    if (!r.table || d >= r.dim) return;
+    if (!cs) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = __builtin_nanf("");
+        return;
+    }
+    if (r.interleaved) {
+        float c[8];
+        load_n<8>(cs + d, c);
+#pragma unroll
+        for (int e = 0; e < 4; e++) turn_pair(x[2 * e], x[2 * e + 1], c[2 * e], c[2 * e + 1]);
+        return;
+    }
+    const int half = r.dim / 2;
+    const bool second = d >= half;
+    const int pair = second ? d - half : d;
+    float c[16], y[8];
+    load_n<16>(cs + 2 * pair, c);
+    load_n<8>(x0 + (second ? pair : d + half), y);
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        if (second) turn_pair(y[e], x[e], c[2 * e], c[2 * e + 1]);
+        else turn_pair(x[e], y[e], c[2 * e], c[2 * e + 1]);
+    }
+}
+
 struct RotaryArgs {
     Rotation r;
     const void *x;

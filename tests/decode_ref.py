@@ -144,7 +144,9 @@ def attention(kind, q, keys, values, *, scale, causal=False, start=0, turn=None)
         # a probability: its score's error, its exponential's, its place as an operand; the sum's is at most that
         top = dx.amax(1, keepdim=True) if n else torch.zeros(L, 1, dtype=torch.float64)
         rel = 2 * torch.expm1(top) + operand + U * (n / 32 + 60)
-        small = n * 2.0 ** -38 * v.abs().amax() if kind == "int8" and n else 0  # fp16's smallest, times 2^-14
+        # P (times its block's scale over the largest) is fp16 times 2^10: below fp16's normal numbers it is off by up to half
+        # of their step 2^-24, 2^-35 of the largest value, and the second operand's by as much
+        small = n * 2.0 ** -34 * v.abs().amax() if kind == "int8" and n else 0
         val[:, h] = out
         tol[:, h] = rel * (p @ v.abs()) + small + HALF[dtype] * out.abs() * 1.01
     return val, tol
