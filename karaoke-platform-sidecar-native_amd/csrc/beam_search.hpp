@@ -133,86 +133,116 @@ struct BeamPlace {
     }
 };
 
+constexpr int BS_VECTORS = 64;
+template <typename T>
+struct BeamVectors {
+    Logits<T> x[BS_VECTORS];
+    int at[BS_VECTORS], skip[BS_VECTORS];
+};
+
 // A wave's best `most` of NV * 8 logits a lane into list, unordered; how many.  floor: a
-// value that `most` of them reach, or -inf.
+// value that `most` of them reach, or -inf.  p: the stretch, x: its vectors, top: theirs.
 template <typename T, int NV>
-VH_DEVICE int collect(Logits<T> (&x)[NV], int thread, int valid, float floor, int most, BeamPick *list) {
+VH_DEVICE int collect(const T *p, bool whole, const Logits<T> (&x)[NV], const float (&top)[NV], int thread, int valid, float floor,
+                      int most, BeamPick *list, BeamVectors<T> &some) {
     const int lane = threadIdx.x & 63;
     const uint64_t below = ((uint64_t)1 << lane) - 1;
     int n = 0;
+    // the vectors that have such a logit, few, are put where all lanes see them
+    int vectors = 0;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-        anew(x[j]);
-        const BeamPlace place(j, thread, valid);
-        // the lane's logits of this vector that reach the floor, as bits
-        uint32_t mine = 0;
-#pragma unroll
-        for (int e = 0; e < 8; e++) mine |= x[j].get(e) >= floor ? 1u << e : 0u;
-        mine &= 0xffu << place.skip;
-        while (__ballot(mine != 0)) {  // one of each lane's at a time
-            const uint64_t m = __ballot(mine != 0);
-            const int e = __ffs((int)mine) - 1, k = n + __popcll(m & below);
-            if (mine && k < BS_LIST) list[k] = {x[j].pick(e), place.at + e};
-            mine &= mine - 1;
+        const bool has = top[j] >= floor;
+        const uint64_t m = __ballot(has);
+        const int k = vectors + __popcll(m & below);
+        if (has && k < BS_VECTORS) {
+            const BeamPlace place(j, thread, valid);
+            some.x[k] = x[j];
+            some.at[k] = place.at;
+            some.skip[k] = place.skip;
+        }
+        vectors += __popcll(m);
+    }
+    if (vectors <= BS_VECTORS) {
+        beam_wave_order();
+        for (int i0 = 0; i0 < 8 * vectors; i0 += 64) {
+            const int i = i0 + lane, k = min(i / 8, BS_VECTORS - 1), e = i % 8;
+            const float v = some.x[k].pick(e);
+            const bool has = i < 8 * vectors && v >= floor && e >= some.skip[k];
+            const uint64_t m = __ballot(has);
+            const int place = n + __popcll(m & below);
+            if (has && place < BS_LIST) list[place] = {v, some.at[k] + e};
             n += __popcll(m);
         }
+        if (n <= BS_LIST) return n;
     }
-    if (n <= BS_LIST) return n;
-    // Too many (many logits alike, or those of one lane all larger than others'): the
-    // value that the most-th best has, bit by bit; those above it, and of its own the
-    // first ones.
-    uint32_t best = 0;
-    for (int bit = 31; bit >= 0; bit--) {
-        const uint32_t trial = best | 1u << bit;
+    // Too many: hardly any above -inf, many alike, or those of a few lanes all larger than
+    // others'.  The value that the most-th best has, between the floor and the largest by
+    // halves; those above it, and of its own the first ones.  The logits are read
+    // once more, a vector at a time: kept, they would take every call's registers.
+    auto again = [&](int j) {
+        const BeamPlace place(j, thread, valid);
+        Logits<T> v;
+        if (whole) v.load(p + place.at);
+        else v.load_few(p, valid);
+        return v;
+    };
+    auto reach = [&](uint32_t least) {  // how many do
         int count = 0;
-#pragma unroll
+#pragma clang loop unroll(disable)
         for (int j = 0; j < NV; j++) {
-            anew(x[j]);
+            const Logits<T> v = again(j);
             const BeamPlace place(j, thread, valid);
-            int mine = 0;
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                mine += x[j].get(e) == x[j].get(e) && ordered(x[j].get(e)) >= trial && e >= place.skip ? 1 : 0;
-            count += mine;
+            for (int e = 0; e < 8; e++) count += v.get(e) == v.get(e) && ordered(v.get(e)) >= least && e >= place.skip ? 1 : 0;
         }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) count += __shfl_xor(count, o, 64);
-        if (count >= most) best = trial;
+        return count;
+    };
+    float largest = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < NV; j++) largest = fmaxf(largest, top[j]);
+    uint32_t best = ordered(floor), high = ordered(wave_max(largest));
+    if (floor == -INFINITY && best < high && reach(best + 1) < most) high = best;  // as where few tokens are allowed
+    while (best < high) {
+        const uint32_t trial = best + (high - best + 1) / 2;
+        if (reach(trial) >= most) best = trial;
+        else high = trial - 1;
     }
     const float limit = from_ordered(best);
     n = 0;
-#pragma unroll
-    for (int pass = 0; pass < 2; pass++) {  // above the limit, then at it while there is room
-        const int room = pass ? most : BS_LIST;
-#pragma unroll
-        for (int j = 0; j < NV; j++) {
-            anew(x[j]);
+#pragma clang loop unroll(disable)
+    for (int pass = 0; pass < 2; pass++)  // above the limit, then at it while there is room
+#pragma clang loop unroll(disable)
+        for (int j = 0; j < NV && n < most; j++) {
+            const Logits<T> v = again(j);
             const BeamPlace place(j, thread, valid);
-            int mine = 0;
+            uint32_t mine = 0;
 #pragma unroll
-            for (int e = 0; e < 8; e++) mine += (pass ? x[j].get(e) == limit : x[j].get(e) > limit) && e >= place.skip ? 1 : 0;
-            int upto = mine;
+            for (int e = 0; e < 8; e++) mine |= (pass ? v.get(e) == limit : v.get(e) > limit) && e >= place.skip ? 1u << e : 0u;
+            int upto = __popc(mine);
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
-                const int v = __shfl_up(upto, o, 64);
-                if (lane >= o) upto += v;
+                const int u = __shfl_up(upto, o, 64);
+                if (lane >= o) upto += u;
             }
-            int k = n + upto - mine;
-            n = min(n + __shfl(upto, 63, 64), room);
+            int k = n + upto - __popc(mine);
+            n = min(n + __shfl(upto, 63, 64), most);
 #pragma unroll
             for (int e = 0; e < 8; e++)
-                if ((pass ? x[j].get(e) == limit : x[j].get(e) > limit) && e >= place.skip) {
-                    if (k < room) list[k] = {x[j].get(e), place.at + e};
+                if (mine >> e & 1) {
+                    if (k < most) list[k] = {v.get(e), place.at + e};
                     k++;
                 }
         }
-    }
     return n;
 }
 
 template <typename T, int NV>
 static __global__ __launch_bounds__(BS_THREADS) void beam_stretch_kernel(BeamArgs a) {
     __shared__ BeamPick lists[BS_WAVES][BS_LIST];
+    __shared__ BeamVectors<T> some[BS_WAVES];
     __shared__ BeamPick sorted[BS_WAVES][BS_MAX_PICKS];
     __shared__ int counts[BS_WAVES];
     __shared__ float tops[BS_WAVES];
@@ -235,12 +265,14 @@ static __global__ __launch_bounds__(BS_THREADS) void beam_stretch_kernel(BeamArg
         if (place.skip) x[j].leave_out(place.skip);
     }
     // the lane's largest, the wave's, and the sum of exponentials (a NaN stays one)
-    float top = -INFINITY;
+    float tops_of[NV], top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         anew(x[j]);
+        tops_of[j] = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 8; e++) top = fmaxf(top, x[j].get(e));
+        for (int e = 0; e < 8; e++) tops_of[j] = fmaxf(tops_of[j], x[j].get(e));
+        top = fmaxf(top, tops_of[j]);
     }
     const float wtop = wave_max(top);
     const float c = 1.4426950408889634f, base = wtop == -INFINITY ? 0.0f : wtop;
@@ -264,11 +296,12 @@ static __global__ __launch_bounds__(BS_THREADS) void beam_stretch_kernel(BeamArg
         if (n >= most) floor = trial;
         if (n == most) break;
     }
-    int n = collect<T, NV>(x, (int)threadIdx.x, valid, floor ? from_ordered(floor) : -INFINITY, most, lists[wave]);
+    int n = collect<T, NV>(p, NV > 1 || a.V >= 8, x, tops_of, (int)threadIdx.x, valid, floor ? from_ordered(floor) : -INFINITY, most, lists[wave], some[wave]);
     beam_wave_order();
     for (int i = lane; i < n; i += 64) {
         const BeamPick mine = lists[wave][i];
         int rank = 0;
+#pragma unroll 4
         for (int k = 0; k < n; k++) rank += beats(lists[wave][k], mine) ? 1 : 0;
         if (rank < a.picks) sorted[wave][rank] = mine;
     }
@@ -332,14 +365,17 @@ VH_DEVICE double score_of(uint64_t a) {
 
 // What the join knows of a beam: 0 as it is, 1 no candidate but -inf, 2 ended.
 struct BeamState {
-    double lse;
+    double lse, score;
     int state;
 };
 // Beam b's candidate `in` of its stretches' lists; (-1, -1): none.
-VH_DEVICE BeamKey candidate(const BeamArgs &a, int s, int beam, int in, const BeamState &st) {
+VH_DEVICE BeamPick listed(const BeamArgs &a, int s, int beam, int in) {
+    const char *p = a.parts + ((int64_t)(s * a.B + beam) * a.stretches + in / a.picks) * a.part_bytes;
+    return reinterpret_cast<const BeamPick *>(p + sizeof(BeamPart))[in % a.picks];
+}
+VH_DEVICE BeamKey candidate(const BeamArgs &a, int beam, int in, const BeamState &st, const BeamPick &pick) {
     const BeamKey none{~0ull, ~0ull};
-    const int row = s * a.B + beam;
-    const double score = (double)a.scores[row];
+    const double score = st.score;
     if (st.state) {  // the end token with the score as it is, then the others in order
         int token = in;
         double v = -INFINITY;
@@ -350,8 +386,6 @@ VH_DEVICE BeamKey candidate(const BeamArgs &a, int s, int beam, int in, const Be
         if (in >= a.picks || token >= a.V) return none;
         return {score_down(v), (uint64_t)beam << 56 | (uint64_t)token};
     }
-    const char *p = a.parts + ((int64_t)row * a.stretches + in / a.picks) * a.part_bytes;
-    const BeamPick pick = reinterpret_cast<const BeamPick *>(p + sizeof(BeamPart))[in % a.picks];
     if (pick.token < 0) return none;
     const double v = score + ((double)pick.x - st.lse);
     const uint32_t down = v == -INFINITY ? 0u : ~ordered(pick.x);
@@ -381,6 +415,10 @@ static __global__ __launch_bounds__(BS_JOIN) void beam_join_kernel(BeamArgs a) {
     __shared__ BeamKey limit;
     __shared__ int left;
     const int s = (int)blockIdx.x, tid = (int)threadIdx.x;
+    const int lists = a.B * a.stretches, per_beam = a.stretches * a.picks, all = a.B * per_beam;
+    // a thread's candidate, where they are as few, asked for while the sums are on their way
+    BeamPick early{0.0f, -1};
+    if (tid < all) early = listed(a, s, tid / per_beam, tid % per_beam);
     // a beam's 16 lanes (a beam after the other): the logarithm of its sum
     if (tid == 0) {
         left = 0;
@@ -413,21 +451,22 @@ static __global__ __launch_bounds__(BS_JOIN) void beam_join_kernel(BeamArgs a) {
             l = (double)all + log(sum);
             if (!(fabs(l) < INFINITY)) st = 1;
         }
-        if (!(fabsf(a.scores[row]) < INFINITY)) st = 1;
-        if (lane == 0) beams[b] = {l, st};
+        const float score = a.scores[row];
+        if (!(fabsf(score) < INFINITY)) st = 1;
+        if (lane == 0) beams[b] = {l, (double)score, st};
     }
     __syncthreads();
-    const int lists = a.B * a.stretches, per_beam = a.stretches * a.picks, all = a.B * per_beam;
     if (lists <= BS_LISTS) {
         const int place = (a.picks + lists - 1) / lists - 1, need = (a.picks + place) / (place + 1);
-        if (tid < lists) {
-            const int beam = tid / a.stretches;
-            keys[tid] = candidate(a, s, beam, tid % a.stretches * a.picks + place, beams[beam]);
+        for (int e = tid; e < all; e += BS_JOIN) {
+            const int beam = e / per_beam, in = e - beam * per_beam;
+            if (in % a.picks == place) keys[e / a.picks] = candidate(a, beam, in, beams[beam], e == tid ? early : listed(a, s, beam, in));
         }
         __syncthreads();
         if (tid < lists) {
             const BeamKey mine = keys[tid];
             int rank = 0;
+#pragma unroll 4
             for (int i = 0; i < lists; i++) rank += key_less(keys[i], mine) ? 1 : 0;
             if (rank == need - 1 && ~mine.a) limit = mine;  // fewer than need: no limit
         }
@@ -435,7 +474,8 @@ static __global__ __launch_bounds__(BS_JOIN) void beam_join_kernel(BeamArgs a) {
         const BeamKey most = limit;
         for (int e = tid; e < all; e += BS_JOIN) {
             const int beam = e / per_beam;
-            const BeamKey key = candidate(a, s, beam, e - beam * per_beam, beams[beam]);
+            const int in = e - beam * per_beam;
+            const BeamKey key = candidate(a, beam, in, beams[beam], e == tid ? early : listed(a, s, beam, in));
             if (~key.a && !key_less(most, key)) keys[atomicAdd(&left, 1)] = key;  // in any order: ranked below
         }
         __syncthreads();
@@ -443,6 +483,7 @@ static __global__ __launch_bounds__(BS_JOIN) void beam_join_kernel(BeamArgs a) {
         for (int i = tid; i < n; i += BS_JOIN) {
             const BeamKey mine = keys[i];
             int rank = 0;
+#pragma unroll 4
             for (int k = 0; k < n; k++) rank += key_less(keys[k], mine) ? 1 : 0;
             if (rank < a.picks) put_pick(a, s, rank, mine);
         }
@@ -454,7 +495,8 @@ static __global__ __launch_bounds__(BS_JOIN) void beam_join_kernel(BeamArgs a) {
         const int take = min(all - done, BS_JOIN - held);
         for (int i = tid; i < BS_JOIN - held; i += BS_JOIN) {
             const int e = done + i, beam = e / per_beam;
-            keys[held + i] = i < take ? candidate(a, s, beam, e - beam * per_beam, beams[beam]) : none;
+            const int in = e - beam * per_beam;
+            keys[held + i] = i < take ? candidate(a, beam, in, beams[beam], listed(a, s, beam, in)) : none;
         }
         __syncthreads();
         for (int k = 2; k <= BS_JOIN; k *= 2)

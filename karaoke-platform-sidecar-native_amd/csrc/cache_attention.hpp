@@ -41,6 +41,7 @@ struct CacheAttentionArgs {
     float scale2;          // |scale| log2(e), at least the smallest normal number
     int negative;          // the scale is: q' is turned instead
     int tiles;             // workgroups of a (sequence, key head)'s rows
+    int by_xcd;            // these pairs are dealt out to the XCDs
     int parts, piece;      // pieces of the keys, and blocks of one
     float *part_o;         // [parts][S][Lq][H][D]
     float2 *part_ml;       // [parts][S][Lq][H]
@@ -141,6 +142,9 @@ struct RawBlocks {
 };
 
 VH_DEVICE float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+// The larger one, or a NaN if one is (the other maximum first makes sure that its
+// operands are quiet, an instruction each).
+VH_DEVICE float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 constexpr float FLT_LEAST = 0x1p-126f;
 constexpr float LAZY = 4.0f;  // P up to 2^LAZY: times P_SCALE it is fp16's
 
@@ -152,14 +156,15 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
     using Op = Operand16<I8>;
     // of q' and P: bf16 out one operand, but two where the cache's bytes are what takes the
     // time; fp32 out as many as 22 bits and more take
-    constexpr int DT = B::DT, QS = D / 32, N = sizeof(T) == 2 ? (SPLIT && !I8 ? 2 : 1) : I8 ? 2 : 3;
-    constexpr int WAVES = SPLIT ? 4 : 1, ROWS = 16 * RG * (SPLIT ? 1 : 4);
+    constexpr int DT = B::DT, QS = D / 32, N = sizeof(T) == 2 ? (RG == 1 && !I8 ? 2 : 1) : I8 ? 2 : 3;
+    constexpr int ROWS = 16 * RG * (SPLIT ? 1 : 4);
     constexpr int PER_FETCH = 64 / KB;
     constexpr float P_SCALE = I8 ? 0x1p10f : 1.0f;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int i = lane & 15, g = lane >> 4;
-    int pair, task;
-    if (!pair_task(a.S * a.p.kv, a.tiles * a.parts, pair, task)) return;
+    const int tasks = a.tiles * a.parts;
+    int pair = (int)blockIdx.x / tasks, task = (int)blockIdx.x % tasks;
+    if (a.by_xcd && !pair_task(a.S * a.p.kv, tasks, pair, task)) return;
     const int s = pair / a.p.kv, head = pair % a.p.kv;
     // causal: a sequence's last rows, which see most, first
     const int tile = a.tiles - 1 - task / a.parts, part = task % a.parts;
@@ -263,6 +268,11 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
         float sk[KB], sv[KB];
         uint32_t there;
     };
+    auto take = [](const char *p) {
+        const u32x4 *from = reinterpret_cast<const u32x4 *>(p);
+        if constexpr (SPLIT && RG == 1) return __builtin_nontemporal_load(from);  // each key is read by one wave
+        else return *from;
+    };
     auto load = [&](Step &st, int step) {
         const int at = step % PER_FETCH * KB;
         if (at == 0) fetch(step);
@@ -272,9 +282,9 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
             const char *p = reinterpret_cast<const char *>((uint64_t)read_lane(at_hi, at + b) << 32 | read_lane(at_lo, at + b));
             const char *from = p + 16 * lane;
 #pragma unroll
-            for (int u = 0; u < B::UNITS; u++) st.k.w[b][u] = *reinterpret_cast<const u32x4 *>(from + 1024 * u);
+            for (int u = 0; u < B::UNITS; u++) st.k.w[b][u] = take(from + 1024 * u);
 #pragma unroll
-            for (int u = 0; u < B::UNITS; u++) st.v.w[b][u] = *reinterpret_cast<const u32x4 *>(from + B::PART + 1024 * u);
+            for (int u = 0; u < B::UNITS; u++) st.v.w[b][u] = take(from + B::PART + 1024 * u);
             if constexpr (I8) {
                 st.sk[b] = __uint_as_float(read_lane(__float_as_uint(sk), at + b));
                 st.sv[b] = __uint_as_float(read_lane(__float_as_uint(sv), at + b));
@@ -323,16 +333,14 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
 #pragma unroll
             for (int b = 0; b < KB; b++) {
                 f[rg][b] = factor[rg];
-                if constexpr (I8) {
-                    f[rg][b] *= st.sk[b];
-                    if (f[rg][b] < FLT_LEAST) f[rg][b] = FLT_LEAST;  // 0 times -inf is no number; a NaN stays
-                }
+                if constexpr (I8) f[rg][b] *= st.sk[b];
+                if (I8 && !whole && f[rg][b] < FLT_LEAST) f[rg][b] = FLT_LEAST;  // 0 times -inf is no number; a NaN stays
                 if (!whole)
 #pragma unroll
                     for (int r = 0; r < 4; r++)
                         if ((st.there >> b & 1) == 0 || first + 16 * b + 4 * g + r >= limit[rg]) x[rg][b][r] = -INFINITY;
-                const float most = fmaxf(fmaxf(x[rg][b][0], x[rg][b][1]), fmaxf(x[rg][b][2], x[rg][b][3]));
-                top[rg] = fmaxf(top[rg], most * f[rg][b]);
+                const float most = larger(larger(x[rg][b][0], x[rg][b][1]), larger(x[rg][b][2], x[rg][b][3]));
+                top[rg] = larger(top[rg], most * f[rg][b]);
             }
             over |= top[rg] > m_run[rg] + LAZY;
         }
@@ -360,7 +368,7 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
         }
         float sv[KB];
         if constexpr (I8) {
-            const float inv = P_SCALE / v_top;
+            const float inv = P_SCALE * __builtin_amdgcn_rcpf(v_top);
 #pragma unroll
             for (int b = 0; b < KB; b++) sv[b] = st.sv[b] * inv;
         }
@@ -410,77 +418,63 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
     // in the values' own units
     const float unit = I8 ? v_top / P_SCALE : 1.0f;
 #pragma unroll
-    for (int rg = 0; rg < RG; rg++) {
-        l_run[rg] += __shfl_xor(l_run[rg], 16, 64);
-        l_run[rg] += __shfl_xor(l_run[rg], 32, 64);
+    for (int rg = 0; rg < RG; rg++)
 #pragma unroll
         for (int t = 0; t < DT; t++) o[rg][t] *= unit;
-    }
-    // a row's D / 4 dims from d on, with its maximum and sum
-    auto put = [&](int row, int d, const float (&v)[4 * DT / (SPLIT ? 4 : 1)], float m, float l) {
-        constexpr int NV = 4 * DT / (SPLIT ? 4 : 1);
-        const int token = (int)((uint32_t)row / a.heads), h = head * a.group + row - token * a.group;
-        if (a.parts > 1) {
-            const int64_t at = (((int64_t)part * a.S + s) * a.Lq + token) * a.H + h;
-            if (l > 0.0f || l != l)
-                store_n<NV>(a.part_o + at * D + d, v);
-            if (d == 0) a.part_ml[at] = {m, l};
-            return;
+
+    // The waves' sums of the same rows lie in the same lanes: half of the waves give theirs
+    // to the others, twice.
+    if constexpr (SPLIT) {
+        __shared__ floatx4 sums[2][RG * DT][64];
+        __shared__ float2 stats[2][RG][64];
+#pragma unroll
+        for (int half = 2; half > 0; half /= 2) {
+            if (wave >= half && wave < 2 * half) {
+#pragma unroll
+                for (int rg = 0; rg < RG; rg++) {
+#pragma unroll
+                    for (int t = 0; t < DT; t++) sums[wave - half][rg * DT + t][lane] = o[rg][t];
+                    stats[wave - half][rg][lane] = {m_run[rg], l_run[rg]};
+                }
+            }
+            __syncthreads();
+            if (wave < half) {
+#pragma unroll
+                for (int rg = 0; rg < RG; rg++) {
+                    const float2 ml = stats[wave][rg][lane];
+                    const float m = fmaxf(m_run[rg], ml.x), base = m == -INFINITY ? 0.0f : m;  // -inf - -inf is no number
+                    const float mine = exp2_of(m_run[rg] - base), other = exp2_of(ml.x - base);
+                    m_run[rg] = m;
+                    l_run[rg] = l_run[rg] * mine + ml.y * other;
+#pragma unroll
+                    for (int t = 0; t < DT; t++) o[rg][t] = o[rg][t] * mine + sums[wave][rg * DT + t][lane] * other;
+                }
+            }
+            if (half > 1) __syncthreads();
         }
-        float y[NV];
+        if (wave > 0) return;
+    }
+#pragma unroll
+    for (int rg = 0; rg < RG; rg++) {
+        float l = l_run[rg];
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        const int row = row0 + 16 * rg + i;
+        if (row >= rows) continue;
+        const int token = row / a.heads, h = head * a.group + row - token * a.group;
+        float y[4 * DT];  // dims 4 DT g ..
+        const bool out = a.parts == 1;
         const float inv = l == 0.0f || token >= qlen ? 0.0f : 1.0f / l;
 #pragma unroll
-        for (int e = 0; e < NV; e++) y[e] = inv == 0.0f ? 0.0f : v[e] * inv;
-        store_n<NV>(reinterpret_cast<T *>(a.out + s * a.os[0] + token * a.os[1] + h * a.os[2]) + d, y);
-    };
-    if constexpr (!SPLIT) {
+        for (int r = 0; r < 4; r++)
 #pragma unroll
-        for (int rg = 0; rg < RG; rg++) {
-            const int row = row0 + 16 * rg + i;
-            if (row >= rows) continue;
-            float v[4 * DT];
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-#pragma unroll
-                for (int t = 0; t < DT; t++) v[DT * r + t] = o[rg][t][r];
-            put(row, 4 * DT * g, v, m_run[rg], l_run[rg]);
-        }
-    } else {
-        constexpr int LROW = D + 4;
-        __shared__ __align__(16) float lo[4][16 * RG * LROW];
-        __shared__ float2 ml[4][16 * RG];
-#pragma unroll
-        for (int rg = 0; rg < RG; rg++) {
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                float v[DT];
-#pragma unroll
-                for (int t = 0; t < DT; t++) v[t] = o[rg][t][r];
-                store_lds<DT>(&lo[wave][(16 * rg + i) * LROW + DT * (4 * g + r)], v);
-            }
-            if (g == 0) ml[wave][16 * rg + i] = {m_run[rg], l_run[rg]};
-        }
-        __syncthreads();
-        // DT dims of a row a thread
-        for (int n = threadIdx.x; n < 16 * RG * 16; n += 256) {
-            const int r = n / 16, d = n % 16 * DT, row = row0 + r;
-            if (row >= rows) continue;
-            float m = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < WAVES; w++) m = fmaxf(m, ml[w][r].x);
-            float v[DT], l = 0.0f;
-#pragma unroll
-            for (int e = 0; e < DT; e++) v[e] = 0.0f;
-#pragma unroll
-            for (int w = 0; w < WAVES; w++) {
-                const float f = ml[w][r].x == -INFINITY ? 0.0f : exp2_of(ml[w][r].x - m);
-                l += ml[w][r].y * f;
-                float x[DT];
-                load_lds<DT>(&lo[w][r * LROW + d], x);
-#pragma unroll
-                for (int e = 0; e < DT; e++) v[e] += x[e] * f;
-            }
-            put(row, d, v, m, l);
+            for (int t = 0; t < DT; t++) y[DT * r + t] = !out ? o[rg][t][r] : inv == 0.0f ? 0.0f : o[rg][t][r] * inv;
+        if (out) {
+            store_n<4 * DT>(reinterpret_cast<T *>(a.out + s * a.os[0] + token * a.os[1] + h * a.os[2]) + 4 * DT * g, y);
+        } else {
+            const int64_t at = (((int64_t)part * a.S + s) * a.Lq + token) * a.H + h;
+            if (l != 0.0f) store_n<4 * DT>(a.part_o + at * D + 4 * DT * g, y);
+            if (g == 0) a.part_ml[at] = {m_run[rg], l};
         }
     }
 }

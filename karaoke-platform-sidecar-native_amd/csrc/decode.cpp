@@ -361,32 +361,36 @@ bool cache_reorder(hipStream_t s, const vh_cache *c, int beams, const int32_t *p
 }
 
 // ----------------------------------------------------------- cache attention
-// How a call is cut into workgroups: of 16 or 32 rows whose waves share the keys, or
-// of more, each wave with its own; and into pieces of the keys.
+// How a call is cut into workgroups: with few rows four waves share them, each every
+// fourth step of the keys, else each wave has its own; and into pieces of the keys.
 struct CacheCut {
-    bool split;
+    bool split, by_xcd;
     int groups, tiles;  // groups of 16 rows a wave has; workgroups of a (sequence, key head)
     int parts = 1, piece;
     int64_t pairs, grid;
 };
 constexpr int CQ_MAX_ROWS = 1 << 30;
-constexpr int wave_groups(int type, int head_dim) { return (head_dim == 64 ? 4 : 2) / (type == VH_TYPE_BF16 ? 1 : 2); }
-constexpr int split_groups(int type, int head_dim) { return type == VH_TYPE_FP32 && head_dim == 128 ? 1 : 2; }
+constexpr int64_t CQ_ENOUGH = 1024;  // workgroups: two a CU, twice
+// Groups of 16 rows of a wave at most: what 256 registers hold.
+constexpr int most_groups(int type, int head_dim) { return (head_dim == 64 ? 4 : 2) / (type == VH_TYPE_BF16 ? 1 : 2); }
 static CacheCut cache_cut(const vh_cache *c, const vh_cache_queries *q) {
     CacheCut cut;
-    const int rows = q->length * (q->heads / c->kv_heads);
-    cut.split = rows <= 128;
-    cut.groups = cut.split ? (rows <= 16 ? 1 : split_groups(q->type, c->head_dim)) : wave_groups(q->type, c->head_dim);
+    const int rows = q->length * (q->heads / c->kv_heads), most = most_groups(q->type, c->head_dim);
+    cut.pairs = (int64_t)c->sequences * c->kv_heads;
+    cut.split = cut.pairs * ((rows + 64 * most - 1) / (64 * most)) < CQ_ENOUGH;
+    cut.groups = !cut.split || rows > 32 ? most : rows > 16 ? std::min(2, most) : 1;
     const int per = 16 * cut.groups * (cut.split ? 1 : 4);
     cut.tiles = (rows + per - 1) / per;
-    cut.pairs = (int64_t)c->sequences * c->kv_heads;
     const int64_t base = cut.pairs * cut.tiles;
     const int blocks = std::max<int>(1, (int)((std::min<int64_t>(q->most_keys, capacity(c)) + PC_BLOCK - 1) / PC_BLOCK));
-    const int64_t want = std::min<int64_t>(1024 / std::max<int64_t>(base, 1), blocks / 32);
+    const int64_t want = std::min<int64_t>(CQ_ENOUGH / std::max<int64_t>(base, 1), blocks / 32);
     const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(want, 64));
     cut.piece = ((blocks + parts - 1) / parts + 15) / 16 * 16;  // whole steps of all waves
     cut.parts = (blocks + cut.piece - 1) / cut.piece;
-    cut.grid = (pairs_by_xcd(cut.pairs) ? (cut.pairs + 7) / 8 * 8 : cut.pairs) * cut.tiles * cut.parts;
+    // (sequence, key head) pairs are dealt out to the XCDs where their rows' workgroups share
+    // an L2's keys, and are many: of few, uneven ones the longest would be one XCD's
+    cut.by_xcd = cut.pairs >= 64 && cut.tiles > 1;
+    cut.grid = (cut.by_xcd ? (cut.pairs + 7) / 8 * 8 : cut.pairs) * cut.tiles * cut.parts;
     return cut;
 }
 static int64_t query_rows(const vh_cache *c, const vh_cache_queries *q) { return (int64_t)c->sequences * q->length * q->heads; }
@@ -425,10 +429,11 @@ size_t cache_workspace_bytes(const vh_cache *c, const vh_cache_queries *q) {
 
 template <typename T, int D, bool I8>
 static void attention_launch(hipStream_t s, const CacheAttentionArgs &a, const CacheCut &cut) {
-    constexpr int TYPE = sizeof(T) == 2 ? VH_TYPE_BF16 : VH_TYPE_FP32;
+    constexpr int MOST = most_groups(sizeof(T) == 2 ? VH_TYPE_BF16 : VH_TYPE_FP32, D);
     const dim3 grid((unsigned)cut.grid);
-    if (!cut.split) hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, wave_groups(TYPE, D), 2, false>), grid, dim3(256), 0, s, a);
-    else if (cut.groups > 1) hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, split_groups(TYPE, D), 2, true>), grid, dim3(256), 0, s, a);
+    if (!cut.split) hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, MOST, 2, false>), grid, dim3(256), 0, s, a);
+    else if (cut.groups == 4) hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, MOST, 2, true>), grid, dim3(256), 0, s, a);
+    else if (cut.groups == 2) hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, MOST < 2 ? MOST : 2, 2, true>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, 1, I8 && D == 64 ? 4 : 2, true>), grid, dim3(256), 0, s, a);
     if (cut.parts == 1) return;
     const int64_t rows = (int64_t)a.S * a.Lq * a.H;
@@ -482,6 +487,7 @@ bool cache_attention(hipStream_t s, const vh_cache *c, const vh_cache_queries *q
     a.scale2 = std::max(fabsf(q->scale) * 1.4426950408889634f, 0x1p-126f);
     a.negative = q->scale < 0.0f;
     a.tiles = cut.tiles;
+    a.by_xcd = cut.by_xcd;
     a.parts = cut.parts;
     a.piece = cut.piece;
     a.part_o = static_cast<float *>(workspace);

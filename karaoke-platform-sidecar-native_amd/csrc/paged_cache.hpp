@@ -112,6 +112,17 @@ struct TokenRange {
     VH_DEVICE bool of_call(int t) const { return t >= lo && t < hi; }
 };
 
+// N consecutive floats of LDS, up to 4 at a time aligned.
+template <int N>
+VH_DEVICE void load_lds(const float *p, float (&v)[N]) {
+    typedef float V __attribute__((ext_vector_type(N < 4 ? N : 4)));
+#pragma unroll
+    for (int e = 0; e < N; e += 4) {
+        const V a = *reinterpret_cast<const V *>(p + e);
+#pragma unroll
+        for (int i = 0; i < (N < 4 ? N : 4); i++) v[e + i] = a[i];
+    }
+}
 // LDS accesses of the wave's lanes before and after stay in that order (the hardware
 // keeps a wave's; this keeps the compiler's).
 VH_DEVICE void cache_wave_order() {
@@ -359,7 +370,15 @@ static __global__ __launch_bounds__(256) void cache_reorder_kernel(ReorderArgs a
     const u32x4 *src = reinterpret_cast<const u32x4 *>(block_at(a.p, source, head, 0, a.block_bytes));
     u32x4 *dst = reinterpret_cast<u32x4 *>(block_at(a.p, target, head, 0, a.block_bytes));
     const int n = blocks * a.block_bytes / 16;
-    for (int i = threadIdx.x; i < n; i += 256) dst[i] = src[i];
+    for (int i0 = threadIdx.x; i0 < n; i0 += 8 * 256) {
+        u32x4 x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (i0 + 256 * j < n) x[j] = src[i0 + 256 * j];
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (i0 + 256 * j < n) dst[i0 + 256 * j] = x[j];
+    }
     if (a.scaled)
         for (int i = threadIdx.x; i < 2 * blocks; i += 256) scale_at(a.p, target, head, 0)[i] = scale_at(a.p, source, head, 0)[i];
 }

@@ -62,29 +62,6 @@ VH_DEVICE void store_n(T *p, const float (&v)[N]) {
     *reinterpret_cast<typename Elements<T, N>::type *>(p) = a;
 }
 
-// The same where N of them (up to 4 at a time) are aligned, as in LDS.
-template <int N>
-VH_DEVICE void load_lds(const float *p, float (&v)[N]) {
-    typedef float V __attribute__((ext_vector_type(N < 4 ? N : 4)));
-#pragma unroll
-    for (int e = 0; e < N; e += 4) {
-        const V a = *reinterpret_cast<const V *>(p + e);
-#pragma unroll
-        for (int i = 0; i < (N < 4 ? N : 4); i++) v[e + i] = a[i];
-    }
-}
-template <int N>
-VH_DEVICE void store_lds(float *p, const float (&v)[N]) {
-    typedef float V __attribute__((ext_vector_type(N < 4 ? N : 4)));
-#pragma unroll
-    for (int e = 0; e < N; e += 4) {
-        V a;
-#pragma unroll
-        for (int i = 0; i < (N < 4 ? N : 4); i++) a[i] = v[e + i];
-        *reinterpret_cast<V *>(p + e) = a;
-    }
-}
-
 // 8 dims of a head from d on (a multiple of 8), turned by the table's row cs (null: NaN).
 // The rotation's dim is a multiple of 16, so they are of one half.
 template <typename T>
