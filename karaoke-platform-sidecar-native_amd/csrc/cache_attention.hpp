@@ -90,11 +90,16 @@ VH_DEVICE void split_n(float (&x)[8], typename Operand16<I8>::type (&o)[N]) {
 }
 
 // Four bytes (numbers plus 128) as fp16.
+template <bool BIASED = false>
 VH_DEVICE void bytes_to_half(uint32_t w, uint32_t &lo, uint32_t &hi) {
     typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
     const halfx2 bias = {(_Float16)-1152.0f, (_Float16)-1152.0f};
-    lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(halfx2, __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) + bias);
-    hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(halfx2, __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) + bias);
+    lo = __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u);
+    hi = __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u);
+    if constexpr (!BIASED) {
+        lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(halfx2, lo) + bias);
+        hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(halfx2, hi) + bias);
+    }
 }
 template <bool I8>
 VH_DEVICE typename Operand16<I8>::type operand_of(u32x2 a, u32x2 b) {
@@ -106,15 +111,16 @@ template <int D, bool I8, int KB>
 struct RawBlocks {
     using B = BlockShape<D, I8>;
     u32x4 w[KB][B::UNITS];
-    // keys' operand m: dims 32 m .. of block b's
+    // keys' operand m: dims 32 m .. of block b's, of 8 bits BIASED by 1152
+    template <bool BIASED>
     VH_DEVICE typename Operand16<I8>::type key(int b, int m) const {
         if constexpr (I8) {
             u32x4 o;
             uint32_t lo, hi;
-            bytes_to_half(w[b][m / 2][2 * (m % 2)], lo, hi);
+            bytes_to_half<BIASED>(w[b][m / 2][2 * (m % 2)], lo, hi);
             o[0] = lo;
             o[1] = hi;
-            bytes_to_half(w[b][m / 2][2 * (m % 2) + 1], lo, hi);
+            bytes_to_half<BIASED>(w[b][m / 2][2 * (m % 2) + 1], lo, hi);
             o[2] = lo;
             o[3] = hi;
             return __builtin_bit_cast(halfx8, o);
@@ -159,6 +165,9 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
     constexpr int DT = B::DT, QS = D / 32, N = sizeof(T) == 2 ? (RG == 1 && !I8 ? 2 : 1) : I8 ? 2 : 3;
     constexpr int ROWS = 16 * RG * (SPLIT ? 1 : 4);
     constexpr int PER_FETCH = 64 / KB;
+    // bf16 out: keys enter as 1152 more than they are, and the scores begin so much lower:
+    // sums 1152 / 40 times as large, whose fp32 roundings stay below those of fp16 queries
+    constexpr bool BIASED = I8 && N == 1;
     constexpr float P_SCALE = I8 ? 0x1p10f : 1.0f;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int i = lane & 15, g = lane >> 4;
@@ -183,6 +192,7 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
     // the wave's rows as columns, made when the first keys are asked for
     typename Op::type qf[RG][QS][N];
     float factor[RG];  // of the scores, in powers of two
+    float origin[RG];  // BIASED: what a score begins with, -1152 times the sum of q'
     int limit[RG];     // keys that the lane's row sees
     auto prepare_rows = [&] {
 #pragma unroll
@@ -218,6 +228,16 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
             }
 #pragma unroll
             for (int m = 0; m < QS; m++) split_n<I8, N>(x[m], qf[rg][m]);
+            origin[rg] = 0.0f;
+            if constexpr (BIASED) {
+#pragma unroll
+                for (int m = 0; m < QS; m++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) origin[rg] += (float)qf[rg][m][0][e];
+                origin[rg] += __shfl_xor(origin[rg], 16, 64);
+                origin[rg] += __shfl_xor(origin[rg], 32, 64);
+                origin[rg] *= -1152.0f;
+            }
         }
     };
 
@@ -268,8 +288,12 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
         float sk[KB], sv[KB];
         uint32_t there;
     };
-    auto take = [](const char *p) {
-        const u32x4 *from = reinterpret_cast<const u32x4 *>(p);
+    // By an address that is known to be global memory's (one made of a number is not, and its
+    // loads are waited for all together), the same in all lanes but for 16 bytes each.
+    auto take = [&](uint64_t at, int offset) {
+        typedef const __attribute__((address_space(1))) char *Bytes;
+        typedef const __attribute__((address_space(1))) u32x4 *Words;
+        const Words from = (Words)((Bytes)at + (uint32_t)(16 * lane) + offset);
         if constexpr (SPLIT && RG == 1) return __builtin_nontemporal_load(from);  // each key is read by one wave
         else return *from;
     };
@@ -279,12 +303,11 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
         st.there = (uint32_t)(there >> at) & ((1u << KB) - 1);
 #pragma unroll
         for (int b = 0; b < KB; b++) {
-            const char *p = reinterpret_cast<const char *>((uint64_t)read_lane(at_hi, at + b) << 32 | read_lane(at_lo, at + b));
-            const char *from = p + 16 * lane;
+            const uint64_t from = (uint64_t)read_lane(at_hi, at + b) << 32 | read_lane(at_lo, at + b);
 #pragma unroll
-            for (int u = 0; u < B::UNITS; u++) st.k.w[b][u] = take(from + 1024 * u);
+            for (int u = 0; u < B::UNITS; u++) st.k.w[b][u] = take(from, 1024 * u);
 #pragma unroll
-            for (int u = 0; u < B::UNITS; u++) st.v.w[b][u] = take(from + B::PART + 1024 * u);
+            for (int u = 0; u < B::UNITS; u++) st.v.w[b][u] = take(from, B::PART + 1024 * u);
             if constexpr (I8) {
                 st.sk[b] = __uint_as_float(read_lane(__float_as_uint(sk), at + b));
                 st.sv[b] = __uint_as_float(read_lane(__float_as_uint(sv), at + b));
@@ -299,12 +322,12 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
 #pragma unroll
         for (int rg = 0; rg < RG; rg++)
 #pragma unroll
-            for (int b = 0; b < KB; b++) x[rg][b] = (floatx4){0, 0, 0, 0};
+            for (int b = 0; b < KB; b++) x[rg][b] = (floatx4){origin[rg], origin[rg], origin[rg], origin[rg]};
 #pragma unroll
         for (int b = 0; b < KB; b++)
 #pragma unroll
             for (int m = 0; m < QS; m++) {
-                const typename Op::type k = st.k.key(b, m);
+                const typename Op::type k = st.k.template key<BIASED>(b, m);
 #pragma unroll
                 for (int rg = 0; rg < RG; rg++)
 #pragma unroll

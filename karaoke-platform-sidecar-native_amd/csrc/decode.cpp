@@ -370,20 +370,20 @@ struct CacheCut {
     int64_t pairs, grid;
 };
 constexpr int CQ_MAX_ROWS = 1 << 30;
-constexpr int64_t CQ_ENOUGH = 1024;  // workgroups: two a CU, twice
+constexpr int64_t CQ_ROWS = 512, CQ_PIECES = 512;
 // Groups of 16 rows of a wave at most: what 256 registers hold.
-constexpr int most_groups(int type, int head_dim) { return (head_dim == 64 ? 4 : 2) / (type == VH_TYPE_BF16 ? 1 : 2); }
+constexpr int most_groups(int type, int head_dim) { return type == VH_TYPE_FP32 && head_dim == 128 ? 1 : 2; }
 static CacheCut cache_cut(const vh_cache *c, const vh_cache_queries *q) {
     CacheCut cut;
     const int rows = q->length * (q->heads / c->kv_heads), most = most_groups(q->type, c->head_dim);
     cut.pairs = (int64_t)c->sequences * c->kv_heads;
-    cut.split = cut.pairs * ((rows + 64 * most - 1) / (64 * most)) < CQ_ENOUGH;
-    cut.groups = !cut.split || rows > 32 ? most : rows > 16 ? std::min(2, most) : 1;
+    cut.split = rows <= 64 || cut.pairs * ((rows + 64 * most - 1) / (64 * most)) < CQ_ROWS;
+    cut.groups = cut.split && rows <= 16 ? 1 : most;
     const int per = 16 * cut.groups * (cut.split ? 1 : 4);
     cut.tiles = (rows + per - 1) / per;
     const int64_t base = cut.pairs * cut.tiles;
     const int blocks = std::max<int>(1, (int)((std::min<int64_t>(q->most_keys, capacity(c)) + PC_BLOCK - 1) / PC_BLOCK));
-    const int64_t want = std::min<int64_t>(CQ_ENOUGH / std::max<int64_t>(base, 1), blocks / 32);
+    const int64_t want = base >= CQ_PIECES / 2 ? 1 : std::min<int64_t>(CQ_PIECES / std::max<int64_t>(base, 1), blocks / 32);
     const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(want, 64));
     cut.piece = ((blocks + parts - 1) / parts + 15) / 16 * 16;  // whole steps of all waves
     cut.parts = (blocks + cut.piece - 1) / cut.piece;
@@ -432,8 +432,7 @@ static void attention_launch(hipStream_t s, const CacheAttentionArgs &a, const C
     constexpr int MOST = most_groups(sizeof(T) == 2 ? VH_TYPE_BF16 : VH_TYPE_FP32, D);
     const dim3 grid((unsigned)cut.grid);
     if (!cut.split) hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, MOST, 2, false>), grid, dim3(256), 0, s, a);
-    else if (cut.groups == 4) hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, MOST, 2, true>), grid, dim3(256), 0, s, a);
-    else if (cut.groups == 2) hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, MOST < 2 ? MOST : 2, 2, true>), grid, dim3(256), 0, s, a);
+    else if (cut.groups > 1) hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, MOST, 2, true>), grid, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, 1, I8 && D == 64 ? 4 : 2, true>), grid, dim3(256), 0, s, a);
     if (cut.parts == 1) return;
     const int64_t rows = (int64_t)a.S * a.Lq * a.H;
