@@ -133,7 +133,7 @@ struct BeamPlace {
     }
 };
 
-constexpr int BS_VECTORS = 64;
+constexpr int BS_VECTORS = 128;
 template <typename T>
 struct BeamVectors {
     Logits<T> x[BS_VECTORS];
@@ -148,14 +148,40 @@ VH_DEVICE int collect(const T *p, bool whole, const Logits<T> (&x)[NV], const fl
     const int lane = threadIdx.x & 63;
     const uint64_t below = ((uint64_t)1 << lane) - 1;
     int n = 0;
-    // the vectors that have such a logit, few, are put where all lanes see them
+    // The vectors that have such a logit, where few, are put where all lanes see them; of more,
+    // those that reach a higher floor, as long as that leaves `most`.
+    auto with = [&](float least) {
+        int vectors = 0;
+#pragma unroll
+        for (int j = 0; j < NV; j++) vectors += __popcll(__ballot(top[j] >= least));
+        return vectors;
+    };
+    float largest = top[0];
+#pragma unroll
+    for (int j = 1; j < NV; j++) largest = fmaxf(largest, top[j]);
+    const uint32_t lowest = ordered(floor), highest = ordered(wave_max(largest));
+    int found = with(floor);
+    if (found > BS_VECTORS) {
+        uint32_t lo = lowest, hi = highest;  // at lo too many, above hi too few
+        while (lo < hi) {
+            const uint32_t trial = lo + (hi - lo + 1) / 2;
+            found = with(from_ordered(trial));
+            if (found >= most) lo = trial;
+            else hi = trial - 1;
+            if (found >= most && found <= BS_VECTORS) {
+                floor = from_ordered(trial);
+                break;
+            }
+        }
+    }
     int vectors = 0;
+    if (found <= BS_VECTORS)
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const bool has = top[j] >= floor;
         const uint64_t m = __ballot(has);
         const int k = vectors + __popcll(m & below);
-        if (has && k < BS_VECTORS) {
+        if (has) {
             const BeamPlace place(j, thread, valid);
             some.x[k] = x[j];
             some.at[k] = place.at;
@@ -163,7 +189,7 @@ VH_DEVICE int collect(const T *p, bool whole, const Logits<T> (&x)[NV], const fl
         }
         vectors += __popcll(m);
     }
-    if (vectors <= BS_VECTORS) {
+    if (found <= BS_VECTORS) {
         beam_wave_order();
         for (int i0 = 0; i0 < 8 * vectors; i0 += 64) {
             const int i = i0 + lane, k = min(i / 8, BS_VECTORS - 1), e = i % 8;
@@ -200,11 +226,8 @@ VH_DEVICE int collect(const T *p, bool whole, const Logits<T> (&x)[NV], const fl
         for (int o = 32; o > 0; o >>= 1) count += __shfl_xor(count, o, 64);
         return count;
     };
-    float largest = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < NV; j++) largest = fmaxf(largest, top[j]);
-    uint32_t best = ordered(floor), high = ordered(wave_max(largest));
-    if (floor == -INFINITY && best < high && reach(best + 1) < most) high = best;  // as where few tokens are allowed
+    uint32_t best = lowest, high = highest;
+    if (lowest == ordered(-INFINITY) && best < high && reach(best + 1) < most) high = best;  // as where few tokens are allowed
     while (best < high) {
         const uint32_t trial = best + (high - best + 1) / 2;
         if (reach(trial) >= most) best = trial;
@@ -240,7 +263,7 @@ VH_DEVICE int collect(const T *p, bool whole, const Logits<T> (&x)[NV], const fl
 }
 
 template <typename T, int NV>
-static __global__ __launch_bounds__(BS_THREADS) void beam_stretch_kernel(BeamArgs a) {
+static __global__ __launch_bounds__(BS_THREADS, 5) void beam_stretch_kernel(BeamArgs a) {
     __shared__ BeamPick lists[BS_WAVES][BS_LIST];
     __shared__ BeamVectors<T> some[BS_WAVES];
     __shared__ BeamPick sorted[BS_WAVES][BS_MAX_PICKS];
@@ -264,7 +287,9 @@ static __global__ __launch_bounds__(BS_THREADS) void beam_stretch_kernel(BeamArg
         const BeamPlace place(j, (int)threadIdx.x, valid);
         if (place.skip) x[j].leave_out(place.skip);
     }
-    // the lane's largest, the wave's, and the sum of exponentials (a NaN stays one)
+    // the vectors' largest, the lane's, the wave's, and the sum of exponentials (a NaN stays
+    // one); in one pass, from the first vector's largest, it took 37.7 us a call instead of
+    // 33.5 (256 rows of 120001): more registers, for the case that this is far too small
     float tops_of[NV], top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
@@ -366,7 +391,7 @@ VH_DEVICE double score_of(uint64_t a) {
 // What the join knows of a beam: 0 as it is, 1 no candidate but -inf, 2 ended.
 struct BeamState {
     double lse, score;
-    int state;
+    int state, ended;
 };
 // Beam b's candidate `in` of its stretches' lists; (-1, -1): none.
 VH_DEVICE BeamPick listed(const BeamArgs &a, int s, int beam, int in) {
@@ -391,24 +416,26 @@ VH_DEVICE BeamKey candidate(const BeamArgs &a, int beam, int in, const BeamState
     const uint32_t down = v == -INFINITY ? 0u : ~ordered(pick.x);
     return {score_down(v), (uint64_t)beam << 56 | (uint64_t)down << 24 | (uint64_t)pick.token};
 }
-VH_DEVICE void put_pick(const BeamArgs &a, int s, int place, const BeamKey &key) {
+VH_DEVICE void put_pick(const BeamArgs &a, int s, int place, const BeamKey &key, const BeamState *beams) {
     const int beam = (int)(key.b >> 56), token = (int)(key.b & 0xffffff);
     const int64_t at = (int64_t)s * a.picks + place;
     a.tokens[at] = token;
     a.parents[at] = beam;
     a.new_scores[at] = (float)score_of(key.a);
-    if (a.new_ended) a.new_ended[at] = (a.ended && a.ended[s * a.B + beam]) || token == a.end_token ? 1 : 0;
+    if (a.new_ended) a.new_ended[at] = beams[beam].ended || token == a.end_token ? 1 : 0;
 }
 
 constexpr int BS_JOIN = 1024;    // threads of the join, and candidates that it sorts at once
 constexpr int BS_LISTS = 512;    // lists whose heads are compared with one another
-constexpr int BS_LEFT = 4096;    // candidates that those leave, at most: picks of `picks` lists
+constexpr int BS_LEFT = 4096;    // candidates that those leave, at most
 
-// A workgroup joins a sequence's beams.  Every list is in order, so with `need` of the
-// lists' candidates at place r at or before a key, need (r + 1) = picks, only candidates
-// at or before it count: those of at most `need` lists with r = 0, else of fewer lists
-// than picks.  They are ranked by counting.  More lists than BS_LISTS are sorted stretch
-// by stretch beside the best so far.
+// A workgroup joins a sequence's beams.  Every list is in order: where `need` lists have
+// their candidate at place r at or before a key, need (r + 1) >= picks, only candidates at
+// or before it count.  r is such that need is about a quarter of the lists (64 lists of
+// 64: from 4096 candidates left with the heads themselves, 835 us, to some 100).  These
+// lists leave at most need * picks candidates, the others r each, BS_LEFT at most, which
+// are ranked by counting.  More lists than BS_LISTS are sorted stretch by stretch beside
+// the best so far.
 static __global__ __launch_bounds__(BS_JOIN) void beam_join_kernel(BeamArgs a) {
     __shared__ __align__(16) BeamKey keys[BS_LEFT];
     __shared__ BeamState beams[BS_MAX_BEAMS];
@@ -428,7 +455,9 @@ static __global__ __launch_bounds__(BS_JOIN) void beam_join_kernel(BeamArgs a) {
         const int b = b0 + tid / 16, lane = tid % 16;
         if (b >= a.B) break;
         const int row = s * a.B + b;
-        int st = a.ended && a.ended[row] ? 2 : 0;
+        const float score = a.scores[row];
+        const int ended = a.ended ? a.ended[row] : 0;
+        int st = ended ? 2 : 0;
         double l = 0.0;
         if (!st) {
             const char *p = a.parts + (int64_t)row * a.stretches * a.part_bytes;
@@ -436,10 +465,10 @@ static __global__ __launch_bounds__(BS_JOIN) void beam_join_kernel(BeamArgs a) {
             double sum = 0.0;
             for (int i = lane; i < a.stretches; i += 16) {
                 const BeamPart h = *reinterpret_cast<const BeamPart *>(p + (int64_t)i * a.part_bytes);
-                const float up = fmaxf(top, h.top);
                 // a stretch of nothing but -inf adds nothing, a NaN stays
-                sum = (top == -INFINITY ? sum : sum * exp((double)top - (double)up)) +
-                      (h.top == -INFINITY ? h.sum : h.sum * exp((double)h.top - (double)up));
+                const float up = fmaxf(top, h.top);
+                if (top != -INFINITY && top != up) sum *= exp((double)top - (double)up);
+                sum += h.top == -INFINITY || h.top == up ? h.sum : h.sum * exp((double)h.top - (double)up);
                 top = up;
             }
             float all = top;
@@ -451,13 +480,12 @@ static __global__ __launch_bounds__(BS_JOIN) void beam_join_kernel(BeamArgs a) {
             l = (double)all + log(sum);
             if (!(fabs(l) < INFINITY)) st = 1;
         }
-        const float score = a.scores[row];
         if (!(fabsf(score) < INFINITY)) st = 1;
-        if (lane == 0) beams[b] = {l, (double)score, st};
+        if (lane == 0) beams[b] = {l, (double)score, st, ended};
     }
     __syncthreads();
     if (lists <= BS_LISTS) {
-        const int place = (a.picks + lists - 1) / lists - 1, need = (a.picks + place) / (place + 1);
+        const int place = min(a.picks, (4 * a.picks + lists - 1) / lists) - 1, need = (a.picks + place) / (place + 1);
         for (int e = tid; e < all; e += BS_JOIN) {
             const int beam = e / per_beam, in = e - beam * per_beam;
             if (in % a.picks == place) keys[e / a.picks] = candidate(a, beam, in, beams[beam], e == tid ? early : listed(a, s, beam, in));
@@ -485,7 +513,7 @@ static __global__ __launch_bounds__(BS_JOIN) void beam_join_kernel(BeamArgs a) {
             int rank = 0;
 #pragma unroll 4
             for (int k = 0; k < n; k++) rank += key_less(keys[k], mine) ? 1 : 0;
-            if (rank < a.picks) put_pick(a, s, rank, mine);
+            if (rank < a.picks) put_pick(a, s, rank, mine, beams);
         }
         return;
     }
@@ -515,7 +543,7 @@ static __global__ __launch_bounds__(BS_JOIN) void beam_join_kernel(BeamArgs a) {
         done += take;
         held = min(a.picks, held + take);
     }
-    if (tid < a.picks) put_pick(a, s, tid, keys[tid]);
+    if (tid < a.picks) put_pick(a, s, tid, keys[tid], beams);
 }
 
 }  // namespace vh

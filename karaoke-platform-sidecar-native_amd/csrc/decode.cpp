@@ -179,7 +179,7 @@ bool rotary_apply(hipStream_t s, const vh_rotary *r, const vh_rotary_rows *rows,
     const int per_row = a.heads * a.units;
     a.per_row = divisor((uint32_t)per_row);
     a.per_head = divisor((uint32_t)a.units);
-    a.rows = std::max(1, std::min(rows->length, 1024 / per_row));
+    a.rows = std::max(1, std::min(rows->length, 512 / per_row));
     a.blocks = (rows->length + a.rows - 1) / a.rows;
     const int64_t groups = (int64_t)a.blocks * rows->sequences;
     if (!groups_ok(what, groups)) return false;
@@ -500,11 +500,11 @@ bool cache_attention(hipStream_t s, const vh_cache *c, const vh_cache_queries *q
 // --------------------------------------------------------------- beam search
 // A stretch of a beam's logits, the vectors of 8 that a thread takes of it (of bf16 up
 // to 8, of fp32 4: the same registers); shorter stretches while there are fewer than
-// two workgroups a CU.
+// half as many workgroups as CUs.
 struct BeamCut {
     int vectors, stretch, stretches, part_bytes;
 };
-constexpr int64_t BS_ENOUGH = 512;
+constexpr int64_t BS_ENOUGH = 128;
 static BeamCut beam_cut(const vh_beam *b) {
     constexpr int ONE = BS_THREADS * 8;
     const int64_t rows = std::max<int64_t>(1, (int64_t)b->sequences * b->beams);

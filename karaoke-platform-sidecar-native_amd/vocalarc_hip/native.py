@@ -534,8 +534,16 @@ class _Plan:
         if any(t.shape[-1] > 1 and t.stride(-1) != 1 for t in tensors.values()):
             self._refuse("a row's elements are consecutive")
 
+    def _whole(self, name, t, dtype, shape, device):
+        """t's address, where it is a contiguous tensor of that type and shape on that device."""
+        if t.dtype is not dtype or t.shape != shape or t.device != device or not t.is_contiguous():
+            self._refuse(f"{name} is a contiguous {dtype} tensor {list(shape)} on {device}")
+        return t.data_ptr()
+
     def _tensor(self, name, like, t):
         """t's address, where it is laid out as `like` was."""
+        if (t.dtype, t.shape, t.stride(), t.device) == self._like[like]:
+            return t.data_ptr()
         dtype, shape, stride, device = self._like[like]
         if t.dtype != dtype or t.shape != shape or t.device != device or \
                 (t.stride() != stride and t.numel() and any(n > 1 and a != b for n, a, b in zip(shape, t.stride(), stride))):
@@ -552,6 +560,17 @@ class _Plan:
     def _on_gpu(self, device):
         if device.type != "cuda" or device.index:  # every context's GPU is the first
             self._refuse(f"the tensors are on {device}, the context's work runs on cuda:0")
+
+
+_torch_module = None
+
+
+def _torch():
+    global _torch_module
+    if _torch_module is None:
+        import torch
+        _torch_module = torch
+    return _torch_module
 
 
 def _rotary_ref(r):
@@ -581,24 +600,23 @@ class Rotary(_Plan):
     def apply(self, x, y, start=None, backward: bool = False):
         """y [S][L][H][D] = x turned from position start[s] (int32 device tensor [S], None: 0) on; y may be x.  backward:
         by the transpose, which takes y's gradient to x's."""
-        key = (x.dtype, x.shape, x.stride(), y.dtype, y.stride())
+        key = (x.dtype, x.shape, x.stride(), y.dtype, y.shape, y.stride())
         rows = self._rows.get(key)
         if rows is None:
-            if x.dim() != 4 or x.shape[3] < self.c.dim:
+            if x.dim() != 4 or x.shape[3] < self.c.dim or y.shape != x.shape:
                 self._refuse(f"x and y are [S][L][H][D] with D from {self.c.dim}")
             self._activations(x=x, y=y)
             S, L, H, D = x.shape
-            rows = CRotaryRows(int(x.element_size() == 2), S, L, H, D, (_I64 * 3)(*x.stride()[:3]), (_I64 * 3)(*y.stride()[:3]))
+            c = CRotaryRows(int(x.element_size() == 2), S, L, H, D, (_I64 * 3)(*x.stride()[:3]), (_I64 * 3)(*y.stride()[:3]))
+            rows = c, ctypes.byref(c), (S,)
             self._rows = {**(self._rows if len(self._rows) < 64 else {}), key: rows}
-        if y.shape != x.shape:
-            self._refuse("y is not of x's shape")
-        if start is not None:
-            self._ints("start", start, x.shape[0])
-        self._same_device((x, y, start))
-        self._on_gpu(x.device)
-        rows.start = _opt(start)
-        _ok(lib().vh_rotary_apply(self.ctx.h, self._ref, ctypes.byref(rows), x.data_ptr(), y.data_ptr(), int(backward)),
-            "vh_rotary_apply")
+        c, ref, sequences = rows
+        device = x.device
+        if y.device != device:
+            self._refuse("tensors on different devices")
+        c.start = self._whole("start", start, _torch().int32, sequences, device) if start is not None else None
+        self._on_gpu(device)
+        _ok(lib().vh_rotary_apply(self.ctx.h, self._ref, ref, x.data_ptr(), y.data_ptr(), int(backward)), "vh_rotary_apply")
 
 
 class PagedCache(_Plan):
@@ -618,6 +636,8 @@ class PagedCache(_Plan):
         _ok(n, "vh_cache_bytes")
         self.pool = torch.empty(n, dtype=torch.uint8, device=device)
         self.c.pool = ptr(self.pool)
+        self._view = CCache.from_buffer_copy(self.c)  # reorder's, filled at each call
+        self._view_ref = ctypes.byref(self._view)
 
     def _with(self, table):
         """The cache seen through a table."""
@@ -640,17 +660,19 @@ class PagedCache(_Plan):
 
     def reorder(self, table, parents, lengths, spare, table_out, spare_out, *, beams: int):
         """The table's rows in the order of their parents (see vh_cache_reorder)."""
-        c = self._with(table)
-        S = c.sequences
+        if table.dim() != 2:
+            self._refuse("the table is [sequences][pages]")
+        shape, device, int32, v = table.shape, self.pool.device, _torch().int32, self._view
+        S = shape[0]
         if beams < 1 or S % beams:
             self._refuse(f"{S} sequences in groups of {beams} beams")
-        for name, t, shape in (("parents", parents, (S,)), ("lengths", lengths, (S // beams,)), ("spare", spare, (S,)),
-                               ("table_out", table_out, tuple(table.shape)), ("spare_out", spare_out, (S,))):
-            self._ints(name, t, *shape)
-        self._same_device((table, parents, lengths, spare, table_out, spare_out))
-        self._on_gpu(table.device)
-        _ok(lib().vh_cache_reorder(self.ctx.h, ctypes.byref(c), beams, ptr(parents), ptr(lengths), ptr(spare), ptr(table_out),
-                                   ptr(spare_out)), "vh_cache_reorder")
+        f = self._whole
+        v.sequences, v.table_pages, v.table = S, shape[1], f("table", table, int32, shape, device)
+        args = (f("parents", parents, int32, (S,), device), f("lengths", lengths, int32, (S // beams,), device),
+                f("spare", spare, int32, (S,), device), f("table_out", table_out, int32, shape, device),
+                f("spare_out", spare_out, int32, (S,), device))
+        self._on_gpu(device)
+        _ok(lib().vh_cache_reorder(self.ctx.h, self._view_ref, beams, *args), "vh_cache_reorder")
 
 
 class CacheTokens(_Plan):
@@ -740,6 +762,7 @@ class BeamSearch(_Plan):
         self._keep(logits=logits)
         self.c = CBeam(int(logits.element_size() == 2), S, B, V, self.picks, end_token, (_I64 * 2)(*logits.stride()[:2]))
         self._ref = ctypes.byref(self.c)
+        self._beams, self._picks = (S, B), (S, self.picks)
         self._device, self._bytes = logits.device, None
 
     def workspace_bytes(self) -> int:
@@ -752,20 +775,16 @@ class BeamSearch(_Plan):
     def select(self, logits, scores, tokens, parents, new_scores, *, ended=None, new_ended=None, workspace):
         """The best `picks` of each sequence: tokens and parents (int32), new_scores (fp32) and new_ended (int32), all
         [sequences][picks]; scores (fp32) and ended (int32) are the beams' [sequences][beams]."""
-        import torch
-        S, B = self.c.sequences, self.c.beams
-        address = self._tensor("logits", "logits", logits)
-        for name, t, shape in (("scores", scores, (S, B)), ("new_scores", new_scores, (S, self.picks))):
-            if t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous():
-                self._refuse(f"{name} is a contiguous fp32 tensor {list(shape)}")
-        for name, t, n in (("ended", ended, B), ("tokens", tokens, self.picks), ("parents", parents, self.picks),
-                           ("new_ended", new_ended, self.picks)):
-            self._ints(name, t, S, n)
-        self._same_device((logits, scores, ended, tokens, parents, new_scores, new_ended))
-        ws = self._buffer("workspace", workspace, self.workspace_bytes(), self._device)
-        self._on_gpu(self._device)
-        _ok(lib().vh_beam_select(self.ctx.h, self._ref, address, ptr(scores), _opt(ended), ptr(tokens), ptr(parents),
-                                 ptr(new_scores), _opt(new_ended), ws), "vh_beam_select")
+        f, device, torch = self._whole, self._device, _torch()
+        beams, picks = self._beams, self._picks
+        args = (self._tensor("logits", "logits", logits), f("scores", scores, torch.float32, beams, device),
+                f("ended", ended, torch.int32, beams, device) if ended is not None else None,
+                f("tokens", tokens, torch.int32, picks, device), f("parents", parents, torch.int32, picks, device),
+                f("new_scores", new_scores, torch.float32, picks, device),
+                f("new_ended", new_ended, torch.int32, picks, device) if new_ended is not None else None,
+                self._buffer("workspace", workspace, self.workspace_bytes(), device))
+        self._on_gpu(device)
+        _ok(lib().vh_beam_select(self.ctx.h, self._ref, *args), "vh_beam_select")
 
 
 class Model:
