@@ -349,19 +349,28 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
         }
         // scores to powers of two, s f; their largest in this lane
         float f[RG][KB], top[RG];
+#pragma unroll
+        for (int rg = 0; rg < RG; rg++)
+#pragma unroll
+            for (int b = 0; b < KB; b++) f[rg][b] = I8 ? factor[rg] * st.sk[b] : factor[rg];
+        if (!whole) {
+#pragma unroll
+            for (int rg = 0; rg < RG; rg++)
+#pragma unroll
+                for (int b = 0; b < KB; b++) {
+                    if (f[rg][b] < FLT_LEAST) f[rg][b] = FLT_LEAST;  // 0 times -inf is no number; a NaN stays
+                    const int keys_of_block = (st.there >> b & 1) ? limit[rg] - (first + 16 * b + 4 * g) : 0;
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+                        if (r >= keys_of_block) x[rg][b][r] = -INFINITY;
+                }
+        }
         bool over = false;
 #pragma unroll
         for (int rg = 0; rg < RG; rg++) {
             top[rg] = -INFINITY;
 #pragma unroll
             for (int b = 0; b < KB; b++) {
-                f[rg][b] = factor[rg];
-                if constexpr (I8) f[rg][b] *= st.sk[b];
-                if (I8 && !whole && f[rg][b] < FLT_LEAST) f[rg][b] = FLT_LEAST;  // 0 times -inf is no number; a NaN stays
-                if (!whole)
-#pragma unroll
-                    for (int r = 0; r < 4; r++)
-                        if ((st.there >> b & 1) == 0 || first + 16 * b + 4 * g + r >= limit[rg]) x[rg][b][r] = -INFINITY;
                 const float most = larger(larger(x[rg][b][0], x[rg][b][1]), larger(x[rg][b][2], x[rg][b][3]));
                 top[rg] = larger(top[rg], most * f[rg][b]);
             }

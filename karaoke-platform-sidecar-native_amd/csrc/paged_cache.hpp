@@ -160,8 +160,8 @@ static __global__ __launch_bounds__(256) void cache_append_kernel(CacheRowsArgs 
         const int t = (lane + 64 * n) / (D / 16), u = (lane + 64 * n) % (D / 16);
         mine[n] = tokens.of_call(t);
         turned[n] = !w.values && a.r.table && u < a.r.dim / 16;
-        at[n] = 16 * u;
-        beside[n] = 16 * u + 8;
+        at[n] = D == 128 && w.values ? 8 * u : 16 * u;
+        beside[n] = D == 128 && w.values ? 64 + 8 * u : 16 * u + 8;
         if (turned[n] && !a.r.interleaved) {
             at[n] = 8 * u;
             beside[n] = a.r.dim / 2 + 8 * u;
@@ -174,6 +174,9 @@ static __global__ __launch_bounds__(256) void cache_append_kernel(CacheRowsArgs 
             load_n<16>((row ? row : a.r.table) + 16 * u, cs[n]);
         }
     }
+    // Of 128 dims, in groups of 4, the even groups lie before the odd ones: a value's unit is
+    // every other group of a row, all of them in banks of their own so.
+    auto column = [](int d) { return D == 64 ? d : (d / 8 + 16 * (d / 4 % 2)) * 4 + d % 4; };
     Raw lo[NU], hi[NU];
     auto load = [&](int head) {
 #pragma unroll
@@ -214,8 +217,8 @@ static __global__ __launch_bounds__(256) void cache_append_kernel(CacheRowsArgs 
             float *to = tile + (lane + 64 * n) / (D / 16) * ROW;
 #pragma unroll
             for (int e = 0; e < 8; e += 4) {
-                st4(to + at[n] + e, (floatx4){x[e], x[e + 1], x[e + 2], x[e + 3]});
-                st4(to + beside[n] + e, (floatx4){y[e], y[e + 1], y[e + 2], y[e + 3]});
+                st4(to + column(at[n] + e), (floatx4){x[e], x[e + 1], x[e + 2], x[e + 3]});
+                st4(to + column(beside[n] + e), (floatx4){y[e], y[e + 1], y[e + 2], y[e + 3]});
             }
         }
         if (h + 1 < w.heads) load(h + 1);
@@ -243,12 +246,17 @@ static __global__ __launch_bounds__(256) void cache_append_kernel(CacheRowsArgs 
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     float v[B::C / 4];
-                    load_lds<B::C / 4>(tile + (4 * g + r) * ROW + DT * i + B::C / 4 * u, v);
+                    load_lds<B::C / 4>(tile + (4 * g + r) * ROW + column(DT * i + B::C / 4 * u), v);
 #pragma unroll
                     for (int e = 0; e < B::C / 4; e++) x[4 * e + r] = v[e];
                 }
             } else {
-                load_lds<B::C>(tile + i * ROW + 64 * (u * B::C / 16) + 16 * g + u * B::C % 16, x);
+#pragma unroll
+                for (int e = 0; e < B::C; e += 4) {
+                    const floatx4 v = ld4(tile + i * ROW + column(64 * (u * B::C / 16) + 16 * g + u * B::C % 16 + e));
+#pragma unroll
+                    for (int j = 0; j < 4; j++) x[e + j] = v[j];
+                }
             }
             u32x4 now;
 #pragma unroll
