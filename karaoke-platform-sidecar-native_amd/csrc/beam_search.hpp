@@ -321,7 +321,9 @@ static __global__ __launch_bounds__(BS_THREADS, 5) void beam_stretch_kernel(Beam
         if (n >= most) floor = trial;
         if (n == most) break;
     }
-    int n = collect<T, NV>(p, NV > 1 || a.V >= 8, x, tops_of, (int)threadIdx.x, valid, floor ? from_ordered(floor) : -INFINITY, most, lists[wave], some[wave]);
+    // what lies below -inf in that order is no number
+    const float least = floor <= ordered(-INFINITY) ? -INFINITY : from_ordered(floor);
+    int n = collect<T, NV>(p, NV > 1 || a.V >= 8, x, tops_of, (int)threadIdx.x, valid, least, most, lists[wave], some[wave]);
     beam_wave_order();
     for (int i = lane; i < n; i += 64) {
         const BeamPick mine = lists[wave][i];
@@ -426,7 +428,7 @@ VH_DEVICE void put_pick(const BeamArgs &a, int s, int place, const BeamKey &key,
 }
 
 constexpr int BS_JOIN = 1024;    // threads of the join, and candidates that it sorts at once
-constexpr int BS_LISTS = 512;    // lists whose heads are compared with one another
+constexpr int BS_LISTS = 1024;   // lists whose candidates at one place are compared with one another
 constexpr int BS_LEFT = 4096;    // candidates that those leave, at most
 
 // A workgroup joins a sequence's beams.  Every list is in order: where `need` lists have

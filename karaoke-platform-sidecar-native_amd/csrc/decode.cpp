@@ -2,6 +2,7 @@
 // beam search (rotary.hpp, paged_cache.hpp, cache_attention.hpp, beam_search.hpp).
 #include "runtime.hpp"
 
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -483,7 +484,7 @@ bool cache_attention(hipStream_t s, const vh_cache *c, const vh_cache_queries *q
     a.Lq = q->length;
     a.most = (int)std::min<int64_t>(q->most_keys, capacity(c));
     a.causal = q->causal ? 1 : 0;
-    a.scale2 = std::max(fabsf(q->scale) * 1.4426950408889634f, 0x1p-126f);
+    a.scale2 = std::min(std::max(fabsf(q->scale) * 1.4426950408889634f, 0x1p-126f), FLT_MAX);
     a.negative = q->scale < 0.0f;
     a.tiles = cut.tiles;
     a.by_xcd = cut.by_xcd;

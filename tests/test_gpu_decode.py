@@ -415,6 +415,35 @@ def test_numbers_that_are_none(ctx):
         assert bool(out[0].isnan().all()) and torch.equal(out[1], clean[1])
 
 
+@pytest.mark.parametrize("kind", ["int8", "bf16"])
+def test_nothing_to_attend_to(ctx, kind):
+    """No keys for anybody, no pages in the table, no rows, no sequences; key lengths below 0 and beyond the table."""
+    w = World(ctx, kind, 2, 1, 64, 16, 48, F32)
+    w.random(1, [0, 0], [48, 20])
+    q = randn(2, 2, 3, 2, 64)
+    assert bool((attend(w, q, start=[0, 0], most=0, keys=[40, 20], scale=0.125, check=False) == 0).all())
+    out = attend(w, q, start=[0, 0], keys=[-4, 10 ** 9], most=10 ** 6, scale=0.125, check=False)
+    assert bool((out[0] == 0).all())
+    # 48 tokens, of which 28 were never appended: what the pool began with, of int8 scales that are no numbers, and the last
+    # block of the first 20 ends in zeros
+    assert bool(out[1].isnan().all())
+    for table in (w.table[:, :0].contiguous(), w.table[:0]):
+        S = table.shape[0]
+        x, o = q[:S].to(DEV), torch.full((S, 3, 2, 64), 7.0, device=DEV)
+        p = w.cache.queries(table, x, o, most_keys=30)
+        p.forward(x, o, workspace=buffer(p.workspace_bytes()))
+        assert bool((o == 0).all())
+        k = torch.ones(S, 5, 1, 64, device=DEV)
+        before = w.cache.pool.clone()
+        w.cache.tokens(table, k, k).append(k, k)
+        assert torch.equal(before, w.cache.pool)
+        w.cache.tokens(table, k, k).read(k, None)
+        assert bool((k == 0).all())
+    x = torch.empty(2, 0, 2, 64, device=DEV)
+    p = w.cache.queries(w.table, x, x, most_keys=30)
+    p.forward(x, x, workspace=buffer(p.workspace_bytes()))
+
+
 def test_attention_strides_and_in_place(ctx):
     """Queries as a slice of a projection, out in their place, and out with heads outside rows."""
     w = World(ctx, "int8", 2, 2, 64, 16, 200, BF16, 64)
@@ -542,6 +571,41 @@ def test_beams_without_numbers(ctx):
         assert [(int(p), int(t)) for p, t in zip(parents[s], tokens[s])] == [(b, t) for _, b, t in want], s
         assert [math.isinf(float(v)) for v in new[s]] == [math.isinf(v) for v, _, _ in want]
     assert tokens[5].tolist() == list(range(8)) and parents[5].tolist() == [0] * 8
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [200, 5000, 40000])
+@pytest.mark.parametrize("allowed,picks", [(0, 64), (3, 64), (3, 5), (40, 64), (64, 64), (300, 64), (1000, 16)])
+def test_beams_few_tokens_allowed(ctx, V, allowed, picks, dtype):
+    """All logits but a few -inf, in one stretch or all over: the others fill up from the lowest token."""
+    g = torch.Generator().manual_seed(V + allowed)
+    allowed = min(allowed, V)
+    for where in (torch.randperm(V, generator=g)[:allowed], torch.arange(V - allowed, V)):
+        x = torch.full((1, 2, V), -math.inf)
+        # of bf16's values, each beam's apart from the other's
+        x[0, 0, where] = (torch.randperm(allowed, generator=g) / 64).float()
+        x[0, 1, where] = (torch.randperm(allowed, generator=g) / 64).float()
+        x = x.to(dtype)
+        scores = torch.tensor([[-1.0, -1.3]])
+        tokens, parents, new, _ = select(ctx, x, scores, picks)
+        want, near = R.beams(x[0], scores[0], picks)
+        assert near > 2.0 ** -19, near
+        assert [(int(p), int(t)) for p, t in zip(parents[0], tokens[0])] == [(b, t) for _, b, t in want]
+        assert [math.isinf(float(v)) for v in new[0]] == [math.isinf(v) for v, _, _ in want]
+
+
+def test_beams_many_lists(ctx):
+    """More lists of candidates than are compared at one place: sorted one part after the other."""
+    B, V, picks = 64, 140_003, 64
+    x = randn(11, 1, B, V)
+    scores = -randn(12, 1, B).abs() / 4
+    s = (torch.log_softmax(x[0].double(), -1) + scores[0].double()[:, None]).flatten()
+    best = s.topk(picks + 1)
+    assert float((best.values[:-1] - best.values[1:]).min()) > 2.0 ** -19
+    for logits in (x, x.to(DEV)[:, :, :]):
+        tokens, parents, new, _ = select(ctx, logits, scores, picks)
+        assert (parents[0].long() * V + tokens[0].long()).tolist() == best.indices[:picks].tolist()
+        assert float((new[0].double() - best.values[:picks]).abs().max()) <= 2.0 ** -20 + R.U * float(best.values.abs().max())
 
 
 def test_beams_strides(ctx):
