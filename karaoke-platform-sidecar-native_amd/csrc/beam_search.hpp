@@ -103,13 +103,6 @@ VH_DEVICE double wave_sum_double(double v) {
     return v;
 }
 
-// LDS accesses of the wave's lanes before and after stay in that order (the hardware
-// keeps a wave's; this keeps the compiler's).
-VH_DEVICE void beam_wave_order() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 // Keeps the compiler from holding what it made of the logits up to here, and from
 // taking up more of them than a vector at a time: else it unpacks all of a thread's
 // logits at once, and spills.
@@ -190,7 +183,7 @@ VH_DEVICE int collect(const T *p, bool whole, const Logits<T> (&x)[NV], const fl
         vectors += __popcll(m);
     }
     if (found <= BS_VECTORS) {
-        beam_wave_order();
+        cache_wave_order();
         for (int i0 = 0; i0 < 8 * vectors; i0 += 64) {
             const int i = i0 + lane, k = min(i / 8, BS_VECTORS - 1), e = i % 8;
             const float v = some.x[k].pick(e);
@@ -324,7 +317,7 @@ static __global__ __launch_bounds__(BS_THREADS, 5) void beam_stretch_kernel(Beam
     // what lies below -inf in that order is no number
     const float least = floor <= ordered(-INFINITY) ? -INFINITY : from_ordered(floor);
     int n = collect<T, NV>(p, NV > 1 || a.V >= 8, x, tops_of, (int)threadIdx.x, valid, least, most, lists[wave], some[wave]);
-    beam_wave_order();
+    cache_wave_order();
     for (int i = lane; i < n; i += 64) {
         const BeamPick mine = lists[wave][i];
         int rank = 0;

@@ -180,6 +180,7 @@ bool rotary_apply(hipStream_t s, const vh_rotary *r, const vh_rotary_rows *rows,
     const int per_row = a.heads * a.units;
     a.per_row = divisor((uint32_t)per_row);
     a.per_head = divisor((uint32_t)a.units);
+    // two units a thread: 6408 tokens there and back 13.7 us, four 15.1, one 14.0
     a.rows = std::max(1, std::min(rows->length, 512 / per_row));
     a.blocks = (rows->length + a.rows - 1) / a.rows;
     const int64_t groups = (int64_t)a.blocks * rows->sequences;
@@ -259,7 +260,7 @@ static bool cache_rows_ok(const char *what, const vh_cache *c, const vh_cache_ro
 }
 
 static bool cache_rows_args(const char *what, const vh_cache *c, const vh_cache_rows *r, const void *k, const void *v,
-                            bool append, CacheRowsArgs &a, int64_t &groups) {
+                            CacheRowsArgs &a, int64_t &groups) {
     if (!paged_args(what, c, a.p) || !aligned16(what, {k, v})) return false;
     const int64_t size = type_bytes(r->type);
     a.k = const_cast<char *>(static_cast<const char *>(k));
@@ -271,15 +272,12 @@ static bool cache_rows_args(const char *what, const vh_cache *c, const vh_cache_
     a.length = r->length;
     // from the first block's last token on at worst
     const int64_t blocks = ((int64_t)r->length + (r->start ? 2 * PC_BLOCK - 2 : PC_BLOCK - 1)) / PC_BLOCK;
-    // a wave of an append takes up to 4 heads, while there are 32 waves a CU
-    a.heads = 1;
-    while (append && a.heads < 4 && a.heads < c->kv_heads && c->sequences * blocks * 2 * c->kv_heads / a.heads > 16384) a.heads *= 2;
-    const int64_t of_block = 2 * ((c->kv_heads + a.heads - 1) / a.heads), each = blocks * of_block, tasks = each * c->sequences;  // below 2^59
+    const int64_t each = blocks * 2 * c->kv_heads, tasks = each * c->sequences;  // below 2^59
     groups = (tasks + 3) / 4;
     if (!groups_ok(what, groups)) return false;
     a.tasks = (int)tasks;
     a.per_sequence = divisor((uint32_t)each);
-    a.per_block = divisor((uint32_t)of_block);
+    a.per_block = divisor(2u * c->kv_heads);
     return true;
 }
 
@@ -307,7 +305,7 @@ bool cache_append(hipStream_t s, const vh_cache *c, const vh_cache_rows *r, cons
         return false;
     }
     int64_t groups;
-    if (!cache_rows_args(what, c, r, k, v, true, a, groups) ||
+    if (!cache_rows_args(what, c, r, k, v, a, groups) ||
         !begins_apart(what, {c->pool}, {k, v, c->table, r->start, r->lengths, a.r.table}))
         return false;
     Scope sc(t, s, "cache_append");
@@ -322,7 +320,7 @@ bool cache_read(hipStream_t s, const vh_cache *c, const vh_cache_rows *r, void *
     if (!c->sequences || !r->length || (!k && !v)) return true;
     CacheRowsArgs a{};
     int64_t groups;
-    if (!cache_rows_args(what, c, r, k, v, false, a, groups) || !begins_apart(what, {k, v}, {c->pool, c->table, r->start, r->lengths}))
+    if (!cache_rows_args(what, c, r, k, v, a, groups) || !begins_apart(what, {k, v}, {c->pool, c->table, r->start, r->lengths}))
         return false;
     Scope sc(t, s, "cache_read");
     if (r->type == VH_TYPE_BF16) rows_dispatch<bf16>(s, c, a, groups, false);
@@ -364,6 +362,17 @@ bool cache_reorder(hipStream_t s, const vh_cache *c, int beams, const int32_t *p
 // ----------------------------------------------------------- cache attention
 // How a call is cut into workgroups: with few rows four waves share them, each every
 // fourth step of the keys, else each wave has its own; and into pieces of the keys.
+// Measured over int8 pages, bf16 queries:
+//   CQ_ROWS   rows of their own from 512 workgroups on: 4 x 512 causal tokens of 32 heads
+//             on 8 of 128 over 4608 keys 165 us, from 1024 on 186; from 256 on, 4 x 517 of
+//             16 heads on 4 of 64 over 4613 take 125 us instead of 66; always shared, 16 x
+//             2048 of 16 on 4 of 64 take 358 instead of 293
+//   CQ_PIECES pieces until there are 512 workgroups: 16 single tokens of 32 heads on 8 of
+//             64, uneven, up to 8192 keys 25.9 us; until 384, 768, 1024: 28.1, 27.8, 29
+//   one piece from 256 workgroups on: 32 tokens of 32 heads on 8 of 128 over 16384 keys
+//             162 us, in two pieces 170
+//   a piece has 512 keys at least: one token of 8 heads over 77 to 8192 keys as long with
+//             256, or 1 us longer
 struct CacheCut {
     bool split, by_xcd;
     int groups, tiles;  // groups of 16 rows a wave has; workgroups of a (sequence, key head)
@@ -372,7 +381,8 @@ struct CacheCut {
 };
 constexpr int CQ_MAX_ROWS = 1 << 30;
 constexpr int64_t CQ_ROWS = 512, CQ_PIECES = 512;
-// Groups of 16 rows of a wave at most: what 256 registers hold.
+// Groups of 16 rows of a wave at most: what 256 registers hold.  The 4 x 517 tokens above
+// 64 us with two, 75 with four (the registers spill); fp32 over 64 dims 39.5 with two, 43 with one.
 constexpr int most_groups(int type, int head_dim) { return type == VH_TYPE_FP32 && head_dim == 128 ? 1 : 2; }
 static CacheCut cache_cut(const vh_cache *c, const vh_cache_queries *q) {
     CacheCut cut;
@@ -386,7 +396,7 @@ static CacheCut cache_cut(const vh_cache *c, const vh_cache_queries *q) {
     const int blocks = std::max<int>(1, (int)((std::min<int64_t>(q->most_keys, capacity(c)) + PC_BLOCK - 1) / PC_BLOCK));
     const int64_t want = base >= CQ_PIECES / 2 ? 1 : std::min<int64_t>(CQ_PIECES / std::max<int64_t>(base, 1), blocks / 32);
     const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(want, 64));
-    cut.piece = ((blocks + parts - 1) / parts + 15) / 16 * 16;  // whole steps of all waves
+    cut.piece = ((blocks + parts - 1) / parts + 4 * CQ_STEP - 1) / (4 * CQ_STEP) * (4 * CQ_STEP);  // whole steps of all waves
     cut.parts = (blocks + cut.piece - 1) / cut.piece;
     // (sequence, key head) pairs are dealt out to the XCDs where their rows' workgroups share
     // an L2's keys, and are many: of few, uneven ones the longest would be one XCD's
@@ -432,9 +442,9 @@ template <typename T, int D, bool I8>
 static void attention_launch(hipStream_t s, const CacheAttentionArgs &a, const CacheCut &cut) {
     constexpr int MOST = most_groups(sizeof(T) == 2 ? VH_TYPE_BF16 : VH_TYPE_FP32, D);
     const dim3 grid((unsigned)cut.grid);
-    if (!cut.split) hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, MOST, 2, false>), grid, dim3(256), 0, s, a);
-    else if (cut.groups > 1) hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, MOST, 2, true>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, 1, I8 && D == 64 ? 4 : 2, true>), grid, dim3(256), 0, s, a);
+    if (!cut.split) hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, MOST, false>), grid, dim3(256), 0, s, a);
+    else if (cut.groups > 1) hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, MOST, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((cache_attention_kernel<T, D, I8, 1, true>), grid, dim3(256), 0, s, a);
     if (cut.parts == 1) return;
     const int64_t rows = (int64_t)a.S * a.Lq * a.H;
     hipLaunchKernelGGL((cache_join_kernel<T, D>), dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, a);
@@ -501,7 +511,9 @@ bool cache_attention(hipStream_t s, const vh_cache *c, const vh_cache_queries *q
 // --------------------------------------------------------------- beam search
 // A stretch of a beam's logits, the vectors of 8 that a thread takes of it (of bf16 up
 // to 8, of fp32 4: the same registers); shorter stretches while there are fewer than
-// half as many workgroups as CUs.
+// half as many workgroups as CUs.  32 x 8 beams over 120001 tokens, 16 picks: 33.5 us with
+// 8 vectors, 38.2 with 4; 16 rows of 32003: 14.1 us, cut down to twice as many workgroups
+// as CUs 14.9 (more lists to join).
 struct BeamCut {
     int vectors, stretch, stretches, part_bytes;
 };

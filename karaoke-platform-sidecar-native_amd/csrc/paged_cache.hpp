@@ -57,23 +57,21 @@ struct CacheRowsArgs {
     int64_t ks[3], vs[3];  // bytes
     const int *start, *lengths;
     int length, tasks;     // rows of a sequence; waves
-    int heads;             // of a task
-    Divisor per_sequence, per_block;  // tasks of a sequence and of a block, 2 * ceil(kv / heads)
+    Divisor per_sequence, per_block;  // tasks of a sequence and of a block, 2 * kv
 };
 
-// A wave's task: 16 tokens' keys or values of one or several heads.
+// A wave's task: 16 tokens' keys or values of a head.
 struct CacheTask {
-    int s, head, heads, values;
+    int s, head, values;
     int64_t first, start;  // positions of the block's first token and of row 0
     int rows, page, slot;
     VH_DEVICE bool take(const CacheRowsArgs &a) {
         const uint32_t t = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
         if (t >= (uint32_t)a.tasks) return false;
         const uint32_t sq = t / a.per_sequence, in = t - sq * a.per_sequence.d, block_of_call = in / a.per_block;
-        const int part = (int)(in - block_of_call * a.per_block.d), groups = (int)a.per_block.d / 2;
-        values = part >= groups;
-        head = (values ? part - groups : part) * a.heads;
-        heads = min(a.heads, a.p.kv - head);
+        const int part = (int)(in - block_of_call * a.per_block.d);
+        values = part >= a.p.kv;
+        head = values ? part - a.p.kv : part;
         s = (int)sq;
         start = max(0, a.start ? __builtin_amdgcn_readfirstlane(a.start[s]) : 0);
         rows = a.lengths ? max(0, min(__builtin_amdgcn_readfirstlane(a.lengths[s]), a.length)) : a.length;
@@ -131,15 +129,18 @@ VH_DEVICE void cache_wave_order() {
 }
 
 // Rows into a block.  A wave's lanes take units of 16 dims of its tokens, beside each
-// other in a row, and turn them by a table row's part that stays in registers from head
-// to head; by way of a tile of LDS they take them up in the block's order, and write.
-// The next head's rows are on their way meanwhile.  Earlier tokens of a block that is not
-// new are rescaled in place.
+// other in a row, turn them, and take them up in the block's order by way of a tile of
+// LDS; earlier tokens of a block that is not new are rescaled in place.
+//
+// Bound by HBM: 32000 tokens of 8 heads of 128, bf16 into 8 bits 47 us (4.1 TB/s, where
+// a copy reaches 5.0), into bf16 54 us (4.8).  Lanes that read what they hold in the
+// block's order, without LDS, took 82 us for 18700 tokens instead of 36: a token's row in
+// pieces of 16 bytes; a lane's units one behind the other 40 us; four heads a wave, for
+// one reading of the table's row, no less than one.
 template <typename T, int D, bool I8>
 static __global__ __launch_bounds__(256) void cache_append_kernel(CacheRowsArgs a) {
     using B = BlockShape<D, I8>;
     constexpr int DT = B::DT, NU = D / 64, ROW = D + 4;  // units of a lane; floats of a tile's row, four banks apart
-    typedef typename Elements<T, 8>::type Raw;
     __shared__ __align__(16) float tiles[4][PC_BLOCK * ROW];
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     float *tile = tiles[threadIdx.x >> 6];
@@ -149,12 +150,15 @@ static __global__ __launch_bounds__(256) void cache_append_kernel(CacheRowsArgs 
     if (tokens.lo >= tokens.hi) return;
     const int64_t *strides = w.values ? a.vs : a.ks;
     const char *rows = (w.values ? a.v : a.k) + w.s * strides[0] + (w.first - w.start) * strides[1] + w.head * strides[2];
-
-    // the lane's units: which token, and where its two times 8 dims are
-    bool mine[NU], turned[NU], off_table[NU];
-    int at[NU], beside[NU];
+    // Of 128 dims, in groups of 4, the even groups lie before the odd ones: a value's unit is
+    // every other group of a row, all of them in banks of their own so.
+    auto column = [](int d) { return D == 64 ? d : (d / 8 + 16 * (d / 4 % 2)) * 4 + d % 4; };
+    // the lane's units, all asked for before the first is turned
+    typedef typename Elements<T, 8>::type Raw;
+    Raw lo[NU], hi[NU];
     float cs[NU][16];
-    const T *from[NU];
+    int at[NU], beside[NU];  // where the unit's two times 8 dims are
+    bool mine[NU], turned[NU], off_table[NU];
 #pragma unroll
     for (int n = 0; n < NU; n++) {
         const int t = (lane + 64 * n) / (D / 16), u = (lane + 64 * n) % (D / 16);
@@ -166,136 +170,122 @@ static __global__ __launch_bounds__(256) void cache_append_kernel(CacheRowsArgs 
             at[n] = 8 * u;
             beside[n] = a.r.dim / 2 + 8 * u;
         }
-        from[n] = reinterpret_cast<const T *>(rows + (mine[n] ? t : tokens.lo) * strides[1]);
+        const T *row = reinterpret_cast<const T *>(rows + (mine[n] ? t : tokens.lo) * strides[1]);
+        lo[n] = *reinterpret_cast<const Raw *>(row + at[n]);
+        hi[n] = *reinterpret_cast<const Raw *>(row + beside[n]);
         off_table[n] = false;
         if (turned[n]) {
-            const float *row = rotation_row(a.r, w.first + t);
-            off_table[n] = !row;
-            load_n<16>((row ? row : a.r.table) + 16 * u, cs[n]);
+            const float *angles = rotation_row(a.r, w.first + t);
+            off_table[n] = !angles;
+            load_n<16>((angles ? angles : a.r.table) + 16 * u, cs[n]);
         }
     }
-    // Of 128 dims, in groups of 4, the even groups lie before the odd ones: a value's unit is
-    // every other group of a row, all of them in banks of their own so.
-    auto column = [](int d) { return D == 64 ? d : (d / 8 + 16 * (d / 4 % 2)) * 4 + d % 4; };
-    Raw lo[NU], hi[NU];
-    auto load = [&](int head) {
+    uint32_t top = 0;
 #pragma unroll
-        for (int n = 0; n < NU; n++) {
-            const T *x = reinterpret_cast<const T *>(reinterpret_cast<const char *>(from[n]) + head * strides[2]);
-            lo[n] = *reinterpret_cast<const Raw *>(x + at[n]);
-            hi[n] = *reinterpret_cast<const Raw *>(x + beside[n]);
-        }
-    };
-    load(0);
-    const bool whole = tokens.lo == 0 && tokens.hi == PC_BLOCK;
-    for (int h = 0; h < w.heads; h++) {
-        uint32_t top = 0;
+    for (int n = 0; n < NU; n++) {
+        float x[8], y[8];
 #pragma unroll
-        for (int n = 0; n < NU; n++) {
-            float x[8], y[8];
+        for (int e = 0; e < 8; e++) x[e] = (float)lo[n][e], y[e] = (float)hi[n][e];
+        if (turned[n]) {
+            if (a.r.interleaved) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = (float)lo[n][e], y[e] = (float)hi[n][e];
-            if (turned[n]) {
-                if (a.r.interleaved) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        turn_pair(x[2 * e], x[2 * e + 1], cs[n][2 * e], cs[n][2 * e + 1]);
-                        turn_pair(y[2 * e], y[2 * e + 1], cs[n][8 + 2 * e], cs[n][9 + 2 * e]);
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; e++) turn_pair(x[e], y[e], cs[n][2 * e], cs[n][2 * e + 1]);
-                }
-                if (off_table[n])
-#pragma unroll
-                    for (int e = 0; e < 8; e++) x[e] = y[e] = __builtin_nanf("");
-            }
-            if constexpr (I8)
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (mine[n]) top = max(top, max(__float_as_uint(x[e]) & 0x7fffffffu, __float_as_uint(y[e]) & 0x7fffffffu));
-            float *to = tile + (lane + 64 * n) / (D / 16) * ROW;
-#pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-                st4(to + column(at[n] + e), (floatx4){x[e], x[e + 1], x[e + 2], x[e + 3]});
-                st4(to + column(beside[n] + e), (floatx4){y[e], y[e + 1], y[e + 2], y[e + 3]});
-            }
-        }
-        if (h + 1 < w.heads) load(h + 1);
-        u32x4 *block = reinterpret_cast<u32x4 *>(block_at(a.p, w.page, w.head + h, w.slot, B::BYTES) + w.values * B::PART) + lane;
-        float inv = 0.0f, earlier = 0.0f;
-        if constexpr (I8) {
-            top = wave_umax(top);
-            float *held = scale_at(a.p, w.page, w.head + h, w.slot) + w.values;
-            float scale = fmaxf(__uint_as_float(top) * (1.0f / 127.0f), 0x1p-100f);
-            float old = 0.0f;
-            if (tokens.lo) {
-                old = *held;
-                if (!(old <= scale)) scale = old;
-            }
-            if (top >= 0x7f800000u) scale = __builtin_nanf("");
-            inv = 1.0f / scale;
-            earlier = old * inv;
-            if (lane == 0) *held = scale;
-        }
-        cache_wave_order();
-#pragma unroll
-        for (int u = 0; u < B::UNITS; u++) {
-            float x[B::C];
-            if (w.values) {
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    float v[B::C / 4];
-                    load_lds<B::C / 4>(tile + (4 * g + r) * ROW + column(DT * i + B::C / 4 * u), v);
-#pragma unroll
-                    for (int e = 0; e < B::C / 4; e++) x[4 * e + r] = v[e];
+                for (int e = 0; e < 4; e++) {
+                    turn_pair(x[2 * e], x[2 * e + 1], cs[n][2 * e], cs[n][2 * e + 1]);
+                    turn_pair(y[2 * e], y[2 * e + 1], cs[n][8 + 2 * e], cs[n][9 + 2 * e]);
                 }
             } else {
 #pragma unroll
-                for (int e = 0; e < B::C; e += 4) {
-                    const floatx4 v = ld4(tile + i * ROW + column(64 * (u * B::C / 16) + 16 * g + u * B::C % 16 + e));
-#pragma unroll
-                    for (int j = 0; j < 4; j++) x[e + j] = v[j];
-                }
+                for (int e = 0; e < 8; e++) turn_pair(x[e], y[e], cs[n][2 * e], cs[n][2 * e + 1]);
             }
-            u32x4 now;
+            if (off_table[n])
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = y[e] = __builtin_nanf("");
+        }
+        if constexpr (I8)
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (mine[n]) top = max(top, max(__float_as_uint(x[e]) & 0x7fffffffu, __float_as_uint(y[e]) & 0x7fffffffu));
+        float *to = tile + (lane + 64 * n) / (D / 16) * ROW;
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+            st4(to + column(at[n] + e), (floatx4){x[e], x[e + 1], x[e + 2], x[e + 3]});
+            st4(to + column(beside[n] + e), (floatx4){y[e], y[e + 1], y[e + 2], y[e + 3]});
+        }
+    }
+    float inv = 0.0f, earlier = 0.0f;
+    if constexpr (I8) {
+        top = wave_umax(top);
+        float *held = scale_at(a.p, w.page, w.head, w.slot) + w.values;
+        float scale = fmaxf(__uint_as_float(top) * (1.0f / 127.0f), 0x1p-100f);
+        float old = 0.0f;
+        if (tokens.lo) {
+            old = *held;
+            if (!(old <= scale)) scale = old;
+        }
+        if (top >= 0x7f800000u) scale = __builtin_nanf("");
+        inv = 1.0f / scale;
+        earlier = old * inv;
+        if (lane == 0) *held = scale;
+    }
+    cache_wave_order();
+    u32x4 *block = reinterpret_cast<u32x4 *>(block_at(a.p, w.page, w.head, w.slot, B::BYTES) + w.values * B::PART) + lane;
+    const bool whole = tokens.lo == 0 && tokens.hi == PC_BLOCK;
+#pragma unroll
+    for (int u = 0; u < B::UNITS; u++) {
+        float x[B::C];
+        if (w.values) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                float v[B::C / 4];
+                load_lds<B::C / 4>(tile + (4 * g + r) * ROW + column(DT * i + B::C / 4 * u), v);
+#pragma unroll
+                for (int e = 0; e < B::C / 4; e++) x[4 * e + r] = v[e];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < B::C; e += 4) {
+                const floatx4 v = ld4(tile + i * ROW + column(64 * (u * B::C / 16) + 16 * g + u * B::C % 16 + e));
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[e + j] = v[j];
+            }
+        }
+        u32x4 now;
+#pragma unroll
+        for (int d = 0; d < 4; d++) {
+            if constexpr (I8) {
+                const float *q = x + 4 * d;
+                now[d] = low_bytes(number_of(q[0], inv), number_of(q[1], inv), number_of(q[2], inv), number_of(q[3], inv));
+            } else {
+                const float *q = x + 2 * d;
+                now[d] = (uint32_t)__builtin_bit_cast(uint16_t, (bf16)q[0]) | (uint32_t)__builtin_bit_cast(uint16_t, (bf16)q[1]) << 16;
+            }
+        }
+        if (!whole) {
+            u32x4 old = {0, 0, 0, 0};
+            if (tokens.lo) old = block[64 * u];
 #pragma unroll
             for (int d = 0; d < 4; d++) {
-                if constexpr (I8) {
-                    const float *q = x + 4 * d;
-                    now[d] = low_bytes(number_of(q[0], inv), number_of(q[1], inv), number_of(q[2], inv), number_of(q[3], inv));
-                } else {
-                    const float *q = x + 2 * d;
-                    now[d] = (uint32_t)__builtin_bit_cast(uint16_t, (bf16)q[0]) | (uint32_t)__builtin_bit_cast(uint16_t, (bf16)q[1]) << 16;
-                }
-            }
-            if (!whole) {
-                u32x4 old = {0, 0, 0, 0};
-                if (tokens.lo) old = block[64 * u];
+                constexpr int N = I8 ? 4 : 2, BITS = 32 / N;
+                constexpr uint32_t MASK = I8 ? 0xffu : 0xffffu;
+                uint32_t word = 0;
 #pragma unroll
-                for (int d = 0; d < 4; d++) {
-                    constexpr int N = I8 ? 4 : 2, BITS = 32 / N;
-                    constexpr uint32_t MASK = I8 ? 0xffu : 0xffffu;
-                    uint32_t word = 0;
-#pragma unroll
-                    for (int e = 0; e < N; e++) {
-                        const int t = w.values ? 4 * g + (N * d + e) % 4 : i;
-                        uint32_t before = old[d] >> (BITS * e) & MASK;
-                        if constexpr (I8) before = number_of((float)((int)before - 128), earlier) & MASK;
-                        const uint32_t value = tokens.of_call(t) ? now[d] >> (BITS * e) & MASK : tokens.earlier(t) ? before : I8 ? 128u : 0u;
-                        word |= value << (BITS * e);
-                    }
-                    now[d] = word;
+                for (int e = 0; e < N; e++) {
+                    const int t = w.values ? 4 * g + (N * d + e) % 4 : i;
+                    uint32_t before = old[d] >> (BITS * e) & MASK;
+                    if constexpr (I8) before = number_of((float)((int)before - 128), earlier) & MASK;
+                    const uint32_t value = tokens.of_call(t) ? now[d] >> (BITS * e) & MASK : tokens.earlier(t) ? before : I8 ? 128u : 0u;
+                    word |= value << (BITS * e);
                 }
+                now[d] = word;
             }
-            block[64 * u] = now;
         }
-        cache_wave_order();
+        block[64 * u] = now;
     }
 }
 
 // A block's rows, one head's: lanes write what they hold in the block's order (of keys a
-// token's 16 dims beside each other, of values D / 16 of four tokens).
+// token's 16 dims beside each other, of values D / 16 of four tokens).  Bound by HBM:
+// 32000 tokens of 8 heads of 128 to bf16, 47 us from 8 bits (4.2 TB/s), 54 us from bf16.
 template <typename T, int D, bool I8>
 static __global__ __launch_bounds__(256) void cache_read_kernel(CacheRowsArgs a) {
     using B = BlockShape<D, I8>;
@@ -354,7 +344,8 @@ struct ReorderArgs {
 };
 
 // A workgroup copies a head's blocks of a row's last page; head 0's writes the row of
-// the table too.
+// the table too.  Bound by HBM: 256 rows of 8 heads of 128, 8 blocks of 8 bits each, 7 of 8
+// rows another's: 19 us (6.0 TB/s).
 static __global__ __launch_bounds__(256) void cache_reorder_kernel(ReorderArgs a) {
     const int row = (int)(blockIdx.x / (uint32_t)a.p.kv), head = (int)(blockIdx.x % (uint32_t)a.p.kv);
     const int group = row / a.beams;
