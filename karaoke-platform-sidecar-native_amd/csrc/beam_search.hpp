@@ -46,7 +46,9 @@ VH_DEVICE uint32_t ordered(float x) {
     return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
 VH_DEVICE float from_ordered(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u ^ 0x80000000u : ~u); }
-VH_DEVICE bool beats(const BeamPick &a, const BeamPick &b) { return a.x > b.x || (a.x == b.x && a.token < b.token); }
+// A logit and its token as one number, the better the larger: (logit, token down).
+VH_DEVICE uint64_t key_of(float x, int token) { return (uint64_t)ordered(x) << 32 | ~(uint32_t)token; }
+VH_DEVICE BeamPick pick_of(uint64_t key) { return {from_ordered((uint32_t)(key >> 32)), (int)~(uint32_t)key}; }
 
 // 8 consecutive logits as they lie in memory, one of them as fp32.
 template <typename T>
@@ -137,7 +139,7 @@ struct BeamVectors {
 // value that `most` of them reach, or -inf.  p: the stretch, x: its vectors, top: theirs.
 template <typename T, int NV>
 VH_DEVICE int collect(const T *p, bool whole, const Logits<T> (&x)[NV], const float (&top)[NV], int thread, int valid, float floor,
-                      int most, BeamPick *list, BeamVectors<T> &some) {
+                      int most, uint64_t *list, BeamVectors<T> &some) {
     const int lane = threadIdx.x & 63;
     const uint64_t below = ((uint64_t)1 << lane) - 1;
     int n = 0;
@@ -190,7 +192,7 @@ VH_DEVICE int collect(const T *p, bool whole, const Logits<T> (&x)[NV], const fl
             const bool has = i < 8 * vectors && v >= floor && e >= some.skip[k];
             const uint64_t m = __ballot(has);
             const int place = n + __popcll(m & below);
-            if (has && place < BS_LIST) list[place] = {v, some.at[k] + e};
+            if (has && place < BS_LIST) list[place] = key_of(v, some.at[k] + e);
             n += __popcll(m);
         }
         if (n <= BS_LIST) return n;
@@ -248,7 +250,7 @@ VH_DEVICE int collect(const T *p, bool whole, const Logits<T> (&x)[NV], const fl
 #pragma unroll
             for (int e = 0; e < 8; e++)
                 if (mine >> e & 1) {
-                    if (k < most) list[k] = {v.get(e), place.at + e};
+                    if (k < most) list[k] = key_of(v.get(e), place.at + e);
                     k++;
                 }
         }
@@ -257,9 +259,9 @@ VH_DEVICE int collect(const T *p, bool whole, const Logits<T> (&x)[NV], const fl
 
 template <typename T, int NV>
 static __global__ __launch_bounds__(BS_THREADS, 5) void beam_stretch_kernel(BeamArgs a) {
-    __shared__ BeamPick lists[BS_WAVES][BS_LIST];
+    __shared__ __align__(16) uint64_t lists[BS_WAVES][BS_LIST + 2];
     __shared__ BeamVectors<T> some[BS_WAVES];
-    __shared__ BeamPick sorted[BS_WAVES][BS_MAX_PICKS];
+    __shared__ uint64_t sorted[BS_WAVES][BS_MAX_PICKS];
     __shared__ int counts[BS_WAVES];
     __shared__ float tops[BS_WAVES];
     __shared__ double sums[BS_WAVES];
@@ -293,15 +295,17 @@ static __global__ __launch_bounds__(BS_THREADS, 5) void beam_stretch_kernel(Beam
         top = fmaxf(top, tops_of[j]);
     }
     const float wtop = wave_max(top);
-    const float c = 1.4426950408889634f, base = wtop == -INFINITY ? 0.0f : wtop;
+    // 2^(c x - base), the exponent rounded once, that of wtop, 64 at most, not at all.  From
+    // 2^30 on values are the largest or 128 below it, and nothing is left of them in any base
+    const float c = fabsf(wtop) < 0x1p30f ? 1.4426950408889634f : 1.0f, base = wtop == -INFINITY ? 0.0f : wtop * c;
     float sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         anew(x[j]);
 #pragma unroll
-        for (int e = 0; e < 8; e++) sum += __builtin_amdgcn_exp2f((x[j].get(e) - base) * c);
+        for (int e = 0; e < 8; e++) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(x[j].get(e), c, -base));
     }
-    const double wsum = wave_sum_double((double)sum);
+    const double wsum = wave_sum_double((double)sum) * (wtop == -INFINITY ? 1.0 : exp2(-(double)__builtin_fmaf(wtop, c, -base)));
 
     // a value that at least `most` of the wave's lanes' largest reach
     const int most = min(a.picks, valid);
@@ -317,12 +321,12 @@ static __global__ __launch_bounds__(BS_THREADS, 5) void beam_stretch_kernel(Beam
     // what lies below -inf in that order is no number
     const float least = floor <= ordered(-INFINITY) ? -INFINITY : from_ordered(floor);
     int n = collect<T, NV>(p, NV > 1 || a.V >= 8, x, tops_of, (int)threadIdx.x, valid, least, most, lists[wave], some[wave]);
+    if (lane < 2) lists[wave][n + lane] = 0;
     cache_wave_order();
     for (int i = lane; i < n; i += 64) {
-        const BeamPick mine = lists[wave][i];
+        const uint64_t mine = lists[wave][i];
         int rank = 0;
-#pragma unroll 4
-        for (int k = 0; k < n; k++) rank += beats(lists[wave][k], mine) ? 1 : 0;
+        for (int k = 0; k < n; k += 2) rank += (lists[wave][k] > mine) + (lists[wave][k + 1] > mine);
         if (rank < a.picks) sorted[wave][rank] = mine;
     }
     n = min(n, a.picks);
@@ -340,19 +344,19 @@ static __global__ __launch_bounds__(BS_THREADS, 5) void beam_stretch_kernel(Beam
     for (int i = threadIdx.x; i < BS_WAVES * a.picks; i += BS_THREADS) {
         const int w = i / a.picks, r = i % a.picks;
         if (r < counts[w]) {
-            const BeamPick mine = sorted[w][r];
-            int rank = r;
-            for (int o = 0; o < BS_WAVES; o++) {
-                if (o == w) continue;
-                int lo = 0, hi = counts[o];
-                while (lo < hi) {
-                    const int mid = (lo + hi) / 2;
-                    if (beats(sorted[o][mid], mine)) lo = mid + 1;
-                    else hi = mid;
+            const uint64_t mine = sorted[w][r];
+            int above[BS_WAVES] = {}, rank = 0;  // of its own list: r
+            for (int step = BS_MAX_PICKS; step > 0; step /= 2)
+#pragma unroll
+                for (int o = 0; o < BS_WAVES; o++) {
+                    const int at = above[o] + step;
+                    const bool more = sorted[o][min(at, BS_MAX_PICKS) - 1] > mine;
+                    if (at <= counts[o] && more) above[o] = at;
                 }
-                rank += lo;
-            }
-            if (rank < a.picks) best[rank] = {mine.x, mine.token + first};
+#pragma unroll
+            for (int o = 0; o < BS_WAVES; o++) rank += above[o];
+            const BeamPick pick = pick_of(mine);
+            if (rank < a.picks) best[rank] = {pick.x, pick.token + first};
         }
         if (i < a.picks && i >= total) best[i] = {0.0f, -1};
     }
@@ -373,7 +377,7 @@ static __global__ __launch_bounds__(BS_THREADS, 5) void beam_stretch_kernel(Beam
 struct BeamKey {
     uint64_t a, b;
 };
-VH_DEVICE bool key_less(const BeamKey &x, const BeamKey &y) { return x.a < y.a || (x.a == y.a && x.b < y.b); }
+VH_DEVICE bool key_less(const BeamKey &x, const BeamKey &y) { return (x.a < y.a) | ((x.a == y.a) & (x.b < y.b)); }
 VH_DEVICE uint64_t score_down(double s) {
     const uint64_t u = (uint64_t)__double_as_longlong(s + 0.0);
     return ~(u ^ ((uint64_t)((int64_t)u >> 63) | 0x8000000000000000ull));

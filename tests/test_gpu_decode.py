@@ -574,6 +574,21 @@ def test_beams_without_numbers(ctx):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("top", [1.0e4, 1.7e7, 5.4e8, 1.07e9, 1.08e9, 2.2e9, 3.3e38, -1.7e7, -1.07e9, -3.3e38])
+def test_beams_large_logits(ctx, top, dtype):
+    """Logits around a large number: the largest one several times, the next numbers of the type, ones far below, -0."""
+    x = torch.full((1, 2, 5000), -0.0 if top > 0 else 1.02 * top)
+    up = torch.tensor(top).to(dtype)
+    for beam, alike in ((0, 3), (1, 4)):
+        v = up.clone()
+        for token in (4990, 17, 2500):
+            x[0, beam, token] = float(v)
+            v = torch.nextafter(v, torch.tensor(-math.inf, dtype=dtype))
+        x[0, beam, 100:100 + alike] = float(up)
+    check_beams(ctx, x.to(dtype), torch.tensor([[-1.0, -1.5]]), 6)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("V", [200, 5000, 40000])
 @pytest.mark.parametrize("allowed,picks", [(0, 64), (3, 64), (3, 5), (40, 64), (64, 64), (300, 64), (1000, 16)])
 def test_beams_few_tokens_allowed(ctx, V, allowed, picks, dtype):
