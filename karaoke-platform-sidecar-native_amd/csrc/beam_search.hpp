@@ -38,6 +38,7 @@ struct BeamArgs {
     float *new_scores;
     char *parts;                      // [sequences * beams][stretches] of part_bytes
     int S, B, V, picks, end_token, stretches, stretch, part_bytes;
+    Divisor per_list, per_beam;       // picks, stretches
 };
 
 // The order of floats as whole numbers; -0 as 0.
@@ -392,12 +393,14 @@ struct BeamState {
     double lse, score;
     int state, ended;
 };
-// Beam b's candidate `in` of its stretches' lists; (-1, -1): none.
-VH_DEVICE BeamPick listed(const BeamArgs &a, int s, int beam, int in) {
-    const char *p = a.parts + ((int64_t)(s * a.B + beam) * a.stretches + in / a.picks) * a.part_bytes;
-    return reinterpret_cast<const BeamPick *>(p + sizeof(BeamPart))[in % a.picks];
+// Candidate r of a sequence's list; (-1, -1): none.
+VH_DEVICE BeamPick listed(const BeamArgs &a, int s, int list, int r) {
+    const char *p = a.parts + ((int64_t)s * a.B * a.stretches + list) * a.part_bytes;
+    return reinterpret_cast<const BeamPick *>(p + sizeof(BeamPart))[r];
 }
-VH_DEVICE BeamKey candidate(const BeamArgs &a, int beam, int in, const BeamState &st, const BeamPick &pick) {
+VH_DEVICE BeamKey candidate(const BeamArgs &a, int list, int r, const BeamState *beams, const BeamPick &pick) {
+    const int beam = (int)((uint32_t)list / a.per_beam), in = (list - beam * a.stretches) * a.picks + r;
+    const BeamState &st = beams[beam];
     const BeamKey none{~0ull, ~0ull};
     const double score = st.score;
     if (st.state) {  // the end token with the score as it is, then the others in order
@@ -441,11 +444,22 @@ static __global__ __launch_bounds__(BS_JOIN) void beam_join_kernel(BeamArgs a) {
     __shared__ BeamKey limit;
     __shared__ int left;
     const int s = (int)blockIdx.x, tid = (int)threadIdx.x;
-    const int lists = a.B * a.stretches, per_beam = a.stretches * a.picks, all = a.B * per_beam;
-    // a thread's candidate, where they are as few, asked for while the sums are on their way
-    BeamPick early{0.0f, -1};
-    if (tid < all) early = listed(a, s, tid / per_beam, tid % per_beam);
-    // a beam's 16 lanes (a beam after the other): the logarithm of its sum
+    const int lists = a.B * a.stretches, all = lists * a.picks;
+    const int place = min(a.picks, (4 * a.picks + lists - 1) / lists) - 1, need = (a.picks + place) / (place + 1);
+    // a thread's candidates, as long as they are few, asked for while the sums are on their way
+    auto place_of = [&](int e) {
+        const int list = (int)((uint32_t)e / a.per_list);
+        return int2{list, e - list * a.picks};
+    };
+    constexpr int EARLY = 4;
+    BeamPick at_place{0.0f, -1}, early[EARLY];
+    if (tid < lists) at_place = listed(a, s, tid, place);
+#pragma unroll
+    for (int k = 0; k < EARLY; k++) {
+        early[k] = {0.0f, -1};
+        const int2 at = place_of(tid + k * BS_JOIN);
+        if (tid + k * BS_JOIN < all) early[k] = listed(a, s, at.x, at.y);
+    }
     if (tid == 0) {
         left = 0;
         limit = {~0ull, ~0ull};
@@ -484,11 +498,7 @@ static __global__ __launch_bounds__(BS_JOIN) void beam_join_kernel(BeamArgs a) {
     }
     __syncthreads();
     if (lists <= BS_LISTS) {
-        const int place = min(a.picks, (4 * a.picks + lists - 1) / lists) - 1, need = (a.picks + place) / (place + 1);
-        for (int e = tid; e < all; e += BS_JOIN) {
-            const int beam = e / per_beam, in = e - beam * per_beam;
-            if (in % a.picks == place) keys[e / a.picks] = candidate(a, beam, in, beams[beam], e == tid ? early : listed(a, s, beam, in));
-        }
+        if (tid < lists) keys[tid] = candidate(a, tid, place, beams, at_place);
         __syncthreads();
         if (tid < lists) {
             const BeamKey mine = keys[tid];
@@ -499,11 +509,17 @@ static __global__ __launch_bounds__(BS_JOIN) void beam_join_kernel(BeamArgs a) {
         }
         __syncthreads();
         const BeamKey most = limit;
-        for (int e = tid; e < all; e += BS_JOIN) {
-            const int beam = e / per_beam;
-            const int in = e - beam * per_beam;
-            const BeamKey key = candidate(a, beam, in, beams[beam], e == tid ? early : listed(a, s, beam, in));
+        auto take = [&](int e, const BeamPick &pick) {
+            const int2 at = place_of(e);
+            const BeamKey key = candidate(a, at.x, at.y, beams, pick);
             if (~key.a && !key_less(most, key)) keys[atomicAdd(&left, 1)] = key;  // in any order: ranked below
+        };
+#pragma unroll
+        for (int k = 0; k < EARLY; k++)
+            if (tid + k * BS_JOIN < all) take(tid + k * BS_JOIN, early[k]);
+        for (int e = tid + EARLY * BS_JOIN; e < all; e += BS_JOIN) {
+            const int2 at = place_of(e);
+            take(e, listed(a, s, at.x, at.y));
         }
         __syncthreads();
         const int n = left;
@@ -521,9 +537,8 @@ static __global__ __launch_bounds__(BS_JOIN) void beam_join_kernel(BeamArgs a) {
     for (int done = 0; done < all;) {
         const int take = min(all - done, BS_JOIN - held);
         for (int i = tid; i < BS_JOIN - held; i += BS_JOIN) {
-            const int e = done + i, beam = e / per_beam;
-            const int in = e - beam * per_beam;
-            keys[held + i] = i < take ? candidate(a, beam, in, beams[beam], listed(a, s, beam, in)) : none;
+            const int2 at = place_of(done + i);
+            keys[held + i] = i < take ? candidate(a, at.x, at.y, beams, listed(a, s, at.x, at.y)) : none;
         }
         __syncthreads();
         for (int k = 2; k <= BS_JOIN; k *= 2)

@@ -606,6 +606,8 @@ bool beam_select(hipStream_t s, const vh_beam *b, const void *logits, const floa
     a.stretches = cut.stretches;
     a.stretch = cut.stretch;
     a.part_bytes = cut.part_bytes;
+    a.per_list = divisor((uint32_t)a.picks);
+    a.per_beam = divisor((uint32_t)a.stretches);
     Scope sc(t, s, "beam_select");
     const int64_t groups = (int64_t)a.S * a.B * a.stretches;
     if (b->type == VH_TYPE_BF16) beam_launch<bf16>(s, a, cut.vectors, groups);
