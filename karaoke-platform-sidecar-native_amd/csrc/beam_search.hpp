@@ -6,7 +6,10 @@
 // of (x down, token), so the vocabulary is looked through once, in x: a workgroup takes
 // a stretch of a beam's logits in registers, adds up its exponentials and finds its
 // best `picks`; a second launch joins the stretches of a sequence's beams, in 64 bits.
-// Bound by HBM: the logits are read once.
+// The logits are read once: 256 rows of 120001 in bf16, 61 MB, 23 us (2.7 TB/s) and 7 us
+// for the join of 16 picks.  Two rounds of workgroups load and then compute; the VALU is
+// busy in 67% of the cycles, half of it for the maximum and the exponentials, half for the
+// best.  A step of one request is two launches, 4 to 6 us each.
 #pragma once
 
 #include "paged_cache.hpp"
@@ -284,8 +287,8 @@ static __global__ __launch_bounds__(BS_THREADS, 5) void beam_stretch_kernel(Beam
         if (place.skip) x[j].leave_out(place.skip);
     }
     // the vectors' largest, the lane's, the wave's, and the sum of exponentials (a NaN stays
-    // one); in one pass, from the first vector's largest, it took 37.7 us a call instead of
-    // 33.5 (256 rows of 120001): more registers, for the case that this is far too small
+    // one); in one pass, from the first vector's largest, 256 rows of 120001 took 13% longer:
+    // more registers, for the case that this is far too small
     float tops_of[NV], top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < NV; j++) {

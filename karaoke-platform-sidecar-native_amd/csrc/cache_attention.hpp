@@ -22,8 +22,8 @@
 // Single tokens are bound by HBM, the cache is read once: 32 of 32 heads on 8 of 128 over
 // 16384 keys each, 8 bits, 1.07 GB in 162 us (6.6 TB/s; with loads that stay in the caches
 // 185, without asking for the next step's 182).  Chunks are bound by the vector
-// instructions, the exponentials and conversions (62 to 75% of the cycles; the matrix
-// instructions 15%): 4 x 517 causal tokens of 16 heads on 4 of 64 over up to 4613 keys
+// instructions, the exponentials and conversions (83% of a busy CU's cycles; the matrix
+// instructions 21%): 4 x 517 causal tokens of 16 heads on 4 of 64 over up to 4613 keys
 // 61 us; with P's base moved at every larger maximum 70, with keys unbiased 64, with 128
 // registers and four waves a SIMD 80 instead of 67.
 #pragma once

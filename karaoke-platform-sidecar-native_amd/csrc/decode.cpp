@@ -511,9 +511,9 @@ bool cache_attention(hipStream_t s, const vh_cache *c, const vh_cache_queries *q
 // --------------------------------------------------------------- beam search
 // A stretch of a beam's logits, the vectors of 8 that a thread takes of it (of bf16 up
 // to 8, of fp32 4: the same registers); shorter stretches while there are fewer than
-// half as many workgroups as CUs.  32 x 8 beams over 120001 tokens, 16 picks: 33.5 us with
-// 8 vectors, 38.2 with 4; 16 rows of 32003: 14.1 us, cut down to twice as many workgroups
-// as CUs 14.9 (more lists to join).
+// half as many workgroups as CUs.  32 x 8 beams over 120001 tokens, 16 picks: 28.6 us with
+// 8 vectors, 31.2 with 4; 8 x 32 over 32003, 64 picks: 32 and 40; 16 rows of 32003: 12.1
+// us, cut down to twice as many workgroups as CUs 12.8 (more lists to join).
 struct BeamCut {
     int vectors, stretch, stretches, part_bytes;
 };
