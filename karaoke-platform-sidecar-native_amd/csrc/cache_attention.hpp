@@ -175,6 +175,12 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
     // bf16 out: keys enter as 1152 more than they are, and the scores begin so much lower:
     // sums 1152 / 40 times as large, whose fp32 roundings stay below those of fp16 queries
     constexpr bool BIASED = I8 && N == 1;
+    // Keys are asked for one step ahead when the last ones are multiplied, values likewise,
+    // each in its one place, where two steps at once do not fit the registers: 4 x 512 causal
+    // tokens of 32 heads on 8 of 128 over 4608 bf16 keys 158 us, twice kept 260 (32 registers
+    // spilled).  Elsewhere two steps are kept: 8 bits 155 us against 167, 64 dims 223 against
+    // 244, fp32 316 against 342.
+    constexpr bool ROLLING = !I8 && D == 128 && RG > 1;
     constexpr float P_SCALE = I8 ? 0x1p10f : 1.0f;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int i = lane & 15, g = lane >> 4;
@@ -304,7 +310,16 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
         if constexpr (SPLIT && RG == 1) return __builtin_nontemporal_load(from);  // each key is read by one wave
         else return *from;
     };
-    auto load = [&](Step &st, int step) {
+    auto load_values = [&](Step &st, int step) {
+        const int at = step % PER_FETCH * KB;
+#pragma unroll
+        for (int b = 0; b < KB; b++) {
+            const uint64_t from = (uint64_t)read_lane(at_hi, at + b) << 32 | read_lane(at_lo, at + b);
+#pragma unroll
+            for (int u = 0; u < B::UNITS; u++) st.v.w[b][u] = take(from, B::PART + 1024 * u);
+        }
+    };
+    auto load = [&](Step &st, int step) {  // keys, and values where both are kept twice
         const int at = step % PER_FETCH * KB;
         if (at == 0) fetch(step);
         st.there = (uint32_t)(there >> at) & ((1u << KB) - 1);
@@ -313,8 +328,9 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
             const uint64_t from = (uint64_t)read_lane(at_hi, at + b) << 32 | read_lane(at_lo, at + b);
 #pragma unroll
             for (int u = 0; u < B::UNITS; u++) st.k.w[b][u] = take(from, 1024 * u);
+            if constexpr (!ROLLING)
 #pragma unroll
-            for (int u = 0; u < B::UNITS; u++) st.v.w[b][u] = take(from, B::PART + 1024 * u);
+                for (int u = 0; u < B::UNITS; u++) st.v.w[b][u] = take(from, B::PART + 1024 * u);
             if constexpr (I8) {
                 st.sk[b] = __uint_as_float(read_lane(__float_as_uint(sk), at + b));
                 st.sv[b] = __uint_as_float(read_lane(__float_as_uint(sv), at + b));
@@ -324,7 +340,8 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
 
     auto compute = [&](Step &st, int step) {
         const int first = block_of(step) * PC_BLOCK;
-        const bool whole = first + KB * PC_BLOCK <= all_see && st.there == (1u << KB) - 1;
+        const uint32_t held = st.there;
+        const bool whole = first + KB * PC_BLOCK <= all_see && held == (1u << KB) - 1;
         floatx4 x[RG][KB];
 #pragma unroll
         for (int rg = 0; rg < RG; rg++)
@@ -340,6 +357,7 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
 #pragma unroll
                     for (int n = N - 1; n >= 0; n--) x[rg][b] = Op::mfma(k, qf[rg][m][n], x[rg][b]);
             }
+        if (ROLLING && step + 1 < steps) load(st, step + 1);
         // bf16: what lies behind the keys may be no number, which a probability of 0 does not hide
         if (!I8 && !whole) {
 #pragma unroll
@@ -350,7 +368,7 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
                     for (int d = 0; d < 4; d++) {
                         // a word holds tokens 4 g + 2 (d % 2) and the next
                         const int key = first + 16 * b + 4 * g + 2 * (d % 2);
-                        uint32_t keep = (st.there >> b & 1) == 0 || key >= upto ? 0u : key + 1 >= upto ? 0xffffu : ~0u;
+                        uint32_t keep = (held >> b & 1) == 0 || key >= upto ? 0u : key + 1 >= upto ? 0xffffu : ~0u;
                         st.v.w[b][u][d] &= keep;
                     }
         }
@@ -366,7 +384,7 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
 #pragma unroll
                 for (int b = 0; b < KB; b++) {
                     if (f[rg][b] < FLT_LEAST) f[rg][b] = FLT_LEAST;  // 0 times -inf is no number; a NaN stays
-                    const int keys_of_block = (st.there >> b & 1) ? limit[rg] - (first + 16 * b + 4 * g) : 0;
+                    const int keys_of_block = (held >> b & 1) ? limit[rg] - (first + 16 * b + 4 * g) : 0;
 #pragma unroll
                     for (int r = 0; r < 4; r++)
                         if (r >= keys_of_block) x[rg][b][r] = -INFINITY;
@@ -440,18 +458,26 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
 #pragma unroll
                     for (int n = N - 1; n >= 0; n--) o[rg][t] = Op::mfma(v, pf[rg][c][n], o[rg][t]);
             }
+        if (ROLLING && step + 1 < steps) load_values(st, step + 1);
     };
 
     // the next step's blocks are on their way while one is computed
     Step even, odd;
-    if (steps > 0) load(even, 0);
+    if (steps > 0) {
+        load(even, 0);
+        if constexpr (ROLLING) load_values(even, 0);
+    }
     prepare_rows();
-    for (int step = 0; step < steps; step += 2) {
-        if (step + 1 < steps) load(odd, step + 1);
-        compute(even, step);
-        if (step + 1 >= steps) break;
-        if (step + 2 < steps) load(even, step + 2);
-        compute(odd, step + 1);
+    for (int step = 0; step < steps; step += ROLLING ? 1 : 2) {
+        if constexpr (ROLLING) {
+            compute(even, step);
+        } else {
+            if (step + 1 < steps) load(odd, step + 1);
+            compute(even, step);
+            if (step + 1 >= steps) break;
+            if (step + 2 < steps) load(even, step + 2);
+            compute(odd, step + 1);
+        }
     }
 
     // in the values' own units
