@@ -12,6 +12,7 @@
 // best.  A step of one request is two launches, 4 to 6 us each.
 #pragma once
 
+#include "beam_floor.hpp"
 #include "paged_cache.hpp"
 
 namespace vh {
@@ -149,38 +150,27 @@ VH_DEVICE int collect(const T *p, bool whole, const Logits<T> (&x)[NV], const fl
     int n = 0;
     // The vectors that have such a logit, where few, are put where all lanes see them; of more,
     // those that reach a higher floor, as long as that leaves `most`.
-    auto with = [&](float least) {
+    auto with = [&](uint32_t least) {
         int vectors = 0;
 #pragma unroll
-        for (int j = 0; j < NV; j++) vectors += __popcll(__ballot(top[j] >= least));
+        for (int j = 0; j < NV; j++) vectors += __popcll(__ballot(top[j] >= from_ordered(least)));
         return vectors;
     };
     float largest = top[0];
 #pragma unroll
     for (int j = 1; j < NV; j++) largest = fmaxf(largest, top[j]);
     const uint32_t lowest = ordered(floor), highest = ordered(wave_max(largest));
-    int found = with(floor);
-    if (found > BS_VECTORS) {
-        uint32_t lo = lowest, hi = highest;  // at lo too many, above hi too few
-        while (lo < hi) {
-            const uint32_t trial = lo + (hi - lo + 1) / 2;
-            found = with(from_ordered(trial));
-            if (found >= most) lo = trial;
-            else hi = trial - 1;
-            if (found >= most && found <= BS_VECTORS) {
-                floor = from_ordered(trial);
-                break;
-            }
-        }
-    }
+    const BeamFloor chosen = beam_floor(lowest, highest, most, BS_VECTORS, with);
+    floor = from_ordered(chosen.least);
+    const bool few = chosen.vectors <= BS_VECTORS;
     int vectors = 0;
-    if (found <= BS_VECTORS)
+    if (few)
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const bool has = top[j] >= floor;
         const uint64_t m = __ballot(has);
         const int k = vectors + __popcll(m & below);
-        if (has) {
+        if (has && k < BS_VECTORS) {
             const BeamPlace place(j, thread, valid);
             some.x[k] = x[j];
             some.at[k] = place.at;
@@ -188,7 +178,7 @@ VH_DEVICE int collect(const T *p, bool whole, const Logits<T> (&x)[NV], const fl
         }
         vectors += __popcll(m);
     }
-    if (found <= BS_VECTORS) {
+    if (few) {
         cache_wave_order();
         for (int i0 = 0; i0 < 8 * vectors; i0 += 64) {
             const int i = i0 + lane, k = min(i / 8, BS_VECTORS - 1), e = i % 8;

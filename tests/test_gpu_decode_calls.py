@@ -1,0 +1,94 @@
+"""Calls of the decoding operators that take each of their kernels' forms: sizes of a batch, and inputs that are masked, equal
+or rounded."""
+
+import math
+
+import pytest
+import torch
+
+import decode_ref as R
+from helpers import gpu_available
+
+pytestmark = pytest.mark.gpu
+
+if gpu_available():
+    from vocalarc_hip import native
+
+DEV = "cuda:0"
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    c = native.Context()
+    yield c
+    c.close()
+
+
+# ---------------------------------------------------------------- beam search
+
+def beam_logits(shape, S, B, V, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(S, B, V, generator=g)
+    if shape == "normal":
+        return (3 * x).to(dtype)
+    if shape == "rounded":
+        return torch.round(3 * x).to(dtype)
+    if shape == "one lane":  # of a wave's 64, whose 8 consecutive logits are all larger than the others'
+        return (x / 8 + 4.0 * (torch.arange(V) // 8 % 64 == 9)).to(dtype)
+    kind, count = shape
+    rest = {"allowed": -math.inf, "filled": -1.0e4, "above": 0.0}[kind]
+    y = torch.full((S, B, V), rest)
+    where = torch.rand(S, B, V, generator=g).topk(count).indices if count else torch.zeros(S, B, 0, dtype=torch.long)
+    values = torch.randint(1, 4, (S, B, count), generator=g).float() if kind == "above" else x[..., :count]
+    return y.scatter(2, where, values).to(dtype)
+
+
+def beam_scores(S, B, seed):
+    return -4 * torch.rand(S, B, generator=torch.Generator().manual_seed(seed))
+
+
+def best_of(logits, scores, picks):
+    """[S][picks] of (score, beam, token) in the order that the header gives, and the smallest distance of two beams' scores
+    that follow each other there."""
+    x = logits.double()
+    v, t = torch.sort(x, dim=2, descending=True, stable=True)
+    v, t = v[..., :picks + 1], t[..., :picks + 1]
+    v = scores.double()[..., None] + (v - torch.logsumexp(x, 2, keepdim=True))
+    found, near = [], math.inf
+    for s in range(x.shape[0]):
+        # a beam's own are in order; those of several that are equal, of the lower beam first
+        c = [(float(a), b, int(i)) for b in range(x.shape[1]) for a, i in zip(v[s, b], t[s, b])]
+        c.sort(key=lambda e: (-e[0], e[1]))
+        near = min([near] + [a[0] - b[0] for a, b in zip(c[:picks], c[1:picks + 1]) if a[1] != b[1] and math.isfinite(a[0])])
+        found.append(c[:picks])
+    return found, near
+
+
+# rows and vocabularies that give a thread 1, 2, 4 and (bf16) 8 vectors of 8 logits
+BEAM_SIZES = [(F32, 2, 4, 5003, 8, 1), (F32, 4, 4, 32003, 64, 2), (F32, 4, 4, 60007, 16, 4), (BF16, 2, 4, 5003, 8, 1),
+              (BF16, 4, 4, 32003, 5, 2), (BF16, 8, 4, 32003, 8, 4), (BF16, 4, 4, 120_001, 16, 8), (BF16, 4, 4, 120_001, 64, 8)]
+BEAM_SHAPES = ["normal", "rounded", "one lane", ("allowed", 4), ("allowed", 12), ("allowed", 60), ("allowed", 200), ("filled", 1),
+               ("filled", 12), ("filled", 700), ("above", 0), ("above", 1), ("above", 7), ("above", 63)]
+
+
+@pytest.mark.parametrize("dtype,S,B,V,picks,vectors", BEAM_SIZES)
+@pytest.mark.parametrize("shape", BEAM_SHAPES, ids=str)
+def test_beams_of_any_logits(ctx, shape, dtype, S, B, V, picks, vectors):
+    """Masked, equal and rounded logits, where few of a wave's vectors stand out or more than there is room for."""
+    logits, scores = beam_logits(shape, S, B, V, dtype, V + picks), beam_scores(S, B, 3)
+    want, near = best_of(logits, scores, picks)
+    assert near > 2.0 ** -19, near  # what the sum of exponentials may be off by, twice
+    g = logits.to(DEV)
+    search = native.BeamSearch(ctx, g, picks=picks)
+    # a list of picks for each stretch of 2048 logits and as many times more as a thread has vectors
+    part = 16 + (picks + 1) // 2 * 16
+    assert search.workspace_bytes() == S * B * -(-V // (2048 * vectors)) * part
+    tokens, parents = (torch.full((S, picks), -5, dtype=torch.int32, device=DEV) for _ in range(2))
+    new = torch.full((S, picks), 5.0, device=DEV)
+    ws = torch.full((search.workspace_bytes(),), 0xff, dtype=torch.uint8, device=DEV)
+    search.select(g, scores.to(DEV), tokens, parents, new, workspace=ws)
+    for s in range(S):
+        assert list(zip(parents[s].tolist(), tokens[s].tolist())) == [(b, t) for _, b, t in want[s]], s
+        for got, (v, _, _) in zip(new[s].tolist(), want[s]):
+            assert got == v if math.isinf(v) else abs(got - v) <= 2.0 ** -20 + R.U * abs(v), s
