@@ -417,8 +417,7 @@ typedef struct {
    row's neighbours see and it does not, causal, may reach it (0 times it is NaN).
    Products run on the matrix cores: over int8 pages, whose whole numbers fp16 holds,
    q' and the probabilities are fp16 times a power of two each (fp32 out: two fp16, 22
-   bits), over bf16 pages bf16 (bf16 out of up to 16 rows, query heads of a key head times
-   length: two, 16 bits; fp32 out: three, 24 bits); the rest is fp32.
+   bits), over bf16 pages two bf16 (16 bits; fp32 out: three, 24 bits); the rest is fp32.
    workspace: vh_cache_workspace_bytes(c, q) bytes of device memory, 16-byte aligned,
    free again when the call's work is done; graphs that may run at once need one each.
    q and out: 16-byte aligned; out may be q (with its strides), else overlaps nothing.

@@ -17,7 +17,7 @@
 // power of two (its largest just below 2^14, so 2^-25 of that is what a small one is
 // off by), the block's scale of keys as a factor of the scores.  P, up to 2^4, enters
 // times the block's scale of values over the largest one so far, times 2^10.  fp32 out: q' and P
-// in two fp16 values each.  Over bf16 pages: bf16, fp32 out: three bf16 values each.
+// in two fp16 values each.  Over bf16 pages: two bf16 values each, fp32 out: three.
 //
 // Single tokens are bound by HBM, the cache is read once: 32 of 32 heads on 8 of 128 over
 // 16384 keys each, 8 bits, 1.07 GB in 162 us (6.6 TB/s; with loads that stay in the caches
@@ -167,9 +167,11 @@ template <typename T, int D, bool I8, int RG, bool SPLIT>
 static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAttentionArgs a) {
     using B = BlockShape<D, I8>;
     using Op = Operand16<I8>;
-    // of q' and P: bf16 out one operand, but two where the cache's bytes are what takes the
-    // time; fp32 out as many as 22 bits and more take
-    constexpr int DT = B::DT, QS = D / 32, N = sizeof(T) == 2 ? (RG == 1 && !I8 ? 2 : 1) : I8 ? 2 : 3;
+    // of q' and P: bf16 out over 8 bits one operand (fp16's 11 bits, three more than out's),
+    // over bf16 pages two, 16 bits: one has no more bits than out, and 4 x 512 causal tokens
+    // over 4608 keys had 1.8 times the error of products in fp32 with it (3.0e-3 of the norm
+    // for 1.66e-3; 161 us, with two 214).  fp32 out as many as 22 bits and more take
+    constexpr int DT = B::DT, QS = D / 32, N = sizeof(T) == 2 ? (I8 ? 1 : 2) : I8 ? 2 : 3;
     constexpr int ROWS = 16 * RG * (SPLIT ? 1 : 4);
     constexpr int KB = CQ_STEP, PER_FETCH = 64 / KB;
     // bf16 out: keys enter as 1152 more than they are, and the scores begin so much lower:
@@ -177,9 +179,9 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
     constexpr bool BIASED = I8 && N == 1;
     // Keys are asked for one step ahead when the last ones are multiplied, values likewise,
     // each in its one place, where two steps at once do not fit the registers: 4 x 512 causal
-    // tokens of 32 heads on 8 of 128 over 4608 bf16 keys 158 us, twice kept 260 (32 registers
-    // spilled).  Elsewhere two steps are kept: 8 bits 155 us against 167, 64 dims 223 against
-    // 244, fp32 316 against 342.
+    // tokens of 32 heads on 8 of 128 over 4608 bf16 keys 211 us, twice kept 885 (74 registers
+    // spilled).  Elsewhere two steps are kept: these tokens over 8 bits 155 us against 167, 16 x
+    // 2048 tokens of 16 heads on 4 of 64 over as many bf16 keys 338 against 334.
     constexpr bool ROLLING = !I8 && D == 128 && RG > 1;
     constexpr float P_SCALE = I8 ? 0x1p10f : 1.0f;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;

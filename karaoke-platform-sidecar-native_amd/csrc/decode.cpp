@@ -382,7 +382,8 @@ struct CacheCut {
 constexpr int CQ_MAX_ROWS = 1 << 30;
 constexpr int64_t CQ_ROWS = 512, CQ_PIECES = 512;
 // Groups of 16 rows of a wave at most: what 256 registers hold.  The 4 x 517 tokens above
-// 64 us with two, 75 with four (the registers spill); fp32 over 64 dims 39.5 with two, 43 with one.
+// 64 us with two, 75 with four (the registers spill); fp32 over 64 dims 39.5 with two, 43 with
+// one; the 4 x 512 tokens over bf16 pages 214 with two, 258 with one.
 constexpr int most_groups(int type, int head_dim) { return type == VH_TYPE_FP32 && head_dim == 128 ? 1 : 2; }
 static CacheCut cache_cut(const vh_cache *c, const vh_cache_queries *q) {
     CacheCut cut;

@@ -112,9 +112,10 @@ class Cache:
 
 # ---------------------------------------------------------------- attention
 
-def attention(kind, q, keys, values, *, scale, causal=False, start=0, turn=None):
+def attention(kind, q, keys, values, *, scale, causal=False, start=0, turn=None, operand=None):
     """q [L][H][D] of one sequence over keys and values [n][KV][D] (any type, 64 bits inside) -> (value, bound).
-    turn: the queries' rotation in 64 bits, q -> q'.  kind: of the cache; the queries' type says how it is rounded."""
+    turn: the queries' rotation in 64 bits, q -> q'.  kind: of the cache; the queries' type says how it is rounded.  operand:
+    what a value of q' and of P may be off by as an operand, where a test holds it to less."""
     dtype = q.dtype
     L, H, D = q.shape
     n, KV = keys.shape[:2]
@@ -123,7 +124,7 @@ def attention(kind, q, keys, values, *, scale, causal=False, start=0, turn=None)
     # what a value of q' and of P is off by as an operand: fp16 2^-11 a piece, bf16 2^-8
     piece, pieces = (2.0 ** -11, 1 if dtype == torch.bfloat16 else 2) if kind == "int8" else \
         (2.0 ** -8, 1 if dtype == torch.bfloat16 else 3)
-    operand = max(piece ** pieces, U)
+    operand = max(piece ** pieces, U) if operand is None else operand
     for h in range(H):
         g = h // (H // KV)
         qh, k, v = q64[:, h], keys[:, g].double(), values[:, g].double()

@@ -8,6 +8,7 @@ import torch
 
 import decode_ref as R
 from helpers import gpu_available
+from test_gpu_decode import World, attend, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -92,3 +93,23 @@ def test_beams_of_any_logits(ctx, shape, dtype, S, B, V, picks, vectors):
         assert list(zip(parents[s].tolist(), tokens[s].tolist())) == [(b, t) for _, b, t in want[s]], s
         for got, (v, _, _) in zip(new[s].tolist(), want[s]):
             assert got == v if math.isinf(v) else abs(got - v) <= 2.0 ** -20 + R.U * abs(v), s
+
+
+# ---------------------------------------------------------------- attention
+
+@pytest.mark.parametrize("L,KV,G,D", [(1, 1, 16, 64), (1, 1, 17, 64), (1, 2, 40, 128), (2, 3, 16, 64), (5, 2, 4, 128), (40, 1, 4, 64),
+                                      (150, 2, 1, 128), (33, 1, 2, 64)])
+@pytest.mark.parametrize("rotary", [None, 32])
+def test_bf16_pages_keep_their_bits(ctx, L, KV, G, D, rotary):
+    """bf16 queries over bf16 pages: q' and P are off by 2^-16, as 2^-8 of 2^-8, for any number of rows."""
+    n = [L + 300, L, 90 + L]
+    w = World(ctx, "bf16", 3, KV, D, 32, 300 + L, BF16, rotary, interleaved=True)
+    w.random(1, [0] * 3, n, gain=1.5)
+    q = randn(2, 3, L, KV * G, D, dtype=BF16)
+    start = [x - L for x in n]
+    out = attend(w, q, start=start, causal=True, scale=D ** -0.5, check=False)
+    for s in range(3):
+        turn = (lambda x, s=s: R.rotary(x[None], [start[s]], rotary, True)[0][0]) if rotary else None
+        val, tol = R.attention("bf16", q[s], w.ref.values(s, 0), w.ref.values(s, 1), scale=D ** -0.5, causal=True, start=start[s],
+                               turn=turn, operand=2.0 ** -16)
+        R.assert_within(out[s], val, tol, f"sequence {s}")
