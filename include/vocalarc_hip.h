@@ -413,11 +413,14 @@ typedef struct {
 /* out = softmax(scale q' k^T) v over the keys that a row sees, q' = q turned by
    `rotary` (may be null; as vh_cache_append's).  A row that sees none is 0.  Keys from
    a sequence's length on and behind the last that a row may see are not read beyond
-   their block of 16, and change nothing (int8: but for a block's NaN); NaN in what a
-   row's neighbours see and it does not, causal, may reach it (0 times it is NaN).
-   Products run on the matrix cores: over int8 pages, whose whole numbers fp16 holds,
-   q' and the probabilities are fp16 times a power of two each (fp32 out: two fp16, 22
-   bits), over bf16 pages two bf16 (16 bits; fp32 out: three, 24 bits); the rest is fp32.
+   their block of 16, and change no bit of it (int8: but by the scale, a NaN's too, of a
+   block that it sees part of; bf16: a NaN or infinity in what a row's neighbours see and
+   it does not, causal, may reach it, as 0 times that is NaN).
+   Products run on the matrix cores: over int8 pages, whose whole numbers fp16 holds, q'
+   is fp16 times a power of two, a probability fp16 times its block's scale of values over
+   the largest scale that the row sees (2^-35 of the largest value is lost; fp32 out: two
+   fp16, 22 bits), over bf16 pages two bf16 (16 bits; fp32 out: three, 24 bits); the rest
+   is fp32.
    workspace: vh_cache_workspace_bytes(c, q) bytes of device memory, 16-byte aligned,
    free again when the call's work is done; graphs that may run at once need one each.
    q and out: 16-byte aligned; out may be q (with its strides), else overlaps nothing.

@@ -16,7 +16,8 @@
 // permute and an addition: 0x6400 + u is 1024 + u); a row of q' enters as fp16 times a
 // power of two (its largest just below 2^14, so 2^-25 of that is what a small one is
 // off by), the block's scale of keys as a factor of the scores.  P, up to 2^4, enters
-// times the block's scale of values over the largest one so far, times 2^10.  fp32 out: q' and P
+// times the block's scale of values over the largest one that the row has seen, times 2^10:
+// what is below 2^-35 of the largest value that a row sees is lost.  fp32 out: q' and P
 // in two fp16 values each.  Over bf16 pages: two bf16 values each, fp32 out: three.
 //
 // Single tokens are bound by HBM, the cache is read once: 32 of 32 heads on 8 of 128 over
@@ -162,9 +163,11 @@ constexpr float FLT_LEAST = 0x1p-126f;
 constexpr float LAZY = 4.0f;  // P up to 2^LAZY: times P_SCALE it is fp16's
 
 // SPLIT: a workgroup's four waves share the rows, each every fourth step of the keys,
-// and join; else each wave has rows of its own.
+// and join; else each wave has rows of its own.  Three waves a SIMD hold fp32's 32 rows of 64
+// dims over 8 bits, with 4 registers spilled: 4 x 300 tokens of 16 heads on 4 over 2613 keys
+// 40.5 us, with two waves and 184 registers 43.
 template <typename T, int D, bool I8, int RG, bool SPLIT>
-static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAttentionArgs a) {
+static __global__ __launch_bounds__(256, D == 64 && I8 ? 3 : 2) void cache_attention_kernel(CacheAttentionArgs a) {
     using B = BlockShape<D, I8>;
     using Op = Operand16<I8>;
     // of q' and P: bf16 out over 8 bits one operand (fp16's 11 bits, three more than out's),
@@ -258,14 +261,15 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
 
     floatx4 o[RG][DT];
     float m_run[RG], l_run[RG];
+    float v_top[RG];  // the largest scale of values that the row has seen so far
 #pragma unroll
     for (int rg = 0; rg < RG; rg++) {
 #pragma unroll
         for (int t = 0; t < DT; t++) o[rg][t] = (floatx4){0, 0, 0, 0};
         m_run[rg] = -INFINITY;
         l_run[rg] = 0.0f;
+        v_top[rg] = 0x1p-100f;
     }
-    float v_top = 0x1p-100f;  // the largest scale of values so far
 
     const int block0 = part * a.piece;
     const int block1 = min(block0 + a.piece, (upto + PC_BLOCK - 1) / PC_BLOCK);
@@ -374,22 +378,27 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
                         st.v.w[b][u][d] &= keep;
                     }
         }
-        // scores to powers of two, s f; their largest in this lane
-        float f[RG][KB], top[RG];
+        // scores to powers of two, s f; their largest in this lane.  A row takes the scales of
+        // the blocks that it sees only: what it sees is all that its result depends on
+        float f[RG][KB], sv[RG][KB], top[RG];
 #pragma unroll
         for (int rg = 0; rg < RG; rg++)
 #pragma unroll
-            for (int b = 0; b < KB; b++) f[rg][b] = I8 ? factor[rg] * st.sk[b] : factor[rg];
+            for (int b = 0; b < KB; b++) {
+                f[rg][b] = I8 ? factor[rg] * st.sk[b] : factor[rg];
+                if constexpr (I8) sv[rg][b] = st.sv[b];
+            }
         if (!whole) {
 #pragma unroll
             for (int rg = 0; rg < RG; rg++)
 #pragma unroll
                 for (int b = 0; b < KB; b++) {
+                    const int keys_of_block = (held >> b & 1) ? limit[rg] - (first + 16 * b) : 0;
+                    if (I8 && keys_of_block <= 0) f[rg][b] = sv[rg][b] = 0.0f;
                     if (f[rg][b] < FLT_LEAST) f[rg][b] = FLT_LEAST;  // 0 times -inf is no number; a NaN stays
-                    const int keys_of_block = (held >> b & 1) ? limit[rg] - (first + 16 * b + 4 * g) : 0;
 #pragma unroll
                     for (int r = 0; r < 4; r++)
-                        if (r >= keys_of_block) x[rg][b][r] = -INFINITY;
+                        if (4 * g + r >= keys_of_block) x[rg][b][r] = -INFINITY;
                 }
         }
         bool over = false;
@@ -402,39 +411,40 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
                 top[rg] = larger(top[rg], most * f[rg][b]);
             }
             over |= top[rg] > m_run[rg] + LAZY;
-        }
-        float v_new = v_top;
-        if constexpr (I8)
+            if constexpr (I8)
 #pragma unroll
-            for (int b = 0; b < KB; b++) v_new = fmaxf(v_new, st.sv[b]);
-        // The exponents' base follows the maximum only when that is 2^LAZY beyond it, and the
-        // values' unit the largest scale: then all that was summed is rescaled.
-        if (__ballot(over || v_new > v_top)) {
-            const float shrink = I8 ? v_top / v_new : 1.0f;
-            v_top = v_new;
+                for (int b = 0; b < KB; b++) over |= sv[rg][b] > v_top[rg];
+        }
+        // A row's exponents' base follows its maximum only when that is 2^LAZY beyond it, and its
+        // values' unit the largest scale: then all that was summed of the row is rescaled, and
+        // that of the others times 1.
+        if (__ballot(over)) {
 #pragma unroll
             for (int rg = 0; rg < RG; rg++) {
                 float m = fmaxf(m_run[rg], top[rg]);
                 m = fmaxf(m, __shfl_xor(m, 16, 64));
                 m = fmaxf(m, __shfl_xor(m, 32, 64));
+                m = m > m_run[rg] + LAZY ? m : m_run[rg];
                 const float alpha = m == -INFINITY ? 0.0f : exp2_of(m_run[rg] - m);  // -inf - -inf is no number
                 m_run[rg] = m;
                 l_run[rg] *= alpha;
-                const float rescale = alpha * shrink;
+                float rescale = alpha;
+                if constexpr (I8) {
+                    float v_new = v_top[rg];
+#pragma unroll
+                    for (int b = 0; b < KB; b++) v_new = fmaxf(v_new, sv[rg][b]);
+                    rescale *= v_top[rg] / v_new;
+                    v_top[rg] = v_new;
+                }
 #pragma unroll
                 for (int t = 0; t < DT; t++) o[rg][t] *= rescale;
             }
-        }
-        float sv[KB];
-        if constexpr (I8) {
-            const float inv = P_SCALE * __builtin_amdgcn_rcpf(v_top);
-#pragma unroll
-            for (int b = 0; b < KB; b++) sv[b] = st.sv[b] * inv;
         }
         typename Op::type pf[RG][KB / 2][N];
 #pragma unroll
         for (int rg = 0; rg < RG; rg++) {
             const float base = m_run[rg] == -INFINITY ? 0.0f : m_run[rg];
+            const float inv = I8 ? P_SCALE * __builtin_amdgcn_rcpf(v_top[rg]) : 1.0f;
             float sum = 0.0f;
 #pragma unroll
             for (int c = 0; c < KB / 2; c++) {
@@ -444,7 +454,7 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
                     const int b = 2 * c + e / 4;
                     p[e] = exp2_of(__builtin_fmaf(x[rg][b][e % 4], f[rg][b], -base));
                     sum += p[e];
-                    if constexpr (I8) p[e] *= sv[b];
+                    if constexpr (I8) p[e] *= sv[rg][b] * inv;
                 }
                 split_n<I8, N>(p, pf[rg][c]);
             }
@@ -483,11 +493,11 @@ static __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAtt
     }
 
     // in the values' own units
-    const float unit = I8 ? v_top / P_SCALE : 1.0f;
+    if constexpr (I8)
 #pragma unroll
-    for (int rg = 0; rg < RG; rg++)
+        for (int rg = 0; rg < RG; rg++)
 #pragma unroll
-        for (int t = 0; t < DT; t++) o[rg][t] *= unit;
+            for (int t = 0; t < DT; t++) o[rg][t] *= v_top[rg] / P_SCALE;
 
     // The waves' sums of the same rows lie in the same lanes: half of the waves give theirs
     // to the others, twice.

@@ -113,3 +113,27 @@ def test_bf16_pages_keep_their_bits(ctx, L, KV, G, D, rotary):
         val, tol = R.attention("bf16", q[s], w.ref.values(s, 0), w.ref.values(s, 1), scale=D ** -0.5, causal=True, start=start[s],
                                turn=turn, operand=2.0 ** -16)
         R.assert_within(out[s], val, tol, f"sequence {s}")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", ["int8", "bf16"])
+@pytest.mark.parametrize("L,KV,G,D,before", [(64, 1, 1, 64, 0), (64, 2, 2, 128, 37), (20, 1, 4, 64, 300), (150, 1, 1, 128, 0), (40, 1, 2, 64, 3000)])
+def test_causal_rows_know_only_what_they_see(ctx, kind, L, KV, G, D, before, dtype):
+    """Later tokens in other blocks, 2^30 times larger or (8 bits) no numbers: a row before them is the same, bit for bit, and
+    as exact as if they were not there."""
+    n = before + L
+    first = -(-(before + L // 2) // 16) * 16  # a block's first token
+    q = randn(2, 1, L, KV * G, D, dtype=dtype)
+    results = []
+    for gain in (1.0, 2.0 ** 30, 2.0 ** -30, math.nan if kind == "int8" else 5.0):
+        w = World(ctx, kind, 1, KV, D, 64, n, dtype, 32)
+        w.random(1, [0], [first])
+        w.random(5, [first], [n - first], gain=gain)
+        out = attend(w, q, start=[before], causal=True, scale=D ** -0.5, check=False)
+        results.append(out[0, :first - before].cpu())
+    turn = lambda x: R.rotary(x[None], [before], 32, False)[0][0]  # noqa: E731
+    val, tol = R.attention(kind, q[0, :first - before], w.ref.values(0, 0, first), w.ref.values(0, 1, first), scale=D ** -0.5,
+                           causal=True, start=before, turn=turn)
+    for got in results:
+        R.assert_within(got, val, tol, "rows before")
+        assert torch.equal(got, results[0])
