@@ -454,7 +454,10 @@ typedef struct {
    log softmax(logits[b])[t] the best `picks`, best first: beams' numbers to parents,
    tokens, scores rounded to fp32, and whether the beam has ended to new_ended (may be
    null).  Scores are compared before they are rounded, in 64 bits; of equal ones the
-   lower beam is first, within a beam the larger logit, then the lower token.
+   lower beam is first, within a beam the larger logit, then the lower token.  A beam's
+   log sum exp, the same for all of its candidates, is made of exponentials and sums of
+   64 in fp32 and off by less than 2^-19 (2^-17 with logits from 2^20 on): candidates of
+   two beams that are closer than twice that may change places.
    scores: device fp32 [sequences][beams]; a beam whose score is not finite, or whose
    logits have a NaN, +inf or nothing but -inf, has candidates of -inf only, lowest
    token first.  ended (may be null; needs an end token): device int32

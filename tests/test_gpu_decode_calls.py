@@ -95,6 +95,41 @@ def test_beams_of_any_logits(ctx, shape, dtype, S, B, V, picks, vectors):
             assert got == v if math.isinf(v) else abs(got - v) <= 2.0 ** -20 + R.U * abs(v), s
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [3000, 8192, 16384])
+@pytest.mark.parametrize("case", ["normal", "flat", "steps", "far", "large", "largest"])
+def test_beams_sum_of_exponentials(ctx, case, V, dtype):
+    """The logarithm of the sum of exponentials is off by less than the header says: a beam's score takes it to nearly 0, of
+    which fp32 loses nothing."""
+    S = 128  # enough for a thread's most vectors
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(S, 1, V, generator=g)
+    if case == "flat":
+        x = 5 * x.clamp(-1, 1)
+    elif case == "steps":  # equal terms below the largest, whose sum is rounded the same way at each step
+        x = torch.linspace(-3, 0, S)[:, None, None].expand(S, 1, V).clone()
+        x[..., 7] = 0.25
+    elif case == "far":
+        x = 4 * x - 1000
+    elif case == "large":
+        x = x + 2.0 ** 21
+    elif case == "largest":
+        x = torch.where(x > 1, 2.0 ** 29 + 2.0 ** 27, 2.0 ** 20)
+    x = x.to(dtype)
+    lse, top = torch.logsumexp(x.double(), 2)[:, 0], x.amax(2)[:, 0].double()
+    scores = (lse - top).float()
+    logits = x.to(DEV)
+    search = native.BeamSearch(ctx, logits, picks=1)
+    tokens, parents = (torch.empty(S, 1, dtype=torch.int32, device=DEV) for _ in range(2))
+    new = torch.empty(S, 1, device=DEV)
+    search.select(logits, scores[:, None].to(DEV), tokens, parents, new,
+                  workspace=torch.empty(search.workspace_bytes(), dtype=torch.uint8, device=DEV))
+    off = new[:, 0].cpu().double() - (scores.double() + (top - lse))
+    loose = 2.0 ** -50 * lse.abs()  # of the definition itself, in 64 bits
+    limit = 2.0 ** -17 if case in ("large", "largest") else 2.0 ** -19
+    assert bool((off.abs() <= limit + loose).all()), float(off.abs().max())
+
+
 # ---------------------------------------------------------------- attention
 
 @pytest.mark.parametrize("L,KV,G,D", [(1, 1, 16, 64), (1, 1, 17, 64), (1, 2, 40, 128), (2, 3, 16, 64), (5, 2, 4, 128), (40, 1, 4, 64),
