@@ -172,3 +172,60 @@ def test_causal_rows_know_only_what_they_see(ctx, kind, L, KV, G, D, before, dty
     for got in results:
         R.assert_within(got, val, tol, "rows before")
         assert torch.equal(got, results[0])
+
+
+def rows_in(w, q, out, s, first, count, start, keys, scale):
+    """Rows first .. of sequence s against the definition."""
+    at = start[s] + first
+    turn = (lambda x: R.rotary(x[None], [at], w.rotary.c.dim, w.interleaved)[0][0]) if w.rotary else None
+    rows = slice(first, first + count)
+    operand = 2.0 ** -16 if w.ref.kind == "bf16" and q.dtype == BF16 else None
+    val, tol = R.attention(w.ref.kind, q[s, rows], w.ref.values(s, 0, keys[s]), w.ref.values(s, 1, keys[s]), scale=scale, causal=True,
+                           start=at, turn=turn, operand=operand)
+    R.assert_within(out[s, rows], val, tol, f"sequence {s}, rows from {first}")
+
+
+# From 64 (sequence, key head) pairs on, workgroups are dealt out to the XCDs pair by pair, and from 512 workgroups of 128
+# rows (fp32 of 128 dims: 64) on, each wave has rows of its own; a wave looks up 64 blocks of the table at a time.
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", ["int8", "bf16"])
+@pytest.mark.parametrize("S,KV,G,D,L,n", [(43, 3, 1, 64, 520, 1500), (43, 3, 1, 128, 520, 1500),  # rows of their own, 129 pairs
+                                          (4, 2, 4, 64, 2048, 2300),  # rows of their own, 8 pairs
+                                          (33, 2, 1, 64, 100, 700), (33, 2, 2, 128, 50, 700)])  # shared rows, 66 pairs
+def test_many_rows(ctx, kind, S, KV, G, D, L, n, dtype):
+    """Pieces of prompts of large batches, uneven, an empty slot among them."""
+    w = World(ctx, kind, S, KV, D, 64, n, dtype, 32, interleaved=True)
+    keys = [n - 37 * s % (n - 20) if s != 1 else 0 for s in range(S)]
+    rows = [min(L, k) for k in keys]
+    start = [k - r for k, r in zip(keys, rows)]
+    w.random(1, [0] * S, keys)
+    q = randn(2, S, L, KV * G, D, dtype=dtype)
+    out = attend(w, q, start=start, query_lengths=rows, causal=True, scale=D ** -0.5, check=False)
+    for s in (0, S // 2, S - 1):
+        for first in (0, rows[s] // 2, max(rows[s] - 9, 0)):
+            rows_in(w, q, out, s, first, min(9, rows[s] - first), start, keys, D ** -0.5)
+    for s in range(S):
+        assert bool((out[s, rows[s]:] == 0).all()) and bool(out[s].isfinite().all()), s
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("kind", ["int8", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_one_piece_of_many_keys(ctx, kind, D, dtype):
+    """Single tokens of 64 sequences of 4 key heads, whose keys are not cut: three sequences are long."""
+    S, KV, n = 64, 4, 4700
+    w = World(ctx, kind, S, KV, D, 64, n, dtype, 32)
+    keys = [7] * S
+    w.random(1, [0] * S, keys)
+    for i, s in enumerate((0, 30, 63)):
+        keys[s] = n - 300 * i
+        k, v = (randn(10 * i + j, 1, keys[s], KV, D, dtype=dtype) for j in (3, 4))
+        w.cache.tokens(w.table[s:s + 1].contiguous(), k.to(DEV), v.to(DEV), rotary=w.rotary).append(k.to(DEV), v.to(DEV))
+        w.ref.append(s, 0, R.turn32(k[0].float(), w.rotary.table.cpu(), 0, False), v[0].float())
+    q = randn(2, S, 1, KV, D, dtype=dtype)
+    g = q.to(DEV)
+    assert w.cache.queries(w.table, g, g, most_keys=n).workspace_bytes() == 16  # no pieces to join
+    start = [x - 1 for x in keys]
+    out = attend(w, q, start=start, keys=keys, scale=D ** -0.5, check=False)
+    for s in (0, 1, 30, 62, 63):
+        rows_in(w, q, out, s, 0, 1, start, keys, D ** -0.5)
