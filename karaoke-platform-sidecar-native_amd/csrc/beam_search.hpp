@@ -8,8 +8,10 @@
 // best `picks`; a second launch joins the stretches of a sequence's beams, in 64 bits.
 // The logits are read once: 256 rows of 120001 in bf16, 61 MB, 23 us (2.7 TB/s) and 7 us
 // for the join of 16 picks.  Two rounds of workgroups load and then compute; the VALU is
-// busy in 67% of the cycles, half of it for the maximum and the exponentials, half for the
-// best.  A step of one request is two launches, 4 to 6 us each.
+// busy in 68% of the cycles, half of it for the maximum and the exponentials, half for the
+// best.  A step of one request is two launches, 4 to 6 us each.  More lists than the join
+// compares at one place (a list is a beam's stretch) cost: 64 beams of 64 picks over 131072
+// tokens in fp32, 1024 lists, 114 us, over 140003, 1152 lists, 1043.
 #pragma once
 
 #include "beam_floor.hpp"

@@ -22,19 +22,19 @@
 //
 // Single tokens are bound by HBM, the cache is read once: 32 of 32 heads on 8 of 128 over
 // 16384 keys each, 8 bits, 1.07 GB in 162 us (6.6 TB/s; with loads that stay in the caches
-// 185, without asking for the next step's 182).  Chunks are bound by the vector
+// 185, without asking for the next step's 182).  Chunks over 8 bits are bound by the vector
 // instructions, the exponentials and conversions (83% of a busy CU's cycles; the matrix
-// instructions 21%): 4 x 517 causal tokens of 16 heads on 4 of 64 over up to 4613 keys
-// 61 us; with P's base moved at every larger maximum 70, with keys unbiased 64, with 128
-// registers and four waves a SIMD 80 instead of 67.
+// instructions 20%): 4 x 517 causal tokens of 16 heads on 4 of 64 over up to 4613 keys 63 us;
+// with P's base moved at every larger maximum 74, with keys unbiased 66, with 128 registers and
+// four waves a SIMD 144 (spilled).  Over bf16 pages of 128 dims by the matrix cores: 4 x 512
+// tokens of 32 heads on 8 over up to 4608 keys are 107 GFLOP, 215 with two operands, in 211 us
+// (1.02 PFLOP/s of the 1.1 to 1.2 of a large product).
 #pragma once
 
 #include "h2.hpp"
 #include "paged_cache.hpp"
 
 namespace vh {
-
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 struct CacheAttentionArgs {
     PagedArgs p;
@@ -108,10 +108,6 @@ VH_DEVICE void bytes_to_half(uint32_t w, uint32_t &lo, uint32_t &hi) {
         hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(halfx2, hi) + bias);
     }
 }
-template <bool I8>
-VH_DEVICE typename Operand16<I8>::type operand_of(u32x2 a, u32x2 b) {
-    return __builtin_bit_cast(typename Operand16<I8>::type, (u32x4){a[0], a[1], b[0], b[1]});
-}
 
 // A step's keys or values in registers, as the page holds them.
 template <int D, bool I8, int KB>
@@ -173,7 +169,7 @@ static __global__ __launch_bounds__(256, D == 64 && I8 ? 3 : 2) void cache_atten
     // of q' and P: bf16 out over 8 bits one operand (fp16's 11 bits, three more than out's),
     // over bf16 pages two, 16 bits: one has no more bits than out, and 4 x 512 causal tokens
     // over 4608 keys had 1.8 times the error of products in fp32 with it (3.0e-3 of the norm
-    // for 1.66e-3; 161 us, with two 214).  fp32 out as many as 22 bits and more take
+    // for 1.66e-3; 161 us, with two 211).  fp32 out as many as 22 bits and more take
     constexpr int DT = B::DT, QS = D / 32, N = sizeof(T) == 2 ? (I8 ? 1 : 2) : I8 ? 2 : 3;
     constexpr int ROWS = 16 * RG * (SPLIT ? 1 : 4);
     constexpr int KB = CQ_STEP, PER_FETCH = 64 / KB;
@@ -183,8 +179,8 @@ static __global__ __launch_bounds__(256, D == 64 && I8 ? 3 : 2) void cache_atten
     // Keys are asked for one step ahead when the last ones are multiplied, values likewise,
     // each in its one place, where two steps at once do not fit the registers: 4 x 512 causal
     // tokens of 32 heads on 8 of 128 over 4608 bf16 keys 211 us, twice kept 885 (74 registers
-    // spilled).  Elsewhere two steps are kept: these tokens over 8 bits 155 us against 167, 16 x
-    // 2048 tokens of 16 heads on 4 of 64 over as many bf16 keys 338 against 334.
+    // spilled).  Elsewhere two steps are kept: 16 x 2048 tokens of 16 heads on 4 of 64 over as
+    // many bf16 keys 338 us against 334.
     constexpr bool ROLLING = !I8 && D == 128 && RG > 1;
     constexpr float P_SCALE = I8 ? 0x1p10f : 1.0f;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -313,7 +309,10 @@ static __global__ __launch_bounds__(256, D == 64 && I8 ? 3 : 2) void cache_atten
         typedef const __attribute__((address_space(1))) char *Bytes;
         typedef const __attribute__((address_space(1))) u32x4 *Words;
         const Words from = (Words)((Bytes)at + (uint32_t)(16 * lane) + offset);
-        if constexpr (SPLIT && RG == 1) return __builtin_nontemporal_load(from);  // each key is read by one wave
+        // Past the caches: up to 16 rows each key is read by one wave.  fp32 queries of 128 dims
+        // have these loads with more rows too, whose workgroups read the same keys, and lose by
+        // it: 512 tokens of 32 heads on 8 over 4608 bf16 keys 191 us, with the others 112
+        if constexpr (SPLIT && RG == 1) return __builtin_nontemporal_load(from);
         else return *from;
     };
     auto load_values = [&](Step &st, int step) {

@@ -364,15 +364,15 @@ bool cache_reorder(hipStream_t s, const vh_cache *c, int beams, const int32_t *p
 // fourth step of the keys, else each wave has its own; and into pieces of the keys.
 // Measured over int8 pages, bf16 queries:
 //   CQ_ROWS   rows of their own from 512 workgroups on: 4 x 512 causal tokens of 32 heads
-//             on 8 of 128 over 4608 keys 165 us, from 1024 on 186; from 256 on, 4 x 517 of
-//             16 heads on 4 of 64 over 4613 take 125 us instead of 66; always shared, 16 x
-//             2048 of 16 on 4 of 64 take 358 instead of 293
+//             on 8 of 128 over 4608 keys 159 us, from 1024 on 171 (bf16 pages 212 and 237); from
+//             256 on, 4 x 517 of 16 heads on 4 of 64 over 4613 take 105 us instead of 63; always
+//             shared, 16 x 2048 of 16 on 4 of 64 take 344 instead of 269
 //   CQ_PIECES pieces until there are 512 workgroups: 16 single tokens of 32 heads on 8 of
-//             64, uneven, up to 8192 keys 25.9 us; until 384, 768, 1024: 28.1, 27.8, 29
+//             64, uneven, up to 8192 keys 24.7 us; until 384, 768, 1024: 27.6, 25.7, 27.2
 //   one piece from 256 workgroups on: 32 tokens of 32 heads on 8 of 128 over 16384 keys
-//             162 us, in two pieces 170
-//   a piece has 512 keys at least: one token of 8 heads over 77 to 8192 keys as long with
-//             256, or 1 us longer
+//             162 us, in two pieces 168
+//   a piece has 512 keys at least: one token of 32 heads on 8 of 128 over 8192 keys 15.8 us,
+//             with 256 16.5
 struct CacheCut {
     bool split, by_xcd;
     int groups, tiles;  // groups of 16 rows a wave has; workgroups of a (sequence, key head)
@@ -383,7 +383,7 @@ constexpr int CQ_MAX_ROWS = 1 << 30;
 constexpr int64_t CQ_ROWS = 512, CQ_PIECES = 512;
 // Groups of 16 rows of a wave at most: what 256 registers hold.  The 4 x 517 tokens above
 // 64 us with two, 75 with four (the registers spill); fp32 over 64 dims 39.5 with two, 43 with
-// one; the 4 x 512 tokens over bf16 pages 214 with two, 258 with one.
+// one; the 4 x 512 tokens over bf16 pages 211 with two, 258 with one.
 constexpr int most_groups(int type, int head_dim) { return type == VH_TYPE_FP32 && head_dim == 128 ? 1 : 2; }
 static CacheCut cache_cut(const vh_cache *c, const vh_cache_queries *q) {
     CacheCut cut;
