@@ -95,6 +95,46 @@ def test_beams_of_any_logits(ctx, shape, dtype, S, B, V, picks, vectors):
             assert got == v if math.isinf(v) else abs(got - v) <= 2.0 ** -20 + R.U * abs(v), s
 
 
+@pytest.mark.parametrize("dtype,S,B,V,picks,vectors", BEAM_SIZES)
+def test_beams_without_numbers_of_any_size(ctx, dtype, S, B, V, picks, vectors):
+    """Beams of nothing but -inf, with a NaN, with an infinity, without a score, and ended ones, beside others."""
+    end = 3
+    x, scores = beam_logits("normal", S, B, V, dtype, V), beam_scores(S, B, 4)
+    x[0, 0] = -math.inf
+    x[0, 1, V - 1] = math.nan
+    x[0, 2, 5] = math.inf
+    scores[1, 0], scores[1, 1] = -math.inf, math.nan
+    ended = torch.zeros(S, B, dtype=torch.int32)
+    ended[1, 2] = ended[S - 1, 3] = 1
+    x[1, 2] = math.nan  # not looked at
+    found = [[] for _ in range(S)]
+    for s in range(S):
+        for b in range(B):
+            v = scores[s, b].double() + torch.log_softmax(x[s, b].double(), 0)
+            if ended[s, b]:
+                v = torch.full((V,), -math.inf, dtype=torch.float64)
+                v[end] = scores[s, b].double()
+            if not bool(v.max() > -math.inf):  # of a NaN too
+                v = torch.full((V,), -math.inf, dtype=torch.float64)
+            a, t = torch.sort(v, descending=True, stable=True)
+            found[s] += [(float(p), b, int(i)) for p, i in zip(a[:picks], t[:picks])]
+        found[s].sort(key=lambda e: (-e[0], e[1]))
+        near = [p[0] - q[0] for p, q in zip(found[s][:picks], found[s][1:]) if p[1] != q[1] and math.isfinite(p[0])]
+        assert min(near, default=1) > 2.0 ** -18
+    g = x.to(DEV)
+    search = native.BeamSearch(ctx, g, picks=picks, end_token=end)
+    tokens, parents, done = (torch.full((S, picks), -5, dtype=torch.int32, device=DEV) for _ in range(3))
+    new = torch.full((S, picks), 5.0, device=DEV)
+    search.select(g, scores.to(DEV), tokens, parents, new, ended=ended.to(DEV), new_ended=done,
+                  workspace=torch.full((search.workspace_bytes(),), 0xff, dtype=torch.uint8, device=DEV))
+    for s in range(S):
+        want = found[s][:picks]
+        assert list(zip(parents[s].tolist(), tokens[s].tolist())) == [(b, t) for _, b, t in want], s
+        assert done[s].tolist() == [int(t == end or bool(ended[s, b])) for _, b, t in want]
+        for got, (v, _, _) in zip(new[s].tolist(), want):
+            assert got == v if math.isinf(v) else abs(got - v) <= 2.0 ** -19 + R.U * abs(v), s
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("V", [3000, 8192, 16384])
 @pytest.mark.parametrize("case", ["normal", "flat", "steps", "far", "large", "largest"])
