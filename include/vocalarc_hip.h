@@ -340,8 +340,9 @@ typedef struct {
     const int32_t *start; /* device [sequences], the position of row 0; null: 0 */
 } vh_rotary_rows;
 /* y = x with every row's heads turned.  y may be x (with its strides), else they do not
-   overlap.  backward: by the transpose, (a c + b s, b c - a s), which takes y's gradient to x's.  Issues
-   kernels only: no allocation, no synchronisation, fit for stream capture. */
+   overlap.  backward: by the transpose, (a c + b s, b c - a s), which takes y's gradient
+   to x's.  Issues kernels only: no allocation, no synchronisation, fit for stream
+   capture. */
 int vh_rotary_apply(vh_context *ctx, const vh_rotary *r, const vh_rotary_rows *rows, const void *x, void *y,
                     int backward);
 

@@ -166,11 +166,11 @@ template <typename T, int D, bool I8, int RG, bool SPLIT>
 static __global__ __launch_bounds__(256, D == 64 && I8 ? 3 : 2) void cache_attention_kernel(CacheAttentionArgs a) {
     using B = BlockShape<D, I8>;
     using Op = Operand16<I8>;
-    // of q' and P: bf16 out over 8 bits one operand (fp16's 11 bits, three more than out's: an
-    // error of 1.69e-3 of the norm, with two, as exact as products in fp32, 1.66e-3; 4 x 517
-    // causal tokens 63 us, with two 85), over bf16 pages two, 16 bits: one has no more bits than out, and 4 x 512 causal tokens
-    // over 4608 keys had 1.8 times the error of products in fp32 with it (3.0e-3 of the norm
-    // for 1.66e-3; 161 us, with two 211).  fp32 out as many as 22 bits and more take
+    // of q' and P.  bf16 out over 8 bits one operand, fp16's 11 bits, three more than out's: an
+    // error of 1.69e-3 of the norm, with two 1.66e-3, which products in fp32 have; 4 x 517 causal
+    // tokens 63 us, with two 85.  bf16 out over bf16 pages two, 16 bits: with one, which has no
+    // more bits than out, 4 x 512 causal tokens over 4608 keys had an error of 3.0e-3 for 1.66e-3
+    // (161 us, with two 211).  fp32 out as many as 22 bits and more take.
     constexpr int DT = B::DT, QS = D / 32, N = sizeof(T) == 2 ? (I8 ? 1 : 2) : I8 ? 2 : 3;
     constexpr int ROWS = 16 * RG * (SPLIT ? 1 : 4);
     constexpr int KB = CQ_STEP, PER_FETCH = 64 / KB;
